@@ -49,6 +49,8 @@ enum intent_b200_status {
 #define INTENT_B200_VIEW2(p) void* p, int64_t p##_d0, int64_t p##_d1, int64_t p##_s0, int64_t p##_s1
 #define INTENT_B200_VIEW3(p) void* p, int64_t p##_d0, int64_t p##_d1, int64_t p##_d2, \
                              int64_t p##_s0, int64_t p##_s1, int64_t p##_s2
+#define INTENT_B200_VIEW4(p) void* p, int64_t p##_d0, int64_t p##_d1, int64_t p##_d2, int64_t p##_d3, \
+                             int64_t p##_s0, int64_t p##_s1, int64_t p##_s2, int64_t p##_s3
 
 /* Library identity: returns a static string "intent_b200 <version> sm_100a". */
 INTENT_B200_API const char* intent_b200_version(void);
@@ -502,6 +504,92 @@ INTENT_B200_API int intent_b200_dequant_bf16_fp4_matmul(INTENT_B200_VIEW2(a0), I
 INTENT_B200_API int intent_b200_quantized_projection(INTENT_B200_VIEW3(a0), INTENT_B200_VIEW2(a1),
                                                      INTENT_B200_VIEW1(a2), void* workspace,
                                                      int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Norms and rotation of queries and keys; append to a paged cache
+ * (no counterpart in the reference: its examples stop at the projections).
+ *   q [T, HQ, D], k and v [T, HK, D]   f16 | bf16, D 64 or 128; rows may lie at any strides that keep each on a
+ *                                      16-byte boundary (slices of one projection's output), the last axis contiguous
+ *   positions [T] i32, rotary [P, R] f32: row p holds the cosines of R / 2 angles, then their sines; R a multiple of
+ *                                      16 up to D
+ *   q_weight, k_weight [D]             the _norm entries: x / sqrt(mean(x^2) + eps) * weight ahead of the rotation
+ *   pairs                              0 = (i, i + R/2), 1 = (2i, 2i + 1);  eps_bits: the f32 eps
+ *   slots [T] i64                      page * PAGE + place in the page; outside the cache (-1): the token is not stored
+ *   k_cache, v_cache [PAGES, HK, PAGE, D]   PAGE a power of two from 16 to 256
+ * f32 arithmetic, one rounding.  A position outside the table gives NaN.  Two tokens with one slot: either is stored.
+ * ------------------------------------------------------------------------ */
+INTENT_B200_API int intent_b200_qk_rope_f16(INTENT_B200_VIEW3(q), INTENT_B200_VIEW3(k), INTENT_B200_VIEW1(positions),
+                                         INTENT_B200_VIEW2(rotary), INTENT_B200_VIEW3(q_out), INTENT_B200_VIEW3(k_out),
+                                         int32_t pairs, void* stream);
+INTENT_B200_API int intent_b200_qk_norm_rope_f16(INTENT_B200_VIEW3(q), INTENT_B200_VIEW3(k), INTENT_B200_VIEW1(positions),
+                                              INTENT_B200_VIEW2(rotary), INTENT_B200_VIEW1(q_weight),
+                                              INTENT_B200_VIEW1(k_weight), INTENT_B200_VIEW3(q_out),
+                                              INTENT_B200_VIEW3(k_out), int32_t eps_bits, int32_t pairs, void* stream);
+INTENT_B200_API int intent_b200_paged_kv_append_f16(INTENT_B200_VIEW3(q), INTENT_B200_VIEW3(k), INTENT_B200_VIEW3(v),
+                                                 INTENT_B200_VIEW1(positions), INTENT_B200_VIEW1(slots),
+                                                 INTENT_B200_VIEW2(rotary), INTENT_B200_VIEW4(k_cache),
+                                                 INTENT_B200_VIEW4(v_cache), INTENT_B200_VIEW3(q_out), int32_t pairs,
+                                                 void* stream);
+INTENT_B200_API int intent_b200_paged_kv_append_norm_f16(INTENT_B200_VIEW3(q), INTENT_B200_VIEW3(k), INTENT_B200_VIEW3(v),
+                                                      INTENT_B200_VIEW1(positions), INTENT_B200_VIEW1(slots),
+                                                      INTENT_B200_VIEW2(rotary), INTENT_B200_VIEW1(q_weight),
+                                                      INTENT_B200_VIEW1(k_weight), INTENT_B200_VIEW4(k_cache),
+                                                      INTENT_B200_VIEW4(v_cache), INTENT_B200_VIEW3(q_out),
+                                                      int32_t eps_bits, int32_t pairs, void* stream);
+INTENT_B200_API int intent_b200_qk_rope_bf16(INTENT_B200_VIEW3(q), INTENT_B200_VIEW3(k), INTENT_B200_VIEW1(positions),
+                                         INTENT_B200_VIEW2(rotary), INTENT_B200_VIEW3(q_out), INTENT_B200_VIEW3(k_out),
+                                         int32_t pairs, void* stream);
+INTENT_B200_API int intent_b200_qk_norm_rope_bf16(INTENT_B200_VIEW3(q), INTENT_B200_VIEW3(k), INTENT_B200_VIEW1(positions),
+                                              INTENT_B200_VIEW2(rotary), INTENT_B200_VIEW1(q_weight),
+                                              INTENT_B200_VIEW1(k_weight), INTENT_B200_VIEW3(q_out),
+                                              INTENT_B200_VIEW3(k_out), int32_t eps_bits, int32_t pairs, void* stream);
+INTENT_B200_API int intent_b200_paged_kv_append_bf16(INTENT_B200_VIEW3(q), INTENT_B200_VIEW3(k), INTENT_B200_VIEW3(v),
+                                                 INTENT_B200_VIEW1(positions), INTENT_B200_VIEW1(slots),
+                                                 INTENT_B200_VIEW2(rotary), INTENT_B200_VIEW4(k_cache),
+                                                 INTENT_B200_VIEW4(v_cache), INTENT_B200_VIEW3(q_out), int32_t pairs,
+                                                 void* stream);
+INTENT_B200_API int intent_b200_paged_kv_append_norm_bf16(INTENT_B200_VIEW3(q), INTENT_B200_VIEW3(k), INTENT_B200_VIEW3(v),
+                                                      INTENT_B200_VIEW1(positions), INTENT_B200_VIEW1(slots),
+                                                      INTENT_B200_VIEW2(rotary), INTENT_B200_VIEW1(q_weight),
+                                                      INTENT_B200_VIEW1(k_weight), INTENT_B200_VIEW4(k_cache),
+                                                      INTENT_B200_VIEW4(v_cache), INTENT_B200_VIEW3(q_out),
+                                                      int32_t eps_bits, int32_t pairs, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Attention over a paged cache (no counterpart in the reference).
+ *   q, out [T, HQ, D]                  q may be strided as above; HQ a multiple of HK
+ *   k_cache, v_cache [PAGES, HK, PAGE, D]
+ *   page_table [B, W] i32              token j of sequence b lies in page page_table[b, j / PAGE]
+ *   query_offsets [B + 1] i32          rows of q of sequence b (paged_attention); row b (paged_decode_attention, T = B)
+ *   kv_lengths [B] i32                 tokens of sequence b in the cache, the new ones among them
+ * Query i of n sees the tokens j <= kv_length - n + i, with window > 0 only the last `window` of them.  No such token: a row
+ * of zeros.  Tokens behind kv_length, ahead of the window, in pages that the table does not name or whose number lies
+ * outside the cache are not read, whatever the memory there holds.  Rows of q that no sequence has are left alone.
+ * scale_bits: the f32 factor of the scores (> 0; 0: 1 / sqrt(D)).  f32 statistics and sums.
+ * workspace: at least ..._workspace_bytes(D) bytes, 16-byte aligned, zero-filled once; every launch leaves its counters
+ * zero again.  Launches that may overlap need separate ones.  Bytes 0..3: INTENT_B200_ERR_TIMEOUT of a bounded wait that
+ * gave up (..._workspace_status reads it and clears the workspace).  The same call gives the same bits.
+ * ------------------------------------------------------------------------ */
+INTENT_B200_API int intent_b200_paged_attention_f16(INTENT_B200_VIEW3(q), INTENT_B200_VIEW4(k_cache), INTENT_B200_VIEW4(v_cache),
+                                                 INTENT_B200_VIEW2(page_table), INTENT_B200_VIEW1(query_offsets),
+                                                 INTENT_B200_VIEW1(kv_lengths), INTENT_B200_VIEW3(out), int32_t scale_bits,
+                                                 int32_t window, void* workspace, int64_t workspace_bytes, void* stream);
+INTENT_B200_API int intent_b200_paged_decode_attention_f16(INTENT_B200_VIEW3(q), INTENT_B200_VIEW4(k_cache),
+                                                        INTENT_B200_VIEW4(v_cache), INTENT_B200_VIEW2(page_table),
+                                                        INTENT_B200_VIEW1(kv_lengths), INTENT_B200_VIEW3(out),
+                                                        int32_t scale_bits, int32_t window, void* workspace,
+                                                        int64_t workspace_bytes, void* stream);
+INTENT_B200_API int intent_b200_paged_attention_bf16(INTENT_B200_VIEW3(q), INTENT_B200_VIEW4(k_cache), INTENT_B200_VIEW4(v_cache),
+                                                 INTENT_B200_VIEW2(page_table), INTENT_B200_VIEW1(query_offsets),
+                                                 INTENT_B200_VIEW1(kv_lengths), INTENT_B200_VIEW3(out), int32_t scale_bits,
+                                                 int32_t window, void* workspace, int64_t workspace_bytes, void* stream);
+INTENT_B200_API int intent_b200_paged_decode_attention_bf16(INTENT_B200_VIEW3(q), INTENT_B200_VIEW4(k_cache),
+                                                        INTENT_B200_VIEW4(v_cache), INTENT_B200_VIEW2(page_table),
+                                                        INTENT_B200_VIEW1(kv_lengths), INTENT_B200_VIEW3(out),
+                                                        int32_t scale_bits, int32_t window, void* workspace,
+                                                        int64_t workspace_bytes, void* stream);
+INTENT_B200_API int64_t intent_b200_paged_attention_workspace_bytes(int64_t dim);
+INTENT_B200_API int intent_b200_paged_attention_workspace_status(void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
  * entry_benchmark counterparts of the reference's native ABI, which exports

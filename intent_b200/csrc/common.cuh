@@ -71,6 +71,10 @@ struct View3 {
   void* p;
   int64_t d0, d1, d2, s0, s1, s2;
 };
+struct View4 {
+  void* p;
+  int64_t d0, d1, d2, d3, s0, s1, s2, s3;
+};
 
 inline bool contiguous(const View1& v) { return v.d0 <= 1 || v.s0 == 1; }
 inline bool contiguous(const View2& v) {
@@ -78,6 +82,14 @@ inline bool contiguous(const View2& v) {
 }
 inline bool contiguous(const View3& v) {
   return (v.d2 <= 1 || v.s2 == 1) && (v.d1 <= 1 || v.s1 == v.d2) && (v.d0 <= 1 || v.s0 == v.d1 * v.d2);
+}
+inline bool contiguous(const View4& v) {
+  return (v.d3 <= 1 || v.s3 == 1) && (v.d2 <= 1 || v.s2 == v.d3) && (v.d1 <= 1 || v.s1 == v.d2 * v.d3) &&
+         (v.d0 <= 1 || v.s0 == v.d1 * v.d2 * v.d3);
+}
+// Rows of 16-bit elements in memory order, each on a 16-byte boundary if the first is, at any (not negative) distance.
+inline bool rows16(const View3& v) {
+  return (v.d2 <= 1 || v.s2 == 1) && (v.d1 <= 1 || (v.s1 >= 0 && v.s1 % 8 == 0)) && (v.d0 <= 1 || (v.s0 >= 0 && v.s0 % 8 == 0));
 }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -126,6 +138,7 @@ cudaError_t launch_programmatic(void (*kernel)(P...), dim3 grid, dim3 block, siz
 #define IB200_VIEW1_ARG(p) ib200::View1{p, p##_d0, p##_s0}
 #define IB200_VIEW2_ARG(p) ib200::View2{p, p##_d0, p##_d1, p##_s0, p##_s1}
 #define IB200_VIEW3_ARG(p) ib200::View3{p, p##_d0, p##_d1, p##_d2, p##_s0, p##_s1, p##_s2}
+#define IB200_VIEW4_ARG(p) ib200::View4{p, p##_d0, p##_d1, p##_d2, p##_d3, p##_s0, p##_s1, p##_s2, p##_s3}
 
 // ---- device side ---------------------------------------------------------
 #ifdef __CUDACC__

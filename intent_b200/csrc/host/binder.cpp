@@ -29,13 +29,14 @@
 namespace {
 
 enum Access { kIn = 0, kOut = 1, kInOut = 2 };
-constexpr int kMaxRank = 3, kMaxPlans = 16;
+constexpr int kMaxRank = 4, kMaxPlans = 16, kMaxSlots = 96;
 
 struct View {
   int access;
   at::ScalarType type;
   int rank;
   int64_t alignment;
+  int rows;                          // only the last axis is contiguous, every row on a 16-byte boundary
 };
 
 // What the Python binder found for one combination of shapes.
@@ -97,6 +98,23 @@ bool modes_active() {
               c10::DispatchKey::Functionalize, c10::DispatchKey::Python}));
 }
 
+// Whether the strides are those that the entry takes.  Not for empty tensors.
+bool layout_taken(const View& v, const at::Tensor& t) {
+  if (t.is_contiguous()) return true;
+  if (!v.rows || (t.size(v.rank - 1) != 1 && t.stride(v.rank - 1) != 1)) return false;
+  for (int d = 0; d + 1 < v.rank; ++d)
+    if (t.size(d) != 1 && t.stride(d) * int64_t(t.element_size()) % 16 != 0) return false;
+  return true;
+}
+
+// Elements from the first to behind the last.
+int64_t span(const at::Tensor& t) {
+  if (t.is_contiguous()) return t.numel();
+  int64_t last = 0;
+  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  return last + 1;
+}
+
 // `explicit_outputs`: every view is supplied; `private_workspace`: such a call owns its workspace, which is not made here
 PyObject* invoke(Binder* self, PyObject* arguments, bool explicit_outputs, bool private_workspace) {
   const auto& views = *self->views;
@@ -115,7 +133,7 @@ PyObject* invoke(Binder* self, PyObject* arguments, bool explicit_outputs, bool 
     if (!THPVariable_CheckExact(object)) return not_plain();
     const at::Tensor& t = THPVariable_Unpack(object);
     if (!t.defined() || t.scalar_type() != views[i].type || t.dim() != views[i].rank || !t.is_cuda() ||
-        t.get_device() != self->device || !plain_keys(t) || t.numel() == 0 || !t.is_contiguous())
+        t.get_device() != self->device || !plain_keys(t) || t.numel() == 0 || !layout_taken(views[i], t))
       return not_plain();
     supplied[i] = &t;
   }
@@ -136,7 +154,7 @@ PyObject* invoke(Binder* self, PyObject* arguments, bool explicit_outputs, bool 
   if (!plan || std::memcmp(plan->selection.data(), self->selection, self->selection_bytes) != 0) return not_plain();
 
   const auto stream = c10::cuda::getCurrentCUDAStream(self->device);
-  int64_t slots[64];
+  int64_t slots[kMaxSlots];
   int at_slot = 0;
   at::Tensor made[16];
   int64_t begin[16], end[16];
@@ -152,9 +170,9 @@ PyObject* invoke(Binder* self, PyObject* arguments, bool explicit_outputs, bool 
     const int rank = views[i].rank;
     const at::Tensor& t = supplied[i] ? *supplied[i] : made[i];
     const int64_t pointer = reinterpret_cast<int64_t>(t.data_ptr());
-    if (pointer % views[i].alignment != 0 || !t.is_contiguous()) return not_plain();
+    if (pointer % views[i].alignment != 0 || !layout_taken(views[i], t)) return not_plain();
     begin[i] = pointer;
-    end[i] = pointer + t.numel() * int64_t(t.element_size());
+    end[i] = pointer + span(t) * int64_t(t.element_size());
     slots[at_slot++] = pointer;
     for (int d = 0; d < rank; ++d) slots[at_slot++] = t.size(d);
     for (int d = 0; d < rank; ++d) slots[at_slot++] = t.stride(d);
@@ -310,7 +328,7 @@ PyObject* binder_forget(PyObject* object, PyObject*) {
 }
 
 // Binder(call address, slots, device, selection address, selection bytes, workspaces | None,
-//        ((access, dtype, rank, alignment), ...), constants)
+//        ((access, dtype, rank, alignment, rows), ...), constants)
 PyObject* binder_new(PyTypeObject* type, PyObject* arguments, PyObject*) {
   unsigned long long call, selection;
   int slots, device;
@@ -319,7 +337,7 @@ PyObject* binder_new(PyTypeObject* type, PyObject* arguments, PyObject*) {
   if (!PyArg_ParseTuple(arguments, "KiiKLOO!O!", &call, &slots, &device, &selection, &selection_bytes, &workspaces,
                         &PyTuple_Type, &views, &PyTuple_Type, &constants))
     return nullptr;
-  if (PyTuple_GET_SIZE(views) > 16 || slots > 63 || (workspaces != Py_None && !PyDict_Check(workspaces))) {
+  if (PyTuple_GET_SIZE(views) > 16 || slots >= kMaxSlots || (workspaces != Py_None && !PyDict_Check(workspaces))) {
     PyErr_SetString(PyExc_ValueError, "unsupported interface");
     return nullptr;
   }
@@ -342,7 +360,7 @@ PyObject* binder_new(PyTypeObject* type, PyObject* arguments, PyObject*) {
       View v;
       PyObject* dtype;
       long long alignment;
-      if (!PyArg_ParseTuple(PyTuple_GET_ITEM(views, i), "iOiL", &v.access, &dtype, &v.rank, &alignment)) {
+      if (!PyArg_ParseTuple(PyTuple_GET_ITEM(views, i), "iOiLi", &v.access, &dtype, &v.rank, &alignment, &v.rows)) {
         Py_DECREF(self);
         return nullptr;
       }

@@ -66,6 +66,18 @@ const Row kRows[] = {
     IB200_PACKED(intent_b200_moe_route_positions),
     IB200_PACKED(intent_b200_moe_route_top2),
     IB200_PACKED(intent_b200_moe_scatter_routes),
+    IB200_PACKED(intent_b200_paged_attention_bf16),
+    IB200_PACKED(intent_b200_paged_attention_f16),
+    IB200_PACKED(intent_b200_paged_decode_attention_bf16),
+    IB200_PACKED(intent_b200_paged_decode_attention_f16),
+    IB200_PACKED(intent_b200_paged_kv_append_bf16),
+    IB200_PACKED(intent_b200_paged_kv_append_f16),
+    IB200_PACKED(intent_b200_paged_kv_append_norm_bf16),
+    IB200_PACKED(intent_b200_paged_kv_append_norm_f16),
+    IB200_PACKED(intent_b200_qk_norm_rope_bf16),
+    IB200_PACKED(intent_b200_qk_norm_rope_f16),
+    IB200_PACKED(intent_b200_qk_rope_bf16),
+    IB200_PACKED(intent_b200_qk_rope_f16),
     IB200_PACKED(intent_b200_quantized_gemm_f16),
     IB200_PACKED(intent_b200_quantized_projection),
     IB200_PACKED(intent_b200_ragged_grouped_gemm_bf16),

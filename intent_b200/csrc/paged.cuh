@@ -1,0 +1,56 @@
+// What the kernels of attention over a paged cache share.
+#pragma once
+
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace ib200 {
+
+constexpr int kPagedCtas = 160;            // most CTAs of a launch
+constexpr int64_t kPagedHeader = 4096;     // bytes of the workspace ahead of the parts: status word, one counter per CTA
+
+struct PagedParams {
+  const uint16_t* q;                 // [T, HQ, D] at these strides (elements)
+  int64_t q_token, q_head;
+  uint16_t* out;                     // [T, HQ, D]
+  const int32_t* page_table;         // [B, table_width]
+  const int32_t* offsets;            // [B + 1] rows of q of every sequence; null: row b is sequence b's only one
+  const int32_t* lengths;            // [B] tokens in the cache, the new ones among them
+  int tokens, batch, q_heads, k_heads, group, table_width;
+  int pages, page_shift, capacity;   // capacity: tokens that a row of the page table can name
+  int window;                        // tokens that a query sees, its own among them; 0 = all
+  float scale;                       // of the scores, times log2(e)
+  int* status;                       // heads of the workspace
+  int* counters;
+  float* parts;
+};
+
+#ifdef __CUDACC__
+
+template <bool B>
+using Bool = std::integral_constant<bool, B>;
+
+struct TokenSpan {
+  int begin, count;
+};
+// rows of q of a sequence; offsets that make no sense are cut to the rows there are
+__device__ __forceinline__ TokenSpan span_of(const PagedParams& p, int b) {
+  if (!p.offsets) return {b, 1};
+  const int begin = min(max(__ldg(p.offsets + b), 0), p.tokens);
+  return {begin, min(max(__ldg(p.offsets + b + 1), begin), p.tokens) - begin};
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+#endif  // __CUDACC__
+
+int64_t paged_rows_workspace_bytes(int64_t dim);
+template <typename T>
+int paged_rows(const PagedParams& p, int64_t dim, const void* k_cache, const void* v_cache, int sms, cudaStream_t stream);
+
+}  // namespace ib200

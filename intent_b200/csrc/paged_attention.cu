@@ -1,0 +1,114 @@
+// Entries of attention over a paged cache: argument checks and the choice of the kernel.
+#include <cmath>
+#include <cstring>
+
+#include "paged.cuh"
+
+namespace ib200 {
+namespace {
+
+int device_sms() {
+  int device = 0, sms = 0;
+  if (cudaGetDevice(&device) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return sms;
+}
+
+template <typename T>
+int attend(const View3& q, const View4& k_cache, const View4& v_cache, const View2& table, const View1* offsets,
+           const View1& lengths, const View3& out, int32_t scale_bits, int32_t window, void* workspace, int64_t workspace_bytes,
+           cudaStream_t stream) {
+  const int64_t tokens = q.d0, heads = q.d1, dim = q.d2, pages = k_cache.d0, k_heads = k_cache.d1, page = k_cache.d2;
+  const int64_t batch = lengths.d0;
+  if (tokens < 0 || batch < 0 || heads <= 0 || k_heads <= 0 || heads % k_heads != 0 || k_cache.d3 != dim || v_cache.d0 != pages ||
+      v_cache.d1 != k_heads || v_cache.d2 != page || v_cache.d3 != dim || table.d0 != batch || out.d0 != tokens ||
+      out.d1 != heads || out.d2 != dim || (offsets ? offsets->d0 != batch + 1 : tokens != batch))
+    return INTENT_B200_ERR_SHAPE;
+  if (dim != 64 && dim != 128) return INTENT_B200_ERR_UNSUPPORTED;
+  if (page < 16 || page > 256 || (page & (page - 1)) != 0 || window < 0) return INTENT_B200_ERR_UNSUPPORTED;
+  constexpr int64_t kMost = (int64_t(1) << 31) - 1;
+  if (heads > 4096 || batch > (1 << 24) || tokens > kMost / heads || pages > kMost / (k_heads * page) || table.d1 > kMost / page)
+    return INTENT_B200_ERR_UNSUPPORTED;
+  float scale;
+  std::memcpy(&scale, &scale_bits, sizeof(float));
+  if (scale == 0.f) scale = 1.f / std::sqrt(float(dim));
+  if (!(scale > 0.f) || std::isinf(scale)) return INTENT_B200_ERR_UNSUPPORTED;
+  if (!rows16(q) || !contiguous(k_cache) || !contiguous(v_cache) || !contiguous(table) || !contiguous(lengths) ||
+      !contiguous(out) || (offsets && !contiguous(*offsets)) || !aligned16(q.p) || !aligned16(k_cache.p) ||
+      !aligned16(v_cache.p) || !aligned16(out.p))
+    return INTENT_B200_ERR_LAYOUT;
+  if (tokens == 0 || batch == 0) return INTENT_B200_OK;
+  if (!q.p || !out.p || !lengths.p || (offsets && !offsets->p)) return INTENT_B200_ERR_NULL;
+  if (pages == 0 || table.d1 == 0) {     // no token anywhere
+    if (observe_sink()) return INTENT_B200_OK;
+    return cuda_status(cudaMemsetAsync(out.p, 0, size_t(tokens * heads * dim) * 2, stream));
+  }
+  if (!k_cache.p || !v_cache.p || !table.p) return INTENT_B200_ERR_NULL;
+  if (!workspace || workspace_bytes < paged_rows_workspace_bytes(dim)) return INTENT_B200_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return INTENT_B200_ERR_LAYOUT;
+  const int sms = device_sms();
+  if (sms <= 0) return INTENT_B200_ERR_CUDA;
+
+  PagedParams p = {};
+  p.q = static_cast<const uint16_t*>(q.p);
+  p.q_token = q.s0, p.q_head = q.s1;
+  p.out = static_cast<uint16_t*>(out.p);
+  p.page_table = static_cast<const int32_t*>(table.p);
+  p.offsets = offsets ? static_cast<const int32_t*>(offsets->p) : nullptr;
+  p.lengths = static_cast<const int32_t*>(lengths.p);
+  p.tokens = int(tokens), p.batch = int(batch), p.q_heads = int(heads), p.k_heads = int(k_heads);
+  p.group = int(heads / k_heads);
+  p.table_width = int(table.d1), p.pages = int(pages), p.capacity = int(table.d1 * page);
+  while ((int64_t(1) << p.page_shift) < page) ++p.page_shift;
+  p.window = window;
+  p.scale = scale * 1.44269504f;         // log2(e): the exponentials are powers of two
+  p.status = static_cast<int*>(workspace);
+  p.counters = p.status + 16;
+  p.parts = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + kPagedHeader);
+  return paged_rows<T>(p, dim, k_cache.p, v_cache.p, sms, stream);
+}
+
+}  // namespace
+}  // namespace ib200
+
+extern "C" int64_t intent_b200_paged_attention_workspace_bytes(int64_t dim) {
+  return ib200::paged_rows_workspace_bytes(dim);
+}
+
+// Reads the status word at the head of a workspace after synchronising `stream`.  A launch that gave up on a bounded wait may
+// have left counters behind: the workspace is then cleared for reuse before the code is returned.
+extern "C" int intent_b200_paged_attention_workspace_status(void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!workspace || workspace_bytes < ib200::kPagedHeader) return INTENT_B200_ERR_WORKSPACE;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int value = 0;
+  cudaError_t e = cudaStreamSynchronize(s);
+  if (e == cudaSuccess) e = cudaMemcpy(&value, workspace, sizeof(int), cudaMemcpyDeviceToHost);
+  if (e == cudaSuccess && value != 0) {
+    e = cudaMemsetAsync(workspace, 0, size_t(ib200::kPagedHeader), s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  }
+  return e == cudaSuccess ? value : ib200::cuda_status(e);
+}
+
+#define IB200_PAGED_ENTRIES(NAME, TYPE)                                                                                    \
+  extern "C" int intent_b200_paged_attention_##NAME(                                                                       \
+      INTENT_B200_VIEW3(a0), INTENT_B200_VIEW4(a1), INTENT_B200_VIEW4(a2), INTENT_B200_VIEW2(a3), INTENT_B200_VIEW1(a4),   \
+      INTENT_B200_VIEW1(a5), INTENT_B200_VIEW3(a6), int32_t scale_bits, int32_t window, void* workspace,                   \
+      int64_t workspace_bytes, void* stream) {                                                                             \
+    const ib200::View1 offsets = IB200_VIEW1_ARG(a4);                                                                      \
+    return ib200::attend<TYPE>(IB200_VIEW3_ARG(a0), IB200_VIEW4_ARG(a1), IB200_VIEW4_ARG(a2), IB200_VIEW2_ARG(a3),         \
+                               &offsets, IB200_VIEW1_ARG(a5), IB200_VIEW3_ARG(a6), scale_bits, window, workspace,          \
+                               workspace_bytes, static_cast<cudaStream_t>(stream));                                        \
+  }                                                                                                                        \
+  extern "C" int intent_b200_paged_decode_attention_##NAME(                                                                \
+      INTENT_B200_VIEW3(a0), INTENT_B200_VIEW4(a1), INTENT_B200_VIEW4(a2), INTENT_B200_VIEW2(a3), INTENT_B200_VIEW1(a4),   \
+      INTENT_B200_VIEW3(a5), int32_t scale_bits, int32_t window, void* workspace, int64_t workspace_bytes, void* stream) { \
+    return ib200::attend<TYPE>(IB200_VIEW3_ARG(a0), IB200_VIEW4_ARG(a1), IB200_VIEW4_ARG(a2), IB200_VIEW2_ARG(a3),         \
+                               nullptr, IB200_VIEW1_ARG(a4), IB200_VIEW3_ARG(a5), scale_bits, window, workspace,           \
+                               workspace_bytes, static_cast<cudaStream_t>(stream));                                        \
+  }
+IB200_PAGED_ENTRIES(f16, __half)
+IB200_PAGED_ENTRIES(bf16, __nv_bfloat16)

@@ -1,0 +1,556 @@
+// Attention over a paged cache for few rows of queries per sequence and key head: a decode step, or short chunks.
+//
+// Program (paged_decode_attention; paged_attention for chunks): query row x at position p of a sequence with n new tokens and
+// L tokens in the cache (p = L - n + i), over the tokens j with max(0, p - W + 1) <= j <= p (W = 0: no window)
+//   o = sum_j softmax_j(scale * x . k_j) * v_j,     zero where there is no such token
+// Token j of sequence b lies in page page_table[b, j / PAGE]; the tokens of a page number outside the cache are not seen.
+// All statistics and sums are in f32; the weights of one product with V are rounded to the 16-bit type (relative to the
+// running maximum, so at most 1), as the tensor core takes them.
+//
+// Bound by HBM: a token's keys and values (4 D bytes per key head) are read once for the whole group of query heads that share
+// them.  What has to be right for that:
+//  * Loads run ahead.  A warp has its own ring of three units of 32 tokens (16 KiB each with D = 128), filled by TMA through
+//    128B-swizzled boxes of one page's rows, so that 192 KiB are asked for per SM whatever the warp is computing.
+//  * Work is cut evenly, not by sequence.  All steps of 128 tokens of all (sequence, key head, row tile) form one line, of
+//    which every CTA takes the same number; a long sequence is shared by many CTAs and a CTA goes through many short ones
+//    while its ring runs on.  A row tile that was cut leaves its parts (maximum, sum, unscaled result) in the workspace, and
+//    the CTA that finishes last puts them together in CTA order: the same bits in every launch.
+//  * Few instructions per token.  Keys are the tensor core's A operand (16 tokens) and the queries its B operand (eight rows,
+//    kept in registers): S^T = K Q^T, then O^T += V^T P^T with V^T from transposing loads and P^T from one movmatrix per
+//    eight tokens.  With up to eight query heads per key head nothing is computed for rows that are not there.
+#include <cstring>
+
+#include "common.cuh"
+#include "paged.cuh"
+#include "tma.cuh"
+
+namespace ib200 {
+namespace {
+
+constexpr int WARPS = 4, THREADS = 32 * WARPS;
+constexpr int UNIT = 32;                 // tokens of a ring slot
+constexpr int STEP = UNIT * WARPS;       // tokens of a CTA's step
+
+template <int D>
+struct Ring {
+  static constexpr int STAGES = D == 128 ? 3 : 6;
+  static constexpr int HALF = UNIT * 128;                 // 64 elements of every token of a unit
+  static constexpr int OPERAND = HALF * (D / 64);         // keys or values of a unit
+  static constexpr int SLOT = 2 * OPERAND;
+  static constexpr int BYTES = WARPS * STAGES * SLOT;
+};
+
+template <int D, int NT>
+constexpr int smem_bytes() {
+  return 1024 + Ring<D>::BYTES + WARPS * 8 * NT * (D + 4) * 4 + 2 * WARPS * 8 * NT * 4 + WARPS * Ring<D>::STAGES * 8 + 64;
+}
+
+// One sequence's share of the line of steps
+struct Sequence {
+  int rows;        // query rows of a key head: new tokens x group
+  int first_row;   // its first token among all
+  int length;      // tokens in the cache
+  int first;       // position of its first query
+  int low;         // first token that any of its queries sees
+  int begin;       // first step
+  int steps;       // of a row tile, one at least: a tile without tokens writes zeros
+  int items;       // row tiles of all key heads
+};
+
+__device__ __forceinline__ Sequence sequence_of(const PagedParams& p, int b, int tile_rows) {
+  Sequence s;
+  const TokenSpan span = span_of(p, b);
+  s.rows = span.count * p.group;
+  s.first_row = span.begin;
+  s.length = min(max(__ldg(p.lengths + b), 0), p.capacity);
+  s.first = s.length - span.count;
+  s.low = p.window > 0 ? min(max(s.first - p.window + 1, 0), s.length) : 0;
+  s.begin = s.low / STEP;
+  s.steps = max((s.length + STEP - 1) / STEP - s.begin, 1);
+  s.items = (s.rows + tile_rows - 1) / tile_rows * p.k_heads;
+  return s;
+}
+
+// A place on the line of steps
+struct Walk {
+  Sequence s;
+  int b, item, step;
+  __device__ __forceinline__ void advance(const PagedParams& p, int tile_rows) {
+    if (++step < s.steps) return;
+    step = 0;
+    if (++item < s.items) return;
+    item = 0;
+    do {
+      if (++b >= p.batch) return;
+      s = sequence_of(p, b, tile_rows);
+    } while (s.items == 0);
+  }
+};
+
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ uint32_t movmatrix(uint32_t v) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
+}
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(THREADS, 1)
+paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedParams p) {
+  using R = Ring<D>;
+  constexpr int ROWS = 8 * NT, PITCH = D + 4;
+  extern __shared__ unsigned char smem_raw[];
+  programmatic_begin();
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  unsigned char* base_ptr = smem_raw + (base - smem_u32(smem_raw));
+  float* join = reinterpret_cast<float*>(base_ptr + R::BYTES);          // [WARPS][ROWS][PITCH]
+  float* join_max = join + WARPS * ROWS * PITCH;                        // [WARPS][ROWS]
+  float* join_sum = join_max + WARPS * ROWS;
+  int* shared = reinterpret_cast<int*>(join_sum + WARPS * ROWS);        // [4], then the warps' sums in 64 bits
+  long long* warp_sums = reinterpret_cast<long long*>(shared + 4);
+  const uint32_t bars = smem_u32(warp_sums + WARPS);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t ring = base + warp * R::STAGES * R::SLOT, full = bars + warp * R::STAGES * 8;
+  if (lane == 0) {
+    for (int s = 0; s < R::STAGES; ++s) mbar_init(full + 8 * s, 1);
+    fence_mbar_init();
+  }
+  programmatic_wait();
+
+  // ---- this CTA's part of the line
+  const int per_thread = (p.batch + THREADS - 1) / THREADS, mine = tid * per_thread;
+  long long sum = 0;
+  for (int b = mine; b < min(mine + per_thread, p.batch); ++b) {
+    const Sequence s = sequence_of(p, b, ROWS);
+    sum += (long long)s.items * s.steps;
+  }
+  long long before = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const long long v = __shfl_up_sync(0xffffffffu, before, d);
+    if (lane >= d) before += v;
+  }
+  if (lane == 31) warp_sums[warp] = before;
+  __syncthreads();
+  long long line = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    if (w < warp) before += warp_sums[w];
+    line += warp_sums[w];
+  }
+  before -= sum;
+  if (line > 0x3fffffff) {               // (only offsets that make no sense name so much)
+    if (tid == 0) atomicExch(p.status, INTENT_B200_ERR_SHAPE);
+    return;
+  }
+  const int total = int(line);
+  const int share = (total + int(gridDim.x) - 1) / int(gridDim.x);     // steps of a CTA
+  const int cta = blockIdx.x;
+  const int begin = min(cta * share, total), end = min(begin + share, total);
+  if (begin >= end) return;
+  if (begin >= before && begin < before + sum) {
+    int b = mine, at = int(before);
+    for (;; ++b) {
+      const Sequence s = sequence_of(p, b, ROWS);
+      if (begin < at + s.items * s.steps) break;
+      at += s.items * s.steps;
+    }
+    shared[0] = b;
+    shared[1] = at;
+  }
+  __syncthreads();
+  Walk load;
+  load.b = shared[0];
+  load.s = sequence_of(p, load.b, ROWS);
+  load.item = (begin - shared[1]) / load.s.steps;
+  load.step = (begin - shared[1]) - load.item * load.s.steps;
+  Walk work = load;
+
+  const float infinity = __int_as_float(0x7f800000);
+  int loading = begin, slot_in = 0, slot_out = 0;
+  uint32_t parity = 0, present = 0;      // a bit per slot; two bits per unit asked for (its halves), the oldest lowest
+  int queued = 0;
+  bool ok = true;
+
+  // asks for the unit of this warp at `load`, and goes on
+  auto ask = [&] {
+    const int tiles = (load.s.rows + ROWS - 1) / ROWS;
+    const int head = load.item / tiles, token = (load.s.begin + load.step) * STEP + warp * UNIT;
+    int row[2];
+    bool here[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int t = token + i * (UNIT / 2);
+      here[i] = t < load.s.length && t + UNIT / 2 > load.s.low;
+      int page = -1;
+      if (here[i]) page = __ldg(p.page_table + int64_t(load.b) * p.table_width + (t >> p.page_shift));
+      here[i] = page >= 0 && page < p.pages;
+      row[i] = ((page * p.k_heads + head) << p.page_shift) + (t & ((1 << p.page_shift) - 1));
+    }
+    const int halves = int(here[0]) + int(here[1]);
+    if (lane == 0 && halves) {
+      const uint32_t bar = full + 8 * slot_in, to = ring + slot_in * R::SLOT;
+      mbar_expect_tx(bar, halves * (R::SLOT / 2));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (!here[i]) continue;
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          tma_load_2d(to + c * R::HALF + i * (R::HALF / 2), &map_k, 64 * c, row[i], bar);
+          tma_load_2d(to + R::OPERAND + c * R::HALF + i * (R::HALF / 2), &map_v, 64 * c, row[i], bar);
+        }
+      }
+    }
+    present |= (uint32_t(here[0]) | (uint32_t(here[1]) << 1)) << (2 * queued);
+    ++queued;
+    if (halves) slot_in = slot_in + 1 == R::STAGES ? 0 : slot_in + 1;
+    ++loading;
+    load.advance(p, ROWS);
+  };
+  for (int i = 0; i < R::STAGES && loading < end; ++i) ask();
+
+  uint32_t qf[NT][D / 16][2];            // queries as B fragments: k = elements, n = rows
+  float o[NT][D / 16][4];                // O^T: elements 16 i + lane / 4 (+ 8) of rows 2 (lane % 4) (+ 1)
+  float top[NT][2], weight_sum[NT][2];
+  int position[NT][2];                   // of this thread's rows; -1 where there is none
+  int least = 0, most = 0;               // positions of the tile's first and last row
+  bool fresh = true;
+  for (int at = begin; at < end; ++at) {
+    const int tiles = (work.s.rows + ROWS - 1) / ROWS;
+    const int head = work.item / tiles, tile_row = (work.item - head * tiles) * ROWS;
+    if (fresh) {
+      fresh = false;
+      const int rows = min(ROWS, work.s.rows - tile_row);
+      least = work.s.first + tile_row / p.group;
+      most = work.s.first + (tile_row + rows - 1) / p.group;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = tile_row + nt * 8 + 2 * (lane & 3) + e;
+          position[nt][e] = r < work.s.rows ? work.s.first + r / p.group : -1;
+          top[nt][e] = -infinity;
+          weight_sum[nt][e] = 0.f;
+        }
+        const int r = min(tile_row + nt * 8 + (lane >> 2), work.s.rows - 1), token = r / p.group;
+        const uint16_t* x = p.q + int64_t(work.s.first_row + token) * p.q_token +
+                            int64_t(head * p.group + r - token * p.group) * p.q_head;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          qf[nt][i][0] = __ldg(reinterpret_cast<const uint32_t*>(x + 16 * i + 2 * (lane & 3)));
+          qf[nt][i][1] = __ldg(reinterpret_cast<const uint32_t*>(x + 16 * i + 8 + 2 * (lane & 3)));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
+        }
+      }
+    }
+    const uint32_t halves = present & 3;
+    present >>= 2;
+    --queued;
+    if (halves) {
+      const int token = (work.s.begin + work.step) * STEP + warp * UNIT;
+      const uint32_t keys = ring + slot_out * R::SLOT, values = keys + R::OPERAND;
+      if (ok) ok = mbar_wait_warp(full + 8 * slot_out, (parity >> slot_out) & 1);
+      parity ^= 1u << slot_out;
+      slot_out = slot_out + 1 == R::STAGES ? 0 : slot_out + 1;
+
+      float s[NT][2][4];                 // S^T: tokens 16 m + lane / 4 (+ 8), rows as in o
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt][m][e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const int r = 16 * m + (lane & 15), c = 2 * (i & 3) + (lane >> 4);
+          uint32_t a[4];
+          ldmatrix_x4(a, keys + (i / 4) * R::HALF + r * 128 + ((c ^ (r & 7)) << 4));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) Elem<T>::mma16816(s[nt][m], a[0], a[1], a[2], a[3], qf[nt][i][0], qf[nt][i][1]);
+        }
+      const bool all = halves == 3 && token + UNIT - 1 <= least && (p.window == 0 || token > most - p.window);
+      uint32_t counted[2][2] = {};       // pairs of tokens 16 m + 2 (lane % 4) (+ 8) that some row of the tile sees
+      if (!all) {
+        const int low = p.window > 0 ? max(least - p.window + 1, 0) : 0;
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const bool there = (halves >> m) & 1;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int t = token + 16 * m + (lane >> 2) + 8 * (e >> 1), at_row = position[nt][e & 1];
+              if (!there || t > at_row || (p.window > 0 && t <= at_row - p.window)) s[nt][m][e] = -infinity;
+            }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            // (what lies behind the tile's last token, or was never loaded, may be no number: 0 * NaN is NaN)
+            const int t = token + 16 * m + 8 * e + 2 * (lane & 3);
+            if (there && t >= low && t <= most) counted[m][e] |= 0xffffu;
+            if (there && t + 1 >= low && t + 1 <= most) counted[m][e] |= 0xffff0000u;
+          }
+        }
+      }
+      uint32_t pf[NT][2][2];             // P^T as B fragments
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float factor[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float most_here = fmaxf(fmaxf(s[nt][0][e], s[nt][0][e + 2]), fmaxf(s[nt][1][e], s[nt][1][e + 2]));
+#pragma unroll
+          for (int d = 4; d < 32; d *= 2) most_here = fmaxf(most_here, __shfl_xor_sync(0xffffffffu, most_here, d));
+          const float old = top[nt][e], now = fmaxf(old, most_here * p.scale);
+          top[nt][e] = now;
+          const float origin = now == -infinity ? 0.f : now;
+          factor[e] = exp2_fast(old - origin);
+          float added = 0.f;
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int f = 0; f < 4; f += 2) {
+              const float w = exp2_fast(fmaf(s[nt][m][e + f], p.scale, -origin));
+              s[nt][m][e + f] = w;
+              added += w;
+            }
+          weight_sum[nt][e] = fmaf(weight_sum[nt][e], factor[e], added);
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          pf[nt][m][0] = movmatrix(Elem<T>::pack2(s[nt][m][0], s[nt][m][1]));
+          pf[nt][m][1] = movmatrix(Elem<T>::pack2(s[nt][m][2], s[nt][m][3]));
+        }
+        if (__any_sync(0xffffffffu, factor[0] != 1.f || factor[1] != 1.f)) {
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[nt][i][e] *= factor[e & 1];
+        }
+      }
+      auto values_of = [&](auto whole, int m, int i, uint32_t (&a)[4]) {   // elements 16 i of tokens 16 m, as A fragments
+        const int r = 16 * m + (lane & 7) + ((lane >> 4) << 3), c = 2 * (i & 3) + ((lane >> 3) & 1);
+        ldmatrix_x4_trans(a, values + (i / 4) * R::HALF + r * 128 + ((c ^ (r & 7)) << 4));
+        if (!decltype(whole)::value)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a[e] &= counted[m][e >> 1];
+      };
+      auto not_finite = [&](auto& loaded) {
+        constexpr uint32_t EXPONENT = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+        bool found = false;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll 2
+          for (int i = 0; i < D / 16; ++i) {
+            uint32_t a[4];
+            loaded(Bool<false>{}, m, i, a);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) found |= (a[e] & EXPONENT) == EXPONENT || ((a[e] >> 16) & EXPONENT) == EXPONENT;
+          }
+        return __any_sync(0xffffffffu, found) != 0;
+      };
+      auto add_values = [&](auto whole) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            uint32_t a[4];
+            values_of(whole, m, i, a);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) Elem<T>::mma16816(o[nt][i], a[0], a[1], a[2], a[3], pf[nt][m][0], pf[nt][m][1]);
+          }
+      };
+      if (all) {
+        add_values(Bool<true>{});
+      } else if (least == most || !not_finite(values_of)) {
+        add_values(Bool<false>{});
+      } else {
+        // Values that are no finite numbers, in tokens that some rows see and others do not: row by row, from what it sees.
+#pragma unroll 1
+        for (int r = 0; r < ROWS; ++r) {
+          const int even = NT == 2 && r >= 8 ? position[NT - 1][0] : position[0][0];
+          const int odd = NT == 2 && r >= 8 ? position[NT - 1][1] : position[0][1];
+          const int at_row = __shfl_sync(0xffffffffu, r & 1 ? odd : even, (r & 7) >> 1);
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            uint32_t sees[2] = {};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int t = token + 16 * m + 8 * (e >> 1) + 2 * (lane & 3) + (e & 1);
+              if (t <= at_row && (p.window == 0 || t > at_row - p.window)) sees[e >> 1] |= e & 1 ? 0xffff0000u : 0xffffu;
+            }
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              uint32_t a[4];
+              values_of(Bool<false>{}, m, i, a);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) a[e] &= sees[e >> 1];
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                float part[4] = {};
+                Elem<T>::mma16816(part, a[0], a[1], a[2], a[3], pf[nt][m][0], pf[nt][m][1]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (nt * 8 + 2 * (lane & 3) + (e & 1) == r) o[nt][i][e] += part[e];
+              }
+            }
+          }
+        }
+      }
+      __syncwarp();                      // every lane is done with the slot
+    }
+    if (loading < end) ask();
+
+    const bool last_step = work.step + 1 == work.s.steps;
+    if (last_step || at + 1 == end) {
+      // ---- the warps' parts, then the CTAs'
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = nt * 8 + 2 * (lane & 3) + e;
+          float sum_all = weight_sum[nt][e];
+#pragma unroll
+          for (int d = 4; d < 32; d *= 2) sum_all += __shfl_xor_sync(0xffffffffu, sum_all, d);
+          if (lane < 4) {
+            join_max[warp * ROWS + r] = top[nt][e];
+            join_sum[warp * ROWS + r] = sum_all;
+          }
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            float* to = join + (warp * ROWS + r) * PITCH + 16 * i + (lane >> 2);
+            to[0] = o[nt][i][e];
+            to[8] = o[nt][i][e + 2];
+          }
+        }
+      }
+      __syncthreads();
+      const int rows = min(ROWS, work.s.rows - tile_row);
+      const int item_begin = at - work.step, item_end = item_begin + work.s.steps;   // on the line
+      const int first_cta = item_begin / share, last_cta = (item_end - 1) / share;
+      const bool whole = first_cta == last_cta;
+      float* part = p.parts + size_t(2 * cta + (cta == first_cta)) * (ROWS * (D + 2));
+      auto store = [&](int r, int c, const float (&x)[8], float l) {
+        const float inverse = l == 0.f ? 0.f : 1.f / l;
+        const int token = (tile_row + r) / p.group, of_group = tile_row + r - token * p.group;
+        uint16_t* to = p.out + (int64_t(work.s.first_row + token) * p.q_heads + head * p.group + of_group) * D + 8 * c;
+        *reinterpret_cast<uint4*>(to) =
+            make_uint4(Elem<T>::pack2(x[0] * inverse, x[1] * inverse), Elem<T>::pack2(x[2] * inverse, x[3] * inverse),
+                       Elem<T>::pack2(x[4] * inverse, x[5] * inverse), Elem<T>::pack2(x[6] * inverse, x[7] * inverse));
+      };
+      for (int w = tid; w < rows * (D / 8); w += THREADS) {
+        const int r = w / (D / 8), c = w - r * (D / 8);
+        float m = -infinity, l = 0.f, x[8] = {};
+#pragma unroll
+        for (int v = 0; v < WARPS; ++v) m = fmaxf(m, join_max[v * ROWS + r]);
+        const float origin = m == -infinity ? 0.f : m;
+#pragma unroll
+        for (int v = 0; v < WARPS; ++v) {
+          const float f = exp2_fast(join_max[v * ROWS + r] - origin);
+          l = fmaf(join_sum[v * ROWS + r], f, l);
+          const float* from = join + (v * ROWS + r) * PITCH + 8 * c;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = fmaf(from[e], f, x[e]);
+        }
+        if (whole) {
+          store(r, c, x, l);
+        } else {
+          float4* to = reinterpret_cast<float4*>(part + r * D + 8 * c);
+          to[0] = make_float4(x[0], x[1], x[2], x[3]);
+          to[1] = make_float4(x[4], x[5], x[6], x[7]);
+          if (c == 0) {
+            part[ROWS * D + r] = m;
+            part[ROWS * (D + 1) + r] = l;
+          }
+        }
+      }
+      if (!whole) {
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) shared[2] = atomicAdd(p.counters + first_cta, 1);
+        __syncthreads();
+        if (shared[2] == last_cta - first_cta) {
+          __threadfence();
+          if (tid == 0) p.counters[first_cta] = 0;
+          for (int w = tid; w < rows * (D / 8); w += THREADS) {
+            const int r = w / (D / 8), c = w - r * (D / 8);
+            float m = -infinity, l = 0.f, x[8] = {};
+            for (int v = first_cta; v <= last_cta; ++v)
+              m = fmaxf(m, __ldcg(p.parts + size_t(2 * v + (v == first_cta)) * (ROWS * (D + 2)) + ROWS * D + r));
+            const float origin = m == -infinity ? 0.f : m;
+#pragma unroll 2
+            for (int v = first_cta; v <= last_cta; ++v) {
+              const float* from = p.parts + size_t(2 * v + (v == first_cta)) * (ROWS * (D + 2));
+              const float f = exp2_fast(__ldcg(from + ROWS * D + r) - origin);
+              l = fmaf(__ldcg(from + ROWS * (D + 1) + r), f, l);
+              const float4 y0 = __ldcg(reinterpret_cast<const float4*>(from + r * D + 8 * c));
+              const float4 y1 = __ldcg(reinterpret_cast<const float4*>(from + r * D + 8 * c) + 1);
+              x[0] = fmaf(y0.x, f, x[0]), x[1] = fmaf(y0.y, f, x[1]), x[2] = fmaf(y0.z, f, x[2]), x[3] = fmaf(y0.w, f, x[3]);
+              x[4] = fmaf(y1.x, f, x[4]), x[5] = fmaf(y1.y, f, x[5]), x[6] = fmaf(y1.z, f, x[6]), x[7] = fmaf(y1.w, f, x[7]);
+            }
+            store(r, c, x, l);
+          }
+        }
+      }
+      __syncthreads();                   // the join's buffer is free again
+      fresh = true;
+    }
+    if (at + 1 < end) work.advance(p, ROWS);
+  }
+  if (!ok) {
+    // (nothing may be on its way to a CTA that is gone)
+    for (int s = 0; s < R::STAGES; ++s) mbar_wait_warp(full + 8 * s, (parity >> s) & 1, 64);
+    if (lane == 0) atomicExch(p.status, INTENT_B200_ERR_TIMEOUT);
+  }
+}
+
+template <typename T, int D, int NT>
+int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, const PagedParams& p, int grid, cudaStream_t stream) {
+  auto kernel = paged_rows_kernel<T, D, NT>;
+  constexpr int smem = smem_bytes<D, NT>();
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return cuda_status(e);
+  if (LaunchFacts* sink = observe_sink())
+    return record_launch(sink, reinterpret_cast<const void*>(kernel),
+                         NT == 1 ? "paged_rows_kernel 8 rows" : "paged_rows_kernel 16 rows", grid, THREADS, smem, 1);
+  e = launch_programmatic(kernel, dim3(unsigned(grid)), dim3(THREADS), smem, stream, 1, map_k, map_v, p);
+  if (e != cudaSuccess) return cuda_status(e);
+  note_launch();
+  return launch_status();
+}
+
+}  // namespace
+
+int64_t paged_rows_workspace_bytes(int64_t dim) {
+  return kPagedHeader + int64_t(2) * kPagedCtas * 16 * (dim + 2) * int64_t(sizeof(float));
+}
+
+template <typename T>
+int paged_rows(const PagedParams& p, int64_t dim, const void* k_cache, const void* v_cache, int sms, cudaStream_t stream) {
+  CUtensorMap map_k, map_v;
+  const uint64_t rows = uint64_t(p.pages) * uint64_t(p.k_heads) << p.page_shift;
+  constexpr auto type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  if (!make_tensor_map_2d(&map_k, type, k_cache, rows, uint64_t(dim), uint64_t(dim) * 2, UNIT / 2, 64,
+                          CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_tensor_map_2d(&map_v, type, v_cache, rows, uint64_t(dim), uint64_t(dim) * 2, UNIT / 2, 64,
+                          CU_TENSOR_MAP_SWIZZLE_128B))
+    return INTENT_B200_ERR_CUDA;
+  const int grid = sms < kPagedCtas ? sms : kPagedCtas;
+  const bool narrow = !p.offsets && p.group <= 8;
+  if (dim == 128)
+    return narrow ? launch<T, 128, 1>(map_k, map_v, p, grid, stream) : launch<T, 128, 2>(map_k, map_v, p, grid, stream);
+  return narrow ? launch<T, 64, 1>(map_k, map_v, p, grid, stream) : launch<T, 64, 2>(map_k, map_v, p, grid, stream);
+}
+template int paged_rows<__half>(const PagedParams&, int64_t, const void*, const void*, int, cudaStream_t);
+template int paged_rows<__nv_bfloat16>(const PagedParams&, int64_t, const void*, const void*, int, cudaStream_t);
+
+}  // namespace ib200

@@ -849,3 +849,134 @@ moe_peer_wait = KernelDefinition(
     "bounded wait until every rank has announced itself at the sync point")
 
 ALL.update({d.name: d for d in (moe_peer_post, moe_peer_wait)})
+
+
+# ---------------------------------------------------------------------------------
+# Attention over a paged cache: norms and rotation, the append, chunks and single tokens
+# ---------------------------------------------------------------------------------
+_PAIRS = {"halves": 0, "neighbours": 1}
+
+
+def _f32_bits(value, name):
+    import struct
+
+    try:
+        return struct.unpack("<i", struct.pack("<f", float(value)))[0]
+    except (TypeError, ValueError, OverflowError):
+        raise CompilationStageError("frontend_kir", f"{name} must be a finite number, got {value!r}") from None
+
+
+def _head_rules():
+    return (_rule(lambda d: d["D"] in (64, 128), lambda d: f"heads must have 64 or 128 elements, got {d['D']}"),)
+
+
+def _cache_rules():
+    return (_rule(lambda d: 16 <= d["PAGE"] <= 256 and d["PAGE"] & (d["PAGE"] - 1) == 0,
+                  lambda d: f"a page must hold a power of two from 16 to 256 tokens, got {d['PAGE']}"),)
+
+
+def _lower_rotation(c, device, *, cache):
+    act = _act_dtype(c)
+    pairs = _PAIRS.get(c["PAIRS"])
+    if pairs is None:
+        raise CompilationStageError("frontend_kir", "PAIRS must be 'halves' or 'neighbours'")
+    eps = _f32_bits(c["EPS"], "EPS")
+    if not 0 <= float(c["EPS"]) < float("inf"):
+        raise CompilationStageError("frontend_kir", "EPS must be a finite number that is not negative")
+    views = []
+
+    def view(name, element, shape, access=IN, alignment=16, layout="contiguous"):
+        views.append(ViewParameter(len(views), name, element, shape, access, alignment, layout))
+
+    view("q", act, ("T", "HQ", "D"), layout="rows")
+    view("k", act, ("T", "HK", "D"), layout="rows")
+    if cache:
+        view("v", act, ("T", "HK", "D"), layout="rows")
+    view("positions", dtypes.i32, ("T",), alignment=4)
+    if cache:
+        view("slots", dtypes.i64, ("T",), alignment=8)
+    view("rotary", dtypes.f32, ("P", "R"))
+    if c["NORM"]:
+        view("q_weight", act, ("D",))
+        view("k_weight", act, ("D",))
+    rules = _head_rules() + (
+        _rule(lambda d: d["HQ"] > 0 and d["HK"] > 0, "q and k must have heads"),
+        _rule(lambda d: d["R"] % 16 == 0 and 0 < d["R"] <= d["D"],
+              lambda d: f"rotary.shape[1] must be a multiple of 16 up to {d['D']}, got {d['R']}"))
+    if cache:
+        view("k_cache", act, ("PAGES", "HK", "PAGE", "D"), INOUT)
+        view("v_cache", act, ("PAGES", "HK", "PAGE", "D"), INOUT)
+        rules += _cache_rules()
+        stem = "paged_kv_append_norm" if c["NORM"] else "paged_kv_append"
+    else:
+        stem = "qk_norm_rope" if c["NORM"] else "qk_rope"
+    view("q_out", act, ("T", "HQ", "D"), OUT)
+    if not cache:
+        view("k_out", act, ("T", "HK", "D"), OUT)
+    return NativeProgram(interface=PublicInterface(tuple(views), dimension_rules=rules), device=device,
+                         entry_name=f"intent_b200_{stem}_{act.name}", constants=(eps, pairs) if c["NORM"] else (pairs,),
+                         empty=lambda d: d["T"] == 0)
+
+
+_ROTATION_CONSTEXPRS = {"ACT_DTYPE": "bf16", "NORM": True, "EPS": 1e-6, "PAIRS": "halves"}
+qk_norm_rope = KernelDefinition(
+    "qk_norm_rope", dict(_ROTATION_CONSTEXPRS), lambda c, d: _lower_rotation(c, d, cache=False),
+    "no counterpart in the reference (its examples stop at the projections)",
+    "q and k normalised per head (NORM) and rotated by position, f32 arithmetic, one rounding")
+paged_kv_append = KernelDefinition(
+    "paged_kv_append", dict(_ROTATION_CONSTEXPRS), lambda c, d: _lower_rotation(c, d, cache=True),
+    "no counterpart in the reference (its examples stop at the projections)",
+    "as qk_norm_rope, the keys and with them the values stored in a paged cache at slots[t] (-1: not stored)")
+
+
+@cache
+def _paged_workspace_bytes(dim):
+    import ctypes
+
+    from .runtime import native
+
+    query = native.library()["intent_b200_paged_attention_workspace_bytes"]
+    query.restype, query.argtypes = ctypes.c_int64, [ctypes.c_int64]
+    return int(query(dim))
+
+
+def _lower_paged(c, device, *, single):
+    act = _act_dtype(c)
+    scale, window = c["SCALE"], c["WINDOW"]
+    if scale is not None and not 0 < float(scale) < float("inf"):
+        raise CompilationStageError("frontend_kir", "SCALE must be a positive number, or None for 1 / sqrt(D)")
+    if not isinstance(window, int) or not 0 <= window < 1 << 31:
+        raise CompilationStageError("frontend_kir", "WINDOW must be a number of tokens, 0 for all")
+    views = [ViewParameter(0, "q", act, ("B" if single else "T", "HQ", "D"), IN, layout="rows"),
+             ViewParameter(1, "k_cache", act, ("PAGES", "HK", "PAGE", "D"), IN),
+             ViewParameter(2, "v_cache", act, ("PAGES", "HK", "PAGE", "D"), IN),
+             ViewParameter(3, "page_table", dtypes.i32, ("B", "W"), IN, alignment=4)]
+    if not single:
+        views.append(ViewParameter(4, "query_offsets", dtypes.i32, ("B_PLUS_1",), IN, alignment=4))
+    views.append(ViewParameter(len(views), "kv_lengths", dtypes.i32, ("B",), IN, alignment=4))
+    views.append(ViewParameter(len(views), "output", act, ("B" if single else "T", "HQ", "D"), OUT))
+    rules = _head_rules() + _cache_rules() + (
+        _rule(lambda d: d["HK"] > 0 and d["HQ"] > 0 and d["HQ"] % d["HK"] == 0,
+              lambda d: f"{d['HQ']} query heads do not share {d['HK']} key heads evenly"),)
+    if not single:
+        rules += (_rule(lambda d: d["B_PLUS_1"] == d["B"] + 1, "query_offsets must have B + 1 entries"),)
+    stem = "paged_decode_attention" if single else "paged_attention"
+    return NativeProgram(interface=PublicInterface(tuple(views), dimension_rules=rules), device=device,
+                         entry_name=f"intent_b200_{stem}_{act.name}",
+                         constants=(_f32_bits(0 if scale is None else scale, "SCALE"), window),
+                         workspace=lambda d: _paged_workspace_bytes(d["D"]),
+                         empty=lambda d: d["B"] == 0 or (not single and d["T"] == 0),
+                         workspace_status="intent_b200_paged_attention_workspace_status")
+
+
+_PAGED_CONSTEXPRS = {"ACT_DTYPE": "bf16", "SCALE": None, "WINDOW": 0}
+paged_attention = KernelDefinition(
+    "paged_attention", dict(_PAGED_CONSTEXPRS), lambda c, d: _lower_paged(c, d, single=False),
+    "no counterpart in the reference (its examples stop at the projections)",
+    "causal attention of each sequence's new tokens over its pages, any number of them per sequence")
+paged_decode_attention = KernelDefinition(
+    "paged_decode_attention", dict(_PAGED_CONSTEXPRS), lambda c, d: _lower_paged(c, d, single=True),
+    "no counterpart in the reference (its examples stop at the projections)",
+    "attention of one new token per sequence over its pages")
+
+ALL.update({d.name: d for d in (qk_norm_rope, paged_kv_append, paged_attention, paged_decode_attention)})

@@ -60,7 +60,7 @@ _OBSERVABLE = ("intent_b200_weight_only_int4_matmul", "intent_b200_w4a16_gemv", 
                "intent_b200_gemm_i8", "intent_b200_w8a8_gemm", "intent_b200_w4a8_packed_matmul",
                "intent_b200_ragged_grouped_gemm", "intent_b200_routed_expert_projection", "intent_b200_moe_expert_ffn",
                "intent_b200_gemm_f16", "intent_b200_bf16_gemm", "intent_b200_quantized_gemm",
-               "intent_b200_moe_grouped_w4a16")
+               "intent_b200_moe_grouped_w4a16", "intent_b200_qk_", "intent_b200_paged_")
 
 
 class _Launched:
@@ -265,8 +265,9 @@ class NativeProgram:
         if not self._binder_asked:
             self._binder_asked = True
             parameters = self.interface.parameters
-            if all(isinstance(p, ViewParameter) and p.layout == "contiguous" for p in parameters):
-                views = tuple((int(p.access), torch_dtype(p.dtype), len(p.shape), p.alignment) for p in parameters)
+            if all(isinstance(p, ViewParameter) and p.layout in ("contiguous", "rows") for p in parameters):
+                views = tuple((int(p.access), torch_dtype(p.dtype), len(p.shape), p.alignment, int(p.layout == "rows"))
+                              for p in parameters)
                 self.binder = native.binder(self.entry_name, self.device, views, self.constants,
                                             None if self._workspace_spec is None else self._stream_workspaces)
         if self.binder is None or not native.PLAIN.issuperset(map(type, bound.arguments)):

@@ -56,7 +56,7 @@ class ViewParameter:
     shape: tuple            # per axis: int (static extent), str (symbolic dimension) or Derived
     access: ViewKind
     alignment: int = 16     # bytes; entry requirement
-    layout: str = "contiguous"
+    layout: str = "contiguous"      # or "rows": only the last axis contiguous, every row on a 16-byte boundary
 
     @property
     def writable(self) -> bool:
@@ -231,6 +231,12 @@ class PublicInterface:
                         message += "; provide explicit output buffers with the required layout"
                     raise NotImplementedError(message)
                 expected *= extent
+        elif parameter.layout == "rows" and not facts.contiguous and not abstract and all(facts.shape):
+            if facts.shape[-1] != 1 and facts.strides[-1] != 1:
+                raise NotImplementedError(f"{parameter.name}: native entry requires a contiguous last axis")
+            if any(extent != 1 and stride * parameter.dtype.bytes % 16
+                   for extent, stride in zip(facts.shape[:-1], facts.strides[:-1])):
+                raise NotImplementedError(f"{parameter.name}: native entry requires rows on 16-byte boundaries")
         if not abstract and facts.pointer is not None and facts.pointer % parameter.alignment:
             raise ValueError(f"{parameter.name}: native entry requires {parameter.alignment}-byte pointer alignment")
 

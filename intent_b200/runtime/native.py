@@ -129,7 +129,8 @@ def _binder_type():
 
 
 def binder(entry_name: str, device: int, views: tuple, constants: tuple, workspaces: dict | None):
-    """A native caller of one entry: ``views`` are (access, torch dtype, rank, alignment) in declaration order.
+    """A native caller of one entry: ``views`` are (access, torch dtype, rank, alignment, rows of their own) in
+    declaration order.
     None where the entry has no packed form."""
     kind = _binder_type()
     if not kind:
@@ -140,8 +141,8 @@ def binder(entry_name: str, device: int, views: tuple, constants: tuple, workspa
         find.restype, find.argtypes = ctypes.c_void_p, [ctypes.c_char_p, ctypes.c_void_p]
         slots = ctypes.c_int32()
         address = find(entry_name.encode(), ctypes.byref(slots))
-        packed = _PACKED[entry_name] = (address, slots.value) if address and slots.value <= 63 else None
-    if packed is None or len(views) > 16 or any(not 1 <= v[2] <= 3 for v in views):
+        packed = _PACKED[entry_name] = (address, slots.value) if address and slots.value <= 95 else None
+    if packed is None or len(views) > 16 or any(not 1 <= v[2] <= 4 for v in views):
         return None
     if sum(1 + 2 * v[2] for v in views) + len(constants) + (0 if workspaces is None else 2) + 1 != packed[1]:
         return None          # not this entry's parameters
