@@ -566,7 +566,7 @@ INTENT_B200_API int intent_b200_paged_kv_append_norm_bf16(INTENT_B200_VIEW3(q), 
  * of zeros.  Tokens behind kv_length, ahead of the window, in pages that the table does not name or whose number lies
  * outside the cache are not read, whatever the memory there holds.  Rows of q that no sequence has are left alone.
  * scale_bits: the f32 factor of the scores (> 0; 0: 1 / sqrt(D)).  f32 statistics and sums.
- * workspace: at least ..._workspace_bytes(D) bytes, 16-byte aligned, zero-filled once; every launch leaves its counters
+ * workspace: at least ..._workspace_bytes(D, 0) bytes (paged_decode_attention: (D, 1)), 16-byte aligned, zero-filled once; every launch leaves its counters
  * zero again.  Launches that may overlap need separate ones.  Bytes 0..3: INTENT_B200_ERR_TIMEOUT of a bounded wait that
  * gave up (..._workspace_status reads it and clears the workspace).  The same call gives the same bits.
  * ------------------------------------------------------------------------ */
@@ -588,7 +588,7 @@ INTENT_B200_API int intent_b200_paged_decode_attention_bf16(INTENT_B200_VIEW3(q)
                                                         INTENT_B200_VIEW1(kv_lengths), INTENT_B200_VIEW3(out),
                                                         int32_t scale_bits, int32_t window, void* workspace,
                                                         int64_t workspace_bytes, void* stream);
-INTENT_B200_API int64_t intent_b200_paged_attention_workspace_bytes(int64_t dim);
+INTENT_B200_API int64_t intent_b200_paged_attention_workspace_bytes(int64_t dim, int32_t single);
 INTENT_B200_API int intent_b200_paged_attention_workspace_status(void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------

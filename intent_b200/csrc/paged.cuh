@@ -8,7 +8,9 @@
 namespace ib200 {
 
 constexpr int kPagedCtas = 160;            // most CTAs of a launch
-constexpr int64_t kPagedHeader = 4096;     // bytes of the workspace ahead of the parts: status word, one counter per CTA
+constexpr int64_t kPagedHeader = 4096;     // bytes of the workspace ahead of the parts: status word, then per CTA a counter
+constexpr int64_t kPagedJoins = 1024;      // and, from here on, the tile that it leaves to others (16 bytes)
+static_assert(64 + 4 * kPagedCtas <= kPagedJoins && kPagedJoins + 16 * kPagedCtas <= kPagedHeader, "room ahead of the parts");
 
 struct PagedParams {
   const uint16_t* q;                 // [T, HQ, D] at these strides (elements)
@@ -23,7 +25,9 @@ struct PagedParams {
   float scale;                       // of the scores, times log2(e)
   int* status;                       // heads of the workspace
   int* counters;
+  void* joins;
   float* parts;
+  int half_tokens;                   // chunks: tokens of half a tile
 };
 
 #ifdef __CUDACC__
@@ -49,8 +53,15 @@ __device__ __forceinline__ float exp2_fast(float x) {
 
 #endif  // __CUDACC__
 
+// few rows per sequence (paged_rows.cu)
 int64_t paged_rows_workspace_bytes(int64_t dim);
 template <typename T>
 int paged_rows(const PagedParams& p, int64_t dim, const void* k_cache, const void* v_cache, int sms, cudaStream_t stream);
+
+// chunks (paged_chunk.cu)
+int64_t paged_chunk_workspace_bytes(int64_t dim);
+bool paged_chunk_takes(const PagedParams& p);
+template <typename T>
+int paged_chunk(PagedParams p, int64_t dim, const void* k_cache, const void* v_cache, int sms, cudaStream_t stream);
 
 }  // namespace ib200

@@ -47,7 +47,7 @@ int attend(const View3& q, const View4& k_cache, const View4& v_cache, const Vie
     return cuda_status(cudaMemsetAsync(out.p, 0, size_t(tokens * heads * dim) * 2, stream));
   }
   if (!k_cache.p || !v_cache.p || !table.p) return INTENT_B200_ERR_NULL;
-  if (!workspace || workspace_bytes < paged_rows_workspace_bytes(dim)) return INTENT_B200_ERR_WORKSPACE;
+  if (!workspace || workspace_bytes < intent_b200_paged_attention_workspace_bytes(dim, offsets ? 0 : 1)) return INTENT_B200_ERR_WORKSPACE;
   if (!aligned16(workspace)) return INTENT_B200_ERR_LAYOUT;
   const int sms = device_sms();
   if (sms <= 0) return INTENT_B200_ERR_CUDA;
@@ -67,15 +67,18 @@ int attend(const View3& q, const View4& k_cache, const View4& v_cache, const Vie
   p.scale = scale * 1.44269504f;         // log2(e): the exponentials are powers of two
   p.status = static_cast<int*>(workspace);
   p.counters = p.status + 16;
+  p.joins = static_cast<unsigned char*>(workspace) + kPagedJoins;
   p.parts = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + kPagedHeader);
+  if (offsets && paged_chunk_takes(p)) return paged_chunk<T>(p, dim, k_cache.p, v_cache.p, sms, stream);
   return paged_rows<T>(p, dim, k_cache.p, v_cache.p, sms, stream);
 }
 
 }  // namespace
 }  // namespace ib200
 
-extern "C" int64_t intent_b200_paged_attention_workspace_bytes(int64_t dim) {
-  return ib200::paged_rows_workspace_bytes(dim);
+extern "C" int64_t intent_b200_paged_attention_workspace_bytes(int64_t dim, int32_t single) {
+  const int64_t rows = ib200::paged_rows_workspace_bytes(dim), chunk = ib200::paged_chunk_workspace_bytes(dim);
+  return single || rows > chunk ? rows : chunk;
 }
 
 // Reads the status word at the head of a workspace after synchronising `stream`.  A launch that gave up on a bounded wait may

@@ -1,0 +1,849 @@
+// Attention of chunks of new tokens over a paged cache on tcgen05 (paged_attention; the definition is in paged_rows.cu).
+//
+// A tile of queries is 256 rows: new tokens of one sequence with all query heads that share a key head (row = token x group +
+// head), in two halves of 128.  For every step of 128 tokens of the cache and each half
+//   S = Q K^T          tcgen05.mma, both operands from shared memory, 128 x 128 f32 in tensor memory
+//   P = 2^(S - m)      128 threads, one row each: no exchange between threads; P goes back over S as 16-bit values
+//   O += P V           tcgen05.mma, P from tensor memory, V as the cache holds it (N-major)
+// Both halves use the same keys and values, and while one half's threads work out exponentials the tensor core has the other
+// half's two products to do.  A row's running maximum m is only raised when it grows by more than 8 (a factor of 256, which
+// 16-bit weights and f32 sums hold without loss): then O is scaled where it lies.  Every sum uses the m its weights were made
+// with, so that the result does not depend on when that is.
+//
+// The steps of all tiles of all sequences form one line, of which every CTA takes the same number (as in paged_rows.cu); how
+// many steps a tile has follows from its last token's position and its first one's window, and the sums of these over the
+// tiles of a sequence are evaluated in closed form (sum of floor((a j + b) / m)), so a CTA finds its place in a few divisions.
+// Tiles that a CTA boundary cuts leave maximum, sum and unscaled result per part, and join_kernel adds the parts in order.
+//
+// Keys and values come through a ring of TMA boxes of one page's rows each (128B swizzle, one lane per box); boxes of tokens
+// that no query of the tile sees are asked for behind the cache's end, where TMA fills in zeros.
+#include <algorithm>
+#include <type_traits>
+
+#include "common.cuh"
+#include "paged.cuh"
+#include "tma.cuh"
+#include "umma.cuh"
+
+namespace ib200 {
+namespace {
+
+constexpr int HALF_ROWS = 128;             // query rows of half a tile
+constexpr int STEP = 128;                  // tokens of a step
+constexpr int LOAD_WARP = 9, MMA_WARP = 8, THREADS = 12 * 32;   // warps 0..3 and 4..7: a half's rows; 10 and 11 only lend registers
+// Registers of a thread: the launch's, then those of a row's thread (128 scores and more) and of the others.
+constexpr int LAUNCH_REGISTERS = 168, ROW_REGISTERS = 224, OTHER_REGISTERS = 56;
+static_assert(2 * ROW_REGISTERS + OTHER_REGISTERS <= 3 * LAUNCH_REGISTERS, "three warpgroups share the launch's registers");
+constexpr int CUBIC = 3;                   // pairs of eight whose exponentials are made by arithmetic
+constexpr float SLACK = 8.f;               // growth of a row's maximum (log2) that its weights are left to absorb
+
+template <int D>
+struct Room {
+  static constexpr int BOX = STEP * 128;                 // 64 elements of 128 rows
+  static constexpr int OPERAND = BOX * (D / 64);
+  static constexpr int SLOTS = D == 128 ? 5 : 10;
+  static constexpr int BYTES = (2 + SLOTS) * OPERAND;
+  static constexpr int SMEM = 1024 + BYTES + 512;
+};
+
+// ---- the line of steps -----------------------------------------------------------------------------------------------
+struct Sequence {
+  int count, first_row, length, first;     // new tokens, their first row of q, tokens in the cache, position of the first
+  int tiles;                               // of a key head
+};
+
+__device__ __forceinline__ Sequence sequence_of(const PagedParams& p, int b) {
+  Sequence s;
+  const TokenSpan span = span_of(p, b);
+  s.count = span.count;
+  s.first_row = span.begin;
+  s.length = min(max(__ldg(p.lengths + b), 0), p.capacity);
+  s.first = s.length - s.count;
+  s.tiles = (s.count + 2 * p.half_tokens - 1) / (2 * p.half_tokens);
+  return s;
+}
+
+// Steps of tile j: from that of the first token its first query sees to that of its last query's own.  (Of queries ahead of the
+// first token, which see nothing, one step each is walked, all of it hidden.)
+__device__ __forceinline__ int first_step(const PagedParams& p, const Sequence& s, int j) {
+  return p.window > 0 ? max(s.first + 2 * j * p.half_tokens - p.window + 1, 0) / STEP : 0;
+}
+__device__ __forceinline__ int steps_of(const PagedParams& p, const Sequence& s, int j) {
+  const int end = max(s.first, 0) + min(s.count, 2 * (j + 1) * p.half_tokens);
+  return (end + STEP - 1) / STEP - first_step(p, s, j);
+}
+
+// sum of floor((a j + b) / m) over j < n
+__device__ __forceinline__ unsigned long long floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
+  unsigned long long sum = 0;
+  while (true) {
+    if (a >= m) {
+      sum += (unsigned long long)n * (n - 1) / 2 * (a / m);
+      a %= m;
+    }
+    if (b >= m) {
+      sum += (unsigned long long)n * (b / m);
+      b %= m;
+    }
+    const unsigned long long last = (unsigned long long)a * n + b;
+    if (last < m) return sum;
+    n = unsigned(last / m);
+    b = unsigned(last % m);
+    const unsigned t = m;
+    m = a;
+    a = t;
+  }
+}
+
+// Steps of tiles 0 .. j - 1 of a key head.
+__device__ __forceinline__ long long steps_before(const PagedParams& p, const Sequence& s, int j) {
+  const int size = 2 * p.half_tokens, start = max(s.first, 0), full = min(j, s.tiles - 1);
+  if (j <= 0) return 0;
+  unsigned long long sum = full > 0 ? floor_sum(full, STEP, size, unsigned(start) + size + STEP - 1) : 0;
+  if (j == s.tiles) sum += (unsigned(start) + s.count + STEP - 1) / STEP;
+  if (p.window > 0) {
+    const int low = s.first - p.window + 1;              // first token that the first tile's first query sees
+    const int from = low >= 0 ? 0 : (-low + size - 1) / size;
+    if (j > from) sum -= floor_sum(j - from, STEP, size, unsigned(low + from * size));
+  }
+  return (long long)sum;
+}
+
+// Goes through the parts of tiles among the steps [at, end); visit(sequence, head, tile, step, steps, all, at) gets the part's
+// first step in its tile, how many it has and how many the tile has, and returns whether to go on.
+struct Start {
+  int b, head, tile, step;
+};
+template <typename Visit>
+__device__ __forceinline__ void walk(const PagedParams& p, const Start& from, int at, int end, Visit visit) {
+  int b = from.b, head = from.head, tile = from.tile, step = from.step;
+  Sequence s = sequence_of(p, b);
+  while (true) {
+    const int all = steps_of(p, s, tile), steps = min(all - step, end - at);
+    if (!visit(s, b, head, tile, step, steps, all, at)) return;
+    at += steps;
+    if (at >= end) return;
+    step = 0;
+    if (++tile < s.tiles) continue;
+    tile = 0;
+    if (++head < p.k_heads) continue;
+    head = 0;
+    do s = sequence_of(p, ++b);
+    while (s.tiles == 0);
+  }
+}
+
+// What a half of a tile sees
+struct Half {
+  int tokens;              // of it
+  int least, most;         // positions of its first and last
+  __device__ __forceinline__ Half(const PagedParams& p, const Sequence& s, int tile, int half) {
+    const int from = (2 * tile + half) * p.half_tokens;
+    tokens = min(max(s.count - from, 0), p.half_tokens);
+    least = s.first + from;
+    most = least + tokens - 1;
+  }
+  // whether any of its queries sees any token of the step that begins with `token`
+  __device__ __forceinline__ bool sees(const PagedParams& p, int token) const {
+    return tokens > 0 && token <= most && (p.window == 0 || token + STEP > least - p.window + 1);
+  }
+  // whether all of them see all of it
+  __device__ __forceinline__ bool sees_all(const PagedParams& p, int token) const {
+    return token + STEP - 1 <= least && (p.window == 0 || token > most - p.window);
+  }
+};
+
+// ---- tensor memory -----------------------------------------------------------------------------------------------------
+// D[tmem] (+)= A[tmem] * B[smem]
+__device__ __forceinline__ void umma_f16_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, bool accumulate) {
+  const uint32_t acc = accumulate ? 1u : 0u;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t tmem_load_one(uint32_t taddr) {
+  uint32_t v;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(v) : "r"(taddr) : "memory");
+  tmem_load_wait();
+  return v;
+}
+
+__device__ __forceinline__ void tmem_load_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// ---- weights -----------------------------------------------------------------------------------------------------------
+// Two f32 in a 64-bit register, and arithmetic on both at once
+__device__ __forceinline__ uint64_t two(float low, float high) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(low), "f"(high));
+  return d;
+}
+__device__ __forceinline__ void apart(uint64_t v, float& low, float& high) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(low), "=f"(high) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_two(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// the largest of three; NaN if any is
+__device__ __forceinline__ float largest(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^x of both for -125 <= x <= SLACK by arithmetic: x = i + f with i an integer and |f| <= 1/2 (adding 1.5 * 2^23 rounds to it
+// and leaves it in the low bits), 2^f by the cubic whose largest relative error there, 7.5e-5, is least (from a linear programme
+// over 4001 points), and i added to the exponent.  Smaller x count as -125.  The exponential unit gives 16 results a cycle and
+// the tensor core would wait for it: a part of the weights is made this way.
+__device__ __forceinline__ void exp2_by_cubic(uint64_t x, float& low, float& high) {
+  float a, b, ta, tb;
+  apart(x, a, b);
+  x = two(fmaxf(a, -125.f), fmaxf(b, -125.f));
+  const uint64_t t = add_two(x, two(12582912.f, 12582912.f));
+  const uint64_t i = add_two(t, two(-12582912.f, -12582912.f));
+  const uint64_t f = fma_two(i, two(-1.f, -1.f), x);
+  uint64_t y = fma_two(f, two(0.05517167f, 0.05517167f), two(0.24261113f, 0.24261113f));
+  y = fma_two(y, f, two(0.69326097f, 0.69326097f));
+  y = fma_two(y, f, two(0.99992806f, 0.99992806f));
+  apart(t, ta, tb);
+  apart(y, a, b);
+  low = __uint_as_float(__float_as_uint(a) + (__float_as_uint(ta) << 23));
+  high = __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23));
+}
+
+// Weights of 32 scores, rounded, and what they add up to.  CUBIC of eight pairs are made by arithmetic.
+template <typename T, int CUBIC>
+__device__ __forceinline__ void weigh(const uint32_t (&v)[32], uint64_t scale, uint64_t origin, uint64_t (&sum)[2], uint32_t (&w)[16]) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const uint64_t x = fma_two(two(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), scale, origin);
+    float a, b;
+    if ((e & 7) < CUBIC) {
+      exp2_by_cubic(x, a, b);
+    } else {
+      apart(x, a, b);
+      a = exp2_fast(a);
+      b = exp2_fast(b);
+    }
+    sum[e & 1] = add_two(sum[e & 1], two(a, b));
+    w[e] = Elem<T>::pack2(a, b);
+  }
+}
+
+struct JoinEntry {
+  int last_cta;            // of the tile that begins in this CTA and ends in another; -1: there is none
+  int row, head, tokens;   // first row of q, key head, tokens from there on in the sequence
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS, 1)
+paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                   const __grid_constant__ CUtensorMap map_v, const PagedParams p) {
+  using R = Room<D>;
+  constexpr int SLOTS = R::SLOTS, BOXES = D / 64;
+  extern __shared__ unsigned char smem_raw[];
+  programmatic_begin();
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  unsigned char* base_ptr = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t queries = base, ring = base + 2 * R::OPERAND;
+  unsigned char* tail = base_ptr + R::BYTES;
+  const uint32_t q_full = base + R::BYTES, q_empty = q_full + 8, kv_full = q_empty + 8, kv_empty = kv_full + 8 * SLOTS,
+                 s_full = kv_empty + 8 * SLOTS, p_full = s_full + 16, o_full = p_full + 32, vote_full = o_full + 16,
+                 tmem_slot = vote_full + 16;
+  // behind the barriers: tensor memory's address, the start, flags
+  volatile uint32_t* tmem_ptr = reinterpret_cast<volatile uint32_t*>(base_ptr + (tmem_slot - base));
+  int* words = reinterpret_cast<int*>(tail + 16 * SLOTS + 112);
+  long long* warp_sums = reinterpret_cast<long long*>(words);          // [12]
+  Start* start = reinterpret_cast<Start*>(words + 24);
+  volatile int* skip = words + 28;                                     // [2]: this half's step has been added to O by its threads
+  volatile uint32_t* vote = reinterpret_cast<uint32_t*>(words) + 30;   // [2]: step + 1 in which a warp of the half asked for that
+  volatile int* unseen = words + 32;                                   // [8]: per step, boxes of pages outside the cache
+  static_assert(16 * SLOTS + 112 + 40 * 4 <= 512, "room behind the operands");
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < SLOTS; ++i) {
+      mbar_init(kv_full + 8 * i, 1);
+      mbar_init(kv_empty + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(p_full + 16 * i, 4);         // weights of the first 64 tokens, then the others
+      mbar_init(p_full + 16 * i + 8, 4);
+      mbar_init(o_full + 8 * i, 1);
+      mbar_init(vote_full + 8 * i, 4);
+      vote[i] = 0;
+    }
+    fence_mbar_init();
+  }
+  if (warp == MMA_WARP) tmem_alloc(tmem_slot, 512);
+  programmatic_wait();
+
+  // ---- this CTA's part of the line
+  const int per_thread = (p.batch + THREADS - 1) / THREADS, mine = tid * per_thread;
+  long long sum = 0;
+  for (int b = mine; b < min(mine + per_thread, p.batch); ++b) {
+    const Sequence s = sequence_of(p, b);
+    sum += steps_before(p, s, s.tiles) * p.k_heads;
+  }
+  long long before = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const long long v = __shfl_up_sync(0xffffffffu, before, d);
+    if (lane >= d) before += v;
+  }
+  if (lane == 31) warp_sums[warp] = before;
+  __syncthreads();
+  long long line = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += warp_sums[w];
+    line += warp_sums[w];
+  }
+  before -= sum;
+  const bool sensible = line <= 0x3fffffff;                            // (only offsets that make no sense name more)
+  const int total = sensible ? int(line) : 0, share = (total + int(gridDim.x) - 1) / int(gridDim.x);
+  const int cta = blockIdx.x, begin = min(cta * share, total), end = min(begin + share, total);
+  if (begin < end && begin >= before && begin < before + sum) {
+    int b = mine;
+    long long at = before;
+    for (;; ++b) {
+      const Sequence s = sequence_of(p, b);
+      const long long steps = steps_before(p, s, s.tiles) * p.k_heads;
+      if (begin < at + steps) break;
+      at += steps;
+    }
+    start->b = b;
+    start->step = begin - int(at);                                     // in the sequence
+  }
+  __syncthreads();
+  if (begin < end && warp == 0) {
+    const Sequence s = sequence_of(p, start->b);
+    const int per_head = int(steps_before(p, s, s.tiles)), head = start->step / per_head, step = start->step - head * per_head;
+    int low = 0, high = s.tiles;                                       // steps_before(low) <= step < steps_before(high)
+    while (high - low > 1) {
+      const int stride = (high - low + 31) / 32, j = low + lane * stride;
+      const int fitting = __popc(__ballot_sync(0xffffffffu, j < high && steps_before(p, s, j) <= step));
+      low += (fitting - 1) * stride;
+      high = min(low + stride, high);
+    }
+    const int within = step - int(steps_before(p, s, low));
+    __syncwarp();
+    if (lane == 0) {
+      start->head = head;
+      start->tile = low;
+      start->step = within;
+    }
+  }
+  JoinEntry* entry = reinterpret_cast<JoinEntry*>(p.joins) + cta;
+  if (tid == 0) {
+    entry->last_cta = -1;
+    if (!sensible) atomicExch(p.status, INTENT_B200_ERR_SHAPE);
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = *tmem_ptr;
+  const uint32_t tmem_s = tmem, tmem_o = tmem + 2 * STEP;              // of both halves, 128 columns apart
+  bool ok = true;
+
+  if (begin >= end) {
+    // nothing to do
+  } else if (warp >= MMA_WARP) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGISTERS));
+    if (warp == LOAD_WARP) {
+      // ------------------------------ loads ---------------------------------------
+      const int rows = min(1 << p.page_shift, STEP);                     // of a box
+      const int boxes = STEP / rows;                                     // of 64 elements of a step
+      const int cache_rows = (p.pages * p.k_heads) << p.page_shift;
+      uint32_t u = 0, tiles = 0;
+      walk(p, *start, begin, end, [&](const Sequence& s, int b, int head, int tile, int step, int steps, int, int) {
+        ok = mbar_wait_warp(q_empty, (tiles & 1) ^ 1);
+        ++tiles;
+        if (!ok) return false;
+        const Half upper(p, s, tile, 0), lower(p, s, tile, 1);
+        if (lane == 0) {
+          mbar_expect_tx(q_full, uint32_t(p.half_tokens * p.group * 128 * BOXES * (lower.tokens > 0 ? 2 : 1)));
+          for (int half = 0; half < (lower.tokens > 0 ? 2 : 1); ++half)
+            for (int c = 0; c < BOXES; ++c)
+              tma_load_3d(queries + half * R::OPERAND + c * R::BOX, &map_q, 64 * c, head * p.group,
+                          s.first_row + (2 * tile + half) * p.half_tokens, q_full);
+        }
+        // tokens that some query of the tile sees: [low, high)
+        const int high = (lower.tokens > 0 ? lower.most : upper.most) + 1, low = p.window > 0 ? max(upper.least - p.window + 1, 0) : 0;
+        const int first = first_step(p, s, tile) + step;
+        for (int i = 0; i < steps; ++i, ++u) {
+          const int box = lane % boxes, column = lane / boxes, token = (first + i) * STEP + box * rows;
+          const bool wanted = token < high && token + rows > low;
+          int page = -1;
+          if (wanted) page = __ldg(p.page_table + int64_t(b) * p.table_width + (token >> p.page_shift));
+          const bool there = page >= 0 && page < p.pages;
+          const int row = there ? ((page * p.k_heads + head) << p.page_shift) + (token & ((1 << p.page_shift) - 1)) : cache_rows;
+          const uint32_t missing = __ballot_sync(0xffffffffu, wanted && !there && column == 0);
+#pragma unroll
+          for (int operand = 0; operand < 2; ++operand) {
+            const uint32_t slot = (2 * u + operand) % SLOTS, turn = (2 * u + operand) / SLOTS;
+            ok = mbar_wait_warp(kv_empty + 8 * slot, (turn & 1) ^ 1);
+            if (!ok) return false;
+            if (lane == 0) {
+              if (operand == 0) unseen[u & 7] = int(missing);
+              mbar_expect_tx(kv_full + 8 * slot, R::OPERAND);
+            }
+            __syncwarp();
+            if (column < BOXES)
+              tma_load_2d(ring + slot * R::OPERAND + column * R::BOX + box * rows * 128, operand == 0 ? &map_k : &map_v, 64 * column,
+                          row, kv_full + 8 * slot);
+            __syncwarp();
+          }
+        }
+        return true;
+      });
+      if (!ok)   // (nothing may be on its way to a CTA that is gone)
+        for (int i = 0; i < SLOTS; ++i)
+          for (int parity = 0; parity < 2; ++parity) mbar_wait_warp(kv_full + 8 * i, parity, 64);
+    } else if (warp == MMA_WARP) {
+      // ------------------------------ products ------------------------------------
+      constexpr uint32_t FORMAT = std::is_same<T, __half>::value ? 0 : 1;
+      constexpr uint32_t scores = umma_idesc(1, FORMAT, FORMAT, 0, 0, HALF_ROWS, STEP);
+      constexpr uint32_t results = umma_idesc(1, FORMAT, FORMAT, 0, 1, HALF_ROWS, D);
+      const bool issue = elect_one();
+      uint32_t u = 0, tiles = 0, taken[2] = {0, 0};
+      walk(p, *start, begin, end, [&](const Sequence& s, int, int, int tile, int step, int steps, int, int) {
+        ok = mbar_wait_warp(q_full, tiles & 1);
+        ++tiles;
+        if (!ok) return false;
+        const Half half[2] = {Half(p, s, tile, 0), Half(p, s, tile, 1)};
+        const int first = first_step(p, s, tile) + step;
+        bool waiting[2] = {false, false}, begun[2] = {false, false};
+        // adds the values of the step before to a half that has its weights
+        auto add = [&](int h, uint32_t slot) {
+          const uint64_t values = umma_desc_mn_major_sw128(ring + slot * R::OPERAND, R::BOX);
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            ok = ok && mbar_wait_warp(p_full + 16 * h + 8 * part, taken[h] & 1);
+            if (!ok) return;
+            tcgen05_fence_after();
+            const bool skipped = skip[h] != 0;
+            if (issue && !skipped) {
+#pragma unroll
+              for (int k = part * (STEP / 32); k < (part + 1) * (STEP / 32); ++k)   // 16 tokens: 8 columns of P, 16 rows of 128 bytes
+                umma_f16_tmem(tmem_o + h * 128, tmem_s + h * STEP + 8 * k, values + uint64_t(128 * k), results, begun[h] || k != 0);
+            }
+          }
+          ++taken[h];
+          waiting[h] = false;
+          begun[h] = true;
+        };
+        for (int i = 0; i < steps; ++i, ++u) {
+          const uint32_t k_slot = (2 * u) % SLOTS, k_turn = (2 * u) / SLOTS;
+          const uint32_t v_slot = (2 * u + SLOTS - 1) % SLOTS, v_turn = (2 * u + SLOTS - 1) / SLOTS - 1;   // of the step before
+          if (i > 0) ok = ok && mbar_wait_warp(kv_full + 8 * v_slot, v_turn & 1);
+          ok = ok && mbar_wait_warp(kv_full + 8 * k_slot, k_turn & 1);
+          if (!ok) return false;
+          tcgen05_fence_after();
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (waiting[h]) add(h, v_slot);
+            if (!ok) return false;
+            if (!half[h].sees(p, (first + i) * STEP)) continue;
+            if (issue) {
+#pragma unroll
+              for (int k = 0; k < D / 16; ++k) {
+                const uint64_t a = umma_desc_k_major_sw128(queries + h * R::OPERAND + (k / 4) * R::BOX) + uint64_t(2 * (k & 3));
+                const uint64_t b = umma_desc_k_major_sw128(ring + k_slot * R::OPERAND + (k / 4) * R::BOX) + uint64_t(2 * (k & 3));
+                umma_f16(tmem_s + h * STEP, a, b, scores, k != 0);
+              }
+              umma_commit(s_full + 8 * h);
+            }
+            waiting[h] = true;
+          }
+          if (issue) {
+            if (i > 0) umma_commit(kv_empty + 8 * v_slot);
+            umma_commit(kv_empty + 8 * k_slot);
+            if (i == steps - 1) umma_commit(q_empty);
+          }
+          __syncwarp();
+        }
+        const uint32_t v_slot = (2 * u + SLOTS - 1) % SLOTS, v_turn = (2 * u + SLOTS - 1) / SLOTS - 1;
+        ok = mbar_wait_warp(kv_full + 8 * v_slot, v_turn & 1);
+        if (!ok) return false;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (waiting[h]) add(h, v_slot);
+          if (!ok) return false;
+          if (issue && begun[h]) umma_commit(o_full + 8 * h);
+        }
+        if (issue) umma_commit(kv_empty + 8 * v_slot);
+        __syncwarp();
+        return true;
+      });
+    }
+  } else {
+    // ------------------------------ weights and results --------------------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(ROW_REGISTERS));
+    const int h = warp >> 2, quadrant = warp & 3, row = quadrant * 32 + lane;
+    const uint32_t lanes = uint32_t(quadrant * 32) << 16;
+    const uint32_t at_s = tmem_s + h * STEP + lanes, at_o = tmem_o + h * 128 + lanes;
+    const float infinity = __int_as_float(0x7f800000);
+    const int row_token = row / p.group;                               // in the half
+    uint32_t u = 0, seen = 0, done = 0, votes = 0;
+    walk(p, *start, begin, end, [&](const Sequence& s, int, int head, int tile, int step, int steps, int all, int at) {
+      const Half half(p, s, tile, h);
+      const bool real = row_token < half.tokens;
+      const int position = real ? half.least + row_token : -1;
+      const int first = first_step(p, s, tile) + step;
+      const int tile_high = s.first + min(s.count, 2 * (tile + 1) * p.half_tokens);     // tokens of the tile: [low, high)
+      const int tile_low = p.window > 0 ? max(s.first + 2 * tile * p.half_tokens - p.window + 1, 0) : 0;
+      float top = -infinity, weight_sum = 0.f;
+      bool begun = false;
+      for (int i = 0; i < steps; ++i, ++u) {
+        const int token = (first + i) * STEP;
+        if (!half.sees(p, token)) continue;
+        ok = mbar_wait_warp(s_full + 8 * h, seen & 1);
+        ++seen;
+        if (!ok) return false;
+        tcgen05_fence_after();
+        uint32_t v[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_load_32x32(at_s + 32 * c, v[c]);
+        tmem_load_wait();
+        const uint32_t missing = uint32_t(unseen[u & 7]);
+        const bool edge = !half.sees_all(p, token) || missing != 0;
+        if (edge) {
+          const int behind = position - token, ahead = p.window > 0 ? behind - p.window : -1;   // seen: (ahead, behind]
+#pragma unroll
+          for (int e = 0; e < STEP; ++e)
+            if (e > behind || e <= ahead) v[e / 32][e % 32] = 0xff800000u;
+          if (missing) {
+            const int shift = min(p.page_shift, 7);
+#pragma unroll
+            for (int e = 0; e < STEP; e += 16)
+              if (missing >> (e >> shift) & 1)
+#pragma unroll
+                for (int f = e; f < e + 16; ++f) v[f / 32][f % 32] = 0xff800000u;
+          }
+        }
+        float most[4] = {-infinity, -infinity, -infinity, -infinity};
+#pragma unroll
+        for (int e = 0; e < 32; e += 2)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) most[c] = largest(most[c], __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
+        const float now = largest(largest(most[0], most[1], most[2]), most[3], -infinity) * p.scale;
+        const bool raise = !(now <= top + SLACK) || top == -infinity;
+        const float factor = raise ? exp2_fast(top - (now == -infinity ? 0.f : now)) : 1.f;
+        if (raise) top = now;
+        weight_sum *= factor;
+        if (begun && __any_sync(0xffffffffu, raise)) {
+          // (S was asked for behind the product that adds the step before, so O is whole)
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
+            tmem_load_32x16(at_o + 16 * c, o);
+            tmem_load_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+            tmem_store_32x16(at_o + 16 * c, o);
+          }
+        }
+        // (a score of +infinity, as one that is no number, makes the row none)
+        const float origin = top == -infinity ? 0.f : top == infinity ? top - top : -top;
+        const uint64_t scales = two(p.scale, p.scale), origins = two(origin, origin);
+        uint64_t added[2] = {0, 0};
+        uint32_t w[16];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (edge) weigh<T, 0>(v[c], scales, origins, added, w);
+          else weigh<T, CUBIC>(v[c], scales, origins, added, w);
+          tmem_store_32x16(at_s + 16 * c, w);
+          if (c == 1 && !edge) {
+            if (lane == 0 && quadrant == 0) skip[h] = 0;
+            tmem_store_wait();
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full + 16 * h);
+          }
+        }
+        float sums[4];
+        apart(added[0], sums[0], sums[1]);
+        apart(added[1], sums[2], sums[3]);
+        weight_sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        bool by_hand = false;
+        if (edge) {
+          // Values that no query of the tile sees may be anything, and 0 * NaN is NaN: they become zeros.
+          const uint32_t slot = (2 * u + 1) % SLOTS, values = ring + slot * R::OPERAND;
+          ok = mbar_wait_warp(kv_full + 8 * slot, ((2 * u + 1) / SLOTS) & 1);
+          if (!ok) return false;
+          unsigned char* mine_row = base_ptr + (values - base) + row * 128;
+          const bool outside = token + row < tile_low || token + row >= tile_high;
+          if (outside) {
+#pragma unroll
+            for (int c = 0; c < BOXES; ++c)
+#pragma unroll
+              for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(mine_row + c * R::BOX + 16 * j) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async();
+          }
+          // Those that some rows see and others do not have to be finite for the product; where they are not, the rows add
+          // them up themselves, each from what it sees.
+          if (!half.sees_all(p, token)) {
+            constexpr uint32_t EXPONENT = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+            bool found = false;
+            if (!outside) {
+#pragma unroll 1
+              for (int j = 0; j < 8 * BOXES; ++j) {
+                const uint4 x = *reinterpret_cast<const uint4*>(mine_row + (j / 8) * R::BOX + 16 * (j % 8));
+                const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  found |= (y[e] & EXPONENT) == EXPONENT || (y[e] >> 16 & EXPONENT) == EXPONENT;
+              }
+            }
+            if (__any_sync(0xffffffffu, found) && lane == 0) vote[h] = u + 1;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(vote_full + 8 * h);
+            ok = mbar_wait_warp(vote_full + 8 * h, votes & 1);
+            ++votes;
+            if (!ok) return false;
+            by_hand = vote[h] == u + 1;
+          }
+          if (by_hand) {
+            tmem_store_wait();
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tmem_load_32x32(at_o + 32 * c, o);
+              tmem_load_wait();
+              if (!begun)
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = 0;
+#pragma unroll 1
+              for (int k = 0; k < STEP; ++k) {
+                __syncwarp();
+                const uint32_t pair = tmem_load_one(at_s + k / 2);
+                const float w = Elem<T>::to_float(uint16_t(k & 1 ? pair >> 16 : pair));
+                const int t = token + k;
+                if (t > position || (p.window > 0 && t <= position - p.window)) continue;
+                const unsigned char* value = base_ptr + (values - base) + (c / 2) * R::BOX + k * 128;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const uint4 x = *reinterpret_cast<const uint4*>(value + ((((c & 1) * 4 + j) ^ (k & 7)) << 4));
+                  const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    o[8 * j + 2 * e] = __float_as_uint(fmaf(w, Elem<T>::to_float(uint16_t(y[e])), __uint_as_float(o[8 * j + 2 * e])));
+                    o[8 * j + 2 * e + 1] =
+                        __float_as_uint(fmaf(w, Elem<T>::to_float(uint16_t(y[e] >> 16)), __uint_as_float(o[8 * j + 2 * e + 1])));
+                  }
+                }
+              }
+              __syncwarp();
+              tmem_store_32x32(at_o + 32 * c, o);
+            }
+          }
+        }
+        begun = true;
+        if (edge && lane == 0 && quadrant == 0) skip[h] = by_hand;
+        tmem_store_wait();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (edge) mbar_arrive(p_full + 16 * h);
+          mbar_arrive(p_full + 16 * h + 8);
+        }
+      }
+
+      // ---- the part's end
+      const bool whole = steps == all;
+      const int first_cta = (at - step) / share;                       // where the tile begins
+      if (tid == 0 && !whole && cta == first_cta) {
+        entry->row = s.first_row + 2 * tile * p.half_tokens;
+        entry->head = head;
+        entry->tokens = s.count - 2 * tile * p.half_tokens;
+        entry->last_cta = (at - step + all - 1) / share;
+      }
+      if (begun) {
+        ok = mbar_wait_warp(o_full + 8 * h, done & 1);
+        ++done;
+        if (!ok) return false;
+        tcgen05_fence_after();
+      }
+      const float inverse = weight_sum == 0.f ? 0.f : 1.f / weight_sum;
+      float* part = p.parts + size_t(2 * cta + (cta == first_cta)) * (2 * HALF_ROWS * (D + 2));
+      uint16_t* to = p.out + (int64_t(s.first_row + (2 * tile + h) * p.half_tokens + row_token) * p.q_heads + head * p.group +
+                              (row - row_token * p.group)) * D;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        if (begun) {
+          tmem_load_32x32(at_o + 32 * c, o);
+          tmem_load_wait();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0;
+        }
+        if (real && whole) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint32_t x[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              x[j] = Elem<T>::pack2(__uint_as_float(o[e + 2 * j]) * inverse, __uint_as_float(o[e + 2 * j + 1]) * inverse);
+            *reinterpret_cast<uint4*>(to + 32 * c + e) = make_uint4(x[0], x[1], x[2], x[3]);
+          }
+        } else if (real) {
+          // [D / 4][256 rows][4]: neighbouring threads write neighbouring 16 bytes
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<uint4*>(part + ((8 * c + e / 4) * 2 * HALF_ROWS + h * HALF_ROWS + row) * 4) =
+                make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        }
+        __syncwarp();
+      }
+      if (!whole && real) {
+        part[2 * HALF_ROWS * D + h * HALF_ROWS + row] = top;
+        part[2 * HALF_ROWS * (D + 1) + h * HALF_ROWS + row] = weight_sum;
+      }
+      tcgen05_fence_before();
+      __syncwarp();
+      return true;
+    });
+  }
+  if (!ok && lane == 0) atomicExch(p.status, INTENT_B200_ERR_TIMEOUT);
+  __syncwarp();
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
+}
+
+// Parts of the tiles that CTA boundaries cut: block (cta, 32 rows), a thread per row and 16 elements.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
+  programmatic_begin();
+  programmatic_wait();
+  const JoinEntry entry = reinterpret_cast<const JoinEntry*>(p.joins)[blockIdx.x];
+  const int first = blockIdx.x, last = entry.last_cta;
+  const int row = blockIdx.y * 32 + (threadIdx.x & 31), c = threadIdx.x >> 5;
+  const int of_half = row % HALF_ROWS, row_token = of_half / p.group, token = row / HALF_ROWS * p.half_tokens + row_token;
+  if (last < 0 || c >= D / 16 || row_token >= p.half_tokens || token >= entry.tokens) return;
+  constexpr size_t SIZE = size_t(2 * HALF_ROWS) * (D + 2);
+  const float infinity = __int_as_float(0x7f800000);
+  float m = -infinity, l = 0.f, x[16] = {};
+  for (int v = first; v <= last; ++v) m = fmaxf(m, __ldcg(p.parts + (2 * v + (v == first)) * SIZE + 2 * HALF_ROWS * D + row));
+  const float origin = m == -infinity ? 0.f : m;
+#pragma unroll 2
+  for (int v = first; v <= last; ++v) {
+    const float* from = p.parts + (2 * v + (v == first)) * SIZE;
+    const float f = exp2_fast(__ldcg(from + 2 * HALF_ROWS * D + row) - origin);
+    l = fmaf(__ldcg(from + 2 * HALF_ROWS * (D + 1) + row), f, l);
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const float4 y = __ldcg(reinterpret_cast<const float4*>(from) + (4 * c + e / 4) * 2 * HALF_ROWS + row);
+      x[e] = fmaf(y.x, f, x[e]), x[e + 1] = fmaf(y.y, f, x[e + 1]);
+      x[e + 2] = fmaf(y.z, f, x[e + 2]), x[e + 3] = fmaf(y.w, f, x[e + 3]);
+    }
+  }
+  const float inverse = l == 0.f ? 0.f : 1.f / l;
+  uint32_t w[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = Elem<T>::pack2(x[2 * e] * inverse, x[2 * e + 1] * inverse);
+  uint16_t* to = p.out + (int64_t(entry.row + token) * p.q_heads + entry.head * p.group + of_half - row_token * p.group) * D + 16 * c;
+  *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+  *reinterpret_cast<uint4*>(to + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+}
+
+template <typename T, int D>
+int launch(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v, const PagedParams& p, int grid,
+           cudaStream_t stream) {
+  auto kernel = paged_chunk_kernel<T, D>;
+  constexpr int smem = Room<D>::SMEM;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return cuda_status(e);
+  // (the kernel shares the launch's registers out anew, which would wait for ever if there were fewer)
+  static const int registers = [kernel] {
+    cudaFuncAttributes attributes;
+    return cudaFuncGetAttributes(&attributes, kernel) == cudaSuccess ? attributes.numRegs : -1;
+  }();
+  if (registers != LAUNCH_REGISTERS) return INTENT_B200_ERR_UNSUPPORTED;
+  if (LaunchFacts* sink = observe_sink())
+    return record_launch(sink, reinterpret_cast<const void*>(kernel), "paged_chunk_kernel 2 x 128 rows, parts joined", grid,
+                         THREADS, smem, 1);
+  e = launch_programmatic(kernel, dim3(unsigned(grid)), dim3(THREADS), smem, stream, 1, map_q, map_k, map_v, p);
+  if (e != cudaSuccess) return cuda_status(e);
+  note_launch();
+  e = launch_programmatic(paged_join_kernel<T, D>, dim3(unsigned(grid), 2 * HALF_ROWS / 32), dim3(256), 0, stream, 1, p);
+  if (e != cudaSuccess) return cuda_status(e);
+  note_launch();
+  return launch_status();
+}
+
+}  // namespace
+
+int64_t paged_chunk_workspace_bytes(int64_t dim) {
+  return kPagedHeader + int64_t(2) * kPagedCtas * 2 * HALF_ROWS * (dim + 2) * int64_t(sizeof(float));
+}
+
+bool paged_chunk_takes(const PagedParams& p) {
+  return p.group <= HALF_ROWS && (p.tokens == 1 || p.q_token > 0) && (p.q_heads == 1 || p.q_head > 0);
+}
+
+template <typename T>
+int paged_chunk(PagedParams p, int64_t dim, const void* k_cache, const void* v_cache, int sms, cudaStream_t stream) {
+  p.half_tokens = HALF_ROWS / p.group;
+  EncodeTiledFn encode = encode_tiled_fn();
+  if (!encode) return INTENT_B200_ERR_CUDA;
+  CUtensorMap map_q, map_k, map_v;
+  const uint64_t rows = uint64_t(p.pages) * uint64_t(p.k_heads) << p.page_shift;
+  constexpr auto type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const uint32_t box = uint32_t(std::min(1 << p.page_shift, STEP));
+  const cuuint64_t dims[3] = {cuuint64_t(dim), cuuint64_t(p.q_heads), cuuint64_t(p.tokens)};
+  const cuuint64_t strides[2] = {cuuint64_t(p.q_heads > 1 ? p.q_head : dim) * 2,
+                                 cuuint64_t(p.tokens > 1 ? p.q_token : p.q_heads * dim) * 2};
+  const cuuint32_t sizes[3] = {64, cuuint32_t(p.group), cuuint32_t(p.half_tokens)}, ones[3] = {1, 1, 1};
+  if (encode(&map_q, type, 3, const_cast<uint16_t*>(p.q), dims, strides, sizes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS ||
+      !make_tensor_map_2d(&map_k, type, k_cache, rows, uint64_t(dim), uint64_t(dim) * 2, box, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_tensor_map_2d(&map_v, type, v_cache, rows, uint64_t(dim), uint64_t(dim) * 2, box, 64, CU_TENSOR_MAP_SWIZZLE_128B))
+    return INTENT_B200_ERR_CUDA;
+  const int grid = std::min(sms, kPagedCtas);
+  return dim == 128 ? launch<T, 128>(map_q, map_k, map_v, p, grid, stream) : launch<T, 64>(map_q, map_k, map_v, p, grid, stream);
+}
+template int paged_chunk<__half>(PagedParams, int64_t, const void*, const void*, int, cudaStream_t);
+template int paged_chunk<__nv_bfloat16>(PagedParams, int64_t, const void*, const void*, int, cudaStream_t);
+
+}  // namespace ib200

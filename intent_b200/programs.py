@@ -930,14 +930,14 @@ paged_kv_append = KernelDefinition(
 
 
 @cache
-def _paged_workspace_bytes(dim):
+def _paged_workspace_bytes(dim, single):
     import ctypes
 
     from .runtime import native
 
     query = native.library()["intent_b200_paged_attention_workspace_bytes"]
-    query.restype, query.argtypes = ctypes.c_int64, [ctypes.c_int64]
-    return int(query(dim))
+    query.restype, query.argtypes = ctypes.c_int64, [ctypes.c_int64, ctypes.c_int32]
+    return int(query(dim, 1 if single else 0))
 
 
 def _lower_paged(c, device, *, single):
@@ -964,7 +964,7 @@ def _lower_paged(c, device, *, single):
     return NativeProgram(interface=PublicInterface(tuple(views), dimension_rules=rules), device=device,
                          entry_name=f"intent_b200_{stem}_{act.name}",
                          constants=(_f32_bits(0 if scale is None else scale, "SCALE"), window),
-                         workspace=lambda d: _paged_workspace_bytes(d["D"]),
+                         workspace=lambda d: _paged_workspace_bytes(d["D"], single),
                          empty=lambda d: d["B"] == 0 or (not single and d["T"] == 0),
                          workspace_status="intent_b200_paged_attention_workspace_status")
 
