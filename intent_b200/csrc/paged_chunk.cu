@@ -18,6 +18,7 @@
 // Keys and values come through a ring of TMA boxes of one page's rows each (128B swizzle, one lane per box); boxes of tokens
 // that no query of the tile sees are asked for behind the cache's end, where TMA fills in zeros.
 #include <algorithm>
+#include <cstddef>
 #include <type_traits>
 
 #include "common.cuh"
@@ -34,7 +35,7 @@ constexpr int LOAD_WARP = 9, MMA_WARP = 8, THREADS = 12 * 32;   // warps 0..3 an
 // Registers of a thread: the launch's, then those of a row's thread (128 scores and more) and of the others.
 constexpr int LAUNCH_REGISTERS = 168, ROW_REGISTERS = 224, OTHER_REGISTERS = 56;
 static_assert(2 * ROW_REGISTERS + OTHER_REGISTERS <= 3 * LAUNCH_REGISTERS, "three warpgroups share the launch's registers");
-constexpr int CUBIC = 3;                   // pairs of eight whose exponentials are made by arithmetic
+constexpr int EARLY = 96;                  // tokens of a step whose weights the products begin with
 constexpr float SLACK = 8.f;               // growth of a row's maximum (log2) that its weights are left to absorb
 
 template <int D>
@@ -43,7 +44,6 @@ struct Room {
   static constexpr int OPERAND = BOX * (D / 64);
   static constexpr int SLOTS = D == 128 ? 5 : 10;
   static constexpr int BYTES = (2 + SLOTS) * OPERAND;
-  static constexpr int SMEM = 1024 + BYTES + 512;
 };
 
 // ---- the line of steps -----------------------------------------------------------------------------------------------
@@ -73,25 +73,25 @@ __device__ __forceinline__ int steps_of(const PagedParams& p, const Sequence& s,
   return (end + STEP - 1) / STEP - first_step(p, s, j);
 }
 
-// sum of floor((a j + b) / m) over j < n
-__device__ __forceinline__ unsigned long long floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
-  unsigned long long sum = 0;
+// sum of floor((a j + b) / 128) over j < n, for n < 2^24: the whole parts of a / 128 and b / 128, then the same with the
+// remainder of a as the divisor
+__device__ __forceinline__ unsigned long long floor_sum(unsigned n, unsigned a, unsigned b) {
+  static_assert(STEP == 128, "the divisor that it begins with");
+  unsigned long long sum = (unsigned long long)(n * (n - 1ull) / 2) * (a >> 7) + (unsigned long long)n * (b >> 7);
+  a &= 127, b &= 127;
+  unsigned m = 128;
   while (true) {
-    if (a >= m) {
-      sum += (unsigned long long)n * (n - 1) / 2 * (a / m);
-      a %= m;
-    }
-    if (b >= m) {
-      sum += (unsigned long long)n * (b / m);
-      b %= m;
-    }
-    const unsigned long long last = (unsigned long long)a * n + b;
+    const unsigned last = a * n + b;                     // (a < 128)
     if (last < m) return sum;
-    n = unsigned(last / m);
-    b = unsigned(last % m);
+    n = last / m;
+    b = last - n * m;
     const unsigned t = m;
     m = a;
-    a = t;
+    a = t / m;
+    sum += (unsigned long long)n * (n - 1ull) / 2 * a;
+    a = t - a * m;
+    sum += (unsigned long long)n * (b / m);
+    b %= m;
   }
 }
 
@@ -99,12 +99,12 @@ __device__ __forceinline__ unsigned long long floor_sum(unsigned n, unsigned m, 
 __device__ __forceinline__ long long steps_before(const PagedParams& p, const Sequence& s, int j) {
   const int size = 2 * p.half_tokens, start = max(s.first, 0), full = min(j, s.tiles - 1);
   if (j <= 0) return 0;
-  unsigned long long sum = full > 0 ? floor_sum(full, STEP, size, unsigned(start) + size + STEP - 1) : 0;
+  unsigned long long sum = full > 0 ? floor_sum(full, size, unsigned(start) + size + STEP - 1) : 0;
   if (j == s.tiles) sum += (unsigned(start) + s.count + STEP - 1) / STEP;
   if (p.window > 0) {
     const int low = s.first - p.window + 1;              // first token that the first tile's first query sees
     const int from = low >= 0 ? 0 : (-low + size - 1) / size;
-    if (j > from) sum -= floor_sum(j - from, STEP, size, unsigned(low + from * size));
+    if (j > from) sum -= floor_sum(j - from, size, unsigned(low + from * size));
   }
   return (long long)sum;
 }
@@ -133,14 +133,22 @@ __device__ __forceinline__ void walk(const PagedParams& p, const Start& from, in
   }
 }
 
+// A CTA's share of a tile, as the loading warp leaves it to the others
+struct Part {
+  int row, head, tokens;   // first row of q, key head, new tokens from there on in the sequence
+  int position;            // of the first of them
+  int first, steps;        // steps of 128 tokens
+  int step, all, at;       // the first one's number in the tile, the tile's steps, the first one's place on the line
+};
+
 // What a half of a tile sees
 struct Half {
   int tokens;              // of it
   int least, most;         // positions of its first and last
-  __device__ __forceinline__ Half(const PagedParams& p, const Sequence& s, int tile, int half) {
-    const int from = (2 * tile + half) * p.half_tokens;
-    tokens = min(max(s.count - from, 0), p.half_tokens);
-    least = s.first + from;
+  __device__ __forceinline__ Half(const PagedParams& p, int tile_tokens, int position, int half) {
+    const int from = half * p.half_tokens;
+    tokens = min(max(tile_tokens - from, 0), p.half_tokens);
+    least = position + from;
     most = least + tokens - 1;
   }
   // whether any of its queries sees any token of the step that begins with `token`
@@ -162,17 +170,6 @@ __device__ __forceinline__ void umma_f16_tmem(uint32_t tmem_d, uint32_t tmem_a, 
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
       ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(acc)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_store_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -226,44 +223,40 @@ __device__ __forceinline__ float largest(float a, float b, float c) {
   return d;
 }
 
-// 2^x of both for -125 <= x <= SLACK by arithmetic: x = i + f with i an integer and |f| <= 1/2 (adding 1.5 * 2^23 rounds to it
-// and leaves it in the low bits), 2^f by the cubic whose largest relative error there, 7.5e-5, is least (from a linear programme
-// over 4001 points), and i added to the exponent.  Smaller x count as -125.  The exponential unit gives 16 results a cycle and
-// the tensor core would wait for it: a part of the weights is made this way.
-__device__ __forceinline__ void exp2_by_cubic(uint64_t x, float& low, float& high) {
-  float a, b, ta, tb;
-  apart(x, a, b);
-  x = two(fmaxf(a, -125.f), fmaxf(b, -125.f));
-  const uint64_t t = add_two(x, two(12582912.f, 12582912.f));
-  const uint64_t i = add_two(t, two(-12582912.f, -12582912.f));
-  const uint64_t f = fma_two(i, two(-1.f, -1.f), x);
-  uint64_t y = fma_two(f, two(0.05517167f, 0.05517167f), two(0.24261113f, 0.24261113f));
-  y = fma_two(y, f, two(0.69326097f, 0.69326097f));
-  y = fma_two(y, f, two(0.99992806f, 0.99992806f));
-  apart(t, ta, tb);
-  apart(y, a, b);
-  low = __uint_as_float(__float_as_uint(a) + (__float_as_uint(ta) << 23));
-  high = __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23));
-}
-
-// Weights of 32 scores, rounded, and what they add up to.  CUBIC of eight pairs are made by arithmetic.
-template <typename T, int CUBIC>
+// Weights of 32 scores, rounded, and what they add up to.
+template <typename T>
 __device__ __forceinline__ void weigh(const uint32_t (&v)[32], uint64_t scale, uint64_t origin, uint64_t (&sum)[2], uint32_t (&w)[16]) {
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
-    const uint64_t x = fma_two(two(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), scale, origin);
     float a, b;
-    if ((e & 7) < CUBIC) {
-      exp2_by_cubic(x, a, b);
-    } else {
-      apart(x, a, b);
-      a = exp2_fast(a);
-      b = exp2_fast(b);
-    }
+    apart(fma_two(two(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), scale, origin), a, b);
+    a = exp2_fast(a);
+    b = exp2_fast(b);
     sum[e & 1] = add_two(sum[e & 1], two(a, b));
     w[e] = Elem<T>::pack2(a, b);
   }
 }
+
+// x * 0 + sum for a pair of 16-bit numbers: NaN where x is no finite number
+template <typename T>
+__device__ __forceinline__ uint32_t add_no_numbers(uint32_t x, uint32_t sum) {
+  if (std::is_same<T, __half>::value) asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(x), "r"(0u));
+  else asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(x), "r"(0u));
+  return sum;
+}
+
+// What lies behind the operands in shared memory
+template <int SLOTS>
+struct Shared {
+  uint64_t q_full, q_empty, kv_full[SLOTS], kv_empty[SLOTS], s_full[2], p_full[2][2], o_full[2], vote_full[2], part_full[4], part_empty[4];
+  long long warp_sums[THREADS / 32];
+  Part parts[4];
+  Start start;
+  volatile uint32_t tmem;
+  volatile int skip[2];                    // this half's step has been added to O by its threads
+  volatile uint32_t vote[2];               // step + 1 in which a warp of the half asked for that
+  volatile uint32_t missing[8];            // per step, boxes of pages outside the cache
+};
 
 struct JoinEntry {
   int last_cta;            // of the tile that begins in this CTA and ends in another; -1: there is none
@@ -281,22 +274,19 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* base_ptr = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t queries = base, ring = base + 2 * R::OPERAND;
-  unsigned char* tail = base_ptr + R::BYTES;
-  const uint32_t q_full = base + R::BYTES, q_empty = q_full + 8, kv_full = q_empty + 8, kv_empty = kv_full + 8 * SLOTS,
-                 s_full = kv_empty + 8 * SLOTS, p_full = s_full + 16, o_full = p_full + 32, vote_full = o_full + 16,
-                 tmem_slot = vote_full + 16;
-  // behind the barriers: tensor memory's address, the start, flags
-  volatile uint32_t* tmem_ptr = reinterpret_cast<volatile uint32_t*>(base_ptr + (tmem_slot - base));
-  int* words = reinterpret_cast<int*>(tail + 16 * SLOTS + 112);
-  long long* warp_sums = reinterpret_cast<long long*>(words);          // [12]
-  Start* start = reinterpret_cast<Start*>(words + 24);
-  volatile int* skip = words + 28;                                     // [2]: this half's step has been added to O by its threads
-  volatile uint32_t* vote = reinterpret_cast<uint32_t*>(words) + 30;   // [2]: step + 1 in which a warp of the half asked for that
-  volatile int* unseen = words + 32;                                   // [8]: per step, boxes of pages outside the cache
-  static_assert(16 * SLOTS + 112 + 40 * 4 <= 512, "room behind the operands");
+  Shared<SLOTS>& sh = *reinterpret_cast<Shared<SLOTS>*>(base_ptr + R::BYTES);
+  const uint32_t bars = base + R::BYTES;
+  const uint32_t q_full = bars + offsetof(Shared<SLOTS>, q_full), q_empty = bars + offsetof(Shared<SLOTS>, q_empty),
+                 kv_full = bars + offsetof(Shared<SLOTS>, kv_full), kv_empty = bars + offsetof(Shared<SLOTS>, kv_empty),
+                 s_full = bars + offsetof(Shared<SLOTS>, s_full), p_full = bars + offsetof(Shared<SLOTS>, p_full),
+                 o_full = bars + offsetof(Shared<SLOTS>, o_full), vote_full = bars + offsetof(Shared<SLOTS>, vote_full),
+                 part_full = bars + offsetof(Shared<SLOTS>, part_full), part_empty = bars + offsetof(Shared<SLOTS>, part_empty);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
+    prefetch_tensormap(&map_q);
+    prefetch_tensormap(&map_k);
+    prefetch_tensormap(&map_v);
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
     for (int i = 0; i < SLOTS; ++i) {
@@ -305,15 +295,19 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + 8 * i, 1);
-      mbar_init(p_full + 16 * i, 4);         // weights of the first 64 tokens, then the others
+      mbar_init(p_full + 16 * i, 4);         // weights of the first EARLY tokens, then the others
       mbar_init(p_full + 16 * i + 8, 4);
       mbar_init(o_full + 8 * i, 1);
       mbar_init(vote_full + 8 * i, 4);
-      vote[i] = 0;
+      sh.vote[i] = 0;
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(part_full + 8 * i, 1);
+      mbar_init(part_empty + 8 * i, 9);      // the warps of both halves and the products'
     }
     fence_mbar_init();
   }
-  if (warp == MMA_WARP) tmem_alloc(tmem_slot, 512);
+  if (warp == MMA_WARP) tmem_alloc(bars + offsetof(Shared<SLOTS>, tmem), 512);
   programmatic_wait();
 
   // ---- this CTA's part of the line
@@ -329,13 +323,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const long long v = __shfl_up_sync(0xffffffffu, before, d);
     if (lane >= d) before += v;
   }
-  if (lane == 31) warp_sums[warp] = before;
+  if (lane == 31) sh.warp_sums[warp] = before;
   __syncthreads();
   long long line = 0;
-#pragma unroll
+#pragma unroll 1
   for (int w = 0; w < THREADS / 32; ++w) {
-    if (w < warp) before += warp_sums[w];
-    line += warp_sums[w];
+    if (w < warp) before += sh.warp_sums[w];
+    line += sh.warp_sums[w];
   }
   before -= sum;
   const bool sensible = line <= 0x3fffffff;                            // (only offsets that make no sense name more)
@@ -344,33 +338,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   if (begin < end && begin >= before && begin < before + sum) {
     int b = mine;
     long long at = before;
-    for (;; ++b) {
+    for (; per_thread > 1; ++b) {
       const Sequence s = sequence_of(p, b);
       const long long steps = steps_before(p, s, s.tiles) * p.k_heads;
       if (begin < at + steps) break;
       at += steps;
     }
-    start->b = b;
-    start->step = begin - int(at);                                     // in the sequence
-  }
-  __syncthreads();
-  if (begin < end && warp == 0) {
-    const Sequence s = sequence_of(p, start->b);
-    const int per_head = int(steps_before(p, s, s.tiles)), head = start->step / per_head, step = start->step - head * per_head;
-    int low = 0, high = s.tiles;                                       // steps_before(low) <= step < steps_before(high)
-    while (high - low > 1) {
-      const int stride = (high - low + 31) / 32, j = low + lane * stride;
-      const int fitting = __popc(__ballot_sync(0xffffffffu, j < high && steps_before(p, s, j) <= step));
-      low += (fitting - 1) * stride;
-      high = min(low + stride, high);
-    }
-    const int within = step - int(steps_before(p, s, low));
-    __syncwarp();
-    if (lane == 0) {
-      start->head = head;
-      start->tile = low;
-      start->step = within;
-    }
+    sh.start.b = b;
+    sh.start.step = begin - int(at);                                   // in the sequence
   }
   JoinEntry* entry = reinterpret_cast<JoinEntry*>(p.joins) + cta;
   if (tid == 0) {
@@ -380,7 +355,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
-  const uint32_t tmem = *tmem_ptr;
+  const uint32_t tmem = sh.tmem;
   const uint32_t tmem_s = tmem, tmem_o = tmem + 2 * STEP;              // of both halves, 128 columns apart
   bool ok = true;
 
@@ -390,25 +365,46 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGISTERS));
     if (warp == LOAD_WARP) {
       // ------------------------------ loads ---------------------------------------
-      const int rows = min(1 << p.page_shift, STEP);                     // of a box
-      const int boxes = STEP / rows;                                     // of 64 elements of a step
+      Start at_first = sh.start;
+      {
+        const Sequence s = sequence_of(p, at_first.b);
+        const int per_head = int(steps_before(p, s, s.tiles));
+        at_first.head = at_first.step / per_head;
+        const int step = at_first.step - at_first.head * per_head;
+        int low = 0, high = s.tiles;                                   // steps_before(low) <= step < steps_before(high)
+        while (high - low > 1) {
+          const int stride = (high - low + 31) / 32, j = low + lane * stride;
+          const int fitting = __popc(__ballot_sync(0xffffffffu, j < high && steps_before(p, s, j) <= step));
+          low += (fitting - 1) * stride;
+          high = min(low + stride, high);
+        }
+        at_first.tile = low;
+        at_first.step = step - int(steps_before(p, s, low));
+      }
+      const int rows = min(1 << p.page_shift, STEP);                   // of a box
+      const int boxes = STEP / rows;                                   // of 64 elements of a step
       const int cache_rows = (p.pages * p.k_heads) << p.page_shift;
-      uint32_t u = 0, tiles = 0;
-      walk(p, *start, begin, end, [&](const Sequence& s, int b, int head, int tile, int step, int steps, int, int) {
-        ok = mbar_wait_warp(q_empty, (tiles & 1) ^ 1);
-        ++tiles;
+      uint32_t u = 0, parts = 0;
+      walk(p, at_first, begin, end, [&](const Sequence& s, int b, int head, int tile, int step, int steps, int all, int at) {
+        const uint32_t place = parts & 3;
+        ok = mbar_wait_warp(part_empty + 8 * place, (parts / 4 & 1) ^ 1) && mbar_wait_warp(q_empty, (parts & 1) ^ 1);
         if (!ok) return false;
-        const Half upper(p, s, tile, 0), lower(p, s, tile, 1);
+        const int from = 2 * tile * p.half_tokens, position = s.first + from, tokens = min(s.count - from, 2 * p.half_tokens);
+        const int first = first_step(p, s, tile) + step, halves = tokens > p.half_tokens ? 2 : 1;
         if (lane == 0) {
-          mbar_expect_tx(q_full, uint32_t(p.half_tokens * p.group * 128 * BOXES * (lower.tokens > 0 ? 2 : 1)));
-          for (int half = 0; half < (lower.tokens > 0 ? 2 : 1); ++half)
+          Part& part = sh.parts[place];
+          part.row = s.first_row + from, part.head = head, part.tokens = s.count - from, part.position = position;
+          part.first = first, part.steps = steps, part.step = step, part.all = all, part.at = at;
+          mbar_arrive(part_full + 8 * place);
+          mbar_expect_tx(q_full, uint32_t(p.half_tokens * p.group * 128 * BOXES * halves));
+          for (int half = 0; half < halves; ++half)
             for (int c = 0; c < BOXES; ++c)
               tma_load_3d(queries + half * R::OPERAND + c * R::BOX, &map_q, 64 * c, head * p.group,
-                          s.first_row + (2 * tile + half) * p.half_tokens, q_full);
+                          s.first_row + from + half * p.half_tokens, q_full);
         }
+        ++parts;
         // tokens that some query of the tile sees: [low, high)
-        const int high = (lower.tokens > 0 ? lower.most : upper.most) + 1, low = p.window > 0 ? max(upper.least - p.window + 1, 0) : 0;
-        const int first = first_step(p, s, tile) + step;
+        const int high = position + tokens, low = p.window > 0 ? max(position - p.window + 1, 0) : 0;
         for (int i = 0; i < steps; ++i, ++u) {
           const int box = lane % boxes, column = lane / boxes, token = (first + i) * STEP + box * rows;
           const bool wanted = token < high && token + rows > low;
@@ -423,7 +419,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             ok = mbar_wait_warp(kv_empty + 8 * slot, (turn & 1) ^ 1);
             if (!ok) return false;
             if (lane == 0) {
-              if (operand == 0) unseen[u & 7] = int(missing);
+              if (operand == 0) sh.missing[u & 7] = missing;
               mbar_expect_tx(kv_full + 8 * slot, R::OPERAND);
             }
             __syncwarp();
@@ -444,76 +440,97 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       constexpr uint32_t scores = umma_idesc(1, FORMAT, FORMAT, 0, 0, HALF_ROWS, STEP);
       constexpr uint32_t results = umma_idesc(1, FORMAT, FORMAT, 0, 1, HALF_ROWS, D);
       const bool issue = elect_one();
-      uint32_t u = 0, tiles = 0, taken[2] = {0, 0};
-      walk(p, *start, begin, end, [&](const Sequence& s, int, int, int tile, int step, int steps, int, int) {
-        ok = mbar_wait_warp(q_full, tiles & 1);
-        ++tiles;
-        if (!ok) return false;
-        const Half half[2] = {Half(p, s, tile, 0), Half(p, s, tile, 1)};
-        const int first = first_step(p, s, tile) + step;
-        bool waiting[2] = {false, false}, begun[2] = {false, false};
-        // adds the values of the step before to a half that has its weights
-        auto add = [&](int h, uint32_t slot) {
-          const uint64_t values = umma_desc_mn_major_sw128(ring + slot * R::OPERAND, R::BOX);
+      const uint64_t query_desc = umma_desc_k_major_sw128(queries), key_desc = umma_desc_k_major_sw128(ring),
+                     value_desc = umma_desc_mn_major_sw128(ring, R::BOX);
+      constexpr uint64_t UNIT = R::OPERAND / 16, BOX_UNIT = R::BOX / 16;       // in descriptors' 16 bytes
+      uint32_t parts = 0, taken[2] = {0, 0};
+      bool waiting[2] = {false, false}, begun[2] = {false, false}, mixed[2] = {false, false};
+      // Places in the ring: of this step's keys, and of the values of the step before.  What is waited for between the products
+      // of two steps leaves the tensor core idle, so all that can be is waited for ahead of the weights.
+      uint32_t k_slot = 0, k_turn = 0, v_slot = SLOTS - 1, v_turn = 1;
+      bool some = false;                                               // there is a step before
+      // adds the values of the step before to a half that has its weights
+      auto add = [&](int h) {
+        const uint64_t values = value_desc + v_slot * UNIT;
 #pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            ok = ok && mbar_wait_warp(p_full + 16 * h + 8 * part, taken[h] & 1);
-            if (!ok) return;
-            tcgen05_fence_after();
-            const bool skipped = skip[h] != 0;
-            if (issue && !skipped) {
-#pragma unroll
-              for (int k = part * (STEP / 32); k < (part + 1) * (STEP / 32); ++k)   // 16 tokens: 8 columns of P, 16 rows of 128 bytes
-                umma_f16_tmem(tmem_o + h * 128, tmem_s + h * STEP + 8 * k, values + uint64_t(128 * k), results, begun[h] || k != 0);
-            }
-          }
-          ++taken[h];
-          waiting[h] = false;
-          begun[h] = true;
-        };
-        for (int i = 0; i < steps; ++i, ++u) {
-          const uint32_t k_slot = (2 * u) % SLOTS, k_turn = (2 * u) / SLOTS;
-          const uint32_t v_slot = (2 * u + SLOTS - 1) % SLOTS, v_turn = (2 * u + SLOTS - 1) / SLOTS - 1;   // of the step before
-          if (i > 0) ok = ok && mbar_wait_warp(kv_full + 8 * v_slot, v_turn & 1);
-          ok = ok && mbar_wait_warp(kv_full + 8 * k_slot, k_turn & 1);
-          if (!ok) return false;
+        for (int c = 0; c < 2; ++c) {
+          ok = ok && mbar_wait_warp(p_full + 16 * h + 8 * c, taken[h] & 1);
+          if (!ok) return;
           tcgen05_fence_after();
+          if (issue && !(mixed[h] && sh.skip[h])) {
+#pragma unroll
+            for (int k = c * (EARLY / 16); k < (c ? STEP / 16 : EARLY / 16); ++k)   // 16 tokens: 8 columns of P, 16 rows of 128 bytes
+              umma_f16_tmem(tmem_o + h * 128, tmem_s + h * STEP + 8 * k, values + uint64_t(128 * k), results, begun[h] || k != 0);
+          }
+        }
+        ++taken[h];
+        waiting[h] = false;
+        begun[h] = true;
+      };
+      // the same for a part's last step
+      auto finish = [&](int h) {
+        if (waiting[h]) add(h);
+        if (ok && issue && begun[h]) umma_commit(o_full + 8 * h);
+        begun[h] = false;
+      };
+      int at = begin;
+      while (ok && at < end) {
+        const uint32_t place = parts & 3;
+        ok = mbar_wait_warp(part_full + 8 * place, parts / 4 & 1);
+        if (!ok) break;
+        const int steps = sh.parts[place].steps, first = sh.parts[place].first, tokens = sh.parts[place].tokens,
+                  position = sh.parts[place].position;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(part_empty + 8 * place);
+        at += steps;
+        const Half half[2] = {Half(p, tokens, position, 0), Half(p, tokens, position, 1)};
+        for (int i = 0; i < steps; ++i) {
+          const int token = (first + i) * STEP;
+          const bool sees[2] = {half[0].sees(p, token), half[1].sees(p, token)};
+          if (some) ok = mbar_wait_warp(kv_full + 8 * v_slot, v_turn & 1);
+          // (ahead of a new tile's first products a half may still have its last results to add)
+          if (i > 0) ok = ok && mbar_wait_warp(kv_full + 8 * k_slot, k_turn & 1);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            if (waiting[h]) add(h, v_slot);
-            if (!ok) return false;
-            if (!half[h].sees(p, (first + i) * STEP)) continue;
+            if (!ok) break;
+            if (i == 0) {
+              finish(h);
+              if (h == 0 && ok) ok = mbar_wait_warp(q_full, parts & 1) && mbar_wait_warp(kv_full + 8 * k_slot, k_turn & 1);
+              tcgen05_fence_after();
+            } else if (waiting[h]) {
+              add(h);
+            }
+            if (!ok || !sees[h]) continue;
             if (issue) {
 #pragma unroll
-              for (int k = 0; k < D / 16; ++k) {
-                const uint64_t a = umma_desc_k_major_sw128(queries + h * R::OPERAND + (k / 4) * R::BOX) + uint64_t(2 * (k & 3));
-                const uint64_t b = umma_desc_k_major_sw128(ring + k_slot * R::OPERAND + (k / 4) * R::BOX) + uint64_t(2 * (k & 3));
-                umma_f16(tmem_s + h * STEP, a, b, scores, k != 0);
-              }
+              for (int k = 0; k < D / 16; ++k)      // 16 elements: 32 bytes of a row of 128
+                umma_f16(tmem_s + h * STEP, query_desc + (h * UNIT + (k / 4) * BOX_UNIT + 2 * (k & 3)),
+                         key_desc + (k_slot * UNIT + (k / 4) * BOX_UNIT + 2 * (k & 3)), scores, k != 0);
               umma_commit(s_full + 8 * h);
             }
             waiting[h] = true;
+            mixed[h] = !half[h].sees_all(p, token);
           }
+          if (!ok) break;
           if (issue) {
-            if (i > 0) umma_commit(kv_empty + 8 * v_slot);
+            if (some) umma_commit(kv_empty + 8 * v_slot);
             umma_commit(kv_empty + 8 * k_slot);
             if (i == steps - 1) umma_commit(q_empty);
           }
           __syncwarp();
+          some = true;
+          v_slot = k_slot + 1, v_turn = k_turn;
+          if (v_slot == SLOTS) v_slot = 0, ++v_turn;
+          k_slot = v_slot + 1, k_turn = v_turn;
+          if (k_slot == SLOTS) k_slot = 0, ++k_turn;
         }
-        const uint32_t v_slot = (2 * u + SLOTS - 1) % SLOTS, v_turn = (2 * u + SLOTS - 1) / SLOTS - 1;
-        ok = mbar_wait_warp(kv_full + 8 * v_slot, v_turn & 1);
-        if (!ok) return false;
+        ++parts;
+      }
+      // the last step's values: no slot is asked for again, but nothing may be on its way to a CTA that is gone
+      ok = ok && mbar_wait_warp(kv_full + 8 * v_slot, v_turn & 1);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (waiting[h]) add(h, v_slot);
-          if (!ok) return false;
-          if (issue && begun[h]) umma_commit(o_full + 8 * h);
-        }
-        if (issue) umma_commit(kv_empty + 8 * v_slot);
-        __syncwarp();
-        return true;
-      });
+      for (int h = 0; h < 2; ++h)
+        if (ok) finish(h);
     }
   } else {
     // ------------------------------ weights and results --------------------------
@@ -523,14 +540,19 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const uint32_t at_s = tmem_s + h * STEP + lanes, at_o = tmem_o + h * 128 + lanes;
     const float infinity = __int_as_float(0x7f800000);
     const int row_token = row / p.group;                               // in the half
-    uint32_t u = 0, seen = 0, done = 0, votes = 0;
-    walk(p, *start, begin, end, [&](const Sequence& s, int, int head, int tile, int step, int steps, int all, int at) {
-      const Half half(p, s, tile, h);
+    uint32_t u = 0, parts = 0, seen = 0, done = 0, votes = 0;
+    int at = begin;
+    while (at < end) {
+      const uint32_t place = parts & 3;
+      ok = mbar_wait_warp(part_full + 8 * place, parts / 4 & 1);
+      if (!ok) break;
+      const volatile Part& part = sh.parts[place];
+      ++parts;
+      const int steps = part.steps, first = part.first, tokens = part.tokens, tile_position = part.position;
+      at += steps;
+      const Half half(p, tokens, tile_position, h);
       const bool real = row_token < half.tokens;
       const int position = real ? half.least + row_token : -1;
-      const int first = first_step(p, s, tile) + step;
-      const int tile_high = s.first + min(s.count, 2 * (tile + 1) * p.half_tokens);     // tokens of the tile: [low, high)
-      const int tile_low = p.window > 0 ? max(s.first + 2 * tile * p.half_tokens - p.window + 1, 0) : 0;
       float top = -infinity, weight_sum = 0.f;
       bool begun = false;
       for (int i = 0; i < steps; ++i, ++u) {
@@ -538,26 +560,28 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         if (!half.sees(p, token)) continue;
         ok = mbar_wait_warp(s_full + 8 * h, seen & 1);
         ++seen;
-        if (!ok) return false;
+        if (!ok) break;
         tcgen05_fence_after();
         uint32_t v[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_load_32x32(at_s + 32 * c, v[c]);
         tmem_load_wait();
-        const uint32_t missing = uint32_t(unseen[u & 7]);
+        const uint32_t missing = sh.missing[u & 7];
         const bool edge = !half.sees_all(p, token) || missing != 0;
         if (edge) {
           const int behind = position - token, ahead = p.window > 0 ? behind - p.window : -1;   // seen: (ahead, behind]
+          const int shift = min(p.page_shift, 7);
 #pragma unroll
-          for (int e = 0; e < STEP; ++e)
-            if (e > behind || e <= ahead) v[e / 32][e % 32] = 0xff800000u;
-          if (missing) {
-            const int shift = min(p.page_shift, 7);
+          for (int c = 0; c < 4; ++c) {
+            // bit e: token 32 c + e is seen
+            const int last = behind - 32 * c, none = ahead - 32 * c + 1;
+            uint32_t shown = last < 0 ? 0u : last >= 31 ? ~0u : (2u << last) - 1;
+            shown &= none <= 0 ? ~0u : none >= 32 ? 0u : ~0u << none;
+            if (missing >> ((32 * c) >> shift) & 1) shown &= 0xffff0000u;
+            if (missing >> ((32 * c + 16) >> shift) & 1) shown &= 0xffffu;
 #pragma unroll
-            for (int e = 0; e < STEP; e += 16)
-              if (missing >> (e >> shift) & 1)
-#pragma unroll
-                for (int f = e; f < e + 16; ++f) v[f / 32][f % 32] = 0xff800000u;
+            for (int e = 0; e < 32; ++e)
+              if (!(shown >> e & 1)) v[c][e] = 0xff800000u;
           }
         }
         float most[4] = {-infinity, -infinity, -infinity, -infinity};
@@ -589,11 +613,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         uint32_t w[16];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          if (edge) weigh<T, 0>(v[c], scales, origins, added, w);
-          else weigh<T, CUBIC>(v[c], scales, origins, added, w);
+          weigh<T>(v[c], scales, origins, added, w);
           tmem_store_32x16(at_s + 16 * c, w);
-          if (c == 1 && !edge) {
-            if (lane == 0 && quadrant == 0) skip[h] = 0;
+          if (c == EARLY / 32 - 1 && !edge) {
+            if (lane == 0 && quadrant == 0) sh.skip[h] = 0;
             tmem_store_wait();
             tcgen05_fence_before();
             __syncwarp();
@@ -609,76 +632,77 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
           // Values that no query of the tile sees may be anything, and 0 * NaN is NaN: they become zeros.
           const uint32_t slot = (2 * u + 1) % SLOTS, values = ring + slot * R::OPERAND;
           ok = mbar_wait_warp(kv_full + 8 * slot, ((2 * u + 1) / SLOTS) & 1);
-          if (!ok) return false;
+          if (!ok) break;
+          const int tile_high = tile_position + min(tokens, 2 * p.half_tokens);
+          const int tile_low = p.window > 0 ? max(tile_position - p.window + 1, 0) : 0;
           unsigned char* mine_row = base_ptr + (values - base) + row * 128;
           const bool outside = token + row < tile_low || token + row >= tile_high;
           if (outside) {
 #pragma unroll
-            for (int c = 0; c < BOXES; ++c)
-#pragma unroll
-              for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(mine_row + c * R::BOX + 16 * j) = make_uint4(0, 0, 0, 0);
+            for (int j = 0; j < 8 * BOXES; ++j) *reinterpret_cast<uint4*>(mine_row + (j / 8) * R::BOX + 16 * (j % 8)) = make_uint4(0, 0, 0, 0);
             fence_proxy_async();
           }
           // Those that some rows see and others do not have to be finite for the product; where they are not, the rows add
           // them up themselves, each from what it sees.
           if (!half.sees_all(p, token)) {
-            constexpr uint32_t EXPONENT = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-            bool found = false;
+            uint32_t sum[2] = {0, 0};
             if (!outside) {
-#pragma unroll 1
+#pragma unroll
               for (int j = 0; j < 8 * BOXES; ++j) {
                 const uint4 x = *reinterpret_cast<const uint4*>(mine_row + (j / 8) * R::BOX + 16 * (j % 8));
-                const uint32_t y[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  found |= (y[e] & EXPONENT) == EXPONENT || (y[e] >> 16 & EXPONENT) == EXPONENT;
+                sum[0] = add_no_numbers<T>(x.x, sum[0]);
+                sum[1] = add_no_numbers<T>(x.y, sum[1]);
+                sum[0] = add_no_numbers<T>(x.z, sum[0]);
+                sum[1] = add_no_numbers<T>(x.w, sum[1]);
               }
             }
-            if (__any_sync(0xffffffffu, found) && lane == 0) vote[h] = u + 1;
+            const bool found = (sum[0] & 0x7fff7fffu) != 0 || (sum[1] & 0x7fff7fffu) != 0;
+            if (__any_sync(0xffffffffu, found) && lane == 0) sh.vote[h] = u + 1;
+            tmem_store_wait();                                         // (the other threads read these weights)
+            tcgen05_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(vote_full + 8 * h);
             ok = mbar_wait_warp(vote_full + 8 * h, votes & 1);
             ++votes;
-            if (!ok) return false;
-            by_hand = vote[h] == u + 1;
+            if (!ok) break;
+            by_hand = sh.vote[h] == u + 1;
           }
           if (by_hand) {
-            tmem_store_wait();
+            tcgen05_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tmem_load_32x32(at_o + 32 * c, o);
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16];
+              tmem_load_32x16(at_o + 16 * c, o);
               tmem_load_wait();
               if (!begun)
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = 0;
+                for (int e = 0; e < 16; ++e) o[e] = 0;
+              const int element = 16 * c, piece = element % 64 / 8;
 #pragma unroll 1
               for (int k = 0; k < STEP; ++k) {
                 __syncwarp();
                 const uint32_t pair = tmem_load_one(at_s + k / 2);
-                const float w = Elem<T>::to_float(uint16_t(k & 1 ? pair >> 16 : pair));
+                const float weight = Elem<T>::to_float(uint16_t(k & 1 ? pair >> 16 : pair));
                 const int t = token + k;
                 if (t > position || (p.window > 0 && t <= position - p.window)) continue;
-                const unsigned char* value = base_ptr + (values - base) + (c / 2) * R::BOX + k * 128;
+                const unsigned char* value = base_ptr + (values - base) + element / 64 * R::BOX + k * 128;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const uint4 x = *reinterpret_cast<const uint4*>(value + ((((c & 1) * 4 + j) ^ (k & 7)) << 4));
+                for (int j = 0; j < 2; ++j) {
+                  const uint4 x = *reinterpret_cast<const uint4*>(value + (((piece + j) ^ (k & 7)) << 4));
                   const uint32_t y[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                  for (int e = 0; e < 4; ++e) {
-                    o[8 * j + 2 * e] = __float_as_uint(fmaf(w, Elem<T>::to_float(uint16_t(y[e])), __uint_as_float(o[8 * j + 2 * e])));
-                    o[8 * j + 2 * e + 1] =
-                        __float_as_uint(fmaf(w, Elem<T>::to_float(uint16_t(y[e] >> 16)), __uint_as_float(o[8 * j + 2 * e + 1])));
-                  }
+                  for (int e = 0; e < 8; ++e)
+                    o[8 * j + e] = __float_as_uint(fmaf(weight, Elem<T>::to_float(uint16_t(y[e / 2] >> (16 * (e & 1)))),
+                                                        __uint_as_float(o[8 * j + e])));
                 }
               }
               __syncwarp();
-              tmem_store_32x32(at_o + 32 * c, o);
+              tmem_store_32x16(at_o + 16 * c, o);
             }
           }
         }
         begun = true;
-        if (edge && lane == 0 && quadrant == 0) skip[h] = by_hand;
+        if (edge && quadrant == 0 && lane == 0) sh.skip[h] = by_hand;
         tmem_store_wait();
         tcgen05_fence_before();
         __syncwarp();
@@ -687,25 +711,29 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
           mbar_arrive(p_full + 16 * h + 8);
         }
       }
+      if (!ok) break;
 
       // ---- the part's end
-      const bool whole = steps == all;
-      const int first_cta = (at - step) / share;                       // where the tile begins
-      if (tid == 0 && !whole && cta == first_cta) {
-        entry->row = s.first_row + 2 * tile * p.half_tokens;
-        entry->head = head;
-        entry->tokens = s.count - 2 * tile * p.half_tokens;
-        entry->last_cta = (at - step + all - 1) / share;
-      }
       if (begun) {
         ok = mbar_wait_warp(o_full + 8 * h, done & 1);
         ++done;
-        if (!ok) return false;
+        if (!ok) break;
         tcgen05_fence_after();
       }
+      const int all = part.all, tile_at = part.at - part.step, head = part.head, tile_row = part.row;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(part_empty + 8 * place);
+      const bool whole = steps == all;
+      const int first_cta = tile_at / share;                           // where the tile begins
+      if (tid == 0 && !whole && cta == first_cta) {
+        entry->row = tile_row;
+        entry->head = head;
+        entry->tokens = tokens;
+        entry->last_cta = (tile_at + all - 1) / share;
+      }
       const float inverse = weight_sum == 0.f ? 0.f : 1.f / weight_sum;
-      float* part = p.parts + size_t(2 * cta + (cta == first_cta)) * (2 * HALF_ROWS * (D + 2));
-      uint16_t* to = p.out + (int64_t(s.first_row + (2 * tile + h) * p.half_tokens + row_token) * p.q_heads + head * p.group +
+      float* to_part = p.parts + size_t(2 * cta + (cta == first_cta)) * (2 * HALF_ROWS * (D + 2));
+      uint16_t* to = p.out + (int64_t(tile_row + h * p.half_tokens + row_token) * p.q_heads + head * p.group +
                               (row - row_token * p.group)) * D;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
@@ -730,19 +758,18 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
           // [D / 4][256 rows][4]: neighbouring threads write neighbouring 16 bytes
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<uint4*>(part + ((8 * c + e / 4) * 2 * HALF_ROWS + h * HALF_ROWS + row) * 4) =
+            *reinterpret_cast<uint4*>(to_part + ((8 * c + e / 4) * 2 * HALF_ROWS + h * HALF_ROWS + row) * 4) =
                 make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         }
         __syncwarp();
       }
       if (!whole && real) {
-        part[2 * HALF_ROWS * D + h * HALF_ROWS + row] = top;
-        part[2 * HALF_ROWS * (D + 1) + h * HALF_ROWS + row] = weight_sum;
+        to_part[2 * HALF_ROWS * D + h * HALF_ROWS + row] = top;
+        to_part[2 * HALF_ROWS * (D + 1) + h * HALF_ROWS + row] = weight_sum;
       }
       tcgen05_fence_before();
       __syncwarp();
-      return true;
-    });
+    }
   }
   if (!ok && lane == 0) atomicExch(p.status, INTENT_B200_ERR_TIMEOUT);
   __syncwarp();
@@ -764,9 +791,10 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
   constexpr size_t SIZE = size_t(2 * HALF_ROWS) * (D + 2);
   const float infinity = __int_as_float(0x7f800000);
   float m = -infinity, l = 0.f, x[16] = {};
+#pragma unroll 8
   for (int v = first; v <= last; ++v) m = fmaxf(m, __ldcg(p.parts + (2 * v + (v == first)) * SIZE + 2 * HALF_ROWS * D + row));
   const float origin = m == -infinity ? 0.f : m;
-#pragma unroll 2
+#pragma unroll 4
   for (int v = first; v <= last; ++v) {
     const float* from = p.parts + (2 * v + (v == first)) * SIZE;
     const float f = exp2_fast(__ldcg(from + 2 * HALF_ROWS * D + row) - origin);
@@ -791,7 +819,8 @@ template <typename T, int D>
 int launch(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v, const PagedParams& p, int grid,
            cudaStream_t stream) {
   auto kernel = paged_chunk_kernel<T, D>;
-  constexpr int smem = Room<D>::SMEM;
+  constexpr int smem = 1024 + Room<D>::BYTES + int(sizeof(Shared<Room<D>::SLOTS>));
+  static_assert(smem <= 227 * 1024, "shared memory of a CTA");
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return cuda_status(e);
   // (the kernel shares the launch's registers out anew, which would wait for ever if there were fewer)
