@@ -778,39 +778,57 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
 }
 
-// Parts of the tiles that CTA boundaries cut: block (cta, 32 rows), a thread per row and 16 elements.
+// Parts of the tiles that CTA boundaries cut: block (cta, 32 rows), a thread per row and 16 elements.  What it costs is the
+// latency of dependent reads, so the maxima and sums of all parts are read at once, by all warps, and the results four parts at a
+// time (8 tiles of 16 parts: 23 us one after another, see the table of measured cases for now).
 template <typename T, int D>
 __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
+  __shared__ float maxima[kPagedCtas][32], sums[kPagedCtas][32];
   programmatic_begin();
   programmatic_wait();
   const JoinEntry entry = reinterpret_cast<const JoinEntry*>(p.joins)[blockIdx.x];
-  const int first = blockIdx.x, last = entry.last_cta;
-  const int row = blockIdx.y * 32 + (threadIdx.x & 31), c = threadIdx.x >> 5;
+  const int first = blockIdx.x, count = entry.last_cta - first + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = blockIdx.y * 32 + lane;
   const int of_half = row % HALF_ROWS, row_token = of_half / p.group, token = row / HALF_ROWS * p.half_tokens + row_token;
-  if (last < 0 || c >= D / 16 || row_token >= p.half_tokens || token >= entry.tokens) return;
+  const bool real = row_token < p.half_tokens && token < entry.tokens;
+  if (entry.last_cta < 0 || !__any_sync(0xffffffffu, real)) return;    // (all warps have the same rows)
   constexpr size_t SIZE = size_t(2 * HALF_ROWS) * (D + 2);
   const float infinity = __int_as_float(0x7f800000);
-  float m = -infinity, l = 0.f, x[16] = {};
-#pragma unroll 8
-  for (int v = first; v <= last; ++v) m = fmaxf(m, __ldcg(p.parts + (2 * v + (v == first)) * SIZE + 2 * HALF_ROWS * D + row));
-  const float origin = m == -infinity ? 0.f : m;
+  auto part = [&](int v) { return p.parts + (2 * (first + v) + (v == 0)) * SIZE; };
 #pragma unroll 4
-  for (int v = first; v <= last; ++v) {
-    const float* from = p.parts + (2 * v + (v == first)) * SIZE;
-    const float f = exp2_fast(__ldcg(from + 2 * HALF_ROWS * D + row) - origin);
-    l = fmaf(__ldcg(from + 2 * HALF_ROWS * (D + 1) + row), f, l);
+  for (int v = warp; v < count; v += 8) {
+    maxima[v][lane] = real ? __ldcg(part(v) + 2 * HALF_ROWS * D + row) : -infinity;
+    sums[v][lane] = real ? __ldcg(part(v) + 2 * HALF_ROWS * (D + 1) + row) : 0.f;
+  }
+  __syncthreads();
+  if (warp >= D / 16 || !real) return;
+  float m = -infinity, l = 0.f, x[16] = {};
+  for (int v = 0; v < count; ++v) m = fmaxf(m, maxima[v][lane]);
+  const float origin = m == -infinity ? 0.f : m;
+  for (int from = 0; from < count; from += 4) {
+    float4 y[4][4];
 #pragma unroll
-    for (int e = 0; e < 16; e += 4) {
-      const float4 y = __ldcg(reinterpret_cast<const float4*>(from) + (4 * c + e / 4) * 2 * HALF_ROWS + row);
-      x[e] = fmaf(y.x, f, x[e]), x[e + 1] = fmaf(y.y, f, x[e + 1]);
-      x[e + 2] = fmaf(y.z, f, x[e + 2]), x[e + 3] = fmaf(y.w, f, x[e + 3]);
+    for (int v = 0; v < 4; ++v)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (from + v < count) y[v][e] = __ldcg(reinterpret_cast<const float4*>(part(from + v)) + (4 * warp + e) * 2 * HALF_ROWS + row);
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      if (from + v >= count) break;
+      const float f = exp2_fast(maxima[from + v][lane] - origin);
+      l = fmaf(sums[from + v][lane], f, l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[4 * e] = fmaf(y[v][e].x, f, x[4 * e]), x[4 * e + 1] = fmaf(y[v][e].y, f, x[4 * e + 1]);
+        x[4 * e + 2] = fmaf(y[v][e].z, f, x[4 * e + 2]), x[4 * e + 3] = fmaf(y[v][e].w, f, x[4 * e + 3]);
+      }
     }
   }
   const float inverse = l == 0.f ? 0.f : 1.f / l;
   uint32_t w[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) w[e] = Elem<T>::pack2(x[2 * e] * inverse, x[2 * e + 1] * inverse);
-  uint16_t* to = p.out + (int64_t(entry.row + token) * p.q_heads + entry.head * p.group + of_half - row_token * p.group) * D + 16 * c;
+  uint16_t* to = p.out + (int64_t(entry.row + token) * p.q_heads + entry.head * p.group + of_half - row_token * p.group) * D + 16 * warp;
   *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
   *reinterpret_cast<uint4*>(to + 8) = make_uint4(w[4], w[5], w[6], w[7]);
 }

@@ -30,6 +30,7 @@ namespace {
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr int UNIT = 32;                 // tokens of a ring slot
 constexpr int STEP = UNIT * WARPS;       // tokens of a CTA's step
+constexpr float SLACK = 8.f;             // growth of a row's maximum (log2) that its weights are left to absorb
 
 template <int D>
 struct Ring {
@@ -40,10 +41,17 @@ struct Ring {
   static constexpr int BYTES = WARPS * STAGES * SLOT;
 };
 
+// Places for the warps' parts of a tile: two where there is room
+template <int D, int NT>
+constexpr int joins() {
+  return NT == 2 ? 1 : 2;
+}
 template <int D, int NT>
 constexpr int smem_bytes() {
-  return 1024 + Ring<D>::BYTES + WARPS * 8 * NT * (D + 4) * 4 + 2 * WARPS * 8 * NT * 4 + WARPS * Ring<D>::STAGES * 8 + 64;
+  return 1024 + Ring<D>::BYTES + joins<D, NT>() * WARPS * 8 * NT * ((D + 4) * 4 + 8) + WARPS * Ring<D>::STAGES * 8 + 64;
 }
+static_assert(smem_bytes<128, 2>() <= 227 * 1024 && smem_bytes<128, 1>() <= 227 * 1024 && smem_bytes<64, 2>() <= 227 * 1024,
+              "shared memory of a CTA");
 
 // One sequence's share of the line of steps
 struct Sequence {
@@ -54,7 +62,7 @@ struct Sequence {
   int low;         // first token that any of its queries sees
   int begin;       // first step
   int steps;       // of a row tile, one at least: a tile without tokens writes zeros
-  int items;       // row tiles of all key heads
+  int tiles;       // row tiles of a key head
 };
 
 __device__ __forceinline__ Sequence sequence_of(const PagedParams& p, int b, int tile_rows) {
@@ -67,23 +75,25 @@ __device__ __forceinline__ Sequence sequence_of(const PagedParams& p, int b, int
   s.low = p.window > 0 ? min(max(s.first - p.window + 1, 0), s.length) : 0;
   s.begin = s.low / STEP;
   s.steps = max((s.length + STEP - 1) / STEP - s.begin, 1);
-  s.items = (s.rows + tile_rows - 1) / tile_rows * p.k_heads;
+  s.tiles = (s.rows + tile_rows - 1) / tile_rows;
   return s;
 }
 
 // A place on the line of steps
 struct Walk {
   Sequence s;
-  int b, item, step;
+  int b, head, tile, step;
   __device__ __forceinline__ void advance(const PagedParams& p, int tile_rows) {
     if (++step < s.steps) return;
     step = 0;
-    if (++item < s.items) return;
-    item = 0;
+    if (++tile < s.tiles) return;
+    tile = 0;
+    if (++head < p.k_heads) return;
+    head = 0;
     do {
       if (++b >= p.batch) return;
       s = sequence_of(p, b, tile_rows);
-    } while (s.items == 0);
+    } while (s.tiles == 0);
   }
 };
 
@@ -110,10 +120,11 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   programmatic_begin();
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* base_ptr = smem_raw + (base - smem_u32(smem_raw));
-  float* join = reinterpret_cast<float*>(base_ptr + R::BYTES);          // [WARPS][ROWS][PITCH]
-  float* join_max = join + WARPS * ROWS * PITCH;                        // [WARPS][ROWS]
-  float* join_sum = join_max + WARPS * ROWS;
-  int* shared = reinterpret_cast<int*>(join_sum + WARPS * ROWS);        // [4], then the warps' sums in 64 bits
+  constexpr int JOINS = joins<D, NT>();
+  float* join = reinterpret_cast<float*>(base_ptr + R::BYTES);          // [JOINS][WARPS][ROWS][PITCH]
+  float* join_max = join + JOINS * WARPS * ROWS * PITCH;                // [JOINS][WARPS][ROWS]
+  float* join_sum = join_max + JOINS * WARPS * ROWS;
+  int* shared = reinterpret_cast<int*>(join_sum + JOINS * WARPS * ROWS);   // [4], then the warps' sums in 64 bits
   long long* warp_sums = reinterpret_cast<long long*>(shared + 4);
   const uint32_t bars = smem_u32(warp_sums + WARPS);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -129,7 +140,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   long long sum = 0;
   for (int b = mine; b < min(mine + per_thread, p.batch); ++b) {
     const Sequence s = sequence_of(p, b, ROWS);
-    sum += (long long)s.items * s.steps;
+    sum += (long long)s.tiles * p.k_heads * s.steps;
   }
   long long before = sum;
 #pragma unroll
@@ -159,8 +170,9 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     int b = mine, at = int(before);
     for (;; ++b) {
       const Sequence s = sequence_of(p, b, ROWS);
-      if (begin < at + s.items * s.steps) break;
-      at += s.items * s.steps;
+      const int steps = s.tiles * p.k_heads * s.steps;
+      if (begin < at + steps) break;
+      at += steps;
     }
     shared[0] = b;
     shared[1] = at;
@@ -169,8 +181,12 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   Walk load;
   load.b = shared[0];
   load.s = sequence_of(p, load.b, ROWS);
-  load.item = (begin - shared[1]) / load.s.steps;
-  load.step = (begin - shared[1]) - load.item * load.s.steps;
+  {
+    const int item = (begin - shared[1]) / load.s.steps;
+    load.step = (begin - shared[1]) - item * load.s.steps;
+    load.head = item / load.s.tiles;
+    load.tile = item - load.head * load.s.tiles;
+  }
   Walk work = load;
 
   const float infinity = __int_as_float(0x7f800000);
@@ -178,42 +194,49 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   uint32_t parity = 0, present = 0;      // a bit per slot; two bits per unit asked for (its halves), the oldest lowest
   int queued = 0;
   bool ok = true;
-
-  // asks for the unit of this warp at `load`, and goes on
-  auto ask = [&] {
-    const int tiles = (load.s.rows + ROWS - 1) / ROWS;
-    const int head = load.item / tiles, token = (load.s.begin + load.step) * STEP + warp * UNIT;
-    int row[2];
-    bool here[2];
+  const int boxes = p.page_shift >= 5 ? 1 : 2;           // pages that a unit lies in
+  int page[2];                           // of the unit at `load`, asked for one unit ahead; -1: not needed
+  auto look_up = [&] {
+    const int token = (load.s.begin + load.step) * STEP + warp * UNIT;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int t = token + i * (UNIT / 2);
-      here[i] = t < load.s.length && t + UNIT / 2 > load.s.low;
-      int page = -1;
-      if (here[i]) page = __ldg(p.page_table + int64_t(load.b) * p.table_width + (t >> p.page_shift));
-      here[i] = page >= 0 && page < p.pages;
-      row[i] = ((page * p.k_heads + head) << p.page_shift) + (t & ((1 << p.page_shift) - 1));
+      page[i] = -1;
+      if (t < load.s.length && t + UNIT / 2 > load.s.low)
+        page[i] = __ldg(p.page_table + int64_t(load.b) * p.table_width + (t >> p.page_shift));
     }
-    const int halves = int(here[0]) + int(here[1]);
-    if (lane == 0 && halves) {
+  };
+  // asks for the unit of this warp at `load`, and goes on
+  auto ask = [&] {
+    const int token = (load.s.begin + load.step) * STEP + warp * UNIT;
+    const bool here[2] = {page[0] >= 0 && page[0] < p.pages, page[1] >= 0 && page[1] < p.pages};
+    const bool any = here[0] || here[1];
+    if (lane == 0 && any) {
       const uint32_t bar = full + 8 * slot_in, to = ring + slot_in * R::SLOT;
-      mbar_expect_tx(bar, halves * (R::SLOT / 2));
+      mbar_expect_tx(bar, boxes == 1 || (here[0] && here[1]) ? R::SLOT : R::SLOT / 2);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        if (!here[i]) continue;
+        // (a unit in one page is one box, whichever of its halves is needed)
+        if (boxes == 1 ? i == 1 : !here[i]) continue;
+        const int number = boxes == 1 && !here[0] ? page[1] : page[i], t = token + i * (UNIT / 2);
+        const int row = ((number * p.k_heads + load.head) << p.page_shift) + (t & ((1 << p.page_shift) - 1));
 #pragma unroll
         for (int c = 0; c < D / 64; ++c) {
-          tma_load_2d(to + c * R::HALF + i * (R::HALF / 2), &map_k, 64 * c, row[i], bar);
-          tma_load_2d(to + R::OPERAND + c * R::HALF + i * (R::HALF / 2), &map_v, 64 * c, row[i], bar);
+          tma_load_2d(to + c * R::HALF + i * (R::HALF / 2), &map_k, 64 * c, row, bar);
+          tma_load_2d(to + R::OPERAND + c * R::HALF + i * (R::HALF / 2), &map_v, 64 * c, row, bar);
         }
       }
     }
     present |= (uint32_t(here[0]) | (uint32_t(here[1]) << 1)) << (2 * queued);
     ++queued;
-    if (halves) slot_in = slot_in + 1 == R::STAGES ? 0 : slot_in + 1;
+    if (any) slot_in = slot_in + 1 == R::STAGES ? 0 : slot_in + 1;
     ++loading;
-    load.advance(p, ROWS);
+    if (loading < end) {
+      load.advance(p, ROWS);
+      look_up();
+    }
   };
+  look_up();
   for (int i = 0; i < R::STAGES && loading < end; ++i) ask();
 
   uint32_t qf[NT][D / 16][2];            // queries as B fragments: k = elements, n = rows
@@ -221,36 +244,35 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   float top[NT][2], weight_sum[NT][2];
   int position[NT][2];                   // of this thread's rows; -1 where there is none
   int least = 0, most = 0;               // positions of the tile's first and last row
-  bool fresh = true;
-  for (int at = begin; at < end; ++at) {
-    const int tiles = (work.s.rows + ROWS - 1) / ROWS;
-    const int head = work.item / tiles, tile_row = (work.item - head * tiles) * ROWS;
-    if (fresh) {
-      fresh = false;
-      const int rows = min(ROWS, work.s.rows - tile_row);
-      least = work.s.first + tile_row / p.group;
-      most = work.s.first + (tile_row + rows - 1) / p.group;
+  // the queries of the tile at `work`
+  auto begin_tile = [&] {
+    const int tile_row = work.tile * ROWS, rows = min(ROWS, work.s.rows - tile_row);
+    least = work.s.first + tile_row / p.group;
+    most = work.s.first + (tile_row + rows - 1) / p.group;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int r = tile_row + nt * 8 + 2 * (lane & 3) + e;
-          position[nt][e] = r < work.s.rows ? work.s.first + r / p.group : -1;
-          top[nt][e] = -infinity;
-          weight_sum[nt][e] = 0.f;
-        }
-        const int r = min(tile_row + nt * 8 + (lane >> 2), work.s.rows - 1), token = r / p.group;
-        const uint16_t* x = p.q + int64_t(work.s.first_row + token) * p.q_token +
-                            int64_t(head * p.group + r - token * p.group) * p.q_head;
+      for (int e = 0; e < 2; ++e) {
+        const int r = tile_row + nt * 8 + 2 * (lane & 3) + e;
+        position[nt][e] = r < work.s.rows ? work.s.first + r / p.group : -1;
+        top[nt][e] = -infinity;
+        weight_sum[nt][e] = 0.f;
+      }
+      const int r = min(tile_row + nt * 8 + (lane >> 2), work.s.rows - 1), token = r / p.group;
+      const uint16_t* x = p.q + int64_t(work.s.first_row + token) * p.q_token +
+                          int64_t(work.head * p.group + r - token * p.group) * p.q_head;
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          qf[nt][i][0] = __ldg(reinterpret_cast<const uint32_t*>(x + 16 * i + 2 * (lane & 3)));
-          qf[nt][i][1] = __ldg(reinterpret_cast<const uint32_t*>(x + 16 * i + 8 + 2 * (lane & 3)));
+      for (int i = 0; i < D / 16; ++i) {
+        qf[nt][i][0] = __ldg(reinterpret_cast<const uint32_t*>(x + 16 * i + 2 * (lane & 3)));
+        qf[nt][i][1] = __ldg(reinterpret_cast<const uint32_t*>(x + 16 * i + 8 + 2 * (lane & 3)));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
-        }
+        for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
       }
     }
+  };
+  begin_tile();
+  int turn = 0;                          // place of the join that is next
+  for (int at = begin; at < end; ++at) {
     const uint32_t halves = present & 3;
     present >>= 2;
     --queued;
@@ -261,13 +283,13 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       parity ^= 1u << slot_out;
       slot_out = slot_out + 1 == R::STAGES ? 0 : slot_out + 1;
 
-      float s[NT][2][4];                 // S^T: tokens 16 m + lane / 4 (+ 8), rows as in o
+      float s[NT][2][4], s_odd[NT][2][4];  // S^T: tokens 16 m + lane / 4 (+ 8), rows as in o; of even and odd pieces of 16 elements
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[nt][m][e] = 0.f;
+          for (int e = 0; e < 4; ++e) s[nt][m][e] = s_odd[nt][m][e] = 0.f;
 #pragma unroll
       for (int i = 0; i < D / 16; ++i)
 #pragma unroll
@@ -276,8 +298,15 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           uint32_t a[4];
           ldmatrix_x4(a, keys + (i / 4) * R::HALF + r * 128 + ((c ^ (r & 7)) << 4));
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) Elem<T>::mma16816(s[nt][m], a[0], a[1], a[2], a[3], qf[nt][i][0], qf[nt][i][1]);
+          for (int nt = 0; nt < NT; ++nt)
+            Elem<T>::mma16816(i & 1 ? s_odd[nt][m] : s[nt][m], a[0], a[1], a[2], a[3], qf[nt][i][0], qf[nt][i][1]);
         }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt][m][e] += s_odd[nt][m][e];
       const bool all = halves == 3 && token + UNIT - 1 <= least && (p.window == 0 || token > most - p.window);
       uint32_t counted[2][2] = {};       // pairs of tokens 16 m + 2 (lane % 4) (+ 8) that some row of the tile sees
       if (!all) {
@@ -301,19 +330,41 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           }
         }
       }
+      // A row's maximum is raised only when a score exceeds it by more than SLACK: until then no lane has to know the others'.
+      bool raise = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float here = fmaxf(fmaxf(s[nt][0][e], s[nt][0][e + 2]), fmaxf(s[nt][1][e], s[nt][1][e + 2]));
+          raise |= here * p.scale > top[nt][e] + SLACK;                // (from -inf: any)
+        }
+      if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float factor[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float here = fmaxf(fmaxf(s[nt][0][e], s[nt][0][e + 2]), fmaxf(s[nt][1][e], s[nt][1][e + 2]));
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) here = fmaxf(here, __shfl_xor_sync(0xffffffffu, here, d));
+            const float now = fmaxf(top[nt][e], here * p.scale);
+            factor[e] = exp2_fast(top[nt][e] - (now == -infinity ? 0.f : now));
+            top[nt][e] = now;
+            weight_sum[nt][e] *= factor[e];
+          }
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[nt][i][e] *= factor[e & 1];
+        }
+      }
       uint32_t pf[NT][2][2];             // P^T as B fragments
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float factor[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float most_here = fmaxf(fmaxf(s[nt][0][e], s[nt][0][e + 2]), fmaxf(s[nt][1][e], s[nt][1][e + 2]));
-#pragma unroll
-          for (int d = 4; d < 32; d *= 2) most_here = fmaxf(most_here, __shfl_xor_sync(0xffffffffu, most_here, d));
-          const float old = top[nt][e], now = fmaxf(old, most_here * p.scale);
-          top[nt][e] = now;
-          const float origin = now == -infinity ? 0.f : now;
-          factor[e] = exp2_fast(old - origin);
+          const float origin = top[nt][e] == -infinity ? 0.f : top[nt][e];
           float added = 0.f;
 #pragma unroll
           for (int m = 0; m < 2; ++m)
@@ -323,18 +374,12 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
               s[nt][m][e + f] = w;
               added += w;
             }
-          weight_sum[nt][e] = fmaf(weight_sum[nt][e], factor[e], added);
+          weight_sum[nt][e] += added;
         }
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
           pf[nt][m][0] = movmatrix(Elem<T>::pack2(s[nt][m][0], s[nt][m][1]));
           pf[nt][m][1] = movmatrix(Elem<T>::pack2(s[nt][m][2], s[nt][m][3]));
-        }
-        if (__any_sync(0xffffffffu, factor[0] != 1.f || factor[1] != 1.f)) {
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[nt][i][e] *= factor[e & 1];
         }
       }
       auto values_of = [&](auto whole, int m, int i, uint32_t (&a)[4]) {   // elements 16 i of tokens 16 m, as A fragments
@@ -411,8 +456,15 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     if (loading < end) ask();
 
     const bool last_step = work.step + 1 == work.s.steps;
-    if (last_step || at + 1 == end) {
-      // ---- the warps' parts, then the CTAs'
+    if (!last_step && at + 1 < end) {
+      ++work.step;
+    } else {
+      // ---- the warps' parts, then the CTAs'.  There are two places for them in turn: when a warp writes to one of them again,
+      // all have passed the barrier of the tile between.
+      float* join_here = join + turn * (WARPS * ROWS * PITCH);
+      float* max_here = join_max + turn * (WARPS * ROWS);
+      float* sum_here = join_sum + turn * (WARPS * ROWS);
+      turn ^= JOINS - 1;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -422,27 +474,31 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 #pragma unroll
           for (int d = 4; d < 32; d *= 2) sum_all += __shfl_xor_sync(0xffffffffu, sum_all, d);
           if (lane < 4) {
-            join_max[warp * ROWS + r] = top[nt][e];
-            join_sum[warp * ROWS + r] = sum_all;
+            max_here[warp * ROWS + r] = top[nt][e];
+            sum_here[warp * ROWS + r] = sum_all;
           }
 #pragma unroll
           for (int i = 0; i < D / 16; ++i) {
-            float* to = join + (warp * ROWS + r) * PITCH + 16 * i + (lane >> 2);
+            float* to = join_here + (warp * ROWS + r) * PITCH + 16 * i + (lane >> 2);
             to[0] = o[nt][i][e];
             to[8] = o[nt][i][e + 2];
           }
         }
       }
-      __syncthreads();
-      const int rows = min(ROWS, work.s.rows - tile_row);
+      const int tile_row = work.tile * ROWS, rows = min(ROWS, work.s.rows - tile_row), head = work.head, first_row = work.s.first_row;
       const int item_begin = at - work.step, item_end = item_begin + work.s.steps;   // on the line
+      if (at + 1 < end) {
+        work.advance(p, ROWS);
+        begin_tile();                    // (its queries are on their way while this tile is put together)
+      }
+      __syncthreads();
       const int first_cta = item_begin / share, last_cta = (item_end - 1) / share;
       const bool whole = first_cta == last_cta;
       float* part = p.parts + size_t(2 * cta + (cta == first_cta)) * (ROWS * (D + 2));
       auto store = [&](int r, int c, const float (&x)[8], float l) {
         const float inverse = l == 0.f ? 0.f : 1.f / l;
         const int token = (tile_row + r) / p.group, of_group = tile_row + r - token * p.group;
-        uint16_t* to = p.out + (int64_t(work.s.first_row + token) * p.q_heads + head * p.group + of_group) * D + 8 * c;
+        uint16_t* to = p.out + (int64_t(first_row + token) * p.q_heads + head * p.group + of_group) * D + 8 * c;
         *reinterpret_cast<uint4*>(to) =
             make_uint4(Elem<T>::pack2(x[0] * inverse, x[1] * inverse), Elem<T>::pack2(x[2] * inverse, x[3] * inverse),
                        Elem<T>::pack2(x[4] * inverse, x[5] * inverse), Elem<T>::pack2(x[6] * inverse, x[7] * inverse));
@@ -451,13 +507,13 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         const int r = w / (D / 8), c = w - r * (D / 8);
         float m = -infinity, l = 0.f, x[8] = {};
 #pragma unroll
-        for (int v = 0; v < WARPS; ++v) m = fmaxf(m, join_max[v * ROWS + r]);
+        for (int v = 0; v < WARPS; ++v) m = fmaxf(m, max_here[v * ROWS + r]);
         const float origin = m == -infinity ? 0.f : m;
 #pragma unroll
         for (int v = 0; v < WARPS; ++v) {
-          const float f = exp2_fast(join_max[v * ROWS + r] - origin);
-          l = fmaf(join_sum[v * ROWS + r], f, l);
-          const float* from = join + (v * ROWS + r) * PITCH + 8 * c;
+          const float f = exp2_fast(max_here[v * ROWS + r] - origin);
+          l = fmaf(sum_here[v * ROWS + r], f, l);
+          const float* from = join_here + (v * ROWS + r) * PITCH + 8 * c;
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = fmaf(from[e], f, x[e]);
         }
@@ -501,10 +557,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           }
         }
       }
-      __syncthreads();                   // the join's buffer is free again
-      fresh = true;
+      if (JOINS == 1) __syncthreads();
     }
-    if (at + 1 < end) work.advance(p, ROWS);
   }
   if (!ok) {
     // (nothing may be on its way to a CTA that is gone)
@@ -538,10 +592,11 @@ template <typename T>
 int paged_rows(const PagedParams& p, int64_t dim, const void* k_cache, const void* v_cache, int sms, cudaStream_t stream) {
   CUtensorMap map_k, map_v;
   const uint64_t rows = uint64_t(p.pages) * uint64_t(p.k_heads) << p.page_shift;
+  const uint32_t box = p.page_shift >= 5 ? UNIT : UNIT / 2;
   constexpr auto type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  if (!make_tensor_map_2d(&map_k, type, k_cache, rows, uint64_t(dim), uint64_t(dim) * 2, UNIT / 2, 64,
+  if (!make_tensor_map_2d(&map_k, type, k_cache, rows, uint64_t(dim), uint64_t(dim) * 2, box, 64,
                           CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !make_tensor_map_2d(&map_v, type, v_cache, rows, uint64_t(dim), uint64_t(dim) * 2, UNIT / 2, 64,
+      !make_tensor_map_2d(&map_v, type, v_cache, rows, uint64_t(dim), uint64_t(dim) * 2, box, 64,
                           CU_TENSOR_MAP_SWIZZLE_128B))
     return INTENT_B200_ERR_CUDA;
   const int grid = sms < kPagedCtas ? sms : kPagedCtas;
