@@ -11,8 +11,11 @@
 // All sums and products are in f32 and every result is rounded once.  A token whose slot is outside the cache (-1: padding)
 // is not stored; one whose position is outside the table gets NaN, as there is no angle for it.
 //
-// A row is held by D / 8 lanes, 16 bytes each: the norm is one sum over them, and the partner of a pair (i, i + R/2) lies
-// R / 16 lanes away in the same group, so a row is read once, and all that leaves the registers is the result.
+// Bound by instructions before it is bound by HBM, so a row costs few of them.  It is held by D / (2 PIECE) lanes in two pieces;
+// with pairs (i, i + R/2) the pieces of a rotated lane lie R/2 apart, so that both elements of a pair and their angle are in one
+// lane and nothing but the norm's sum is exchanged.  Several rows of one kind (queries, keys, values) of one token share what does
+// not depend on the row: weight times cosine and weight times sine, worked out once, turn a row into two packed operations per
+// two elements, one more scales it by the norm.  Calls of few rows take one row per group of lanes, as there the latency counts.
 #include <cstring>
 
 #include "common.cuh"
@@ -21,6 +24,9 @@ namespace ib200 {
 namespace {
 
 constexpr int THREADS = 256;
+constexpr int PIECE_OF = 4;             // elements of a lane's piece of a row, of which it has two
+constexpr int SHARED_ROWS = 4;          // rows of a group in calls of many rows
+constexpr uint32_t MANY = 20000;        // rows from which on a call has many
 
 struct RotateParams {
   const uint16_t *q, *k, *v;
@@ -32,125 +38,225 @@ struct RotateParams {
   uint16_t* v_out;
   int64_t q_token, q_head, k_token, k_head, v_token, v_head;   // strides in elements
   int64_t table_rows, slot_count;
-  uint32_t rows;                       // T * heads of a token
-  uint32_t heads, q_heads, k_heads;    // of a token: queries, keys (and values)
+  uint32_t tokens, q_heads, k_heads;                           // k_heads: keys' and values'
   int rotary_dim, page_shift;
   float eps;
 };
 
-// Eight 16-bit elements as floats and back
-template <typename T>
-__device__ __forceinline__ void widen(const uint4& v, float (&x)[8]) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = Elem<T>::to_float(uint16_t(w[i]));
-    x[2 * i + 1] = Elem<T>::to_float(uint16_t(w[i] >> 16));
-  }
+// Two f32 in a 64-bit register, and arithmetic on both at once
+__device__ __forceinline__ uint64_t two(float low, float high) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(low), "f"(high));
+  return d;
 }
-template <typename T>
-__device__ __forceinline__ uint4 narrow(const float (&x)[8]) {
-  return make_uint4(Elem<T>::pack2(x[0], x[1]), Elem<T>::pack2(x[2], x[3]), Elem<T>::pack2(x[4], x[5]),
-                    Elem<T>::pack2(x[6], x[7]));
+__device__ __forceinline__ float2 apart(uint64_t v) {
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(v));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul_two(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 
-template <typename T, int D, bool NORM, bool NEIGHBOURS, bool CACHE>
+// A piece of a row: PIECE 16-bit elements
+template <int PIECE>
+struct Piece {
+  uint32_t w[PIECE / 2];
+};
+template <int PIECE, bool STREAM>
+__device__ __forceinline__ Piece<PIECE> load_piece(const uint16_t* from) {
+  Piece<PIECE> d;
+  if constexpr (PIECE == 8) {
+    const uint4 v = STREAM ? ldg_stream_v4(from) : __ldg(reinterpret_cast<const uint4*>(from));
+    d.w[0] = v.x, d.w[1] = v.y, d.w[2] = v.z, d.w[3] = v.w;
+  } else {
+    const uint2 v = STREAM ? ldg_stream_v2(from) : __ldg(reinterpret_cast<const uint2*>(from));
+    d.w[0] = v.x, d.w[1] = v.y;
+  }
+  return d;
+}
+template <int PIECE>
+__device__ __forceinline__ void store_piece(uint16_t* to, const Piece<PIECE>& v) {
+  if constexpr (PIECE == 8) *reinterpret_cast<uint4*>(to) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+  else *reinterpret_cast<uint2*>(to) = make_uint2(v.w[0], v.w[1]);
+}
+
+template <typename T, int D, bool NORM, bool NEIGHBOURS, bool CACHE, int ROWS>
 __global__ void __launch_bounds__(THREADS) rotate_kernel(const RotateParams p) {
-  constexpr int LANES = D / 8;                       // of a row
+  constexpr int PIECE = PIECE_OF, PAIRS = PIECE / 2, LANES = D / (2 * PIECE);   // lanes of a row
   programmatic_begin();
-  const int lane = threadIdx.x & 31, chunk = lane % LANES;
+  const int lane = threadIdx.x & 31, j = lane % LANES;
+  // groups of a token: of its queries, its keys, its values
+  const uint32_t q_groups = (p.q_heads + ROWS - 1) / ROWS, k_groups = (p.k_heads + ROWS - 1) / ROWS;
+  const uint32_t groups = q_groups + (CACHE ? 2 : 1) * k_groups;
   const uint32_t at = blockIdx.x * uint32_t(THREADS / LANES) + threadIdx.x / LANES;
-  const bool live = at < p.rows;                     // (all lanes stay for the exchanges)
-  const uint32_t token = live ? at / p.heads : 0, head = live ? at - token * p.heads : 0;
-  const bool is_q = head < p.q_heads, is_v = CACHE && head >= p.q_heads + p.k_heads;
-  const uint32_t h = is_q ? head : head - p.q_heads - (is_v ? p.k_heads : 0);
-  const uint16_t* row = is_q   ? p.q + token * p.q_token + h * p.q_head
-                        : is_v ? p.v + token * p.v_token + h * p.v_head
-                               : p.k + token * p.k_token + h * p.k_head;
+  const bool live = at < p.tokens * groups;          // (all lanes stay for the norms' sums)
+  const uint32_t token = live ? at / groups : 0, group = at - token * groups;
+  const bool is_q = group < q_groups, is_v = CACHE && group >= q_groups + k_groups;
+  const uint32_t first = (is_q ? group : group - q_groups - (is_v ? k_groups : 0)) * ROWS;
+  const uint32_t rows = live ? min((is_q ? p.q_heads : p.k_heads) - first, uint32_t(ROWS)) : 0;
+  const int half = p.rotary_dim / 2;
+  const bool turned = 2 * PIECE * j < p.rotary_dim;
+  // this lane's two pieces of a row
+  const int low = (NEIGHBOURS || !turned ? 2 : 1) * PIECE * j, high = NEIGHBOURS || !turned ? low + PIECE : half + low;
+  const int64_t step = is_q ? p.q_head : is_v ? p.v_head : p.k_head;
+  const uint16_t* from = (is_q ? p.q + token * p.q_token : is_v ? p.v + token * p.v_token : p.k + token * p.k_token) + first * step;
   programmatic_wait();
-  const uint4 raw = live ? ldg_stream_v4(row + 8 * chunk) : make_uint4(0, 0, 0, 0);
+
+  Piece<PIECE> raw[ROWS][2];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    raw[i][0] = raw[i][1] = Piece<PIECE>{};
+    if (i < rows) {
+      raw[i][0] = load_piece<PIECE, true>(from + i * step + low);
+      raw[i][1] = load_piece<PIECE, true>(from + i * step + high);
+    }
+  }
   const int64_t position = __ldg(p.positions + token);
   const bool known = position >= 0 && position < p.table_rows;
-  const float* angles = p.rotary + (known ? position : 0) * p.rotary_dim;
-  const int half = p.rotary_dim / 2, first = 8 * chunk;
-  const bool turned = known && !is_v && first < p.rotary_dim;
-  float c[8], s[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) c[i] = 1.f, s[i] = 0.f;
-  if (turned) {
-    // angles of this lane's pairs: eight from its place in its half on, or those of four neighbours
-    const int from = NEIGHBOURS ? first / 2 : first < half ? first : first - half;
-#pragma unroll
-    for (int i = 0; i < (NEIGHBOURS ? 4 : 8); i += 4) {
-      const float4 cc = __ldg(reinterpret_cast<const float4*>(angles + from + i));
-      const float4 ss = __ldg(reinterpret_cast<const float4*>(angles + half + from + i));
-      c[i] = cc.x, c[i + 1] = cc.y, c[i + 2] = cc.z, c[i + 3] = cc.w;
-      s[i] = ss.x, s[i + 1] = ss.y, s[i + 2] = ss.z, s[i + 3] = ss.w;
-    }
-  }
-  float x[8];
-  widen<T>(raw, x);
-  if (NORM) {
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
-#pragma unroll
-    for (int d = LANES / 2; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (!is_v) {
-      const float scale = rsqrtf(sum * (1.f / D) + p.eps);
-      float w[8];
-      widen<T>(__ldg(reinterpret_cast<const uint4*>((is_q ? p.q_weight : p.k_weight) + first)), w);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = x[i] * scale * w[i];
-    }
-  }
-  float y[8];
-  if (NEIGHBOURS) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      y[2 * i] = x[2 * i] * c[i] - x[2 * i + 1] * s[i];
-      y[2 * i + 1] = x[2 * i + 1] * c[i] + x[2 * i] * s[i];
-    }
+  uint16_t* to;                                      // the group's first row
+  int64_t next = D;                                  // elements from one row to the next
+  bool kept = true;
+  if (CACHE && !is_q) {
+    const int64_t slot = __ldg(p.slots + token);
+    kept = slot >= 0 && slot < p.slot_count;
+    const int64_t row = (((slot >> p.page_shift) * p.k_heads + first) << p.page_shift) + (slot & ((int64_t(1) << p.page_shift) - 1));
+    to = (is_v ? p.v_out : p.k_out) + (kept ? row * D : 0);
+    next = int64_t(D) << p.page_shift;
   } else {
-    const int step = half / 8;                       // lanes between the halves of a pair
-    const int partner = first < half ? lane + step : lane - step;
-    const float sign = first < half ? -1.f : 1.f;
+    to = (is_q ? p.q_out + size_t(token) * p.q_heads * D : p.k_out + size_t(token) * p.k_heads * D) + size_t(first) * D;
+  }
+  if (is_v) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float other = __shfl_sync(0xffffffffu, x[i], turned ? partner : lane);
-      y[i] = turned ? x[i] * c[i] + sign * (other * s[i]) : x[i];
+    for (int i = 0; i < ROWS; ++i)
+      if (i < rows && kept) {
+        store_piece(to + i * next + low, raw[i][0]);
+        store_piece(to + i * next + high, raw[i][1]);
+      }
+  }
+
+  // What an element is multiplied with, and what its partner is for it: weight times cosine, weight times (minus) sine.
+  uint64_t own[2][PAIRS], cross[2][PAIRS];
+  {
+    float c[PIECE], s[PIECE];                        // of this lane's PIECE pairs
+#pragma unroll
+    for (int e = 0; e < PIECE; ++e) c[e] = known ? 1.f : __int_as_float(0x7fc00000), s[e] = 0.f;
+    if (known && turned && !is_v) {
+      const float* angles = p.rotary + position * p.rotary_dim + PIECE * j;
+#pragma unroll
+      for (int e = 0; e < PIECE; e += 4) {
+        const float4 cosine = __ldg(reinterpret_cast<const float4*>(angles + e));
+        const float4 sine = __ldg(reinterpret_cast<const float4*>(angles + half + e));
+        c[e] = cosine.x, c[e + 1] = cosine.y, c[e + 2] = cosine.z, c[e + 3] = cosine.w;
+        s[e] = sine.x, s[e + 1] = sine.y, s[e + 2] = sine.z, s[e + 3] = sine.w;
+      }
     }
-  }
-  if (!known && !is_v) {
+    float w[2][PIECE];
+    if (NORM) {
+      const uint16_t* weight = is_q ? p.q_weight : p.k_weight;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = __int_as_float(0x7fc00000);
+      for (int side = 0; side < 2; ++side) {
+        const Piece<PIECE> v = load_piece<PIECE, false>(weight + (side ? high : low));
+#pragma unroll
+        for (int e = 0; e < PIECE; ++e) w[side][e] = Elem<T>::to_float(uint16_t(v.w[e / 2] >> (16 * (e & 1))));
+      }
+    }
+#pragma unroll
+    for (int side = 0; side < 2; ++side)
+#pragma unroll
+      for (int e = 0; e < PAIRS; ++e) {
+        float a[2], b[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          // element 2 e + i of the piece: its pair among the lane's, its partner
+          const int pair = NEIGHBOURS ? side * PAIRS + e : 2 * e + i;
+          const float sign = (NEIGHBOURS ? i : side) ? 1.f : -1.f;
+          const float mine = NORM ? w[side][2 * e + i] : 1.f;
+          const float partner = NORM ? (NEIGHBOURS ? w[side][2 * e + 1 - i] : w[1 - side][2 * e + i]) : 1.f;
+          a[i] = mine * c[pair];
+          b[i] = sign * (partner * s[pair]);
+        }
+        own[side][e] = two(a[0], a[1]);
+        cross[side][e] = two(b[0], b[1]);
+      }
   }
-  if (!live) return;
-  const uint4 out = is_v ? raw : narrow<T>(y);
-  if (is_q || !CACHE) {
-    uint16_t* to = is_q ? p.q_out + (size_t(token) * p.q_heads + h) * D : p.k_out + (size_t(token) * p.k_heads + h) * D;
-    *reinterpret_cast<uint4*>(to + first) = out;
-    return;
+  const bool partly = p.rotary_dim < D;
+
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    uint64_t x[2][PAIRS];
+#pragma unroll
+    for (int side = 0; side < 2; ++side)
+#pragma unroll
+      for (int e = 0; e < PAIRS; ++e)
+        x[side][e] = two(Elem<T>::to_float(uint16_t(raw[i][side].w[e])), Elem<T>::to_float(uint16_t(raw[i][side].w[e] >> 16)));
+    uint64_t scale = 0;
+    if (NORM) {
+      uint64_t squares = mul_two(x[0][0], x[0][0]);
+#pragma unroll
+      for (int e = 1; e < 2 * PAIRS; ++e) squares = fma_two(x[e / PAIRS][e % PAIRS], x[e / PAIRS][e % PAIRS], squares);
+      const float2 both = apart(squares);
+      float sum = both.x + both.y;
+#pragma unroll
+      for (int d = LANES / 2; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      const float r = rsqrtf(sum * (1.f / D) + p.eps);
+      scale = two(r, r);
+    }
+    if (i >= rows || !kept || is_v) continue;
+    Piece<PIECE> out[2];
+#pragma unroll
+    for (int side = 0; side < 2; ++side)
+#pragma unroll
+      for (int e = 0; e < PAIRS; ++e) {
+        uint64_t partner;
+        if (NEIGHBOURS) {
+          const float2 v = apart(x[side][e]);
+          partner = two(v.y, v.x);
+        } else {
+          partner = x[1 - side][e];
+        }
+        if (partly && !turned) partner = 0;          // (what is not rotated has none, and may be infinite)
+        uint64_t y = fma_two(x[side][e], own[side][e], mul_two(partner, cross[side][e]));
+        if (NORM) y = mul_two(y, scale);
+        const float2 v = apart(y);
+        out[side].w[e] = Elem<T>::pack2(v.x, v.y);
+      }
+    store_piece(to + i * next + low, out[0]);
+    store_piece(to + i * next + high, out[1]);
   }
-  const int64_t slot = __ldg(p.slots + token);
-  if (slot < 0 || slot >= p.slot_count) return;
-  const int64_t page = slot >> p.page_shift, inside = slot & ((int64_t(1) << p.page_shift) - 1);
-  uint16_t* to = (is_v ? p.v_out : p.k_out) + (((page * p.k_heads + h) << p.page_shift) + inside) * D;
-  *reinterpret_cast<uint4*>(to + first) = out;
 }
 
-template <typename T, int D, bool NORM, bool CACHE>
+template <typename T, int D, bool NORM, bool CACHE, int ROWS>
 int launch(const RotateParams& p, bool neighbours, cudaStream_t stream) {
-  constexpr uint32_t PER_CTA = THREADS / (D / 8);
-  auto kernel = neighbours ? rotate_kernel<T, D, NORM, true, CACHE> : rotate_kernel<T, D, NORM, false, CACHE>;
-  const uint32_t grid = (p.rows + PER_CTA - 1) / PER_CTA;
+  constexpr uint32_t PER_CTA = THREADS / (D / (2 * PIECE_OF));
+  auto kernel = neighbours ? rotate_kernel<T, D, NORM, true, CACHE, ROWS> : rotate_kernel<T, D, NORM, false, CACHE, ROWS>;
+  const uint32_t groups = (p.q_heads + ROWS - 1) / ROWS + (CACHE ? 2 : 1) * ((p.k_heads + ROWS - 1) / ROWS);
+  const uint32_t grid = (p.tokens * groups + PER_CTA - 1) / PER_CTA;
   if (LaunchFacts* sink = observe_sink())
-    return record_launch(sink, reinterpret_cast<const void*>(kernel), CACHE ? "rotate_kernel into pages" : "rotate_kernel",
-                         int(grid), THREADS, 0, 1);
+    return record_launch(sink, reinterpret_cast<const void*>(kernel),
+                         ROWS == 1 ? "rotate_kernel a row per group" : "rotate_kernel several rows per group", int(grid), THREADS, 0, 1);
   const cudaError_t e = launch_programmatic(kernel, dim3(grid), dim3(THREADS), 0, stream, 1, p);
   if (e != cudaSuccess) return cuda_status(e);
   note_launch();
   return launch_status();
+}
+
+template <typename T, bool CACHE>
+int choose(const RotateParams& p, int64_t dim, bool neighbours, cudaStream_t stream) {
+  const bool many = p.tokens * (p.q_heads + (CACHE ? 2 : 1) * p.k_heads) >= MANY;
+#define IB200_ROTATE(D_, NORM_)                                                        \
+  (many ? launch<T, D_, NORM_, CACHE, SHARED_ROWS>(p, neighbours, stream)              \
+        : launch<T, D_, NORM_, CACHE, 1>(p, neighbours, stream))
+  if (p.q_weight) return dim == 128 ? IB200_ROTATE(128, true) : IB200_ROTATE(64, true);
+  return dim == 128 ? IB200_ROTATE(128, false) : IB200_ROTATE(64, false);
+#undef IB200_ROTATE
 }
 
 // Checks what both programs share and fills the parameters in.
@@ -187,10 +293,9 @@ int prepare(RotateParams& p, const View3& q, const View3& k, const View1& positi
   return INTENT_B200_OK;
 }
 
-int count_rows(RotateParams& p, int64_t tokens, int64_t heads) {
+int set_rows(RotateParams& p, int64_t tokens, int64_t heads) {
   if (heads > (1 << 20) || tokens > ((int64_t(1) << 31) - 1) / heads) return INTENT_B200_ERR_UNSUPPORTED;
-  p.heads = uint32_t(heads);
-  p.rows = uint32_t(tokens * heads);
+  p.tokens = uint32_t(tokens);
   return INTENT_B200_OK;
 }
 
@@ -203,12 +308,11 @@ int norm_rope(const View3& q, const View3& k, const View1& positions, const View
   if (status != INTENT_B200_OK) return status;
   if (k_out.d0 != k.d0 || k_out.d1 != k.d1 || k_out.d2 != k.d2) return INTENT_B200_ERR_SHAPE;
   if (!contiguous(k_out) || !aligned16(k_out.p)) return INTENT_B200_ERR_LAYOUT;
-  if ((status = count_rows(p, q.d0, q.d1 + k.d1)) != INTENT_B200_OK) return status;
-  if (p.rows == 0) return INTENT_B200_OK;
+  if ((status = set_rows(p, q.d0, q.d1 + k.d1)) != INTENT_B200_OK) return status;
+  if (p.tokens == 0) return INTENT_B200_OK;
   if (!k_out.p) return INTENT_B200_ERR_NULL;
   p.k_out = static_cast<uint16_t*>(k_out.p);
-  if (q_weight) return q.d2 == 128 ? launch<T, 128, true, false>(p, pairs, stream) : launch<T, 64, true, false>(p, pairs, stream);
-  return q.d2 == 128 ? launch<T, 128, false, false>(p, pairs, stream) : launch<T, 64, false, false>(p, pairs, stream);
+  return choose<T, false>(p, q.d2, pairs, stream);
 }
 
 template <typename T>
@@ -227,8 +331,8 @@ int append(const View3& q, const View3& k, const View3& v, const View1& position
   if (!rows16(v) || !contiguous(slots) || !contiguous(k_cache) || !contiguous(v_cache) || !aligned16(v.p) ||
       !aligned16(k_cache.p) || !aligned16(v_cache.p))
     return INTENT_B200_ERR_LAYOUT;
-  if ((status = count_rows(p, q.d0, q.d1 + 2 * k.d1)) != INTENT_B200_OK) return status;
-  if (p.rows == 0) return INTENT_B200_OK;
+  if ((status = set_rows(p, q.d0, q.d1 + 2 * k.d1)) != INTENT_B200_OK) return status;
+  if (p.tokens == 0) return INTENT_B200_OK;
   if (!v.p || !slots.p || (k_cache.d0 > 0 && (!k_cache.p || !v_cache.p))) return INTENT_B200_ERR_NULL;
   p.v = static_cast<const uint16_t*>(v.p);
   p.v_token = v.s0, p.v_head = v.s1;
@@ -237,8 +341,7 @@ int append(const View3& q, const View3& k, const View3& v, const View1& position
   p.v_out = static_cast<uint16_t*>(v_cache.p);
   p.slot_count = k_cache.d0 * page;
   while ((int64_t(1) << p.page_shift) < page) ++p.page_shift;
-  if (q_weight) return q.d2 == 128 ? launch<T, 128, true, true>(p, pairs, stream) : launch<T, 64, true, true>(p, pairs, stream);
-  return q.d2 == 128 ? launch<T, 128, false, true>(p, pairs, stream) : launch<T, 64, false, true>(p, pairs, stream);
+  return choose<T, true>(p, q.d2, pairs, stream);
 }
 
 }  // namespace
