@@ -11,7 +11,7 @@
 // them.  What has to be right for that:
 //  * Loads run ahead.  A warp has its own ring of three units of 32 tokens (16 KiB each with D = 128), filled by TMA through
 //    128B-swizzled boxes of one page's rows, so that 192 KiB are asked for per SM whatever the warp is computing.
-//  * Work is cut evenly, not by sequence.  All steps of 128 tokens of all (sequence, key head, row tile) form one line, of
+//  * Work is cut evenly, not by sequence.  All steps (32 tokens for each warp) of all (sequence, key head, row tile) form one line, of
 //    which every CTA takes the same number; a long sequence is shared by many CTAs and a CTA goes through many short ones
 //    while its ring runs on.  A row tile that was cut leaves its parts (maximum, sum, unscaled result) in the workspace, and
 //    the CTA that finishes last puts them together in CTA order: the same bits in every launch.
@@ -27,14 +27,16 @@
 namespace ib200 {
 namespace {
 
-constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr int UNIT = 32;                 // tokens of a ring slot
-constexpr int STEP = UNIT * WARPS;       // tokens of a CTA's step
 constexpr float SLACK = 8.f;             // growth of a row's maximum (log2) that its weights are left to absorb
 
 template <int D>
 struct Ring {
-  static constexpr int STAGES = D == 128 ? 3 : 6;
+  // Heads of 64 give a warp half the bytes for nearly the same instructions: with four warps, one per scheduler, their latency
+  // was what bounded the kernel (200 histories, 16 heads: 211 us; see below for eight).
+  static constexpr int WARPS = D == 128 ? 4 : 8;
+  static constexpr int STAGES = 3;
+  static constexpr int STEP = UNIT * WARPS;               // tokens of a CTA's step
   static constexpr int HALF = UNIT * 128;                 // 64 elements of every token of a unit
   static constexpr int OPERAND = HALF * (D / 64);         // keys or values of a unit
   static constexpr int SLOT = 2 * OPERAND;
@@ -48,7 +50,8 @@ constexpr int joins() {
 }
 template <int D, int NT>
 constexpr int smem_bytes() {
-  return 1024 + Ring<D>::BYTES + joins<D, NT>() * WARPS * 8 * NT * ((D + 4) * 4 + 8) + WARPS * Ring<D>::STAGES * 8 + 64;
+  return 1024 + Ring<D>::BYTES + joins<D, NT>() * Ring<D>::WARPS * 8 * NT * (D * 4 + 8) +
+         Ring<D>::WARPS * Ring<D>::STAGES * 8 + 16 + 8 * Ring<D>::WARPS;
 }
 static_assert(smem_bytes<128, 2>() <= 227 * 1024 && smem_bytes<128, 1>() <= 227 * 1024 && smem_bytes<64, 2>() <= 227 * 1024,
               "shared memory of a CTA");
@@ -65,6 +68,7 @@ struct Sequence {
   int tiles;       // row tiles of a key head
 };
 
+template <int STEP>
 __device__ __forceinline__ Sequence sequence_of(const PagedParams& p, int b, int tile_rows) {
   Sequence s;
   const TokenSpan span = span_of(p, b);
@@ -80,6 +84,7 @@ __device__ __forceinline__ Sequence sequence_of(const PagedParams& p, int b, int
 }
 
 // A place on the line of steps
+template <int STEP>
 struct Walk {
   Sequence s;
   int b, head, tile, step;
@@ -92,7 +97,7 @@ struct Walk {
     head = 0;
     do {
       if (++b >= p.batch) return;
-      s = sequence_of(p, b, tile_rows);
+      s = sequence_of<STEP>(p, b, tile_rows);
     } while (s.tiles == 0);
   }
 };
@@ -112,10 +117,10 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t v) {
 }
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(32 * Ring<D>::WARPS, 1)
 paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedParams p) {
   using R = Ring<D>;
-  constexpr int ROWS = 8 * NT, PITCH = D + 4;
+  constexpr int ROWS = 8 * NT, PITCH = D, WARPS = R::WARPS, THREADS = 32 * WARPS, STEP = R::STEP;
   extern __shared__ unsigned char smem_raw[];
   programmatic_begin();
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -139,7 +144,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   const int per_thread = (p.batch + THREADS - 1) / THREADS, mine = tid * per_thread;
   long long sum = 0;
   for (int b = mine; b < min(mine + per_thread, p.batch); ++b) {
-    const Sequence s = sequence_of(p, b, ROWS);
+    const Sequence s = sequence_of<STEP>(p, b, ROWS);
     sum += (long long)s.tiles * p.k_heads * s.steps;
   }
   long long before = sum;
@@ -169,7 +174,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   if (begin >= before && begin < before + sum) {
     int b = mine, at = int(before);
     for (;; ++b) {
-      const Sequence s = sequence_of(p, b, ROWS);
+      const Sequence s = sequence_of<STEP>(p, b, ROWS);
       const int steps = s.tiles * p.k_heads * s.steps;
       if (begin < at + steps) break;
       at += steps;
@@ -178,16 +183,16 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     shared[1] = at;
   }
   __syncthreads();
-  Walk load;
+  Walk<STEP> load;
   load.b = shared[0];
-  load.s = sequence_of(p, load.b, ROWS);
+  load.s = sequence_of<STEP>(p, load.b, ROWS);
   {
     const int item = (begin - shared[1]) / load.s.steps;
     load.step = (begin - shared[1]) - item * load.s.steps;
     load.head = item / load.s.tiles;
     load.tile = item - load.head * load.s.tiles;
   }
-  Walk work = load;
+  Walk<STEP> work = load;
 
   const float infinity = __int_as_float(0x7f800000);
   int loading = begin, slot_in = 0, slot_out = 0;
@@ -479,9 +484,10 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           }
 #pragma unroll
           for (int i = 0; i < D / 16; ++i) {
-            float* to = join_here + (warp * ROWS + r) * PITCH + 16 * i + (lane >> 2);
-            to[0] = o[nt][i][e];
-            to[8] = o[nt][i][e + 2];
+            // (pieces of eight elements change places with the row, so that a store meets 32 banks)
+            float* to = join_here + (warp * ROWS + r) * PITCH + (lane >> 2);
+            to[((2 * i) ^ (lane & 3)) * 8] = o[nt][i][e];
+            to[((2 * i + 1) ^ (lane & 3)) * 8] = o[nt][i][e + 2];
           }
         }
       }
@@ -513,7 +519,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         for (int v = 0; v < WARPS; ++v) {
           const float f = exp2_fast(max_here[v * ROWS + r] - origin);
           l = fmaf(sum_here[v * ROWS + r], f, l);
-          const float* from = join_here + (v * ROWS + r) * PITCH + 8 * c;
+          const float* from = join_here + (v * ROWS + r) * PITCH + 8 * (c ^ (r >> 1 & 3));
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = fmaf(from[e], f, x[e]);
         }
@@ -575,8 +581,8 @@ int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, const PagedParams
   if (e != cudaSuccess) return cuda_status(e);
   if (LaunchFacts* sink = observe_sink())
     return record_launch(sink, reinterpret_cast<const void*>(kernel),
-                         NT == 1 ? "paged_rows_kernel 8 rows" : "paged_rows_kernel 16 rows", grid, THREADS, smem, 1);
-  e = launch_programmatic(kernel, dim3(unsigned(grid)), dim3(THREADS), smem, stream, 1, map_k, map_v, p);
+                         NT == 1 ? "paged_rows_kernel 8 rows" : "paged_rows_kernel 16 rows", grid, 32 * Ring<D>::WARPS, smem, 1);
+  e = launch_programmatic(kernel, dim3(unsigned(grid)), dim3(32 * Ring<D>::WARPS), smem, stream, 1, map_k, map_v, p);
   if (e != cudaSuccess) return cuda_status(e);
   note_launch();
   return launch_status();
