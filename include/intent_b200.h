@@ -566,9 +566,9 @@ INTENT_B200_API int intent_b200_paged_kv_append_norm_bf16(INTENT_B200_VIEW3(q), 
  * of zeros.  Tokens behind kv_length, ahead of the window, in pages that the table does not name or whose number lies
  * outside the cache are not read, whatever the memory there holds.  Rows of q that no sequence has are left alone.
  * scale_bits: the f32 factor of the scores (> 0; 0: 1 / sqrt(D)).  f32 statistics and sums.
- * workspace: at least ..._workspace_bytes(D, 0) bytes (paged_decode_attention: (D, 1)), 16-byte aligned, zero-filled once; every launch leaves its counters
- * zero again.  Launches that may overlap need separate ones.  Bytes 0..3: INTENT_B200_ERR_TIMEOUT of a bounded wait that
- * gave up (..._workspace_status reads it and clears the workspace).  The same call gives the same bits.
+ * workspace: at least ..._workspace_bytes(D, 0) bytes (paged_decode_attention: (D, 1)), 16-byte aligned, its first four zero
+ * before the first launch.  Launches that may overlap need separate ones.  Bytes 0..3: INTENT_B200_ERR_TIMEOUT of a bounded
+ * wait that gave up (..._workspace_status reads and clears it).  The same call gives the same bits.
  * ------------------------------------------------------------------------ */
 INTENT_B200_API int intent_b200_paged_attention_f16(INTENT_B200_VIEW3(q), INTENT_B200_VIEW4(k_cache), INTENT_B200_VIEW4(v_cache),
                                                  INTENT_B200_VIEW2(page_table), INTENT_B200_VIEW1(query_offsets),

@@ -8,9 +8,10 @@
 namespace ib200 {
 
 constexpr int kPagedCtas = 160;            // most CTAs of a launch
-constexpr int64_t kPagedHeader = 4096;     // bytes of the workspace ahead of the parts: status word, then per CTA a counter
-constexpr int64_t kPagedJoins = 1024;      // and, from here on, the tile that it leaves to others (16 bytes)
-static_assert(64 + 4 * kPagedCtas <= kPagedJoins && kPagedJoins + 16 * kPagedCtas <= kPagedHeader, "room ahead of the parts");
+constexpr int64_t kPagedHeader = 4096;     // bytes of the workspace ahead of the parts: status word
+constexpr int64_t kPagedJoins = 64;        // and, from here on, the tile that a CTA leaves to others
+constexpr int64_t kPagedEntry = 24;        // bytes of its description, at most
+static_assert(kPagedJoins + kPagedEntry * kPagedCtas <= kPagedHeader, "room ahead of the parts");
 
 struct PagedParams {
   const uint16_t* q;                 // [T, HQ, D] at these strides (elements)
@@ -23,8 +24,7 @@ struct PagedParams {
   int pages, page_shift, capacity;   // capacity: tokens that a row of the page table can name
   int window;                        // tokens that a query sees, its own among them; 0 = all
   float scale;                       // of the scores, times log2(e)
-  int* status;                       // heads of the workspace
-  int* counters;
+  int* status;                       // head of the workspace
   void* joins;
   float* parts;
   int half_tokens;                   // chunks: tokens of half a tile
@@ -49,6 +49,14 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// x * 0 + sum for a pair of 16-bit numbers: NaN where x is no finite number
+template <typename T>
+__device__ __forceinline__ uint32_t add_no_numbers(uint32_t x, uint32_t sum) {
+  if (std::is_same<T, __half>::value) asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(x), "r"(0u));
+  else asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(x), "r"(0u));
+  return sum;
 }
 
 #endif  // __CUDACC__

@@ -66,10 +66,13 @@ int attend(const View3& q, const View4& k_cache, const View4& v_cache, const Vie
   p.window = window;
   p.scale = scale * 1.44269504f;         // log2(e): the exponentials are powers of two
   p.status = static_cast<int*>(workspace);
-  p.counters = p.status + 16;
   p.joins = static_cast<unsigned char*>(workspace) + kPagedJoins;
   p.parts = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + kPagedHeader);
-  if (offsets && paged_chunk_takes(p)) return paged_chunk<T>(p, dim, k_cache.p, v_cache.p, sms, stream);
+  // Up to sixteen rows of queries per sequence and key head on average are one tile of the rows kernel, which is then bound by
+  // HBM; with more it reads and multiplies the cache once for every sixteen.  us for 64 sequences of up to 4000 tokens, 32 heads
+  // of 128 on 8 key heads, 1 / 4 / 8 / 16 new tokens each: rows 98 / 110 / 189 / 345, chunk 146 / 146 / 147 / 146; one sequence
+  // of 8000: rows 16 / 30 / 20 / 30, chunk 24 throughout.
+  if (offsets && paged_chunk_takes(p) && tokens * p.group > 16 * batch) return paged_chunk<T>(p, dim, k_cache.p, v_cache.p, sms, stream);
   return paged_rows<T>(p, dim, k_cache.p, v_cache.p, sms, stream);
 }
 
@@ -81,8 +84,7 @@ extern "C" int64_t intent_b200_paged_attention_workspace_bytes(int64_t dim, int3
   return single || rows > chunk ? rows : chunk;
 }
 
-// Reads the status word at the head of a workspace after synchronising `stream`.  A launch that gave up on a bounded wait may
-// have left counters behind: the workspace is then cleared for reuse before the code is returned.
+// Reads the status word at the head of a workspace after synchronising `stream`, and clears it.
 extern "C" int intent_b200_paged_attention_workspace_status(void* workspace, int64_t workspace_bytes, void* stream) {
   if (!workspace || workspace_bytes < ib200::kPagedHeader) return INTENT_B200_ERR_WORKSPACE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

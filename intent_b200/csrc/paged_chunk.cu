@@ -237,14 +237,6 @@ __device__ __forceinline__ void weigh(const uint32_t (&v)[32], uint64_t scale, u
   }
 }
 
-// x * 0 + sum for a pair of 16-bit numbers: NaN where x is no finite number
-template <typename T>
-__device__ __forceinline__ uint32_t add_no_numbers(uint32_t x, uint32_t sum) {
-  if (std::is_same<T, __half>::value) asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(x), "r"(0u));
-  else asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(x), "r"(0u));
-  return sum;
-}
-
 // What lies behind the operands in shared memory
 template <int SLOTS>
 struct Shared {

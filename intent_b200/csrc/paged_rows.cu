@@ -13,8 +13,8 @@
 //    128B-swizzled boxes of one page's rows, so that 192 KiB are asked for per SM whatever the warp is computing.
 //  * Work is cut evenly, not by sequence.  All steps (32 tokens for each warp) of all (sequence, key head, row tile) form one line, of
 //    which every CTA takes the same number; a long sequence is shared by many CTAs and a CTA goes through many short ones
-//    while its ring runs on.  A row tile that was cut leaves its parts (maximum, sum, unscaled result) in the workspace, and
-//    the CTA that finishes last puts them together in CTA order: the same bits in every launch.
+//    while its ring runs on.  A row tile that was cut leaves its parts (maximum, sum, unscaled result) in the workspace,
+//    which paged_rows_join_kernel puts together in CTA order: the same bits in every launch.
 //  * Few instructions per token.  Keys are the tensor core's A operand (16 tokens) and the queries its B operand (eight rows,
 //    kept in registers): S^T = K Q^T, then O^T += V^T P^T with V^T from transposing loads and P^T from one movmatrix per
 //    eight tokens.  With up to eight query heads per key head nothing is computed for rows that are not there.
@@ -116,6 +116,12 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t v) {
   return d;
 }
 
+struct JoinEntry {
+  int last_cta;            // of the tile that begins in this CTA and ends in another; -1: there is none
+  int row, head;           // first row of q of its sequence, key head
+  int tile_row, rows;      // its first row among the sequence's, how many it has
+};
+
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(32 * Ring<D>::WARPS, 1)
 paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedParams p) {
@@ -162,13 +168,13 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     line += warp_sums[w];
   }
   before -= sum;
-  if (line > 0x3fffffff) {               // (only offsets that make no sense name so much)
-    if (tid == 0) atomicExch(p.status, INTENT_B200_ERR_SHAPE);
-    return;
-  }
-  const int total = int(line);
+  const bool sensible = line <= 0x3fffffff;              // (only offsets that make no sense name more)
+  if (!sensible && tid == 0) atomicExch(p.status, INTENT_B200_ERR_SHAPE);
+  const int total = sensible ? int(line) : 0;
   const int share = (total + int(gridDim.x) - 1) / int(gridDim.x);     // steps of a CTA
   const int cta = blockIdx.x;
+  JoinEntry* entry = reinterpret_cast<JoinEntry*>(p.joins) + cta;
+  if (tid == 0) entry->last_cta = -1;
   const int begin = min(cta * share, total), end = min(begin + share, total);
   if (begin >= end) return;
   if (begin >= before && begin < before + sum) {
@@ -394,19 +400,21 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 #pragma unroll
           for (int e = 0; e < 4; ++e) a[e] &= counted[m][e >> 1];
       };
-      auto not_finite = [&](auto& loaded) {
-        constexpr uint32_t EXPONENT = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-        bool found = false;
+      auto not_finite = [&] {
+        // (a loop that stays one: code that few calls reach has to be fetched when they do)
+        uint32_t sum[2] = {};
+#pragma unroll 1
+        for (int i = 0; i < D / 16; ++i) {
+          uint32_t a[4], b[4];
+          values_of(Bool<false>{}, 0, i, a);
+          values_of(Bool<false>{}, 1, i, b);
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll 2
-          for (int i = 0; i < D / 16; ++i) {
-            uint32_t a[4];
-            loaded(Bool<false>{}, m, i, a);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) found |= (a[e] & EXPONENT) == EXPONENT || ((a[e] >> 16) & EXPONENT) == EXPONENT;
+          for (int e = 0; e < 4; ++e) {
+            sum[0] = add_no_numbers<T>(a[e], sum[0]);
+            sum[1] = add_no_numbers<T>(b[e], sum[1]);
           }
-        return __any_sync(0xffffffffu, found) != 0;
+        }
+        return __any_sync(0xffffffffu, ((sum[0] | sum[1]) & 0x7fff7fffu) != 0) != 0;
       };
       auto add_values = [&](auto whole) {
 #pragma unroll
@@ -421,7 +429,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       };
       if (all) {
         add_values(Bool<true>{});
-      } else if (least == most || !not_finite(values_of)) {
+      } else if (least == most || !not_finite()) {
         add_values(Bool<false>{});
       } else {
         // Values that are no finite numbers, in tokens that some rows see and others do not: row by row, from what it sees.
@@ -501,13 +509,9 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       const int first_cta = item_begin / share, last_cta = (item_end - 1) / share;
       const bool whole = first_cta == last_cta;
       float* part = p.parts + size_t(2 * cta + (cta == first_cta)) * (ROWS * (D + 2));
-      auto store = [&](int r, int c, const float (&x)[8], float l) {
-        const float inverse = l == 0.f ? 0.f : 1.f / l;
+      auto place = [&](int r) {
         const int token = (tile_row + r) / p.group, of_group = tile_row + r - token * p.group;
-        uint16_t* to = p.out + (int64_t(first_row + token) * p.q_heads + head * p.group + of_group) * D + 8 * c;
-        *reinterpret_cast<uint4*>(to) =
-            make_uint4(Elem<T>::pack2(x[0] * inverse, x[1] * inverse), Elem<T>::pack2(x[2] * inverse, x[3] * inverse),
-                       Elem<T>::pack2(x[4] * inverse, x[5] * inverse), Elem<T>::pack2(x[6] * inverse, x[7] * inverse));
+        return p.out + (int64_t(first_row + token) * p.q_heads + head * p.group + of_group) * D;
       };
       for (int w = tid; w < rows * (D / 8); w += THREADS) {
         const int r = w / (D / 8), c = w - r * (D / 8);
@@ -524,7 +528,10 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           for (int e = 0; e < 8; ++e) x[e] = fmaf(from[e], f, x[e]);
         }
         if (whole) {
-          store(r, c, x, l);
+          const float inverse = l == 0.f ? 0.f : 1.f / l;
+          *reinterpret_cast<uint4*>(place(r) + 8 * c) =
+              make_uint4(Elem<T>::pack2(x[0] * inverse, x[1] * inverse), Elem<T>::pack2(x[2] * inverse, x[3] * inverse),
+                         Elem<T>::pack2(x[4] * inverse, x[5] * inverse), Elem<T>::pack2(x[6] * inverse, x[7] * inverse));
         } else {
           float4* to = reinterpret_cast<float4*>(part + r * D + 8 * c);
           to[0] = make_float4(x[0], x[1], x[2], x[3]);
@@ -535,33 +542,12 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           }
         }
       }
-      if (!whole) {
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) shared[2] = atomicAdd(p.counters + first_cta, 1);
-        __syncthreads();
-        if (shared[2] == last_cta - first_cta) {
-          __threadfence();
-          if (tid == 0) p.counters[first_cta] = 0;
-          for (int w = tid; w < rows * (D / 8); w += THREADS) {
-            const int r = w / (D / 8), c = w - r * (D / 8);
-            float m = -infinity, l = 0.f, x[8] = {};
-            for (int v = first_cta; v <= last_cta; ++v)
-              m = fmaxf(m, __ldcg(p.parts + size_t(2 * v + (v == first_cta)) * (ROWS * (D + 2)) + ROWS * D + r));
-            const float origin = m == -infinity ? 0.f : m;
-#pragma unroll 2
-            for (int v = first_cta; v <= last_cta; ++v) {
-              const float* from = p.parts + size_t(2 * v + (v == first_cta)) * (ROWS * (D + 2));
-              const float f = exp2_fast(__ldcg(from + ROWS * D + r) - origin);
-              l = fmaf(__ldcg(from + ROWS * (D + 1) + r), f, l);
-              const float4 y0 = __ldcg(reinterpret_cast<const float4*>(from + r * D + 8 * c));
-              const float4 y1 = __ldcg(reinterpret_cast<const float4*>(from + r * D + 8 * c) + 1);
-              x[0] = fmaf(y0.x, f, x[0]), x[1] = fmaf(y0.y, f, x[1]), x[2] = fmaf(y0.z, f, x[2]), x[3] = fmaf(y0.w, f, x[3]);
-              x[4] = fmaf(y1.x, f, x[4]), x[5] = fmaf(y1.y, f, x[5]), x[6] = fmaf(y1.z, f, x[6]), x[7] = fmaf(y1.w, f, x[7]);
-            }
-            store(r, c, x, l);
-          }
-        }
+      if (tid == 0 && !whole && cta == first_cta) {
+        entry->row = first_row;
+        entry->head = head;
+        entry->tile_row = tile_row;
+        entry->rows = rows;
+        entry->last_cta = last_cta;
       }
       if (JOINS == 1) __syncthreads();
     }
@@ -571,6 +557,51 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     for (int s = 0; s < R::STAGES; ++s) mbar_wait_warp(full + 8 * s, (parity >> s) & 1, 64);
     if (lane == 0) atomicExch(p.status, INTENT_B200_ERR_TIMEOUT);
   }
+}
+
+// Parts of the tiles that CTA boundaries cut: a block per CTA in which such a tile begins, a thread per row and four elements.
+// What it costs is the latency of dependent reads: all maxima and sums are read at once, then the results of eight parts at a time.
+// (The CTA that finishes a tile last did this before: one multiprocessor for 16 rows of 16 parts, 7 us; see the table of measured
+// cases for the kernel of its own.)
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(ROWS * D / 4) paged_rows_join_kernel(const PagedParams p) {
+  __shared__ float maxima[kPagedCtas][ROWS], sums[kPagedCtas][ROWS];
+  programmatic_begin();
+  programmatic_wait();
+  const JoinEntry entry = reinterpret_cast<const JoinEntry*>(p.joins)[blockIdx.x];
+  const int first = blockIdx.x, count = entry.last_cta - first + 1, r = threadIdx.x / (D / 4), c = threadIdx.x % (D / 4);
+  if (entry.last_cta < 0) return;
+  constexpr size_t SIZE = size_t(ROWS) * (D + 2);
+  const float infinity = __int_as_float(0x7f800000);
+  auto part = [&](int v) { return p.parts + (2 * (first + v) + (v == 0)) * SIZE; };
+  for (int i = threadIdx.x; i < count * ROWS; i += ROWS * D / 4) {
+    const int v = i / ROWS, row = i % ROWS;
+    maxima[v][row] = row < entry.rows ? __ldcg(part(v) + ROWS * D + row) : -infinity;
+    sums[v][row] = row < entry.rows ? __ldcg(part(v) + ROWS * (D + 1) + row) : 0.f;
+  }
+  __syncthreads();
+  if (r >= entry.rows) return;
+  float m = -infinity, l = 0.f, x[4] = {};
+  for (int v = 0; v < count; ++v) m = fmaxf(m, maxima[v][r]);
+  const float origin = m == -infinity ? 0.f : m;
+#pragma unroll 1
+  for (int from = 0; from < count; from += 8) {
+    float4 y[8];
+#pragma unroll
+    for (int v = 0; v < 8; ++v)
+      if (from + v < count) y[v] = __ldcg(reinterpret_cast<const float4*>(part(from + v) + r * D) + c);
+#pragma unroll
+    for (int v = 0; v < 8; ++v) {
+      if (from + v >= count) break;
+      const float f = exp2_fast(maxima[from + v][r] - origin);
+      l = fmaf(sums[from + v][r], f, l);
+      x[0] = fmaf(y[v].x, f, x[0]), x[1] = fmaf(y[v].y, f, x[1]), x[2] = fmaf(y[v].z, f, x[2]), x[3] = fmaf(y[v].w, f, x[3]);
+    }
+  }
+  const float inverse = l == 0.f ? 0.f : 1.f / l;
+  const int token = (entry.tile_row + r) / p.group, of_group = entry.tile_row + r - token * p.group;
+  *reinterpret_cast<uint2*>(p.out + (int64_t(entry.row + token) * p.q_heads + entry.head * p.group + of_group) * D + 4 * c) =
+      make_uint2(Elem<T>::pack2(x[0] * inverse, x[1] * inverse), Elem<T>::pack2(x[2] * inverse, x[3] * inverse));
 }
 
 template <typename T, int D, int NT>
@@ -583,6 +614,9 @@ int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, const PagedParams
     return record_launch(sink, reinterpret_cast<const void*>(kernel),
                          NT == 1 ? "paged_rows_kernel 8 rows" : "paged_rows_kernel 16 rows", grid, 32 * Ring<D>::WARPS, smem, 1);
   e = launch_programmatic(kernel, dim3(unsigned(grid)), dim3(32 * Ring<D>::WARPS), smem, stream, 1, map_k, map_v, p);
+  if (e != cudaSuccess) return cuda_status(e);
+  note_launch();
+  e = launch_programmatic(paged_rows_join_kernel<T, D, 8 * NT>, dim3(unsigned(grid)), dim3(8 * NT * D / 4), 0, stream, 1, p);
   if (e != cudaSuccess) return cuda_status(e);
   note_launch();
   return launch_status();
