@@ -328,7 +328,7 @@ PyObject* binder_forget(PyObject* object, PyObject*) {
 }
 
 // Binder(call address, slots, device, selection address, selection bytes, workspaces | None,
-//        ((access, dtype, rank, alignment, rows), ...), constants)
+//        ((access, dtype, rank, alignment[, rows]), ...), constants)
 PyObject* binder_new(PyTypeObject* type, PyObject* arguments, PyObject*) {
   unsigned long long call, selection;
   int slots, device;
@@ -360,7 +360,8 @@ PyObject* binder_new(PyTypeObject* type, PyObject* arguments, PyObject*) {
       View v;
       PyObject* dtype;
       long long alignment;
-      if (!PyArg_ParseTuple(PyTuple_GET_ITEM(views, i), "iOiLi", &v.access, &dtype, &v.rank, &alignment, &v.rows)) {
+      v.rows = 0;
+      if (!PyArg_ParseTuple(PyTuple_GET_ITEM(views, i), "iOiL|i", &v.access, &dtype, &v.rank, &alignment, &v.rows)) {
         Py_DECREF(self);
         return nullptr;
       }
