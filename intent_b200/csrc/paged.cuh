@@ -28,6 +28,8 @@ struct PagedParams {
   void* joins;
   float* parts;
   int half_tokens;                   // chunks: tokens of half a tile
+  int few;                           // rows of queries per key head up to which a sequence is the rows kernel's; those with more
+                                     // are the chunk kernel's (either may get all: INT_MAX, 0)
 };
 
 #ifdef __CUDACC__

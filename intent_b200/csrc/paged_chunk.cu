@@ -55,7 +55,7 @@ struct Sequence {
 __device__ __forceinline__ Sequence sequence_of(const PagedParams& p, int b) {
   Sequence s;
   const TokenSpan span = span_of(p, b);
-  s.count = span.count;
+  s.count = span.count * p.group > p.few ? span.count : 0;
   s.first_row = span.begin;
   s.length = min(max(__ldg(p.lengths + b), 0), p.capacity);
   s.first = s.length - s.count;
@@ -554,12 +554,44 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         ++seen;
         if (!ok) break;
         tcgen05_fence_after();
+        const uint32_t missing = sh.missing[u & 7];
+        const bool mixed = !half.sees_all(p, token), edge = mixed || missing != 0;
+        const uint32_t slot = (2 * u + 1) % SLOTS, values = ring + slot * R::OPERAND;
+        if (edge) {
+          // Values that no query of the tile sees may be anything, and 0 * NaN is NaN: they become zeros.
+          ok = mbar_wait_warp(kv_full + 8 * slot, ((2 * u + 1) / SLOTS) & 1);
+          if (!ok) break;
+          const int tile_high = tile_position + min(tokens, 2 * p.half_tokens);
+          const int tile_low = p.window > 0 ? max(tile_position - p.window + 1, 0) : 0;
+          unsigned char* mine_row = base_ptr + (values - base) + row * 128;     // (pieces in another order for every row: 32 banks)
+          const bool outside = token + row < tile_low || token + row >= tile_high;
+          if (outside) {
+#pragma unroll 1
+            for (int j = 0; j < 8 * BOXES; ++j)
+              *reinterpret_cast<uint4*>(mine_row + (j / 8) * R::BOX + 16 * ((j ^ row) & 7)) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async();
+          }
+          // Those that some rows see and others do not have to be finite for the product; where they are not, the rows add
+          // them up themselves, each from what it sees.  The warps of the half ask one another, and hear it after the weights.
+          uint32_t sum[2] = {0, 0};
+          if (mixed && !outside && (token + row > half.least || (p.window > 0 && token + row <= half.most - p.window))) {
+#pragma unroll 4
+            for (int j = 0; j < 8 * BOXES; ++j) {
+              const uint4 x = *reinterpret_cast<const uint4*>(mine_row + (j / 8) * R::BOX + 16 * ((j ^ row) & 7));
+              sum[0] = add_no_numbers<T>(x.x, sum[0]);
+              sum[1] = add_no_numbers<T>(x.y, sum[1]);
+              sum[0] = add_no_numbers<T>(x.z, sum[0]);
+              sum[1] = add_no_numbers<T>(x.w, sum[1]);
+            }
+          }
+          if (__any_sync(0xffffffffu, ((sum[0] | sum[1]) & 0x7fff7fffu) != 0) && lane == 0) sh.vote[h] = u + 1;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(vote_full + 8 * h);
+        }
         uint32_t v[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_load_32x32(at_s + 32 * c, v[c]);
         tmem_load_wait();
-        const uint32_t missing = sh.missing[u & 7];
-        const bool edge = !half.sees_all(p, token) || missing != 0;
         if (edge) {
           const int behind = position - token, ahead = p.window > 0 ? behind - p.window : -1;   // seen: (ahead, behind]
           const int shift = min(p.page_shift, 7);
@@ -571,6 +603,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             shown &= none <= 0 ? ~0u : none >= 32 ? 0u : ~0u << none;
             if (missing >> ((32 * c) >> shift) & 1) shown &= 0xffff0000u;
             if (missing >> ((32 * c + 16) >> shift) & 1) shown &= 0xffffu;
+            if (missing == 0 && token + 32 * c + 31 <= half.least && (p.window == 0 || token + 32 * c > half.most - p.window)) continue;
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (!(shown >> e & 1)) v[c][e] = 0xff800000u;
@@ -608,7 +641,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
           weigh<T>(v[c], scales, origins, added, w);
           tmem_store_32x16(at_s + 16 * c, w);
           if (c == EARLY / 32 - 1 && !edge) {
-            if (lane == 0 && quadrant == 0) sh.skip[h] = 0;
             tmem_store_wait();
             tcgen05_fence_before();
             __syncwarp();
@@ -621,46 +653,12 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         weight_sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
         bool by_hand = false;
         if (edge) {
-          // Values that no query of the tile sees may be anything, and 0 * NaN is NaN: they become zeros.
-          const uint32_t slot = (2 * u + 1) % SLOTS, values = ring + slot * R::OPERAND;
-          ok = mbar_wait_warp(kv_full + 8 * slot, ((2 * u + 1) / SLOTS) & 1);
+          ok = mbar_wait_warp(vote_full + 8 * h, votes & 1);
+          ++votes;
           if (!ok) break;
-          const int tile_high = tile_position + min(tokens, 2 * p.half_tokens);
-          const int tile_low = p.window > 0 ? max(tile_position - p.window + 1, 0) : 0;
-          unsigned char* mine_row = base_ptr + (values - base) + row * 128;
-          const bool outside = token + row < tile_low || token + row >= tile_high;
-          if (outside) {
-#pragma unroll
-            for (int j = 0; j < 8 * BOXES; ++j) *reinterpret_cast<uint4*>(mine_row + (j / 8) * R::BOX + 16 * (j % 8)) = make_uint4(0, 0, 0, 0);
-            fence_proxy_async();
-          }
-          // Those that some rows see and others do not have to be finite for the product; where they are not, the rows add
-          // them up themselves, each from what it sees.
-          if (!half.sees_all(p, token)) {
-            uint32_t sum[2] = {0, 0};
-            if (!outside) {
-#pragma unroll
-              for (int j = 0; j < 8 * BOXES; ++j) {
-                const uint4 x = *reinterpret_cast<const uint4*>(mine_row + (j / 8) * R::BOX + 16 * (j % 8));
-                sum[0] = add_no_numbers<T>(x.x, sum[0]);
-                sum[1] = add_no_numbers<T>(x.y, sum[1]);
-                sum[0] = add_no_numbers<T>(x.z, sum[0]);
-                sum[1] = add_no_numbers<T>(x.w, sum[1]);
-              }
-            }
-            const bool found = (sum[0] & 0x7fff7fffu) != 0 || (sum[1] & 0x7fff7fffu) != 0;
-            if (__any_sync(0xffffffffu, found) && lane == 0) sh.vote[h] = u + 1;
-            tmem_store_wait();                                         // (the other threads read these weights)
-            tcgen05_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(vote_full + 8 * h);
-            ok = mbar_wait_warp(vote_full + 8 * h, votes & 1);
-            ++votes;
-            if (!ok) break;
-            by_hand = sh.vote[h] == u + 1;
-          }
+          by_hand = sh.vote[h] == u + 1;
           if (by_hand) {
-            tcgen05_fence_after();
+            tmem_store_wait();
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
               uint32_t o[16];

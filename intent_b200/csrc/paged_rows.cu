@@ -72,7 +72,7 @@ template <int STEP>
 __device__ __forceinline__ Sequence sequence_of(const PagedParams& p, int b, int tile_rows) {
   Sequence s;
   const TokenSpan span = span_of(p, b);
-  s.rows = span.count * p.group;
+  s.rows = span.count * p.group <= p.few ? span.count * p.group : 0;
   s.first_row = span.begin;
   s.length = min(max(__ldg(p.lengths + b), 0), p.capacity);
   s.first = s.length - span.count;
@@ -129,6 +129,10 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   constexpr int ROWS = 8 * NT, PITCH = D, WARPS = R::WARPS, THREADS = 32 * WARPS, STEP = R::STEP;
   extern __shared__ unsigned char smem_raw[];
   programmatic_begin();
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&map_k);
+    prefetch_tensormap(&map_v);
+  }
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* base_ptr = smem_raw + (base - smem_u32(smem_raw));
   constexpr int JOINS = joins<D, NT>();
@@ -247,9 +251,6 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       look_up();
     }
   };
-  look_up();
-  for (int i = 0; i < R::STAGES && loading < end; ++i) ask();
-
   uint32_t qf[NT][D / 16][2];            // queries as B fragments: k = elements, n = rows
   float o[NT][D / 16][4];                // O^T: elements 16 i + lane / 4 (+ 8) of rows 2 (lane % 4) (+ 1)
   float top[NT][2], weight_sum[NT][2];
@@ -281,7 +282,9 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       }
     }
   };
+  look_up();
   begin_tile();
+  for (int i = 0; i < R::STAGES && loading < end; ++i) ask();
   int turn = 0;                          // place of the join that is next
   for (int at = begin; at < end; ++at) {
     const uint32_t halves = present & 3;
