@@ -30,8 +30,8 @@ int attend(const View3& q, const View4& k_cache, const View4& v_cache, const Vie
     return INTENT_B200_ERR_SHAPE;
   if (dim != 64 && dim != 128) return INTENT_B200_ERR_UNSUPPORTED;
   if (page < 16 || page > 256 || (page & (page - 1)) != 0 || window < 0) return INTENT_B200_ERR_UNSUPPORTED;
-  constexpr int64_t kMost = (int64_t(1) << 31) - 1;
-  if (heads > 4096 || batch > (1 << 24) || tokens > kMost / heads || pages > kMost / (k_heads * page) || table.d1 > kMost / page)
+  constexpr int64_t kMost = (int64_t(1) << 31) - 1, kHalf = int64_t(1) << 30;   // (differences of positions are 32 bits, too)
+  if (heads > 4096 || batch > (1 << 24) || tokens > kHalf / heads || pages > kMost / (k_heads * page) || table.d1 > kHalf / page)
     return INTENT_B200_ERR_UNSUPPORTED;
   float scale;
   std::memcpy(&scale, &scale_bits, sizeof(float));
@@ -64,7 +64,7 @@ int attend(const View3& q, const View4& k_cache, const View4& v_cache, const Vie
   p.group = int(heads / k_heads);
   p.table_width = int(table.d1), p.pages = int(pages), p.capacity = int(table.d1 * page);
   while ((int64_t(1) << p.page_shift) < page) ++p.page_shift;
-  p.window = window;
+  p.window = window < p.capacity ? window : 0;   // (a query that sees as many tokens as there may be sees all)
   p.scale = scale * 1.44269504f;         // log2(e): the exponentials are powers of two
   p.status = static_cast<int*>(workspace);
   p.joins = static_cast<unsigned char*>(workspace) + kPagedJoins;

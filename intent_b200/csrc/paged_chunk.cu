@@ -128,8 +128,10 @@ __device__ __forceinline__ void walk(const PagedParams& p, const Start& from, in
     tile = 0;
     if (++head < p.k_heads) continue;
     head = 0;
-    do s = sequence_of(p, ++b);
-    while (s.tiles == 0);
+    do {
+      if (++b >= p.batch) return;            // (not unless the lengths change under the launch)
+      s = sequence_of(p, b);
+    } while (s.tiles == 0);
   }
 }
 
@@ -329,15 +331,16 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   const int cta = blockIdx.x, begin = min(cta * share, total), end = min(begin + share, total);
   if (begin < end && begin >= before && begin < before + sum) {
     int b = mine;
-    long long at = before;
+    long long at = before, steps = sum;
     for (; per_thread > 1; ++b) {
       const Sequence s = sequence_of(p, b);
-      const long long steps = steps_before(p, s, s.tiles) * p.k_heads;
-      if (begin < at + steps) break;
+      steps = steps_before(p, s, s.tiles) * p.k_heads;
+      if (begin < at + steps || b + 1 >= min(mine + per_thread, p.batch)) break;
       at += steps;
     }
     sh.start.b = b;
     sh.start.step = begin - int(at);                                   // in the sequence
+    sh.start.head = max(int(steps) / p.k_heads, 1);                    // steps of a key head
   }
   JoinEntry* entry = reinterpret_cast<JoinEntry*>(p.joins) + cta;
   if (tid == 0) {
@@ -360,7 +363,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       Start at_first = sh.start;
       {
         const Sequence s = sequence_of(p, at_first.b);
-        const int per_head = int(steps_before(p, s, s.tiles));
+        const int per_head = at_first.head;
         at_first.head = at_first.step / per_head;
         const int step = at_first.step - at_first.head * per_head;
         int low = 0, high = s.tiles;                                   // steps_before(low) <= step < steps_before(high)

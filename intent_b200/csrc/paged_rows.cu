@@ -186,7 +186,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     for (;; ++b) {
       const Sequence s = sequence_of<STEP>(p, b, ROWS);
       const int steps = s.tiles * p.k_heads * s.steps;
-      if (begin < at + steps) break;
+      if (begin < at + steps || b + 1 >= min(mine + per_thread, p.batch)) break;
       at += steps;
     }
     shared[0] = b;

@@ -301,3 +301,52 @@ def test_refusals(cuda_device):
     for constexprs in ({"SCALE": 0.0}, {"SCALE": -1.0}, {"WINDOW": -1}, {"WINDOW": 1.5}, {"ACT_DTYPE": "f32"}, {"CAUSAL": 1}):
         with pytest.raises(ib.CompilationStageError):
             ib.compile(ib.programs.paged_attention, constexprs=constexprs)
+
+
+@pytest.mark.parametrize("single", [True, False])
+def test_a_window_of_any_size(cuda_device, single):
+    """One that is wider than any history is none."""
+    data = make([70, 300], [1, 1] if single else [90, 40], 2, 1, 64, 16, "bf16")
+    expected, weight = oracle.paged_attention(*data)
+    program = ib.programs.paged_decode_attention if single else ib.programs.paged_attention
+    for window in (304, 305, (1 << 31) - 1):
+        assert_close(run(ib.compile(program, constexprs={"WINDOW": window}), cuda_device, *data, single), expected, weight, "bf16")
+
+
+def test_few_and_many_rows_in_one_call(cuda_device):
+    """Sequences on both sides of the choice between the kernels, with empty ones between them."""
+    counts = [1, 4, 5, 0, 17, 64, 65, 1, 2, 130, 3, 0]
+    lengths = [200, 4, 90, 60, 17, 300, 65, 1, 129, 140, 40, 0]
+    both(cuda_device, lengths, counts, 8, 2, 128, 16, "bf16")
+    both(cuda_device, lengths, counts, 7, 1, 64, 32, "f16", window=50)
+
+
+def test_values_that_are_no_numbers_beside_few_rows(cuda_device):
+    """The same as above for rows that are taken sixteen at a time."""
+    q, k, v, table, offsets, n = make([64, 33, 50], [2, 4, 1], 4, 2, 64, 16, "bf16")
+    for b, (token, value) in enumerate(((63, math.nan), (30, math.inf))):
+        v[int(table[b, token // 16]), 1, token % 16, 7] = value
+    expected, weight = oracle.paged_attention(q, k, v, table, offsets, n)
+    out = run(ib.compile(ib.programs.paged_attention), cuda_device, q, k, v, table, offsets, n, False).cpu()
+    fine = expected.isfinite()
+    assert 0 < int((~fine).sum()) < 20
+    assert torch.equal(out.isfinite(), fine) and torch.equal(out.isnan(), expected.isnan())
+    bound = (HALF_UNIT["bf16"] + 2e-4) * weight + HALF_UNIT["bf16"] * expected.abs() + 2.0 ** -24
+    assert ((out.double() - expected).abs() <= bound)[fine].all()
+
+
+def test_heads_that_no_tile_holds(cuda_device):
+    """More query heads per key head than half a tile has rows."""
+    both(cuda_device, [40, 70], [9, 30], 130, 1, 64, 16, "bf16")
+
+
+def test_a_status_word_raises(cuda_device):
+    """What a bounded wait that gave up leaves in the workspace is reported by ``check`` and cleared."""
+    q, k, v, table, _, n = (t.to(cuda_device) for t in make([40], [1], 4, 2, 64, 16, "bf16"))
+    call = ib.compile(ib.programs.paged_decode_attention).prepare(q, k, v, table, n)
+    call.launch()
+    call.check()
+    call._workspace[0][:4].view(torch.int32)[0] = 4
+    with pytest.raises(ib.CompilationStageError):
+        call.check()
+    call.check()
