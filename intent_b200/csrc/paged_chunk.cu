@@ -772,10 +772,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
 }
 
 // Parts of the tiles that CTA boundaries cut: block (cta, 32 rows), a thread per row and 16 elements.  What it costs is the
-// latency of dependent reads, so the maxima and sums of all parts are read at once, by all warps, and the results four parts at a
-// time (8 tiles of 16 parts: 23 us one after another, see the table of measured cases for now).
+// latency of dependent reads, so the maxima and sums of all parts are read at once, by all warps, and the results two parts at a
+// time: four take registers that three blocks of a multiprocessor have not (three prompts, heads of 64: 115 -> 113 us with two).
 template <typename T, int D>
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
+__global__ void __launch_bounds__(256, 3) paged_join_kernel(const PagedParams p) {
   __shared__ float maxima[kPagedCtas][32], sums[kPagedCtas][32];
   programmatic_begin();
   programmatic_wait();
@@ -798,15 +798,15 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
   float m = -infinity, l = 0.f, x[16] = {};
   for (int v = 0; v < count; ++v) m = fmaxf(m, maxima[v][lane]);
   const float origin = m == -infinity ? 0.f : m;
-  for (int from = 0; from < count; from += 4) {
-    float4 y[4][4];
+  for (int from = 0; from < count; from += 2) {
+    float4 y[2][4];
 #pragma unroll
-    for (int v = 0; v < 4; ++v)
+    for (int v = 0; v < 2; ++v)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (from + v < count) y[v][e] = __ldcg(reinterpret_cast<const float4*>(part(from + v)) + (4 * warp + e) * 2 * HALF_ROWS + row);
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
+    for (int v = 0; v < 2; ++v) {
       if (from + v >= count) break;
       const float f = exp2_fast(maxima[from + v][lane] - origin);
       l = fmaf(sums[from + v][lane], f, l);
