@@ -63,10 +63,11 @@ __device__ __forceinline__ uint32_t add_no_numbers(uint32_t x, uint32_t sum) {
 
 #endif  // __CUDACC__
 
-// few rows per sequence (paged_rows.cu)
+// few rows per sequence, in tiles of eight (`narrow`) or sixteen (paged_rows.cu)
 int64_t paged_rows_workspace_bytes(int64_t dim);
 template <typename T>
-int paged_rows(const PagedParams& p, int64_t dim, const void* k_cache, const void* v_cache, int sms, cudaStream_t stream);
+int paged_rows(const PagedParams& p, int64_t dim, bool narrow, const void* k_cache, const void* v_cache, int sms,
+               cudaStream_t stream);
 
 // chunks (paged_chunk.cu)
 int64_t paged_chunk_workspace_bytes(int64_t dim);

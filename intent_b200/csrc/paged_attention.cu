@@ -71,22 +71,24 @@ int attend(const View3& q, const View4& k_cache, const View4& v_cache, const Vie
   p.parts = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + kPagedHeader);
   // Up to sixteen rows of queries per sequence and key head on average are one tile of the rows kernel, which is then bound by
   // HBM; with more it reads and multiplies the cache once for every sixteen.  us for 64 sequences of up to 4000 tokens, 32 heads
-  // of 128 on 8 key heads, 1 / 4 / 8 / 16 new tokens each: rows 98 / 110 / 189 / 345, chunk 146 / 146 / 147 / 146; one sequence
-  // of 8000: rows 16 / 30 / 20 / 30, chunk 24 throughout.
-  // In a call of more rows and many sequences, those of up to sixteen rows still are the rows kernel's, so that tokens that are
-  // decoded beside prompts are not multiplied as tiles of 256 (20 beside 4 chunks of up to 500 tokens: 169 -> 160 us).  In a
-  // call of few sequences the two launches cost more than that (3 prompts: 120 -> 128 us).
+  // of 128 on 8 key heads, 1 / 4 / 8 / 16 new tokens each: rows 98 / 103 / 189 / 345, chunk 146 / 146 / 147 / 146; one sequence
+  // of 8000: rows 14 / 17 / 20 / 30, chunk 24 throughout.  With heads of 64 two tiles still are (64 heads on 8, 4 / 8 new tokens:
+  // rows 105 / 185, chunk 128 / 130).
+  // In a call of more rows and many sequences, those of one tile still are the rows kernel's, so that tokens that are decoded
+  // beside prompts are not multiplied as tiles of 256 (20 beside 4 chunks of up to 500 tokens: 169 -> 160 us, with tiles of eight 144).  In a call of few
+  // sequences the two launches cost more than that (3 prompts: 120 -> 128 us).
   constexpr int FEW = 16, MANY = 8;
+  const int64_t rows = tokens * p.group;
   p.few = std::numeric_limits<int>::max();
-  if (offsets && paged_chunk_takes(p) && tokens * p.group > FEW * batch) {
-    p.few = batch >= MANY ? FEW : 0;
-    if (p.few > 0) {
-      const int status = paged_rows<T>(p, dim, k_cache.p, v_cache.p, sms, stream);
-      if (status != INTENT_B200_OK) return status;
-    }
-    return paged_chunk<T>(p, dim, k_cache.p, v_cache.p, sms, stream);
+  if (!offsets || !paged_chunk_takes(p) || rows <= (dim == 64 ? 2 * FEW : FEW) * batch)
+    return paged_rows<T>(p, dim, rows <= FEW / 2 * batch, k_cache.p, v_cache.p, sms, stream);
+  const bool narrow = p.group <= FEW / 2;
+  p.few = batch < MANY ? 0 : narrow ? FEW / 2 : FEW;
+  if (p.few > 0) {
+    const int status = paged_rows<T>(p, dim, narrow, k_cache.p, v_cache.p, sms, stream);
+    if (status != INTENT_B200_OK) return status;
   }
-  return paged_rows<T>(p, dim, k_cache.p, v_cache.p, sms, stream);
+  return paged_chunk<T>(p, dim, k_cache.p, v_cache.p, sms, stream);
 }
 
 }  // namespace

@@ -632,7 +632,8 @@ int64_t paged_rows_workspace_bytes(int64_t dim) {
 }
 
 template <typename T>
-int paged_rows(const PagedParams& p, int64_t dim, const void* k_cache, const void* v_cache, int sms, cudaStream_t stream) {
+int paged_rows(const PagedParams& p, int64_t dim, bool narrow, const void* k_cache, const void* v_cache, int sms,
+               cudaStream_t stream) {
   CUtensorMap map_k, map_v;
   const uint64_t rows = uint64_t(p.pages) * uint64_t(p.k_heads) << p.page_shift;
   const uint32_t box = p.page_shift >= 5 ? UNIT : UNIT / 2;
@@ -643,12 +644,11 @@ int paged_rows(const PagedParams& p, int64_t dim, const void* k_cache, const voi
                           CU_TENSOR_MAP_SWIZZLE_128B))
     return INTENT_B200_ERR_CUDA;
   const int grid = sms < kPagedCtas ? sms : kPagedCtas;
-  const bool narrow = !p.offsets && p.group <= 8;
   if (dim == 128)
     return narrow ? launch<T, 128, 1>(map_k, map_v, p, grid, stream) : launch<T, 128, 2>(map_k, map_v, p, grid, stream);
   return narrow ? launch<T, 64, 1>(map_k, map_v, p, grid, stream) : launch<T, 64, 2>(map_k, map_v, p, grid, stream);
 }
-template int paged_rows<__half>(const PagedParams&, int64_t, const void*, const void*, int, cudaStream_t);
-template int paged_rows<__nv_bfloat16>(const PagedParams&, int64_t, const void*, const void*, int, cudaStream_t);
+template int paged_rows<__half>(const PagedParams&, int64_t, bool, const void*, const void*, int, cudaStream_t);
+template int paged_rows<__nv_bfloat16>(const PagedParams&, int64_t, bool, const void*, const void*, int, cudaStream_t);
 
 }  // namespace ib200
