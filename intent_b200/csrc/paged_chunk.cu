@@ -771,12 +771,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
 }
 
-// Parts of the tiles that CTA boundaries cut: block (cta, 32 rows), a thread per row and 16 elements.  What it costs is the
-// latency of dependent reads, so the maxima and sums of all parts are read at once, by all warps, and the results two parts at a
-// time: four take registers that three blocks of a multiprocessor have not (three prompts, heads of 64: 115 -> 113 us with two).
+// Parts of the tiles that CTA boundaries cut: block (cta, 32 rows), a thread per row and eight elements.  What it costs is the
+// latency of dependent reads (0.5 us each): the maxima and sums of all parts are read at once, by all warps, and the results four
+// parts at a time (8 tiles of 16 parts, 33 tokens behind 7967: 28.1 us a call with two at a time and sixteen elements per thread).
 template <typename T, int D>
-__global__ void __launch_bounds__(256, 3) paged_join_kernel(const PagedParams p) {
+__global__ void __launch_bounds__(4 * D, 1024 / (4 * D)) paged_join_kernel(const PagedParams p) {
   __shared__ float maxima[kPagedCtas][32], sums[kPagedCtas][32];
+  constexpr int WARPS = D / 8;
   programmatic_begin();
   programmatic_wait();
   const JoinEntry entry = reinterpret_cast<const JoinEntry*>(p.joins)[blockIdx.x];
@@ -789,41 +790,41 @@ __global__ void __launch_bounds__(256, 3) paged_join_kernel(const PagedParams p)
   const float infinity = __int_as_float(0x7f800000);
   auto part = [&](int v) { return p.parts + (2 * (first + v) + (v == 0)) * SIZE; };
 #pragma unroll 4
-  for (int v = warp; v < count; v += 8) {
+  for (int v = warp; v < count; v += WARPS) {
     maxima[v][lane] = real ? __ldcg(part(v) + 2 * HALF_ROWS * D + row) : -infinity;
     sums[v][lane] = real ? __ldcg(part(v) + 2 * HALF_ROWS * (D + 1) + row) : 0.f;
   }
   __syncthreads();
-  if (warp >= D / 16 || !real) return;
-  float m = -infinity, l = 0.f, x[16] = {};
+  if (!real) return;
+  float m = -infinity, l = 0.f, x[8] = {};
   for (int v = 0; v < count; ++v) m = fmaxf(m, maxima[v][lane]);
   const float origin = m == -infinity ? 0.f : m;
-  for (int from = 0; from < count; from += 2) {
-    float4 y[2][4];
+#pragma unroll 1
+  for (int from = 0; from < count; from += 4) {
+    float4 y[4][2];
 #pragma unroll
-    for (int v = 0; v < 2; ++v)
+    for (int v = 0; v < 4; ++v)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (from + v < count) y[v][e] = __ldcg(reinterpret_cast<const float4*>(part(from + v)) + (4 * warp + e) * 2 * HALF_ROWS + row);
+      for (int e = 0; e < 2; ++e)
+        if (from + v < count) y[v][e] = __ldcg(reinterpret_cast<const float4*>(part(from + v)) + (2 * warp + e) * 2 * HALF_ROWS + row);
 #pragma unroll
-    for (int v = 0; v < 2; ++v) {
+    for (int v = 0; v < 4; ++v) {
       if (from + v >= count) break;
       const float f = exp2_fast(maxima[from + v][lane] - origin);
       l = fmaf(sums[from + v][lane], f, l);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < 2; ++e) {
         x[4 * e] = fmaf(y[v][e].x, f, x[4 * e]), x[4 * e + 1] = fmaf(y[v][e].y, f, x[4 * e + 1]);
         x[4 * e + 2] = fmaf(y[v][e].z, f, x[4 * e + 2]), x[4 * e + 3] = fmaf(y[v][e].w, f, x[4 * e + 3]);
       }
     }
   }
   const float inverse = l == 0.f ? 0.f : 1.f / l;
-  uint32_t w[8];
+  uint32_t w[4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = Elem<T>::pack2(x[2 * e] * inverse, x[2 * e + 1] * inverse);
-  uint16_t* to = p.out + (int64_t(entry.row + token) * p.q_heads + entry.head * p.group + of_half - row_token * p.group) * D + 16 * warp;
+  for (int e = 0; e < 4; ++e) w[e] = Elem<T>::pack2(x[2 * e] * inverse, x[2 * e + 1] * inverse);
+  uint16_t* to = p.out + (int64_t(entry.row + token) * p.q_heads + entry.head * p.group + of_half - row_token * p.group) * D + 8 * warp;
   *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-  *reinterpret_cast<uint4*>(to + 8) = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
 template <typename T, int D>
@@ -846,7 +847,7 @@ int launch(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap
   e = launch_programmatic(kernel, dim3(unsigned(grid)), dim3(THREADS), smem, stream, 1, map_q, map_k, map_v, p);
   if (e != cudaSuccess) return cuda_status(e);
   note_launch();
-  e = launch_programmatic(paged_join_kernel<T, D>, dim3(unsigned(grid), 2 * HALF_ROWS / 32), dim3(256), 0, stream, 1, p);
+  e = launch_programmatic(paged_join_kernel<T, D>, dim3(unsigned(grid), 2 * HALF_ROWS / 32), dim3(4 * D), 0, stream, 1, p);
   if (e != cudaSuccess) return cuda_status(e);
   note_launch();
   return launch_status();
