@@ -48,7 +48,8 @@ int attend(const View3& q, const View4& k_cache, const View4& v_cache, const Vie
     return cuda_status(cudaMemsetAsync(out.p, 0, size_t(tokens * heads * dim) * 2, stream));
   }
   if (!k_cache.p || !v_cache.p || !table.p) return INTENT_B200_ERR_NULL;
-  if (!workspace || workspace_bytes < intent_b200_paged_attention_workspace_bytes(dim, offsets ? 0 : 1)) return INTENT_B200_ERR_WORKSPACE;
+  if (!workspace || workspace_bytes < intent_b200_paged_attention_workspace_bytes(dim, offsets ? 0 : 1))
+    return INTENT_B200_ERR_WORKSPACE;
   if (!aligned16(workspace)) return INTENT_B200_ERR_LAYOUT;
   const int sms = device_sms();
   if (sms <= 0) return INTENT_B200_ERR_CUDA;
@@ -75,8 +76,8 @@ int attend(const View3& q, const View4& k_cache, const View4& v_cache, const Vie
   // of 8000: rows 14 / 17 / 20 / 30, chunk 24 throughout.  With heads of 64 two tiles still are (64 heads on 8, 4 / 8 new tokens:
   // rows 105 / 185, chunk 128 / 130).
   // In a call of more rows and many sequences, those of one tile still are the rows kernel's, so that tokens that are decoded
-  // beside prompts are not multiplied as tiles of 256 (20 beside 4 chunks of up to 500 tokens: 169 -> 160 us, with tiles of eight 144).  In a call of few
-  // sequences the two launches cost more than that (3 prompts: 120 -> 128 us).
+  // beside prompts are not multiplied as tiles of 256 (20 beside 4 chunks of up to 500 tokens: 169 -> 160 us, with tiles of
+  // eight 144).  In a call of few sequences the two launches cost more than that (3 prompts: 120 -> 128 us).
   constexpr int FEW = 16, MANY = 8;
   const int64_t rows = tokens * p.group;
   p.few = std::numeric_limits<int>::max();
