@@ -44,6 +44,7 @@ constexpr int LOAD_WARP = 9, MMA_WARP = 8, THREADS = 12 * 32;   // warps 0..3 an
 // Registers of a thread: the launch's, then those of a row's thread (128 scores and more) and of the others.
 constexpr int LAUNCH_REGISTERS = 168, ROW_REGISTERS = 224, OTHER_REGISTERS = 56;
 static_assert(2 * ROW_REGISTERS + OTHER_REGISTERS <= 3 * LAUNCH_REGISTERS, "three warpgroups share the launch's registers");
+constexpr int BEGIN = 2;                   // places on the line ahead of the steps of a tile
 constexpr int EARLY = 96;                  // tokens of a step whose weights the products begin with
 constexpr float SLACK = 8.f;               // growth of a row's maximum (log2) that its weights are left to absorb
 
@@ -71,6 +72,9 @@ __device__ __forceinline__ Sequence sequence_of(const PagedParams& p, int b) {
   s.tiles = (s.count + 2 * p.half_tokens - 1) / (2 * p.half_tokens);
   return s;
 }
+
+// A tile takes its steps' places on the line and BEGIN more ahead of them, for what it costs beside its steps: queries, the
+// steps that hide some of their tokens, the results' way out.
 
 // Steps of tile j: from that of the first token its first query sees to that of its last query's own.  (Of queries ahead of the
 // first token, which see nothing, one step each is walked, all of it hidden.)
@@ -104,8 +108,8 @@ __device__ __forceinline__ unsigned long long floor_sum(unsigned n, unsigned a, 
   }
 }
 
-// Steps of tiles 0 .. j - 1 of a key head.
-__device__ __forceinline__ long long steps_before(const PagedParams& p, const Sequence& s, int j) {
+// Places of tiles 0 .. j - 1 of a key head.
+__device__ __forceinline__ long long places_before(const PagedParams& p, const Sequence& s, int j) {
   const int size = 2 * p.half_tokens, start = max(s.first, 0), full = min(j, s.tiles - 1);
   if (j <= 0) return 0;
   unsigned long long sum = full > 0 ? floor_sum(full, size, unsigned(start) + size + STEP - 1) : 0;
@@ -115,24 +119,25 @@ __device__ __forceinline__ long long steps_before(const PagedParams& p, const Se
     const int from = low >= 0 ? 0 : (-low + size - 1) / size;
     if (j > from) sum -= floor_sum(j - from, size, unsigned(low + from * size));
   }
-  return (long long)sum;
+  return (long long)sum + (long long)BEGIN * j;
 }
 
-// Goes through the parts of tiles among the steps [at, end); visit(sequence, head, tile, step, steps, all, at) gets the part's
-// first step in its tile, how many it has and how many the tile has, and returns whether to go on.
+// Goes through the parts of tiles among the places [at, end); visit(sequence, head, tile, step, steps, all, at) gets the part's
+// first step in its tile, how many it has, how many the tile has and the first one's place, and returns whether to go on.
 struct Start {
-  int b, head, tile, step;
+  int b, head, tile, place;
 };
 template <typename Visit>
 __device__ __forceinline__ void walk(const PagedParams& p, const Start& from, int at, int end, Visit visit) {
-  int b = from.b, head = from.head, tile = from.tile, step = from.step;
+  int b = from.b, head = from.head, tile = from.tile, place = from.place;
   Sequence s = sequence_of(p, b);
   while (true) {
-    const int all = steps_of(p, s, tile), steps = min(all - step, end - at);
-    if (!visit(s, b, head, tile, step, steps, all, at)) return;
-    at += steps;
+    const int all = steps_of(p, s, tile), places = min(BEGIN + all - place, end - at);
+    const int step = max(place - BEGIN, 0), steps = place + places - BEGIN - step;
+    if (steps > 0 && !visit(s, b, head, tile, step, steps, all, at + max(BEGIN - place, 0))) return;
+    at += places;
     if (at >= end) return;
-    step = 0;
+    place = 0;
     if (++tile < s.tiles) continue;
     tile = 0;
     if (++head < p.k_heads) continue;
@@ -150,6 +155,7 @@ struct Part {
   int position;            // of the first of them
   int first, steps;        // steps of 128 tokens
   int step, all, at;       // the first one's number in the tile, the tile's steps, the first one's place on the line
+                           // (steps = 0: there are no more)
 };
 
 // What a half of a tile sees
@@ -319,7 +325,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   long long sum = 0;
   for (int b = mine; b < min(mine + per_thread, p.batch); ++b) {
     const Sequence s = sequence_of(p, b);
-    sum += steps_before(p, s, s.tiles) * p.k_heads;
+    sum += places_before(p, s, s.tiles) * p.k_heads;
   }
   long long before = sum;
 #pragma unroll
@@ -344,13 +350,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     long long at = before, steps = sum;
     for (; per_thread > 1; ++b) {
       const Sequence s = sequence_of(p, b);
-      steps = steps_before(p, s, s.tiles) * p.k_heads;
+      steps = places_before(p, s, s.tiles) * p.k_heads;
       if (begin < at + steps || b + 1 >= min(mine + per_thread, p.batch)) break;
       at += steps;
     }
     sh.start.b = b;
-    sh.start.step = begin - int(at);                                   // in the sequence
-    sh.start.head = max(int(steps) / p.k_heads, 1);                    // steps of a key head
+    sh.start.place = begin - int(at);                                   // in the sequence
+    sh.start.head = max(int(steps) / p.k_heads, 1);                    // places of a key head
   }
   JoinEntry* entry = reinterpret_cast<JoinEntry*>(p.joins) + cta;
   if (tid == 0) {
@@ -374,17 +380,17 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       {
         const Sequence s = sequence_of(p, at_first.b);
         const int per_head = at_first.head;
-        at_first.head = at_first.step / per_head;
-        const int step = at_first.step - at_first.head * per_head;
-        int low = 0, high = s.tiles;                                   // steps_before(low) <= step < steps_before(high)
+        at_first.head = at_first.place / per_head;
+        const int place = at_first.place - at_first.head * per_head;
+        int low = 0, high = s.tiles;                                   // places_before(low) <= place < places_before(high)
         while (high - low > 1) {
           const int stride = (high - low + 31) / 32, j = low + lane * stride;
-          const int fitting = __popc(__ballot_sync(0xffffffffu, j < high && steps_before(p, s, j) <= step));
+          const int fitting = __popc(__ballot_sync(0xffffffffu, j < high && places_before(p, s, j) <= place));
           low += (fitting - 1) * stride;
           high = min(low + stride, high);
         }
         at_first.tile = low;
-        at_first.step = step - int(steps_before(p, s, low));
+        at_first.place = place - int(places_before(p, s, low));
       }
       const int rows = min(1 << p.page_shift, STEP);                   // of a box
       const int boxes = STEP / rows;                                   // of 64 elements of a step
@@ -436,6 +442,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         }
         return true;
       });
+      ok = ok && mbar_wait_warp(part_empty + 8 * (parts & 3), (parts / 4 & 1) ^ 1);
+      if (ok && lane == 0) {
+        sh.parts[parts & 3].steps = 0;
+        mbar_arrive(part_full + 8 * (parts & 3));
+      }
       if (!ok)   // (nothing may be on its way to a CTA that is gone)
         for (int i = 0; i < SLOTS; ++i)
           for (int parity = 0; parity < 2; ++parity) mbar_wait_warp(kv_full + 8 * i, parity, 64);
@@ -478,16 +489,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         if (ok && issue && begun[h]) umma_commit(o_full + 8 * h);
         begun[h] = false;
       };
-      int at = begin;
-      while (ok && at < end) {
+      while (ok) {
         const uint32_t place = parts & 3;
         ok = mbar_wait_warp(part_full + 8 * place, parts / 4 & 1);
-        if (!ok) break;
+        if (!ok || sh.parts[place].steps == 0) break;
         const int steps = sh.parts[place].steps, first = sh.parts[place].first, tokens = sh.parts[place].tokens,
                   position = sh.parts[place].position;
         __syncwarp();
         if (lane == 0) mbar_arrive(part_empty + 8 * place);
-        at += steps;
         const Half half[2] = {Half(p, tokens, position, 0), Half(p, tokens, position, 1)};
         for (int i = 0; i < steps; ++i) {
           const int token = (first + i) * STEP;
@@ -532,7 +541,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         ++parts;
       }
       // the last step's values: no slot is asked for again, but nothing may be on its way to a CTA that is gone
-      ok = ok && mbar_wait_warp(kv_full + 8 * v_slot, v_turn & 1);
+      if (some) ok = ok && mbar_wait_warp(kv_full + 8 * v_slot, v_turn & 1);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         if (ok) finish(h);
@@ -546,15 +555,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const float infinity = __int_as_float(0x7f800000);
     const int row_token = row / p.group;                               // in the half
     uint32_t u = 0, parts = 0, seen = 0, done = 0, votes = 0;
-    int at = begin;
-    while (at < end) {
+    while (true) {
       const uint32_t place = parts & 3;
       ok = mbar_wait_warp(part_full + 8 * place, parts / 4 & 1);
-      if (!ok) break;
+      if (!ok || sh.parts[place].steps == 0) break;
       const volatile Part& part = sh.parts[place];
       ++parts;
       const int steps = part.steps, first = part.first, tokens = part.tokens, tile_position = part.position;
-      at += steps;
       const Half half(p, tokens, tile_position, h);
       const bool real = row_token < half.tokens;
       const int position = real ? half.least + row_token : -1;
