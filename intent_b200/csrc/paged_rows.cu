@@ -12,7 +12,7 @@
 //  * Loads run ahead.  A warp has its own ring of three units of 32 tokens (16 KiB each with D = 128), filled by TMA through
 //    128B-swizzled boxes of one page's rows, so that 192 KiB are asked for per SM whatever the warp is computing.
 //  * Work is cut evenly, not by sequence.  All steps (32 tokens for each warp) of all (sequence, key head, row tile) form one
-//    line, of which every CTA takes the same number; a long sequence is shared by many CTAs and a CTA goes through many short ones
+//    line, of which every CTA takes the same length; a long sequence is shared by many CTAs and a CTA goes through many short ones
 //    while its ring runs on.  A row tile that was cut leaves its parts (maximum, sum, unscaled result) in the workspace,
 //    which paged_rows_join_kernel puts together in CTA order: the same bits in every launch.
 //  * Few instructions per token.  Keys are the tensor core's A operand (16 tokens) and the queries its B operand (eight rows,
@@ -21,7 +21,7 @@
 //    shared between lanes only when it grows.
 //
 // Measured on one B200 (6530 GB/s copied): 64 histories of up to 8192 tokens, 32 heads of 128 on 8 key heads, bf16: 181 us, 6.24
-// TB/s; 4 of up to 131072 on 4 key heads: 108 us, 5.9 TB/s; 200 of up to 2048, 16 heads of 64: 154 us, 5.7 TB/s.  One history of
+// TB/s; 4 of up to 131072 on 4 key heads: 108 us, 5.9 TB/s; 200 of up to 2048, 16 heads of 64: 149 us, 5.9 TB/s.  One history of
 // 1000 tokens, 7.3 us: the reads one after another of a launch (lengths, page numbers, keys, parts) and its join.
 #include <cstring>
 
@@ -38,7 +38,7 @@ constexpr float SLACK = 8.f;             // growth of a row's maximum (log2) tha
 template <int D>
 struct Ring {
   // Heads of 64 give a warp half the bytes for nearly the same instructions: with four warps, one per scheduler, their latency
-  // was what bounded the kernel (200 histories of up to 2048 tokens, 16 heads: 211 us; with eight 154).
+  // was what bounded the kernel (200 histories of up to 2048 tokens, 16 heads: 211 us; with eight 149).
   static constexpr int WARPS = D == 128 ? 4 : 8;
   static constexpr int STAGES = 3;
   static constexpr int STEP = UNIT * WARPS;               // tokens of a CTA's step
@@ -46,6 +46,10 @@ struct Ring {
   static constexpr int OPERAND = HALF * (D / 64);         // keys or values of a unit
   static constexpr int SLOT = 2 * OPERAND;
   static constexpr int BYTES = WARPS * STAGES * SLOT;
+  // Places on the line ahead of the steps of a tile, for what it costs beside them: with eight warps to put together about a
+  // step's time (200 histories of up to 2048 tokens, 16 heads of 64: 154 us without, 149 with one, 151 with two); with four not
+  // enough to show (64 histories of up to 8192, 8 heads of 128: 184 us without, 185 with one, 184 with two).
+  static constexpr int BEGIN = D == 128 ? 0 : 1;
 };
 
 // Places for the warps' parts of a tile: two where there is room
@@ -88,11 +92,19 @@ __device__ __forceinline__ Sequence sequence_of(const PagedParams& p, int b, int
   return s;
 }
 
-// A place on the line of steps
-template <int STEP>
+// Places of a sequence on the line
+template <int BEGIN>
+__device__ __forceinline__ long long places_of(const PagedParams& p, const Sequence& s) {
+  return (long long)s.tiles * p.k_heads * (s.steps + BEGIN);
+}
+
+// A step on the line
+template <int STEP, int BEGIN>
 struct Walk {
   Sequence s;
   int b, head, tile, step;
+  // how many places on the next one is
+  __device__ __forceinline__ int distance() const { return step + 1 < s.steps ? 1 : 1 + BEGIN; }
   __device__ __forceinline__ void advance(const PagedParams& p, int tile_rows) {
     if (++step < s.steps) return;
     step = 0;
@@ -131,7 +143,7 @@ template <typename T, int D, int NT>
 __global__ void __launch_bounds__(32 * Ring<D>::WARPS, 1)
 paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedParams p) {
   using R = Ring<D>;
-  constexpr int ROWS = 8 * NT, PITCH = D, WARPS = R::WARPS, THREADS = 32 * WARPS, STEP = R::STEP;
+  constexpr int ROWS = 8 * NT, PITCH = D, WARPS = R::WARPS, THREADS = 32 * WARPS, STEP = R::STEP, BEGIN = R::BEGIN;
   extern __shared__ unsigned char smem_raw[];
   programmatic_begin();
   if (threadIdx.x == 0) {
@@ -160,7 +172,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   long long sum = 0;
   for (int b = mine; b < min(mine + per_thread, p.batch); ++b) {
     const Sequence s = sequence_of<STEP>(p, b, ROWS);
-    sum += (long long)s.tiles * p.k_heads * s.steps;
+    sum += places_of<BEGIN>(p, s);
   }
   long long before = sum;
 #pragma unroll
@@ -180,7 +192,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   const bool sensible = line <= 0x3fffffff;              // (only offsets that make no sense name more)
   if (!sensible && tid == 0) atomicExch(p.status, INTENT_B200_ERR_SHAPE);
   const int total = sensible ? int(line) : 0;
-  const int share = (total + int(gridDim.x) - 1) / int(gridDim.x);     // steps of a CTA
+  const int share = (total + int(gridDim.x) - 1) / int(gridDim.x);     // places of a CTA
   const int cta = blockIdx.x;
   JoinEntry* entry = reinterpret_cast<JoinEntry*>(p.joins) + cta;
   if (tid == 0) entry->last_cta = -1;
@@ -190,27 +202,30 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     int b = mine, at = int(before);
     for (;; ++b) {
       const Sequence s = sequence_of<STEP>(p, b, ROWS);
-      const int steps = s.tiles * p.k_heads * s.steps;
-      if (begin < at + steps || b + 1 >= min(mine + per_thread, p.batch)) break;
-      at += steps;
+      const int places = int(places_of<BEGIN>(p, s));
+      if (begin < at + places || b + 1 >= min(mine + per_thread, p.batch)) break;
+      at += places;
     }
     shared[0] = b;
     shared[1] = at;
   }
   __syncthreads();
-  Walk<STEP> load;
+  Walk<STEP, BEGIN> load;
   load.b = shared[0];
   load.s = sequence_of<STEP>(p, load.b, ROWS);
   {
-    const int item = (begin - shared[1]) / load.s.steps;
-    load.step = (begin - shared[1]) - item * load.s.steps;
+    const int item = (begin - shared[1]) / (load.s.steps + BEGIN);
+    load.step = (begin - shared[1]) - item * (load.s.steps + BEGIN) - BEGIN;
     load.head = item / load.s.tiles;
     load.tile = item - load.head * load.s.tiles;
   }
-  Walk<STEP> work = load;
+  const int first_place = begin + max(-load.step, 0);    // of a step
+  if (first_place >= end) return;
+  load.step = max(load.step, 0);
+  Walk<STEP, BEGIN> work = load;
 
   const float infinity = __int_as_float(0x7f800000);
-  int loading = begin, slot_in = 0, slot_out = 0;
+  int loading = first_place, slot_in = 0, slot_out = 0;
   uint32_t parity = 0, present = 0;      // a bit per slot; two bits per unit asked for (its halves), the oldest lowest
   int queued = 0;
   bool ok = true;
@@ -250,7 +265,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     present |= (uint32_t(here[0]) | (uint32_t(here[1]) << 1)) << (2 * queued);
     ++queued;
     if (any) slot_in = slot_in + 1 == R::STAGES ? 0 : slot_in + 1;
-    ++loading;
+    loading += load.distance();
     if (loading < end) {
       load.advance(p, ROWS);
       look_up();
@@ -291,7 +306,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   begin_tile();
   for (int i = 0; i < R::STAGES && loading < end; ++i) ask();
   int turn = 0;                          // place of the join that is next
-  for (int at = begin; at < end; ++at) {
+  for (int at = first_place, next; at < end; at = next) {
     const uint32_t halves = present & 3;
     present >>= 2;
     --queued;
@@ -477,7 +492,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     if (loading < end) ask();
 
     const bool last_step = work.step + 1 == work.s.steps;
-    if (!last_step && at + 1 < end) {
+    next = at + work.distance();
+    if (!last_step && next < end) {
       ++work.step;
     } else {
       // ---- the warps' parts, then the CTAs'.  There are two places for them in turn: when a warp writes to one of them again,
@@ -510,7 +526,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       const int tile_row = work.tile * ROWS, rows = min(ROWS, work.s.rows - tile_row), head = work.head;
       const int first_row = work.s.first_row;
       const int item_begin = at - work.step, item_end = item_begin + work.s.steps;   // on the line
-      if (at + 1 < end) {
+      if (next < end) {
         work.advance(p, ROWS);
         begin_tile();                    // (its queries are on their way while this tile is put together)
       }
