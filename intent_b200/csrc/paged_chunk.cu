@@ -24,8 +24,15 @@
 // one half, scores to registers, exponentials (1450), weights back, which two halves do not hide altogether.  With the arithmetic
 // on the scores left out the same call takes 0.80 ms.  Tried and not kept: a part of the exponentials by a cubic on the FMA units
 // (fewer cycles, the same time at the power cap), two threads per row (0.94 -> 1.04 ms, they have to exchange the maximum every
-// step), heads of 64 with weights beside the scores in tensor memory (115 -> 123 us for three prompts: both halves then want the
-// exponential unit at once), the maximum looked for only when a sum says so (0.91 -> 0.90 ms, short calls 3 % slower).
+// step), the maximum looked for only when a sum says so (0.91 -> 0.90 ms, short calls 3 % slower), scores read in two loads with the
+// first one's maximum between them (0.91 -> 0.93 ms).
+//
+// Heads of 64: a step takes 3500 cycles as well (1024 tokens behind 7168, 32 heads on 4 key heads: 111 us).  The products take half
+// as long, but a half's chain is what counts: scores into registers 360, maximum 450, weights 1700, handed over and multiplied by V
+// 400, the next scores 600.  Not kept for them: weights beside the scores in tensor memory, which takes the products off the chain
+// (three prompts with a window 115 -> 123 us, 111 -> 127 with one half's products between the other's two: the halves then do the
+// same things at the same time and each takes longer, 3770 cycles a step); a cubic for an eighth or a quarter of the exponentials
+// (111 -> 113 and 114).
 #include <algorithm>
 #include <cstddef>
 #include <type_traits>
@@ -793,7 +800,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
 
 // Parts of the tiles that CTA boundaries cut: block (cta, 32 rows), a thread per row and eight elements.  What it costs is the
 // latency of dependent reads (0.5 us each): the maxima and sums of all parts are read at once, by all warps, and the results four
-// parts at a time (8 tiles of 16 parts, 33 tokens behind 7967: 28.1 us a call with two at a time and sixteen elements per thread).
+// parts at a time (8 tiles of 16 parts, 33 tokens behind 7967, a call alone: 39.7 us; with two at a time and sixteen elements per
+// thread 40.4).
 template <typename T, int D>
 __global__ void __launch_bounds__(4 * D, 1024 / (4 * D)) paged_join_kernel(const PagedParams p) {
   __shared__ float maxima[kPagedCtas][32], sums[kPagedCtas][32];
