@@ -313,6 +313,17 @@ def test_a_window_of_any_size(cuda_device, single):
         assert_close(run(ib.compile(program, constexprs={"WINDOW": window}), cuda_device, *data, single), expected, weight, "bf16")
 
 
+@pytest.mark.parametrize("batch", [37, 75, 150, 223])
+@pytest.mark.parametrize("single", [True, False])
+@pytest.mark.parametrize("D", [64, 128])
+def test_tiles_of_few_steps(cuda_device, batch, single, D):
+    """Shares of the multiprocessors that begin and end anywhere in tiles of one to three steps, and between tiles."""
+    g = torch.Generator().manual_seed(batch)
+    counts = [1] * batch if single else torch.randint(9, 40, (batch,), generator=g).tolist()
+    lengths = [n + int(torch.randint(0, 600 if single else 300, (1,), generator=g)) for n in counts]
+    both(cuda_device, lengths, counts, 4, 2, D, 32, "bf16", seed=batch)
+
+
 def test_few_and_many_rows_in_one_call(cuda_device):
     """Sequences on both sides of the choice between the kernels, with empty ones between them."""
     counts = [1, 4, 5, 0, 17, 64, 65, 1, 2, 130, 3, 0]
