@@ -568,8 +568,9 @@ INTENT_B200_API int intent_b200_paged_kv_append_norm_bf16(INTENT_B200_VIEW3(q), 
  * Limits: T * HQ and W * PAGE up to 2^30, PAGES * HK * PAGE below 2^31 rows (any number of elements), HQ up to 4096.
  * scale_bits: the f32 factor of the scores (> 0; 0: 1 / sqrt(D)).  f32 statistics and sums.
  * workspace: at least ..._workspace_bytes(D, 0) bytes (paged_decode_attention: (D, 1)), 16-byte aligned, its first four zero
- * before the first launch.  Launches that may overlap need separate ones.  Bytes 0..3: INTENT_B200_ERR_TIMEOUT of a bounded
- * wait that gave up (..._workspace_status reads and clears it).  The same call gives the same bits.
+ * before the first launch.  Launches that may overlap need separate ones; host threads that call on one stream may share one.
+ * Bytes 0..3: INTENT_B200_ERR_TIMEOUT of a bounded wait that gave up (..._workspace_status reads and clears it).  The same call
+ * gives the same bits.
  * ------------------------------------------------------------------------ */
 INTENT_B200_API int intent_b200_paged_attention_f16(INTENT_B200_VIEW3(q), INTENT_B200_VIEW4(k_cache), INTENT_B200_VIEW4(v_cache),
                                                  INTENT_B200_VIEW2(page_table), INTENT_B200_VIEW1(query_offsets),

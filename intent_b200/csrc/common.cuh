@@ -26,6 +26,20 @@ inline int cuda_status(cudaError_t error) {
 // would also see sticky errors of unrelated work; cudaGetLastError clears ours).
 inline int launch_status() { return cuda_status(cudaGetLastError()); }
 
+// Held by an entry while it makes the launches of one call, if these hand data to one another through its workspace.  Host
+// threads on one stream share that stream's workspace: a launch of one call between two of another would leave the second its
+// own data.
+class WorkspaceTurn {
+ public:
+  explicit WorkspaceTurn(const void* workspace);
+  ~WorkspaceTurn();
+  WorkspaceTurn(const WorkspaceTurn&) = delete;
+  WorkspaceTurn& operator=(const WorkspaceTurn&) = delete;
+
+ private:
+  int place_;
+};
+
 // Dry-run observation of a launch: while a sink is installed on the calling thread (intent_b200_observe_begin),
 // the main compute kernels' launch sites fill it with what they WOULD launch - the kernel instance's resource
 // usage from cudaFuncGetAttributes and the launch plan - and launch nothing.

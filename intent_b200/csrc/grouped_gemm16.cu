@@ -530,6 +530,7 @@ int routed_expert_projection(View2 x, View1 offsets, View1 members, View3 w, Vie
     return INTENT_B200_ERR_LAYOUT;
   if (K % 8 != 0) return INTENT_B200_ERR_UNSUPPORTED;
   if (!workspace || !aligned16(workspace) || workspace_bytes < align256(R * K * 2)) return INTENT_B200_ERR_WORKSPACE;
+  const WorkspaceTurn turn(workspace);
   int status = gather<false>(x.p, tokens, K, static_cast<const int32_t*>(members.p), R, top_k, nullptr, 0, workspace,
                              stream);
   if (status != INTENT_B200_OK) return status;
@@ -562,6 +563,7 @@ int moe_expert_ffn(View2 x, View1 offsets, View1 members, View1 route_token, Vie
   void* hidden = static_cast<unsigned char*>(workspace) + gathered_bytes;
   const int32_t* member_ptr = static_cast<const int32_t*>(members.p);
   const int32_t* token_ptr = static_cast<const int32_t*>(route_token.p);
+  const WorkspaceTurn turn(workspace);
   int status = gather<true>(x.p, tokens, D, member_ptr, R, 1, token_ptr, NR, gathered, stream);
   if (status != INTENT_B200_OK) return status;
   Problem up{gathered, R, D, F, E, w1.p, static_cast<const int32_t*>(offsets.p), hidden, R, nullptr, nullptr, nullptr, 0};

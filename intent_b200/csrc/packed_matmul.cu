@@ -161,6 +161,7 @@ extern "C" int intent_b200_w4a8_packed_matmul(INTENT_B200_VIEW2(a0), INTENT_B200
   if (status != INTENT_B200_OK) return status;
   if (K == 0 || K % 32 != 0 || M % 16 != 0) return INTENT_B200_ERR_UNSUPPORTED;
   if (!workspace || !aligned16(workspace) || workspace_bytes < align256(N * K)) return INTENT_B200_ERR_WORKSPACE;
+  const WorkspaceTurn turn(workspace);
   if (!observe_sink()) {      // (the contraction behind the expansion is what gets observed)
     const int64_t vectors = N * P / 16;
     status = cuda_status(launch_programmatic(expand_w4_kernel, grid_for(vectors, 256), 256, 0, stream, 1,
@@ -193,6 +194,7 @@ extern "C" int intent_b200_bitnet_int2_matmul(INTENT_B200_VIEW2(a0), INTENT_B200
     return status;
   }
   if (!workspace || !aligned16(workspace) || workspace_bytes < align256(N * K)) return INTENT_B200_ERR_WORKSPACE;
+  const WorkspaceTurn turn(workspace);
   const int64_t words = N * P / 4;
   status = cuda_status(launch_programmatic(expand_int2_kernel, grid_for(words, 256), 256, 0, stream, 1,
                                            static_cast<const uint32_t*>(a1), static_cast<uint4*>(workspace), words));
@@ -216,6 +218,7 @@ extern "C" int intent_b200_dequant_bf16_fp4_matmul(INTENT_B200_VIEW2(a0), INTENT
   const int64_t decoded_bytes = align256(N * K * 2);
   if (!workspace || !aligned16(workspace) || workspace_bytes < decoded_bytes + 256) return INTENT_B200_ERR_WORKSPACE;
   int32_t* row_span = reinterpret_cast<int32_t*>(static_cast<unsigned char*>(workspace) + decoded_bytes);
+  const WorkspaceTurn turn(workspace);
   const int64_t words = N * P / 4;
   status = cuda_status(launch_programmatic(expand_fp4_kernel, grid_for(words, 256), 256, 0, stream, 1,
                                            static_cast<const uint32_t*>(a1), static_cast<uint4*>(workspace), words, row_span,

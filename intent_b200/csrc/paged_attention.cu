@@ -79,6 +79,7 @@ int attend(const View3& q, const View4& k_cache, const View4& v_cache, const Vie
   // beside prompts are not multiplied as tiles of 256 (20 beside 4 chunks of up to 500 tokens: 169 -> 160 us, with tiles of
   // eight 144).  In a call of few sequences the two launches cost more than that (3 prompts: 120 -> 128 us).
   constexpr int FEW = 16, MANY = 8;
+  const WorkspaceTurn turn(workspace);
   const int64_t rows = tokens * p.group;
   p.few = std::numeric_limits<int>::max();
   if (!offsets || !paged_chunk_takes(p) || rows <= (dim == 64 ? 2 * FEW : FEW) * batch)

@@ -145,6 +145,7 @@ extern "C" int intent_b200_quantized_projection(INTENT_B200_VIEW3(a0), INTENT_B2
   if (N > (1 << 30) || G > (1 << 20)) return INTENT_B200_ERR_UNSUPPORTED;
   if (G > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < align256(G * kQ8Bytes)))
     return INTENT_B200_ERR_WORKSPACE;
+  const WorkspaceTurn turn(workspace);
   if (G > 0) {
     const int status = cuda_status(launch_programmatic(q8_k_quantize_kernel, int((G + 7) / 8), 256, 0, stream, 1,
                                                        static_cast<const float*>(a1), int(G),
