@@ -268,7 +268,7 @@ __device__ __forceinline__ void weigh(const uint32_t (&v)[32], uint64_t scale, u
 template <int SLOTS>
 struct Shared {
   uint64_t q_full, q_empty, kv_full[SLOTS], kv_empty[SLOTS], s_full[2], p_full[2][2], o_full[2], vote_full[2], part_full[4],
-      part_empty[4];
+      part_empty[4], products_over;
   long long warp_sums[THREADS / 32];
   Part parts[4];
   Start start;
@@ -300,7 +300,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                  kv_full = bars + offsetof(Shared<SLOTS>, kv_full), kv_empty = bars + offsetof(Shared<SLOTS>, kv_empty),
                  s_full = bars + offsetof(Shared<SLOTS>, s_full), p_full = bars + offsetof(Shared<SLOTS>, p_full),
                  o_full = bars + offsetof(Shared<SLOTS>, o_full), vote_full = bars + offsetof(Shared<SLOTS>, vote_full),
-                 part_full = bars + offsetof(Shared<SLOTS>, part_full), part_empty = bars + offsetof(Shared<SLOTS>, part_empty);
+                 part_full = bars + offsetof(Shared<SLOTS>, part_full), part_empty = bars + offsetof(Shared<SLOTS>, part_empty),
+                 products_over = bars + offsetof(Shared<SLOTS>, products_over);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -321,6 +322,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       mbar_init(vote_full + 8 * i, 4);
       sh.vote[i] = 0;
     }
+    mbar_init(products_over, 1);
     for (int i = 0; i < 4; ++i) {
       mbar_init(part_full + 8 * i, 1);
       mbar_init(part_empty + 8 * i, 9);      // the warps of both halves and the products'
@@ -405,7 +407,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       const int rows = min(1 << p.page_shift, STEP);                   // of a box
       const int boxes = STEP / rows;                                   // of 64 elements of a step
       const int cache_rows = (p.pages * p.k_heads) << p.page_shift;
-      uint32_t u = 0, parts = 0;
+      uint32_t u = 0, parts = 0, odd = 0;                              // odd: keys asked for whose values were given up on
       walk(p, at_first, begin, end, [&](const Sequence& s, int b, int head, int tile, int step, int steps, int all, int at) {
         const uint32_t place = parts & 3;
         ok = mbar_wait_warp(part_empty + 8 * place, (parts / 4 & 1) ^ 1) && mbar_wait_warp(q_empty, (parts & 1) ^ 1);
@@ -438,7 +440,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
           for (int operand = 0; operand < 2; ++operand) {
             const uint32_t slot = (2 * u + operand) % SLOTS, turn = (2 * u + operand) / SLOTS;
             ok = mbar_wait_warp(kv_empty + 8 * slot, (turn & 1) ^ 1);
-            if (!ok) return false;
+            if (!ok) {
+              odd = operand;
+              return false;
+            }
             if (lane == 0) {
               if (operand == 0) sh.missing[u & 7] = missing;
               mbar_expect_tx(kv_full + 8 * slot, R::OPERAND);
@@ -457,9 +462,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         sh.parts[parts & 3].steps = 0;
         mbar_arrive(part_full + 8 * (parts & 3));
       }
-      if (!ok)   // (nothing may be on its way to a CTA that is gone)
-        for (int i = 0; i < SLOTS; ++i)
-          for (int parity = 0; parity < 2; ++parity) mbar_wait_warp(kv_full + 8 * i, parity, 64);
+      // (also where another warp gave up: no load may be on its way to a CTA that is gone)
+      if (parts > 0) mbar_wait_warp(q_full, (parts - 1) & 1);
+      const uint32_t loads = 2 * u + odd;
+      for (uint32_t i = loads > SLOTS ? loads - SLOTS : 0; i < loads; ++i) mbar_wait_warp(kv_full + 8 * (i % SLOTS), i / SLOTS & 1);
     } else if (warp == MMA_WARP) {
       // ------------------------------ products ------------------------------------
       constexpr uint32_t FORMAT = std::is_same<T, __half>::value ? 0 : 1;
@@ -555,6 +561,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         if (ok) finish(h);
+      // (also where a warp gave up: no product may be under way in tensor memory that is given back)
+      if (issue) umma_commit(products_over);
+      __syncwarp();
+      mbar_wait_warp(products_over, 0);
     }
   } else {
     // ------------------------------ weights and results --------------------------

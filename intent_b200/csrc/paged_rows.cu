@@ -489,7 +489,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       }
       __syncwarp();                      // every lane is done with the slot
     }
-    if (loading < end) ask();
+    if (ok && loading < end) ask();      // (a slot that was given up on may still be on its way)
 
     const bool last_step = work.step + 1 == work.s.steps;
     next = at + work.distance();
@@ -578,8 +578,10 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     }
   }
   if (!ok) {
-    // (nothing may be on its way to a CTA that is gone)
-    for (int s = 0; s < R::STAGES; ++s) mbar_wait_warp(full + 8 * s, (parity >> s) & 1, 64);
+    // Nothing may be on its way to a CTA that is gone.  (Which phase a slot is in has not been counted since the wait that gave
+    // up: of the two parities the wait for one is for the current phase, the other is over.)
+    for (int s = 0; s < R::STAGES; ++s)
+      for (int of_phase = 0; of_phase < 2; ++of_phase) mbar_wait_warp(full + 8 * s, of_phase, 64);
     if (lane == 0) atomicExch(p.status, INTENT_B200_ERR_TIMEOUT);
   }
 }
