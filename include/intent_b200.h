@@ -569,8 +569,9 @@ INTENT_B200_API int intent_b200_paged_kv_append_norm_bf16(INTENT_B200_VIEW3(q), 
  * scale_bits: the f32 factor of the scores (> 0; 0: 1 / sqrt(D)).  f32 statistics and sums.
  * workspace: at least ..._workspace_bytes(D, 0) bytes (paged_decode_attention: (D, 1)), 16-byte aligned, its first four zero
  * before the first launch.  Launches that may overlap need separate ones; host threads that call on one stream may share one.
- * Bytes 0..3: INTENT_B200_ERR_TIMEOUT of a bounded wait that gave up (..._workspace_status reads and clears it).  The same call
- * gives the same bits.
+ * Bytes 0..3: INTENT_B200_ERR_TIMEOUT of a bounded wait that gave up, INTENT_B200_ERR_SHAPE where a multiprocessor would
+ * have 2^30 or more steps of 128 tokens to go through (many minutes; nothing is written then); ..._workspace_status reads and
+ * clears it.  The same call gives the same bits.
  * ------------------------------------------------------------------------ */
 INTENT_B200_API int intent_b200_paged_attention_f16(INTENT_B200_VIEW3(q), INTENT_B200_VIEW4(k_cache), INTENT_B200_VIEW4(v_cache),
                                                  INTENT_B200_VIEW2(page_table), INTENT_B200_VIEW1(query_offsets),

@@ -47,6 +47,18 @@ __device__ __forceinline__ TokenSpan span_of(const PagedParams& p, int b) {
   return {begin, min(max(__ldg(p.offsets + b + 1), begin), p.tokens) - begin};
 }
 
+// Places of a CTA, of a line of so many; negative where a CTA has no count for them.  (The line is in 64 bits: 2^20 new tokens of 64
+// heads on 8 are 2^30 places.  Within a CTA places are counted from its first one, in 32.)
+__device__ __forceinline__ int share_of(long long line) {
+  constexpr int MOST = 0x3fffffff;
+  if (line <= MOST) return (int(line) + int(gridDim.x) - 1) / int(gridDim.x);
+  const long long share = (line + gridDim.x - 1) / gridDim.x;
+  return share <= MOST ? int(share) : -1;
+}
+__device__ __forceinline__ int divide(long long a, long long b) {     // for quotients of 31 bits
+  return (a | b) >> 31 == 0 ? int(unsigned(a) / unsigned(b)) : int(a / b);
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -132,14 +132,14 @@ __device__ __forceinline__ long long places_before(const PagedParams& p, const S
   return (long long)sum + (long long)BEGIN * j;
 }
 
-// Goes through the parts of tiles among the places [at, end); visit(sequence, head, tile, step, steps, all, at) gets the part's
+// Goes through the parts of tiles among a CTA's places [0, end); visit(sequence, head, tile, step, steps, all, at) gets the part's
 // first step in its tile, how many it has, how many the tile has and the first one's place, and returns whether to go on.
 struct Start {
   int b, head, tile, place;
 };
 template <typename Visit>
-__device__ __forceinline__ void walk(const PagedParams& p, const Start& from, int at, int end, Visit visit) {
-  int b = from.b, head = from.head, tile = from.tile, place = from.place;
+__device__ __forceinline__ void walk(const PagedParams& p, const Start& from, int end, Visit visit) {
+  int b = from.b, head = from.head, tile = from.tile, place = from.place, at = 0;
   Sequence s = sequence_of(p, b);
   while (true) {
     const int all = steps_of(p, s, tile), places = min(BEGIN + all - place, end - at);
@@ -164,7 +164,7 @@ struct Part {
   int row, head, tokens;   // first row of q, key head, new tokens from there on in the sequence
   int position;            // of the first of them
   int first, steps;        // steps of 128 tokens
-  int step, all, at;       // the first one's number in the tile, the tile's steps, the first one's place on the line
+  int step, all, at;       // the first one's number in the tile, the tile's steps, the first one's place among the CTA's
                            // (steps = 0: there are no more)
 };
 
@@ -271,7 +271,8 @@ struct Shared {
       part_empty[4], products_over;
   long long warp_sums[THREADS / 32];
   Part parts[4];
-  Start start;
+  long long start, start_head;             // this CTA's first place, counted in the sequence; places of a key head of it
+  int start_sequence;
   volatile uint32_t tmem;
   volatile int skip[2];                    // this half's step has been added to O by its threads
   volatile uint32_t vote[2];               // step + 1 in which a warp of the half asked for that
@@ -334,10 +335,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
 
   // ---- this CTA's part of the line
   const int per_thread = (p.batch + THREADS - 1) / THREADS, mine = tid * per_thread;
-  long long sum = 0;
+  long long sum = 0, each = 0;
   for (int b = mine; b < min(mine + per_thread, p.batch); ++b) {
     const Sequence s = sequence_of(p, b);
-    sum += places_before(p, s, s.tiles) * p.k_heads;
+    each = places_before(p, s, s.tiles);
+    sum += each * p.k_heads;
   }
   long long before = sum;
 #pragma unroll
@@ -354,26 +356,26 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     line += sh.warp_sums[w];
   }
   before -= sum;
-  const bool sensible = line <= 0x3fffffff;                            // (only offsets that make no sense name more)
-  const int total = sensible ? int(line) : 0, share = (total + int(gridDim.x) - 1) / int(gridDim.x);
-  const int cta = blockIdx.x, begin = min(cta * share, total), end = min(begin + share, total);
-  if (begin < end && begin >= before && begin < before + sum) {
+  const int share = share_of(line), cta = blockIdx.x;
+  const long long begin = (long long)cta * share;
+  const int end = share > 0 && begin < line ? int(min((long long)share, line - begin)) : 0;   // of this CTA's places, from its first on
+  if (end > 0 && begin >= before && begin < before + sum) {
     int b = mine;
-    long long at = before, steps = sum;
+    long long at = before, of_head = each;
     for (; per_thread > 1; ++b) {
       const Sequence s = sequence_of(p, b);
-      steps = places_before(p, s, s.tiles) * p.k_heads;
-      if (begin < at + steps || b + 1 >= min(mine + per_thread, p.batch)) break;
-      at += steps;
+      of_head = places_before(p, s, s.tiles);
+      if (begin < at + of_head * p.k_heads || b + 1 >= min(mine + per_thread, p.batch)) break;
+      at += of_head * p.k_heads;
     }
-    sh.start.b = b;
-    sh.start.place = begin - int(at);                                   // in the sequence
-    sh.start.head = max(int(steps) / p.k_heads, 1);                    // places of a key head
+    sh.start_sequence = b;
+    sh.start = begin - at;
+    sh.start_head = of_head;
   }
   JoinEntry* entry = reinterpret_cast<JoinEntry*>(p.joins) + cta;
   if (tid == 0) {
     entry->last_cta = -1;
-    if (!sensible) atomicExch(p.status, INTENT_B200_ERR_SHAPE);
+    if (share < 0) atomicExch(p.status, INTENT_B200_ERR_SHAPE);
   }
   tcgen05_fence_before();
   __syncthreads();
@@ -382,18 +384,18 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   const uint32_t tmem_s = tmem, tmem_o = tmem + 2 * STEP;              // of both halves, 128 columns apart
   bool ok = true;
 
-  if (begin >= end) {
+  if (end == 0) {
     // nothing to do
   } else if (warp >= MMA_WARP) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGISTERS));
     if (warp == LOAD_WARP) {
       // ------------------------------ loads ---------------------------------------
-      Start at_first = sh.start;
+      Start at_first;
+      at_first.b = sh.start_sequence;
       {
         const Sequence s = sequence_of(p, at_first.b);
-        const int per_head = at_first.head;
-        at_first.head = at_first.place / per_head;
-        const int place = at_first.place - at_first.head * per_head;
+        at_first.head = divide(sh.start, sh.start_head);
+        const long long place = sh.start - at_first.head * sh.start_head;
         int low = 0, high = s.tiles;                                   // places_before(low) <= place < places_before(high)
         while (high - low > 1) {
           const int stride = (high - low + 31) / 32, j = low + lane * stride;
@@ -402,13 +404,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
           high = min(low + stride, high);
         }
         at_first.tile = low;
-        at_first.place = place - int(places_before(p, s, low));
+        at_first.place = int(place - places_before(p, s, low));
       }
       const int rows = min(1 << p.page_shift, STEP);                   // of a box
       const int boxes = STEP / rows;                                   // of 64 elements of a step
       const int cache_rows = (p.pages * p.k_heads) << p.page_shift;
       uint32_t u = 0, parts = 0, odd = 0;                              // odd: keys asked for whose values were given up on
-      walk(p, at_first, begin, end, [&](const Sequence& s, int b, int head, int tile, int step, int steps, int all, int at) {
+      walk(p, at_first, end, [&](const Sequence& s, int b, int head, int tile, int step, int steps, int all, int at) {
         const uint32_t place = parts & 3;
         ok = mbar_wait_warp(part_empty + 8 * place, (parts / 4 & 1) ^ 1) && mbar_wait_warp(q_empty, (parts & 1) ^ 1);
         if (!ok) return false;
@@ -754,15 +756,15 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       __syncwarp();
       if (lane == 0) mbar_arrive(part_empty + 8 * place);
       const bool whole = steps == all;
-      const int first_cta = tile_at / share;                           // where the tile begins
-      if (tid == 0 && !whole && cta == first_cta) {
+      const bool begins = tile_at >= 0;                                // the tile, in this CTA
+      if (tid == 0 && !whole && begins) {
         entry->row = tile_row;
         entry->head = head;
         entry->tokens = tokens;
-        entry->last_cta = (tile_at + all - 1) / share;
+        entry->last_cta = cta + (tile_at + all - 1) / share;
       }
       const float inverse = weight_sum == 0.f ? 0.f : 1.f / weight_sum;
-      float* to_part = p.parts + size_t(2 * cta + (cta == first_cta)) * (2 * HALF_ROWS * (D + 2));
+      float* to_part = p.parts + size_t(2 * cta + begins) * (2 * HALF_ROWS * (D + 2));
       uint16_t* to = p.out + (int64_t(tile_row + h * p.half_tokens + row_token) * p.q_heads + head * p.group +
                               (row - row_token * p.group)) * D;
 #pragma unroll 1

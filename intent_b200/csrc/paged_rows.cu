@@ -156,7 +156,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   float* join = reinterpret_cast<float*>(base_ptr + R::BYTES);          // [JOINS][WARPS][ROWS][PITCH]
   float* join_max = join + JOINS * WARPS * ROWS * PITCH;                // [JOINS][WARPS][ROWS]
   float* join_sum = join_max + JOINS * WARPS * ROWS;
-  int* shared = reinterpret_cast<int*>(join_sum + JOINS * WARPS * ROWS);   // [4], then the warps' sums in 64 bits
+  int* shared = reinterpret_cast<int*>(join_sum + JOINS * WARPS * ROWS);   // a number, a 64-bit one, the warps' 64-bit sums
   long long* warp_sums = reinterpret_cast<long long*>(shared + 4);
   const uint32_t bars = smem_u32(warp_sums + WARPS);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -189,37 +189,39 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     line += warp_sums[w];
   }
   before -= sum;
-  const bool sensible = line <= 0x3fffffff;              // (only offsets that make no sense name more)
-  if (!sensible && tid == 0) atomicExch(p.status, INTENT_B200_ERR_SHAPE);
-  const int total = sensible ? int(line) : 0;
-  const int share = (total + int(gridDim.x) - 1) / int(gridDim.x);     // places of a CTA
-  const int cta = blockIdx.x;
+  const int share = share_of(line), cta = blockIdx.x;
   JoinEntry* entry = reinterpret_cast<JoinEntry*>(p.joins) + cta;
-  if (tid == 0) entry->last_cta = -1;
-  const int begin = min(cta * share, total), end = min(begin + share, total);
-  if (begin >= end) return;
+  if (tid == 0) {
+    entry->last_cta = -1;
+    if (share < 0) atomicExch(p.status, INTENT_B200_ERR_SHAPE);
+  }
+  const long long begin = (long long)cta * share;
+  if (share <= 0 || begin >= line) return;
+  const int end = int(min((long long)share, line - begin));            // of this CTA's places, counted from its first one
   if (begin >= before && begin < before + sum) {
-    int b = mine, at = int(before);
+    int b = mine;
+    long long at = before;
     for (;; ++b) {
       const Sequence s = sequence_of<STEP>(p, b, ROWS);
-      const int places = int(places_of<BEGIN>(p, s));
+      const long long places = places_of<BEGIN>(p, s);
       if (begin < at + places || b + 1 >= min(mine + per_thread, p.batch)) break;
       at += places;
     }
     shared[0] = b;
-    shared[1] = at;
+    *reinterpret_cast<long long*>(shared + 2) = begin - at;            // place in the sequence
   }
   __syncthreads();
   Walk<STEP, BEGIN> load;
   load.b = shared[0];
   load.s = sequence_of<STEP>(p, load.b, ROWS);
   {
-    const int item = (begin - shared[1]) / (load.s.steps + BEGIN);
-    load.step = (begin - shared[1]) - item * (load.s.steps + BEGIN) - BEGIN;
+    const long long place = *reinterpret_cast<const long long*>(shared + 2);
+    const int item = divide(place, load.s.steps + BEGIN);
+    load.step = int(place - (long long)item * (load.s.steps + BEGIN)) - BEGIN;
     load.head = item / load.s.tiles;
     load.tile = item - load.head * load.s.tiles;
   }
-  const int first_place = begin + max(-load.step, 0);    // of a step
+  const int first_place = max(-load.step, 0);            // of a step
   if (first_place >= end) return;
   load.step = max(load.step, 0);
   Walk<STEP, BEGIN> work = load;
@@ -525,15 +527,14 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       }
       const int tile_row = work.tile * ROWS, rows = min(ROWS, work.s.rows - tile_row), head = work.head;
       const int first_row = work.s.first_row;
-      const int item_begin = at - work.step, item_end = item_begin + work.s.steps;   // on the line
+      const int item_begin = at - work.step, item_end = item_begin + work.s.steps;   // the tile's places, maybe of other CTAs
       if (next < end) {
         work.advance(p, ROWS);
         begin_tile();                    // (its queries are on their way while this tile is put together)
       }
       __syncthreads();
-      const int first_cta = item_begin / share, last_cta = (item_end - 1) / share;
-      const bool whole = first_cta == last_cta;
-      float* part = p.parts + size_t(2 * cta + (cta == first_cta)) * (ROWS * (D + 2));
+      const bool begins = item_begin >= 0, whole = begins && item_end <= share;
+      float* part = p.parts + size_t(2 * cta + begins) * (ROWS * (D + 2));
       auto place = [&](int r) {
         const int token = (tile_row + r) / p.group, of_group = tile_row + r - token * p.group;
         return p.out + (int64_t(first_row + token) * p.q_heads + head * p.group + of_group) * D;
@@ -567,12 +568,12 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           }
         }
       }
-      if (tid == 0 && !whole && cta == first_cta) {
+      if (tid == 0 && !whole && begins) {
         entry->row = first_row;
         entry->head = head;
         entry->tile_row = tile_row;
         entry->rows = rows;
-        entry->last_cta = last_cta;
+        entry->last_cta = cta + (item_end - 1) / share;
       }
       if (JOINS == 1) __syncthreads();
     }
