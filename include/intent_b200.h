@@ -563,7 +563,7 @@ INTENT_B200_API int intent_b200_paged_kv_append_norm_bf16(INTENT_B200_VIEW3(q), 
  *   query_offsets [B + 1] i32          rows of q of sequence b (paged_attention); row b (paged_decode_attention, T = B)
  *   kv_lengths [B] i32                 tokens of sequence b in the cache, the new ones among them
  * Query i of n sees the tokens j <= kv_length - n + i, with window > 0 only the last `window` of them.  No such token: a row
- * of zeros.  Tokens behind kv_length, ahead of the window, in pages that the table does not name or whose number lies
+ * of zeros; a row all of whose scores are -infinity, as one with a score of +infinity, is NaN.  Tokens behind kv_length, ahead of the window, in pages that the table does not name or whose number lies
  * outside the cache are not read, whatever the memory there holds.  Rows of q that no sequence has are left alone.
  * Limits: T * HQ and W * PAGE up to 2^30, PAGES * HK * PAGE below 2^31 rows (any number of elements), HQ up to 4096.
  * scale_bits: the f32 factor of the scores (> 0; 0: 1 / sqrt(D)).  f32 statistics and sums.

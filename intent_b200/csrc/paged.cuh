@@ -59,6 +59,20 @@ __device__ __forceinline__ int divide(long long a, long long b) {     // for quo
   return (a | b) >> 31 == 0 ? int(unsigned(a) / unsigned(b)) : int(a / b);
 }
 
+// The factor of a row whose weights add up to nothing: zero where it sees no token; where it does, all its scores are -infinity,
+// and their softmax is no number.  `row`: of q.
+__device__ __forceinline__ float of_nothing(const PagedParams& p, int b, int row) {
+  const TokenSpan span = span_of(p, b);
+  const int position = min(max(__ldg(p.lengths + b), 0), p.capacity) - span.count + row - span.begin;
+  const int from = p.window > 0 ? max(position - p.window + 1, 0) : 0;
+#pragma unroll 1
+  for (int i = from >> p.page_shift; i <= position >> p.page_shift; ++i) {
+    const int page = __ldg(p.page_table + int64_t(b) * p.table_width + i);
+    if (page >= 0 && page < p.pages) return __int_as_float(0x7fc00000);
+  }
+  return 0.f;
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

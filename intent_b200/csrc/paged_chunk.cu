@@ -162,6 +162,7 @@ __device__ __forceinline__ void walk(const PagedParams& p, const Start& from, in
 // A CTA's share of a tile, as the loading warp leaves it to the others
 struct Part {
   int row, head, tokens;   // first row of q, key head, new tokens from there on in the sequence
+  int sequence;
   int position;            // of the first of them
   int first, steps;        // steps of 128 tokens
   int step, all, at;       // the first one's number in the tile, the tile's steps, the first one's place among the CTA's
@@ -282,7 +283,9 @@ struct Shared {
 struct JoinEntry {
   int last_cta;            // of the tile that begins in this CTA and ends in another; -1: there is none
   int row, head, tokens;   // first row of q, key head, tokens from there on in the sequence
+  int sequence;
 };
+static_assert(sizeof(JoinEntry) <= kPagedEntry, "room ahead of the parts");
 
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -419,6 +422,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         if (lane == 0) {
           Part& part = sh.parts[place];
           part.row = s.first_row + from, part.head = head, part.tokens = s.count - from, part.position = position;
+          part.sequence = b;
           part.first = first, part.steps = steps, part.step = step, part.all = all, part.at = at;
           mbar_arrive(part_full + 8 * place);
           mbar_expect_tx(q_full, uint32_t(p.half_tokens * p.group * 128 * BOXES * halves));
@@ -752,7 +756,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         if (!ok) break;
         tcgen05_fence_after();
       }
-      const int all = part.all, tile_at = part.at - part.step, head = part.head, tile_row = part.row;
+      const int all = part.all, tile_at = part.at - part.step, head = part.head, tile_row = part.row, sequence = part.sequence;
       __syncwarp();
       if (lane == 0) mbar_arrive(part_empty + 8 * place);
       const bool whole = steps == all;
@@ -761,9 +765,12 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         entry->row = tile_row;
         entry->head = head;
         entry->tokens = tokens;
+        entry->sequence = sequence;
         entry->last_cta = cta + (tile_at + all - 1) / share;
       }
-      const float inverse = weight_sum == 0.f ? 0.f : 1.f / weight_sum;
+      float inverse = 0.f;
+      if (whole && real)
+        inverse = weight_sum == 0.f ? of_nothing(p, sequence, tile_row + h * p.half_tokens + row_token) : 1.f / weight_sum;
       float* to_part = p.parts + size_t(2 * cta + begins) * (2 * HALF_ROWS * (D + 2));
       uint16_t* to = p.out + (int64_t(tile_row + h * p.half_tokens + row_token) * p.q_heads + head * p.group +
                               (row - row_token * p.group)) * D;
@@ -859,7 +866,7 @@ __global__ void __launch_bounds__(4 * D, 1024 / (4 * D)) paged_join_kernel(const
       }
     }
   }
-  const float inverse = l == 0.f ? 0.f : 1.f / l;
+  const float inverse = l == 0.f ? of_nothing(p, entry.sequence, entry.row + token) : 1.f / l;
   uint32_t w[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) w[e] = Elem<T>::pack2(x[2 * e] * inverse, x[2 * e + 1] * inverse);

@@ -2,7 +2,7 @@
 //
 // Program (paged_decode_attention; paged_attention for chunks): query row x at position p of a sequence with n new tokens and
 // L tokens in the cache (p = L - n + i), over the tokens j with max(0, p - W + 1) <= j <= p (W = 0: no window)
-//   o = sum_j softmax_j(scale * x . k_j) * v_j,     zero where there is no such token
+//   o = sum_j softmax_j(scale * x . k_j) * v_j,     zero where there is no such token, NaN where all scores are -infinity
 // Token j of sequence b lies in page page_table[b, j / PAGE]; the tokens of a page number outside the cache are not seen.
 // All statistics and sums are in f32; the weights of one product with V are rounded to the 16-bit type (relative to the
 // running maximum, so at most 1), as the tensor core takes them.
@@ -137,7 +137,9 @@ struct JoinEntry {
   int last_cta;            // of the tile that begins in this CTA and ends in another; -1: there is none
   int row, head;           // first row of q of its sequence, key head
   int tile_row, rows;      // its first row among the sequence's, how many it has
+  int sequence;
 };
+static_assert(sizeof(JoinEntry) <= kPagedEntry, "room ahead of the parts");
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(32 * Ring<D>::WARPS, 1)
@@ -526,7 +528,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         }
       }
       const int tile_row = work.tile * ROWS, rows = min(ROWS, work.s.rows - tile_row), head = work.head;
-      const int first_row = work.s.first_row;
+      const int first_row = work.s.first_row, sequence = work.b;
       const int item_begin = at - work.step, item_end = item_begin + work.s.steps;   // the tile's places, maybe of other CTAs
       if (next < end) {
         work.advance(p, ROWS);
@@ -554,7 +556,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           for (int e = 0; e < 8; ++e) x[e] = fmaf(from[e], f, x[e]);
         }
         if (whole) {
-          const float inverse = l == 0.f ? 0.f : 1.f / l;
+          const float inverse = l == 0.f ? of_nothing(p, sequence, first_row + (tile_row + r) / p.group) : 1.f / l;
           *reinterpret_cast<uint4*>(place(r) + 8 * c) =
               make_uint4(Elem<T>::pack2(x[0] * inverse, x[1] * inverse), Elem<T>::pack2(x[2] * inverse, x[3] * inverse),
                          Elem<T>::pack2(x[4] * inverse, x[5] * inverse), Elem<T>::pack2(x[6] * inverse, x[7] * inverse));
@@ -573,6 +575,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         entry->head = head;
         entry->tile_row = tile_row;
         entry->rows = rows;
+        entry->sequence = sequence;
         entry->last_cta = cta + (item_end - 1) / share;
       }
       if (JOINS == 1) __syncthreads();
@@ -626,8 +629,8 @@ __global__ void __launch_bounds__(ROWS * D / 4) paged_rows_join_kernel(const Pag
       x[0] = fmaf(y[v].x, f, x[0]), x[1] = fmaf(y[v].y, f, x[1]), x[2] = fmaf(y[v].z, f, x[2]), x[3] = fmaf(y[v].w, f, x[3]);
     }
   }
-  const float inverse = l == 0.f ? 0.f : 1.f / l;
   const int token = (entry.tile_row + r) / p.group, of_group = entry.tile_row + r - token * p.group;
+  const float inverse = l == 0.f ? of_nothing(p, entry.sequence, entry.row + token) : 1.f / l;
   *reinterpret_cast<uint2*>(p.out + (int64_t(entry.row + token) * p.q_heads + entry.head * p.group + of_group) * D + 4 * c) =
       make_uint2(Elem<T>::pack2(x[0] * inverse, x[1] * inverse), Elem<T>::pack2(x[2] * inverse, x[3] * inverse));
 }
