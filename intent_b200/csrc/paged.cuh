@@ -8,10 +8,11 @@
 namespace ib200 {
 
 constexpr int kPagedCtas = 160;            // most CTAs of a launch
-constexpr int64_t kPagedHeader = 4096;     // bytes of the workspace ahead of the parts: status word
-constexpr int64_t kPagedJoins = 64;        // and, from here on, the tile that a CTA leaves to others
-constexpr int64_t kPagedEntry = 24;        // bytes of its description, at most
-static_assert(kPagedJoins + kPagedEntry * kPagedCtas <= kPagedHeader, "room ahead of the parts");
+// The workspace: status word; descriptions of the tile that each CTA leaves to others, those of the rows kernel, then those of the
+// chunk kernel; parts of the rows kernel, then those of the chunk kernel
+constexpr int64_t kPagedEntry = 24;        // bytes of a description, at most
+constexpr int64_t kPagedRowsJoins = 64, kPagedChunkJoins = kPagedRowsJoins + kPagedEntry * kPagedCtas, kPagedHeader = 8192;
+static_assert(kPagedChunkJoins + kPagedEntry * kPagedCtas <= kPagedHeader, "room ahead of the parts");
 
 struct PagedParams {
   const uint16_t* q;                 // [T, HQ, D] at these strides (elements)
@@ -25,7 +26,7 @@ struct PagedParams {
   int window;                        // tokens that a query sees, its own among them; 0 = all
   float scale;                       // of the scores, times log2(e)
   int* status;                       // head of the workspace
-  void* joins;
+  void* joins;                       // a kernel's own
   float* parts;
   int half_tokens;                   // chunks: tokens of half a tile
   int few;                           // rows of queries per key head up to which a sequence is the rows kernel's; those with more
@@ -89,16 +90,22 @@ __device__ __forceinline__ uint32_t add_no_numbers(uint32_t x, uint32_t sum) {
 
 #endif  // __CUDACC__
 
-// few rows per sequence, in tiles of eight (`narrow`) or sixteen (paged_rows.cu)
-int64_t paged_rows_workspace_bytes(int64_t dim);
+// few rows per sequence, in tiles of so many (8 or 16; paged_rows.cu)
+int64_t paged_rows_parts_bytes(int64_t dim);
 template <typename T>
-int paged_rows(const PagedParams& p, int64_t dim, bool narrow, const void* k_cache, const void* v_cache, int sms,
+int paged_rows(const PagedParams& p, int64_t dim, int tile_rows, const void* k_cache, const void* v_cache, int grid,
                cudaStream_t stream);
 
 // chunks (paged_chunk.cu)
-int64_t paged_chunk_workspace_bytes(int64_t dim);
+int64_t paged_chunk_parts_bytes(int64_t dim);
 bool paged_chunk_takes(const PagedParams& p);
+int paged_chunk_half_tokens(const PagedParams& p);
 template <typename T>
-int paged_chunk(PagedParams p, int64_t dim, const void* k_cache, const void* v_cache, int sms, cudaStream_t stream);
+int paged_chunk(const PagedParams& p, int64_t dim, const void* k_cache, const void* v_cache, int grid, cudaStream_t stream);
+
+// the parts that paged_rows (tile_rows > 0) and paged_chunk (`chunks`) leave (paged_join.cu)
+template <typename T>
+int paged_join(const PagedParams& rows, int tile_rows, const PagedParams& chunk, bool chunks, int64_t dim, int grid,
+               cudaStream_t stream);
 
 }  // namespace ib200

@@ -1,4 +1,5 @@
 // Entries of attention over a paged cache: argument checks and the choice of the kernel.
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <limits>
@@ -68,37 +69,52 @@ int attend(const View3& q, const View4& k_cache, const View4& v_cache, const Vie
   p.window = window < p.capacity ? window : 0;   // (a query that sees as many tokens as there may be sees all)
   p.scale = scale * 1.44269504f;         // log2(e): the exponentials are powers of two
   p.status = static_cast<int*>(workspace);
-  p.joins = static_cast<unsigned char*>(workspace) + kPagedJoins;
+  p.joins = static_cast<unsigned char*>(workspace) + kPagedRowsJoins;
   p.parts = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + kPagedHeader);
-  // Up to sixteen rows of queries per sequence and key head on average are one tile of the rows kernel, which is then bound by
-  // HBM; with more it reads and multiplies the cache once for every sixteen.  us for 64 sequences of up to 4000 tokens, 32 heads
-  // of 128 on 8 key heads, 1 / 4 / 8 / 16 new tokens each: rows 98 / 103 / 189 / 345, chunk 146 / 146 / 147 / 146; one sequence
-  // of 8000: rows 14 / 17 / 20 / 30, chunk 24 throughout.  With heads of 64 two tiles still are (64 heads on 8, 4 / 8 new tokens:
-  // rows 105 / 185, chunk 128 / 130).
-  // In a call of more rows and many sequences, those of one tile still are the rows kernel's, so that tokens that are decoded
-  // beside prompts are not multiplied as tiles of 256 (20 beside 4 chunks of up to 500 tokens: 169 -> 160 us, with tiles of
-  // eight 144).  In a call of few sequences the two launches cost more than that (3 prompts: 120 -> 128 us).
-  constexpr int FEW = 16, MANY = 8;
+  // Which kernel takes a sequence goes by its rows (new tokens x query heads of a key head).  Those of one tile, up to sixteen
+  // rows, are bound by HBM in the rows kernel; with more rows it reads and multiplies the cache once for every tile.  us for 64
+  // sequences of up to 4000 tokens, 32 heads of 128 on 8 key heads, 1 / 4 / 8 / 16 new tokens each: rows 98 / 103 / 189 / 345, chunk
+  // 146 / 146 / 147 / 146; one sequence of 8000: rows 14 / 17 / 20 / 30, chunk 24 throughout.  With heads of 64 two tiles still are
+  // (64 heads on 8, 4 / 8 new tokens: rows 105 / 185, chunk 128 / 130).
+  // The host knows the number of all rows only, so a call may need both kernels, each for its sequences (`few`):
+  //  * more rows than one tile each on average: the chunk kernel, in calls of many sequences beside the rows kernel for those of
+  //    one tile (20 single tokens beside 4 chunks of up to 500: 169 -> 160 us, with tiles of eight 144; of few sequences the two
+  //    launches cost more than that: 3 prompts 120 -> 128);
+  //  * no more: the rows kernel, and the chunk kernel for those of more than two tiles.  768 tokens beside 255 single ones (up to
+  //    8192, as above): 1375 us by the rows kernel alone, 802 by both; 2000 beside 199 (16 heads on 16): 1175 and 618; 128 beside
+  //    64: 163 and 135.  Where no sequence turns out to have so many that costs a launch (64 of 4 tokens 111 and 118), so calls in
+  //    which none can have more than MOST rows, if each has a token, leave it out: 49 tokens beside 15 single ones 62 and 66 (but of
+  //    up to 16384 189 and 139), 16 of 4 tokens 40 and 47.
+  constexpr int FEW = 16, MANY = 8, MOST = 256;
   const WorkspaceTurn turn(workspace);
-  const int64_t rows = tokens * p.group;
-  p.few = std::numeric_limits<int>::max();
-  if (!offsets || !paged_chunk_takes(p) || rows <= (dim == 64 ? 2 * FEW : FEW) * batch)
-    return paged_rows<T>(p, dim, rows <= FEW / 2 * batch, k_cache.p, v_cache.p, sms, stream);
-  const bool narrow = p.group <= FEW / 2;
-  p.few = batch < MANY ? 0 : narrow ? FEW / 2 : FEW;
-  if (p.few > 0) {
-    const int status = paged_rows<T>(p, dim, narrow, k_cache.p, v_cache.p, sms, stream);
+  const int grid = std::min(sms, kPagedCtas);
+  const int64_t rows = tokens * p.group, most = tokens < batch ? rows : (tokens - batch + 1) * p.group;
+  const bool usual = rows <= (dim == 64 ? 2 * FEW : FEW) * batch;
+  const bool narrow = rows <= FEW / 2 * batch || (!usual && p.group <= FEW / 2);
+  const bool chunks = offsets && paged_chunk_takes(p) && !(usual && (batch < MANY || most <= MOST));
+  p.few = !chunks ? std::numeric_limits<int>::max() : batch < MANY ? 0 : usual ? 2 * FEW : narrow ? FEW / 2 : FEW;
+  if (p.few < p.group) p.few = 0;          // (no sequence has so few)
+  const int tile_rows = p.few == 0 ? 0 : narrow ? FEW / 2 : FEW;
+  PagedParams chunk = p;
+  if (tile_rows > 0) {
+    const int status = paged_rows<T>(p, dim, tile_rows, k_cache.p, v_cache.p, grid, stream);
     if (status != INTENT_B200_OK) return status;
   }
-  return paged_chunk<T>(p, dim, k_cache.p, v_cache.p, sms, stream);
+  if (chunks) {
+    chunk.joins = static_cast<unsigned char*>(workspace) + kPagedChunkJoins;
+    chunk.parts += paged_rows_parts_bytes(dim) / int64_t(sizeof(float));
+    chunk.half_tokens = paged_chunk_half_tokens(p);
+    const int status = paged_chunk<T>(chunk, dim, k_cache.p, v_cache.p, grid, stream);
+    if (status != INTENT_B200_OK) return status;
+  }
+  return paged_join<T>(p, tile_rows, chunk, chunks, dim, grid, stream);
 }
 
 }  // namespace
 }  // namespace ib200
 
 extern "C" int64_t intent_b200_paged_attention_workspace_bytes(int64_t dim, int32_t single) {
-  const int64_t rows = ib200::paged_rows_workspace_bytes(dim), chunk = ib200::paged_chunk_workspace_bytes(dim);
-  return single || rows > chunk ? rows : chunk;
+  return ib200::kPagedHeader + ib200::paged_rows_parts_bytes(dim) + (single ? 0 : ib200::paged_chunk_parts_bytes(dim));
 }
 
 // Reads the status word at the head of a workspace after synchronising `stream`, and clears it.

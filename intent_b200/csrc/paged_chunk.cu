@@ -13,7 +13,7 @@
 // The steps of all tiles of all sequences form one line, of which every CTA takes the same length (as in paged_rows.cu); how
 // many steps a tile has follows from its last token's position and its first one's window, and the sums of these over the
 // tiles of a sequence are evaluated in closed form (sum of floor((a j + b) / m)), so a CTA finds its place in a few divisions.
-// Tiles that a CTA boundary cuts leave maximum, sum and unscaled result per part, and join_kernel adds the parts in order.
+// Tiles that a CTA boundary cuts leave maximum, sum and unscaled result per part, and join_chunk adds the parts in order.
 //
 // Keys and values come through a ring of TMA boxes of one page's rows each (128B swizzle, one lane per box); boxes of tokens
 // that no query of the tile sees are asked for behind the cache's end, where TMA fills in zeros.
@@ -39,13 +39,13 @@
 
 #include "common.cuh"
 #include "paged.cuh"
+#include "paged_join.cuh"
 #include "tma.cuh"
 #include "umma.cuh"
 
 namespace ib200 {
 namespace {
 
-constexpr int HALF_ROWS = 128;             // query rows of half a tile
 constexpr int STEP = 128;                  // tokens of a step
 constexpr int LOAD_WARP = 9, MMA_WARP = 8, THREADS = 12 * 32;   // warps 0..3 and 4..7: a half's rows; 10 and 11 only lend registers
 // Registers of a thread: the launch's, then those of a row's thread (128 scores and more) and of the others.
@@ -280,13 +280,6 @@ struct Shared {
   volatile uint32_t missing[8];            // per step, boxes of pages outside the cache
 };
 
-struct JoinEntry {
-  int last_cta;            // of the tile that begins in this CTA and ends in another; -1: there is none
-  int row, head, tokens;   // first row of q, key head, tokens from there on in the sequence
-  int sequence;
-};
-static_assert(sizeof(JoinEntry) <= kPagedEntry, "room ahead of the parts");
-
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS, 1)
 paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -375,7 +368,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     sh.start = begin - at;
     sh.start_head = of_head;
   }
-  JoinEntry* entry = reinterpret_cast<JoinEntry*>(p.joins) + cta;
+  ChunkJoin* entry = static_cast<ChunkJoin*>(p.joins) + cta;
   if (tid == 0) {
     entry->last_cta = -1;
     if (share < 0) atomicExch(p.status, INTENT_B200_ERR_SHAPE);
@@ -817,63 +810,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
 }
 
-// Parts of the tiles that CTA boundaries cut: block (cta, 32 rows), a thread per row and eight elements.  What it costs is the
-// latency of dependent reads (0.5 us each): the maxima and sums of all parts are read at once, by all warps, and the results four
-// parts at a time (8 tiles of 16 parts, 33 tokens behind 7967, a call alone: 39.7 us; with two at a time and sixteen elements per
-// thread 40.4).
-template <typename T, int D>
-__global__ void __launch_bounds__(4 * D, 1024 / (4 * D)) paged_join_kernel(const PagedParams p) {
-  __shared__ float maxima[kPagedCtas][32], sums[kPagedCtas][32];
-  constexpr int WARPS = D / 8;
-  programmatic_begin();
-  programmatic_wait();
-  const JoinEntry entry = reinterpret_cast<const JoinEntry*>(p.joins)[blockIdx.x];
-  const int first = blockIdx.x, count = entry.last_cta - first + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int row = blockIdx.y * 32 + lane;
-  const int of_half = row % HALF_ROWS, row_token = of_half / p.group, token = row / HALF_ROWS * p.half_tokens + row_token;
-  const bool real = row_token < p.half_tokens && token < entry.tokens;
-  if (entry.last_cta < 0 || !__any_sync(0xffffffffu, real)) return;    // (all warps have the same rows)
-  constexpr size_t SIZE = size_t(2 * HALF_ROWS) * (D + 2);
-  const float infinity = __int_as_float(0x7f800000);
-  auto part = [&](int v) { return p.parts + (2 * (first + v) + (v == 0)) * SIZE; };
-#pragma unroll 4
-  for (int v = warp; v < count; v += WARPS) {
-    maxima[v][lane] = real ? __ldcg(part(v) + 2 * HALF_ROWS * D + row) : -infinity;
-    sums[v][lane] = real ? __ldcg(part(v) + 2 * HALF_ROWS * (D + 1) + row) : 0.f;
-  }
-  __syncthreads();
-  if (!real) return;
-  float m = -infinity, l = 0.f, x[8] = {};
-  for (int v = 0; v < count; ++v) m = fmaxf(m, maxima[v][lane]);
-  const float origin = m == -infinity ? 0.f : m;
-#pragma unroll 1
-  for (int from = 0; from < count; from += 4) {
-    float4 y[4][2];
-#pragma unroll
-    for (int v = 0; v < 4; ++v)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        if (from + v < count) y[v][e] = __ldcg(reinterpret_cast<const float4*>(part(from + v)) + (2 * warp + e) * 2 * HALF_ROWS + row);
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      if (from + v >= count) break;
-      const float f = exp2_fast(maxima[from + v][lane] - origin);
-      l = fmaf(sums[from + v][lane], f, l);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        x[4 * e] = fmaf(y[v][e].x, f, x[4 * e]), x[4 * e + 1] = fmaf(y[v][e].y, f, x[4 * e + 1]);
-        x[4 * e + 2] = fmaf(y[v][e].z, f, x[4 * e + 2]), x[4 * e + 3] = fmaf(y[v][e].w, f, x[4 * e + 3]);
-      }
-    }
-  }
-  const float inverse = l == 0.f ? of_nothing(p, entry.sequence, entry.row + token) : 1.f / l;
-  uint32_t w[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) w[e] = Elem<T>::pack2(x[2 * e] * inverse, x[2 * e + 1] * inverse);
-  uint16_t* to = p.out + (int64_t(entry.row + token) * p.q_heads + entry.head * p.group + of_half - row_token * p.group) * D + 8 * warp;
-  *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 template <typename T, int D>
 int launch(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v, const PagedParams& p, int grid,
            cudaStream_t stream) {
@@ -894,25 +830,23 @@ int launch(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap
   e = launch_programmatic(kernel, dim3(unsigned(grid)), dim3(THREADS), smem, stream, 1, map_q, map_k, map_v, p);
   if (e != cudaSuccess) return cuda_status(e);
   note_launch();
-  e = launch_programmatic(paged_join_kernel<T, D>, dim3(unsigned(grid), 2 * HALF_ROWS / 32), dim3(4 * D), 0, stream, 1, p);
-  if (e != cudaSuccess) return cuda_status(e);
-  note_launch();
   return launch_status();
 }
 
 }  // namespace
 
-int64_t paged_chunk_workspace_bytes(int64_t dim) {
-  return kPagedHeader + int64_t(2) * kPagedCtas * 2 * HALF_ROWS * (dim + 2) * int64_t(sizeof(float));
+int64_t paged_chunk_parts_bytes(int64_t dim) {
+  return int64_t(2) * kPagedCtas * 2 * HALF_ROWS * (dim + 2) * int64_t(sizeof(float));
 }
 
 bool paged_chunk_takes(const PagedParams& p) {
   return p.group <= HALF_ROWS && (p.tokens == 1 || p.q_token > 0) && (p.q_heads == 1 || p.q_head > 0);
 }
 
+int paged_chunk_half_tokens(const PagedParams& p) { return HALF_ROWS / p.group; }
+
 template <typename T>
-int paged_chunk(PagedParams p, int64_t dim, const void* k_cache, const void* v_cache, int sms, cudaStream_t stream) {
-  p.half_tokens = HALF_ROWS / p.group;
+int paged_chunk(const PagedParams& p, int64_t dim, const void* k_cache, const void* v_cache, int grid, cudaStream_t stream) {
   EncodeTiledFn encode = encode_tiled_fn();
   if (!encode) return INTENT_B200_ERR_CUDA;
   CUtensorMap map_q, map_k, map_v;
@@ -928,10 +862,9 @@ int paged_chunk(PagedParams p, int64_t dim, const void* k_cache, const void* v_c
       !make_tensor_map_2d(&map_k, type, k_cache, rows, uint64_t(dim), uint64_t(dim) * 2, box, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
       !make_tensor_map_2d(&map_v, type, v_cache, rows, uint64_t(dim), uint64_t(dim) * 2, box, 64, CU_TENSOR_MAP_SWIZZLE_128B))
     return INTENT_B200_ERR_CUDA;
-  const int grid = std::min(sms, kPagedCtas);
   return dim == 128 ? launch<T, 128>(map_q, map_k, map_v, p, grid, stream) : launch<T, 64>(map_q, map_k, map_v, p, grid, stream);
 }
-template int paged_chunk<__half>(PagedParams, int64_t, const void*, const void*, int, cudaStream_t);
-template int paged_chunk<__nv_bfloat16>(PagedParams, int64_t, const void*, const void*, int, cudaStream_t);
+template int paged_chunk<__half>(const PagedParams&, int64_t, const void*, const void*, int, cudaStream_t);
+template int paged_chunk<__nv_bfloat16>(const PagedParams&, int64_t, const void*, const void*, int, cudaStream_t);
 
 }  // namespace ib200

@@ -14,7 +14,7 @@
 //  * Work is cut evenly, not by sequence.  All steps (32 tokens for each warp) of all (sequence, key head, row tile) form one
 //    line, of which every CTA takes the same length; a long sequence is shared by many CTAs and a CTA goes through many short ones
 //    while its ring runs on.  A row tile that was cut leaves its parts (maximum, sum, unscaled result) in the workspace,
-//    which paged_rows_join_kernel puts together in CTA order: the same bits in every launch.
+//    which join_rows puts together in CTA order: the same bits in every launch.
 //  * Few instructions per token.  Keys are the tensor core's A operand (16 tokens) and the queries its B operand (eight rows,
 //    kept in registers): S^T = K Q^T, then O^T += V^T P^T with V^T from transposing loads and P^T from one movmatrix per
 //    eight tokens.  With up to eight query heads per key head nothing is computed for rows that are not there.  A maximum is
@@ -27,6 +27,7 @@
 
 #include "common.cuh"
 #include "paged.cuh"
+#include "paged_join.cuh"
 #include "tma.cuh"
 
 namespace ib200 {
@@ -133,14 +134,6 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t v) {
   return d;
 }
 
-struct JoinEntry {
-  int last_cta;            // of the tile that begins in this CTA and ends in another; -1: there is none
-  int row, head;           // first row of q of its sequence, key head
-  int tile_row, rows;      // its first row among the sequence's, how many it has
-  int sequence;
-};
-static_assert(sizeof(JoinEntry) <= kPagedEntry, "room ahead of the parts");
-
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(32 * Ring<D>::WARPS, 1)
 paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedParams p) {
@@ -192,7 +185,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   }
   before -= sum;
   const int share = share_of(line), cta = blockIdx.x;
-  JoinEntry* entry = reinterpret_cast<JoinEntry*>(p.joins) + cta;
+  RowsJoin* entry = static_cast<RowsJoin*>(p.joins) + cta;
   if (tid == 0) {
     entry->last_cta = -1;
     if (share < 0) atomicExch(p.status, INTENT_B200_ERR_SHAPE);
@@ -590,51 +583,6 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   }
 }
 
-// Parts of the tiles that CTA boundaries cut: a block per CTA in which such a tile begins, a thread per row and four elements.
-// What it costs is the latency of dependent reads: all maxima and sums are read at once, then the results of eight parts at a time.
-// (When the CTA that finished a tile last did this, one multiprocessor had 16 rows of 16 parts to read: four tokens behind 8000,
-// 32 heads on 8, took 31 us a call; with this kernel 17.)
-template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(ROWS * D / 4) paged_rows_join_kernel(const PagedParams p) {
-  __shared__ float maxima[kPagedCtas][ROWS], sums[kPagedCtas][ROWS];
-  programmatic_begin();
-  programmatic_wait();
-  const JoinEntry entry = reinterpret_cast<const JoinEntry*>(p.joins)[blockIdx.x];
-  const int first = blockIdx.x, count = entry.last_cta - first + 1, r = threadIdx.x / (D / 4), c = threadIdx.x % (D / 4);
-  if (entry.last_cta < 0) return;
-  constexpr size_t SIZE = size_t(ROWS) * (D + 2);
-  const float infinity = __int_as_float(0x7f800000);
-  auto part = [&](int v) { return p.parts + (2 * (first + v) + (v == 0)) * SIZE; };
-  for (int i = threadIdx.x; i < count * ROWS; i += ROWS * D / 4) {
-    const int v = i / ROWS, row = i % ROWS;
-    maxima[v][row] = row < entry.rows ? __ldcg(part(v) + ROWS * D + row) : -infinity;
-    sums[v][row] = row < entry.rows ? __ldcg(part(v) + ROWS * (D + 1) + row) : 0.f;
-  }
-  __syncthreads();
-  if (r >= entry.rows) return;
-  float m = -infinity, l = 0.f, x[4] = {};
-  for (int v = 0; v < count; ++v) m = fmaxf(m, maxima[v][r]);
-  const float origin = m == -infinity ? 0.f : m;
-#pragma unroll 1
-  for (int from = 0; from < count; from += 8) {
-    float4 y[8];
-#pragma unroll
-    for (int v = 0; v < 8; ++v)
-      if (from + v < count) y[v] = __ldcg(reinterpret_cast<const float4*>(part(from + v) + r * D) + c);
-#pragma unroll
-    for (int v = 0; v < 8; ++v) {
-      if (from + v >= count) break;
-      const float f = exp2_fast(maxima[from + v][r] - origin);
-      l = fmaf(sums[from + v][r], f, l);
-      x[0] = fmaf(y[v].x, f, x[0]), x[1] = fmaf(y[v].y, f, x[1]), x[2] = fmaf(y[v].z, f, x[2]), x[3] = fmaf(y[v].w, f, x[3]);
-    }
-  }
-  const int token = (entry.tile_row + r) / p.group, of_group = entry.tile_row + r - token * p.group;
-  const float inverse = l == 0.f ? of_nothing(p, entry.sequence, entry.row + token) : 1.f / l;
-  *reinterpret_cast<uint2*>(p.out + (int64_t(entry.row + token) * p.q_heads + entry.head * p.group + of_group) * D + 4 * c) =
-      make_uint2(Elem<T>::pack2(x[0] * inverse, x[1] * inverse), Elem<T>::pack2(x[2] * inverse, x[3] * inverse));
-}
-
 template <typename T, int D, int NT>
 int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, const PagedParams& p, int grid, cudaStream_t stream) {
   auto kernel = paged_rows_kernel<T, D, NT>;
@@ -647,20 +595,17 @@ int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, const PagedParams
   e = launch_programmatic(kernel, dim3(unsigned(grid)), dim3(32 * Ring<D>::WARPS), smem, stream, 1, map_k, map_v, p);
   if (e != cudaSuccess) return cuda_status(e);
   note_launch();
-  e = launch_programmatic(paged_rows_join_kernel<T, D, 8 * NT>, dim3(unsigned(grid)), dim3(8 * NT * D / 4), 0, stream, 1, p);
-  if (e != cudaSuccess) return cuda_status(e);
-  note_launch();
   return launch_status();
 }
 
 }  // namespace
 
-int64_t paged_rows_workspace_bytes(int64_t dim) {
-  return kPagedHeader + int64_t(2) * kPagedCtas * 16 * (dim + 2) * int64_t(sizeof(float));
+int64_t paged_rows_parts_bytes(int64_t dim) {
+  return int64_t(2) * kPagedCtas * 16 * (dim + 2) * int64_t(sizeof(float));
 }
 
 template <typename T>
-int paged_rows(const PagedParams& p, int64_t dim, bool narrow, const void* k_cache, const void* v_cache, int sms,
+int paged_rows(const PagedParams& p, int64_t dim, int tile_rows, const void* k_cache, const void* v_cache, int grid,
                cudaStream_t stream) {
   CUtensorMap map_k, map_v;
   const uint64_t rows = uint64_t(p.pages) * uint64_t(p.k_heads) << p.page_shift;
@@ -671,12 +616,13 @@ int paged_rows(const PagedParams& p, int64_t dim, bool narrow, const void* k_cac
       !make_tensor_map_2d(&map_v, type, v_cache, rows, uint64_t(dim), uint64_t(dim) * 2, box, 64,
                           CU_TENSOR_MAP_SWIZZLE_128B))
     return INTENT_B200_ERR_CUDA;
-  const int grid = sms < kPagedCtas ? sms : kPagedCtas;
   if (dim == 128)
-    return narrow ? launch<T, 128, 1>(map_k, map_v, p, grid, stream) : launch<T, 128, 2>(map_k, map_v, p, grid, stream);
-  return narrow ? launch<T, 64, 1>(map_k, map_v, p, grid, stream) : launch<T, 64, 2>(map_k, map_v, p, grid, stream);
+    return tile_rows == 8 ? launch<T, 128, 1>(map_k, map_v, p, grid, stream)
+                          : launch<T, 128, 2>(map_k, map_v, p, grid, stream);
+  return tile_rows == 8 ? launch<T, 64, 1>(map_k, map_v, p, grid, stream)
+                        : launch<T, 64, 2>(map_k, map_v, p, grid, stream);
 }
-template int paged_rows<__half>(const PagedParams&, int64_t, bool, const void*, const void*, int, cudaStream_t);
-template int paged_rows<__nv_bfloat16>(const PagedParams&, int64_t, bool, const void*, const void*, int, cudaStream_t);
+template int paged_rows<__half>(const PagedParams&, int64_t, int, const void*, const void*, int, cudaStream_t);
+template int paged_rows<__nv_bfloat16>(const PagedParams&, int64_t, int, const void*, const void*, int, cudaStream_t);
 
 }  // namespace ib200

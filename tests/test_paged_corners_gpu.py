@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import intent_b200 as ib
+from intent_b200.runtime import native
 from oracle import attention as oracle
 from test_paged_attention_gpu import HALF_UNIT, assert_close, make, run
 
@@ -50,3 +51,38 @@ def test_rows_whose_scores_are_all_minus_infinity(cuda_device, lengths, counts, 
     if single:
         assert_numbers(attend(cuda_device, (q, k, v, table, offsets, n), single=True, kernel=kernel, WINDOW=window), expected,
                        weight, "bf16")
+
+
+def lengths_of(counts, seed, most=150):
+    g = torch.Generator().manual_seed(seed)
+    return [n + int(torch.randint(0, most, (1,), generator=g)) if n else 0 for n in counts]
+
+
+@pytest.mark.parametrize("counts,HQ,HK,D,launches", [
+    ([150] + [1] * 59, 8, 2, 128, 3),                              # in tiles of sixteen rows, and the chunk by itself
+    ([1] * 50 + [90] + [1] * 49, 8, 2, 128, 3),                    # in tiles of eight
+    ([8, 9, 70, 0, 1, 3, 33] + [1] * 80, 8, 2, 64, 3),             # sequences of up to four tiles, more than that, none
+    ([300] + [1] * 40, 16, 1, 64, 3),
+    ([60] + [1] * 30, 4, 4, 64, 2),                                # so few that one kernel takes all
+    ([4] * 12, 4, 2, 128, 2),
+    ([1] * 70, 32, 1, 64, 2),
+    ([0] * 90 + [75] + [0] * 9, 8, 2, 64, 3),                      # (a step of a fixed number of places, most of them empty)
+])
+def test_a_chunk_beside_many_single_tokens(cuda_device, counts, HQ, HK, D, launches):
+    """What takes a sequence goes by its own new tokens, whatever the others have on average."""
+    data = make(lengths_of(counts, len(counts)), counts, HQ, HK, D, 16, "bf16")
+    expected, weight = oracle.paged_attention(*data)
+    artifact = ib.compile(ib.programs.paged_attention)
+    assert_close(run(artifact, cuda_device, *data, False), expected, weight, "bf16")
+    before = native.launch_count()
+    assert_close(run(artifact, cuda_device, *data, False), expected, weight, "bf16")
+    assert native.launch_count() - before == launches
+    artifact.check()
+
+
+def test_heads_too_many_for_the_rows_kernel(cuda_device):
+    """With more query heads per key head than it takes rows of a sequence, a call launches the chunk kernel alone."""
+    counts = [50] + [1] * 9
+    data = make(lengths_of(counts, 1), counts, 40, 1, 128, 16, "bf16")
+    expected, weight = oracle.paged_attention(*data)
+    assert_close(attend(cuda_device, data, kernel=CHUNK), expected, weight, "bf16")
