@@ -654,7 +654,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
 #pragma unroll
           for (int c = 0; c < 4; ++c) most[c] = largest(most[c], __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
         const float now = largest(largest(most[0], most[1], most[2]), most[3], -infinity) * p.scale;
-        const bool raise = !(now <= top + SLACK) || top == -infinity;
+        // (rows that are no query's hold what was in shared memory, or other sequences' queries, maybe no numbers: they ask for nothing)
+        const bool raise = real && (!(now <= top + SLACK) || top == -infinity);
         const float factor = raise ? exp2_fast(top - (now == -infinity ? 0.f : now)) : 1.f;
         if (raise) top = now;
         weight_sum *= factor;

@@ -86,3 +86,14 @@ def test_heads_too_many_for_the_rows_kernel(cuda_device):
     data = make(lengths_of(counts, 1), counts, 40, 1, 128, 16, "bf16")
     expected, weight = oracle.paged_attention(*data)
     assert_close(attend(cuda_device, data, kernel=CHUNK), expected, weight, "bf16")
+
+
+def test_queries_that_are_no_numbers_stay_among_themselves(cuda_device):
+    """Rows of a tile that belong to the next sequence, or to none, do not reach the tile's own."""
+    counts, lengths = [40, 70, 3], [200, 300, 90]
+    q, k, v, table, offsets, n = make(lengths, counts, 10, 2, 64, 16, "bf16")
+    q[40:110] = math.nan
+    expected, weight = oracle.paged_attention(q, k, v, table, offsets, n)
+    out = attend(cuda_device, (q, k, v, table, offsets, n), kernel=CHUNK)
+    assert expected[40:110].isnan().all() and not expected[:40].isnan().any()
+    assert_numbers(out, expected, weight, "bf16")
