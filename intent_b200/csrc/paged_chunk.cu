@@ -34,6 +34,7 @@
 // same things at the same time and each takes longer, 3770 cycles a step); a cubic for an eighth or a quarter of the exponentials
 // (111 -> 113 and 114).
 #include <algorithm>
+#include <atomic>
 #include <cstddef>
 #include <type_traits>
 
@@ -820,11 +821,14 @@ int launch(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return cuda_status(e);
   // (the kernel shares the launch's registers out anew, which would wait for ever if there were fewer)
-  static const int registers = [kernel] {
+  static std::atomic<int> registers{0};    // (asked for until the answer comes: a call that fails does not decide for those after it)
+  if (registers.load(std::memory_order_relaxed) == 0) {
     cudaFuncAttributes attributes;
-    return cudaFuncGetAttributes(&attributes, kernel) == cudaSuccess ? attributes.numRegs : -1;
-  }();
-  if (registers != LAUNCH_REGISTERS) return INTENT_B200_ERR_UNSUPPORTED;
+    e = cudaFuncGetAttributes(&attributes, kernel);
+    if (e != cudaSuccess) return cuda_status(e);
+    registers.store(attributes.numRegs, std::memory_order_relaxed);
+  }
+  if (registers.load(std::memory_order_relaxed) != LAUNCH_REGISTERS) return INTENT_B200_ERR_UNSUPPORTED;
   if (LaunchFacts* sink = observe_sink())
     return record_launch(sink, reinterpret_cast<const void*>(kernel), "paged_chunk_kernel 2 x 128 rows, parts joined", grid,
                          THREADS, smem, 1);
