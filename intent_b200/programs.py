@@ -943,8 +943,9 @@ def _paged_workspace_bytes(dim, single):
 def _lower_paged(c, device, *, single):
     act = _act_dtype(c)
     scale, window = c["SCALE"], c["WINDOW"]
-    if scale is not None and not 0 < float(scale) < float("inf"):
-        raise CompilationStageError("frontend_kir", "SCALE must be a positive number, or None for 1 / sqrt(D)")
+    bits = _f32_bits(0 if scale is None else scale, "SCALE")
+    if scale is not None and not 0 < bits < 0x7f800000:      # (as the f32 that it becomes: 0 would stand for the default)
+        raise CompilationStageError("frontend_kir", "SCALE must be a positive f32 number, or None for 1 / sqrt(D)")
     if not isinstance(window, int) or not 0 <= window < 1 << 31:
         raise CompilationStageError("frontend_kir", "WINDOW must be a number of tokens, 0 for all")
     views = [ViewParameter(0, "q", act, ("B" if single else "T", "HQ", "D"), IN, layout="rows"),
@@ -963,7 +964,7 @@ def _lower_paged(c, device, *, single):
     stem = "paged_decode_attention" if single else "paged_attention"
     return NativeProgram(interface=PublicInterface(tuple(views), dimension_rules=rules), device=device,
                          entry_name=f"intent_b200_{stem}_{act.name}",
-                         constants=(_f32_bits(0 if scale is None else scale, "SCALE"), window),
+                         constants=(bits, window),
                          workspace=lambda d: _paged_workspace_bytes(d["D"], single),
                          empty=lambda d: d["B"] == 0 or (not single and d["T"] == 0),
                          workspace_status="intent_b200_paged_attention_workspace_status")
