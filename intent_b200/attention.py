@@ -86,7 +86,7 @@ class PagedKVCache:
 
     def step(self, new_tokens: dict) -> AttentionStep:
         """Room for so many new tokens of each sequence, and where they go.  Where there are not enough pages left,
-        MemoryError, and nothing has changed."""
+        MemoryError; a step that fails, in this way or another, changes nothing."""
         import numpy as np
         import torch
 
@@ -98,10 +98,10 @@ class PagedKVCache:
         missing = [-(-length // size) - len(self._pages.get(name, ())) for name, length in zip(names, lengths)]
         if sum(missing) > len(self._free):
             raise MemoryError(f"{sum(missing)} pages are needed and {len(self._free)} are free")
-        for name, length, more in zip(names, lengths, missing):
-            held = self._pages.setdefault(name, [])
-            held.extend(self._free.pop() for _ in range(more))
-            self._lengths[name] = length
+        pages, free = [], len(self._free)
+        for name, more in zip(names, missing):
+            pages.append(self._pages.get(name, []) + self._free[free - more:free][::-1])
+            free -= more
         tokens, batch = sum(counts), len(names)
         width = max(1, max(-(-length // size) for length in lengths))
         words = np.zeros(tokens + batch * width + 2 * batch + 1, dtype=np.int32)
@@ -110,8 +110,8 @@ class PagedKVCache:
         table = table.reshape(batch, width)
         table[:] = -1
         at = 0
-        for row, (name, count, length) in enumerate(zip(names, counts, lengths)):
-            held = np.asarray(self._pages[name], dtype=np.int64)
+        for row, (count, length) in enumerate(zip(counts, lengths)):
+            held = np.asarray(pages[row], dtype=np.int64)
             table[row, :len(held)] = held
             place = np.arange(length - count, length)
             positions[at:at + count] = place
@@ -124,7 +124,11 @@ class PagedKVCache:
         if device.type == "cuda":        # (the allocator of pinned memory waits for copies under way before it gives it again)
             copies = [c.pin_memory().to(device, non_blocking=True) for c in copies]
         parts = torch.split(copies[0], [tokens, batch * width, batch + 1, batch])
-        return AttentionStep(parts[0], copies[1], parts[1].view(batch, width), parts[2], parts[3], all(n == 1 for n in counts))
+        step = AttentionStep(parts[0], copies[1], parts[1].view(batch, width), parts[2], parts[3], all(n == 1 for n in counts))
+        del self._free[free:]
+        self._pages.update(zip(names, pages))
+        self._lengths.update(zip(names, lengths))
+        return step
 
     def release(self, sequence) -> None:
         """Ends a sequence; its pages are free again (for steps that follow on the same stream)."""

@@ -2,8 +2,10 @@
 import math
 
 import pytest
+import torch
 
 import intent_b200 as ib
+from intent_b200.attention import PagedKVCache
 
 
 @pytest.mark.parametrize("program", ["paged_attention", "paged_decode_attention"])
@@ -18,3 +20,24 @@ def test_scales_that_are_no_positive_f32(program, scale):
 def test_scales_that_are_one(scale):
     artifact = ib.compile(ib.programs.paged_attention, constexprs={"SCALE": scale}, resolve_target=False)
     assert (artifact.runtime.constants[0] == 0) == (scale is None)
+
+
+@pytest.mark.parametrize("failing", ["from_numpy", "split"])
+def test_a_step_that_fails_changes_nothing(monkeypatch, failing):
+    """Memory for its tensors, say, may run out after the pages were found."""
+    store = PagedKVCache(layers=1, pages=8, kv_heads=2, head_dim=64, page_size=16, device="cpu")
+    store.step({"a": 20})
+    with monkeypatch.context() as patch:
+        def fail(*_):
+            raise RuntimeError("out of memory")
+
+        patch.setattr(torch, failing, fail)
+        with pytest.raises(RuntimeError):
+            store.step({"a": 30, "b": 5})
+    assert store.free_pages == 6 and store.length("a") == 20 and store.length("b") == 0
+    with pytest.raises(KeyError):
+        store.release("b")
+    step = store.step({"b": 5, "a": 30})
+    assert step.kv_lengths.tolist() == [5, 50] and step.positions.tolist() == [*range(5), *range(20, 50)]
+    used = step.page_table[0, :1].tolist() + step.page_table[1, :4].tolist()
+    assert sorted(used) == sorted(set(used)) and store.free_pages == 3
