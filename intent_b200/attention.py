@@ -46,6 +46,7 @@ class AttentionStep:
     query_offsets: Any    # [B + 1] i32, the sequences' rows
     kv_lengths: Any       # [B] i32, the new tokens among them
     single: bool          # every sequence has one new token
+    longest: int = 0      # positions end here: tokens of the longest sequence that has new ones
 
 
 class PagedKVCache:
@@ -124,7 +125,8 @@ class PagedKVCache:
         if device.type == "cuda":        # (the allocator of pinned memory waits for copies under way before it gives it again)
             copies = [c.pin_memory().to(device, non_blocking=True) for c in copies]
         parts = torch.split(copies[0], [tokens, batch * width, batch + 1, batch])
-        step = AttentionStep(parts[0], copies[1], parts[1].view(batch, width), parts[2], parts[3], all(n == 1 for n in counts))
+        step = AttentionStep(parts[0], copies[1], parts[1].view(batch, width), parts[2], parts[3], all(n == 1 for n in counts),
+                             max((length for count, length in zip(counts, lengths) if count), default=0))
         del self._free[free:]
         self._pages.update(zip(names, pages))
         self._lengths.update(zip(names, lengths))
@@ -174,6 +176,8 @@ class W4A16Attention:
         tokens, heads = x.shape[0], self.heads + 2 * self.kv_heads
         if step.positions.shape[0] != tokens:
             raise ValueError(f"the step has {step.positions.shape[0]} tokens, x has {tokens}")
+        if step.longest > rotary.shape[0]:      # (the keys of positions without an angle would be stored as NaN)
+            raise ValueError(f"a sequence has {step.longest} tokens, the rotary table {rotary.shape[0]} positions")
         qkv = self.project.run(x, weights.qkv_packed, weights.qkv_scales)
         if qkv.shape[1] != heads * self.head_dim:
             raise ValueError(f"the projection has {qkv.shape[1]} columns, not {heads * self.head_dim}")

@@ -41,3 +41,10 @@ def test_a_step_that_fails_changes_nothing(monkeypatch, failing):
     assert step.kv_lengths.tolist() == [5, 50] and step.positions.tolist() == [*range(5), *range(20, 50)]
     used = step.page_table[0, :1].tolist() + step.page_table[1, :4].tolist()
     assert sorted(used) == sorted(set(used)) and store.free_pages == 3
+
+
+def test_where_the_positions_of_a_step_end():
+    store = PagedKVCache(layers=1, pages=8, kv_heads=2, head_dim=64, page_size=16, device="cpu")
+    assert store.step({"a": 20, "b": 3}).longest == 20
+    assert store.step({"b": 1}).longest == 4
+    assert store.step({"a": 0, "b": 2}).longest == 6 and store.step({"a": 0}).longest == 0
