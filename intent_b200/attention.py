@@ -176,6 +176,10 @@ class W4A16Attention:
         tokens, heads = x.shape[0], self.heads + 2 * self.kv_heads
         if step.positions.shape[0] != tokens:
             raise ValueError(f"the step has {step.positions.shape[0]} tokens, x has {tokens}")
+        if x.shape[1] != self.hidden:
+            raise ValueError(f"x has {x.shape[1]} columns, not {self.hidden}")
+        if weights.out_packed.shape[0] * 8 != self.heads * self.head_dim or weights.out_packed.shape[1] != self.hidden:
+            raise ValueError(f"the output projection must be packed from [{self.heads * self.head_dim}, {self.hidden}]")
         if step.longest > rotary.shape[0]:      # (the keys of positions without an angle would be stored as NaN)
             raise ValueError(f"a sequence has {step.longest} tokens, the rotary table {rotary.shape[0]} positions")
         qkv = self.project.run(x, weights.qkv_packed, weights.qkv_scales)

@@ -35,3 +35,20 @@ def test_positions_beyond_the_rotary_table(cuda_device):
     with pytest.raises(ValueError, match="rotary"):
         layer.forward(x[:3], w, table, *cache.layer(0), step)
     assert torch.equal(cache.k, before)
+
+
+def test_sizes_other_than_the_layers(cuda_device):
+    """Refused before the keys are stored, not by the last projection."""
+    cache = PagedKVCache(layers=1, pages=8, kv_heads=KV_HEADS, head_dim=DIM, page_size=16, device=cuda_device)
+    cache.k.zero_(), cache.v.zero_()
+    layer, w = W4A16Attention(hidden=HIDDEN, heads=HEADS, kv_heads=KV_HEADS, head_dim=DIM), make_weights(cuda_device)
+    table = rotary_table(32, DIM, device=cuda_device)
+    wide = make_weights(cuda_device, hidden=384)
+    more = make_weights(cuda_device, heads=8)
+    mixed = AttentionWeights(w.qkv_packed, w.qkv_scales, more.out_packed, more.out_scales, w.q_norm, w.k_norm)
+    broad = AttentionWeights(w.qkv_packed, w.qkv_scales, wide.out_packed, wide.out_scales, w.q_norm, w.k_norm)
+    step = cache.step({"a": 3})
+    for hidden, weights in ((384, wide), (HIDDEN, mixed), (HIDDEN, broad)):
+        with pytest.raises(ValueError):
+            layer.forward(torch.randn((3, hidden), device=cuda_device).bfloat16(), weights, table, *cache.layer(0), step)
+    assert not cache.k.any() and not cache.v.any()
