@@ -13,15 +13,15 @@ def rotate(x, positions, rotary, weight=None, eps=1e-6, pairs="halves"):
         y = y / torch.sqrt((y * y).mean(-1, keepdim=True) + eps) * weight.double()
     R = rotary.shape[1]
     out = y.clone()
-    for t, p in enumerate(positions.tolist()):
-        if R and not 0 <= p < rotary.shape[0]:
-            out[t] = math.nan
-            continue
-        for i in range(R // 2):
-            a, b = (i, i + R // 2) if pairs == "halves" else (2 * i, 2 * i + 1)
-            cos, sin = float(rotary[p, i]), float(rotary[p, R // 2 + i])
-            out[t, :, a] = y[t, :, a] * cos - y[t, :, b] * sin
-            out[t, :, b] = y[t, :, b] * cos + y[t, :, a] * sin
+    known = (positions >= 0) & (positions < rotary.shape[0])
+    angles = rotary.double()[torch.where(known, positions, 0).long()] if known.any() else rotary.new_zeros((len(y), R)).double()
+    for i in range(R // 2):
+        a, b = (i, i + R // 2) if pairs == "halves" else (2 * i, 2 * i + 1)
+        cos, sin = angles[:, None, i], angles[:, None, R // 2 + i]
+        out[..., a] = y[..., a] * cos - y[..., b] * sin
+        out[..., b] = y[..., b] * cos + y[..., a] * sin
+    if R:
+        out[~known] = math.nan
     return out
 
 

@@ -97,3 +97,92 @@ def test_queries_that_are_no_numbers_stay_among_themselves(cuda_device):
     out = attend(cuda_device, (q, k, v, table, offsets, n), kernel=CHUNK)
     assert expected[40:110].isnan().all() and not expected[:40].isnan().any()
     assert_numbers(out, expected, weight, "bf16")
+
+
+@pytest.mark.parametrize("D,HQ", [(64, 6), (128, 14)])
+def test_strided_queries_of_chunks(cuda_device, D, HQ):
+    counts, lengths = [70, 200], [90, 200]
+    q, k, v, table, offsets, n = make(lengths, counts, HQ, 2, D, 16, "bf16")
+    expected, weight = oracle.paged_attention(q, k, v, table, offsets, n)
+    wide = torch.full((270, HQ + 4, D + 8), math.nan, dtype=torch.bfloat16, device=cuda_device)
+    wide[:, 3:3 + HQ, :D] = q.to(cuda_device)
+    turned = q.to(cuda_device).transpose(0, 1).contiguous().transpose(0, 1)     # heads ahead of tokens
+    artifact = ib.compile(ib.programs.paged_attention)
+    rest = [t.to(cuda_device) for t in (k, v, table, offsets, n)]
+    for view in (wide[:, 3:3 + HQ, :D], turned):
+        assert not view.is_contiguous()
+        for _ in range(2):
+            assert_close(artifact.run(view, *rest), expected, weight, "bf16")
+        assert artifact.observation.kernel.startswith(CHUNK)
+    artifact.check()
+
+
+@pytest.mark.parametrize("scale", [0.01, 1.0, 3.0])
+def test_scales_of_chunks(cuda_device, scale):
+    data = make([300, 140], [200, 90], 4, 2, 64, 16, "f16")
+    data = (data[0] * 0.5, *data[1:])
+    expected, weight = oracle.paged_attention(*data, scale=scale)
+    assert_close(attend(cuda_device, data, "f16", kernel=CHUNK, SCALE=scale), expected, weight, "f16")
+
+
+def test_scores_of_both_infinities_in_chunks(cuda_device):
+    """Rows ahead of the key that makes a score +inf are close, those that see it are no numbers; a key of -inf counts nothing."""
+    lengths, counts = [200, 240], [100, 150]
+    q, k, v, table, offsets, n = make(lengths, counts, 4, 2, 64, 16, "f16", poison=False)
+    q[:] = q.abs() + 0.1
+    for b, t, value in ((0, 19, -math.inf), (0, 150, -math.inf), (1, 130, math.inf)):
+        k[int(table[b, t // 16]), 1, t % 16] = value
+    expected, weight = oracle.paged_attention(q, k, v, table, offsets, n)
+    out = attend(cuda_device, (q, k, v, table, offsets, n), "f16", kernel=CHUNK)
+    assert expected[100 + 40:, 2:].isnan().all() and not expected[:100 + 40].isnan().any()
+    assert_numbers(out, expected, weight, "f16")
+
+
+def test_lengths_of_chunks_beyond_the_table(cuda_device):
+    """A length that the table cannot name counts as what it can name."""
+    data = make([144], [100], 2, 1, 64, 16, "f16")
+    expected, weight = oracle.paged_attention(*data)
+    for length in (145, (1 << 31) - 1):
+        longer = (*data[:5], torch.tensor([length], dtype=torch.int32))
+        assert_close(attend(cuda_device, longer, "f16", kernel=CHUNK), expected, weight, "f16")
+
+
+def test_offsets_of_chunks_beyond_the_queries(cuda_device):
+    """Offsets are cut to the rows there are; rows that no sequence has are left alone."""
+    data = make([148, 90], [80, 60], 2, 1, 64, 16, "f16")
+    expected, weight = oracle.paged_attention(*data)
+    artifact = ib.compile(ib.programs.paged_attention, constexprs={"ACT_DTYPE": "f16"})
+    moved = [t.to(cuda_device) for t in data]
+    out = torch.full((140, 2, 64), 7.0, dtype=torch.float16, device=cuda_device)
+    for offsets, rows in (([0, 80, 1 << 30], 140), ([-9, 80, 80], 80)):
+        out.fill_(7.0)
+        artifact.launch(*moved[:4], torch.tensor(offsets, dtype=torch.int32, device=cuda_device), moved[5], out)
+        assert_close(out[:rows], expected[:rows], weight[:rows], "f16")
+        assert (out[rows:] == 7).all() and artifact.observation.kernel.startswith(CHUNK)
+
+
+@pytest.mark.parametrize("window", [0, 1, 20, 128])
+@pytest.mark.parametrize("D", [64, 128])
+def test_chunks_of_more_tokens_than_the_cache_holds(cuda_device, window, D):
+    """Queries ahead of the first token see nothing: rows of zeros, also where whole tiles are ahead of it."""
+    counts, lengths = [150, 700, 60, 300], [30, 40, 0, 300]
+    data = make(lengths, counts, 4, 2, D, 16, "bf16")
+    expected, weight = oracle.paged_attention(*data, window=window)
+    assert not expected[:120].any() and not expected[150:810].any() and expected[:150].any()
+    assert_close(attend(cuda_device, data, kernel=CHUNK, WINDOW=window), expected, weight, "bf16")
+
+
+@pytest.mark.parametrize("HQ,HK", [(28, 4), (40, 8), (9, 3), (64, 1), (128, 1)])
+@pytest.mark.parametrize("window", [0, 70])
+def test_groups_of_chunks(cuda_device, HQ, HK, window):
+    """Tiles that hold 2 x floor(128 / group) tokens, from 1 to 128 of them."""
+    data = make([210, 150], [60, 130], HQ, HK, 64, 32, "bf16")
+    expected, weight = oracle.paged_attention(*data, window=window)
+    assert_close(attend(cuda_device, data, kernel=CHUNK, WINDOW=window), expected, weight, "bf16")
+
+
+def test_chunks_as_torch_op(cuda_device):
+    data = make([90, 220], [60, 150], 4, 2, 64, 16, "bf16")
+    expected, weight = oracle.paged_attention(*data)
+    op = ib.compile(ib.programs.paged_attention).as_torch_op("intent_b200_test::paged_chunks")
+    assert_close(op(*(t.to(cuda_device) for t in data)), expected, weight, "bf16")
