@@ -226,25 +226,6 @@ __device__ __forceinline__ void tmem_store_32x16(uint32_t taddr, const uint32_t 
 }
 
 // ---- weights -----------------------------------------------------------------------------------------------------------
-// Two f32 in a 64-bit register, and arithmetic on both at once
-__device__ __forceinline__ uint64_t two(float low, float high) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(low), "f"(high));
-  return d;
-}
-__device__ __forceinline__ void apart(uint64_t v, float& low, float& high) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(low), "=f"(high) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add_two(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 // the largest of three; NaN if any is
 __device__ __forceinline__ float largest(float a, float b, float c) {
   float d;
@@ -257,10 +238,8 @@ template <typename T>
 __device__ __forceinline__ void weigh(const uint32_t (&v)[32], uint64_t scale, uint64_t origin, uint64_t (&sum)[2], uint32_t (&w)[16]) {
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
-    float a, b;
-    apart(fma_two(two(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), scale, origin), a, b);
-    a = exp2_fast(a);
-    b = exp2_fast(b);
+    const float2 x = apart(fma_two(two(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), scale, origin));
+    const float a = exp2_fast(x.x), b = exp2_fast(x.y);
     sum[e & 1] = add_two(sum[e & 1], two(a, b));
     w[e] = Elem<T>::pack2(a, b);
   }
@@ -688,10 +667,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             if (lane == 0) mbar_arrive(p_full + 16 * h);
           }
         }
-        float sums[4];
-        apart(added[0], sums[0], sums[1]);
-        apart(added[1], sums[2], sums[3]);
-        weight_sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        const float2 sums[2] = {apart(added[0]), apart(added[1])};
+        weight_sum += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
         bool by_hand = false;
         if (edge) {
           ok = mbar_wait_warp(vote_full + 8 * h, votes & 1);

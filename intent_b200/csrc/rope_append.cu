@@ -48,28 +48,6 @@ struct RotateParams {
   float eps;
 };
 
-// Two f32 in a 64-bit register, and arithmetic on both at once
-__device__ __forceinline__ uint64_t two(float low, float high) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(low), "f"(high));
-  return d;
-}
-__device__ __forceinline__ float2 apart(uint64_t v) {
-  float2 d;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(v));
-  return d;
-}
-__device__ __forceinline__ uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t mul_two(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
 // A piece of a row: PIECE 16-bit elements
 template <int PIECE>
 struct Piece {
