@@ -19,6 +19,41 @@ int device_sms() {
   return sms;
 }
 
+// Which kernel takes a sequence goes by its rows (new tokens x query heads of a key head).  Those of one tile, up to sixteen
+// rows, are bound by HBM in the rows kernel; with more rows it reads and multiplies the cache once for every tile.  us for 64
+// sequences of up to 4000 tokens, 32 heads of 128 on 8 key heads, 1 / 4 / 8 / 16 new tokens each: rows 98 / 103 / 189 / 345, chunk
+// 146 / 146 / 147 / 146; one sequence of 8000: rows 14 / 17 / 20 / 30, chunk 24 throughout.  With heads of 64 two tiles still are
+// (64 heads on 8, 4 / 8 new tokens: rows 105 / 185, chunk 128 / 130).
+// The host knows the number of all rows only, so a call may need both kernels, each for its sequences (`few`):
+//  * more rows than one tile each on average: the chunk kernel, in calls of many sequences beside the rows kernel for those of
+//    one tile (20 single tokens beside 4 chunks of up to 500: 169 -> 160 us, with tiles of eight 144; of few sequences the two
+//    launches cost more than that: 3 prompts 120 -> 128);
+//  * no more: the rows kernel, and the chunk kernel for those of more than two tiles.  768 tokens beside 255 single ones (up to
+//    8192, as above): 1375 us by the rows kernel alone, 802 by both; 2000 beside 199 (16 heads on 16): 1175 and 618; 128 beside
+//    64: 163 and 135.  Where no sequence turns out to have so many that costs a launch (64 of 4 tokens 111 and 118), so calls in
+//    which none can have more than MOST rows, if each has a token, leave it out: 49 tokens beside 15 single ones 62 and 66 (but of
+//    up to 16384 189 and 139), 16 of 4 tokens 40 and 47.
+struct Choice {
+  int tile_rows;           // of the rows kernel; 0: it is not needed
+  int few;                 // rows up to which a sequence is its
+  bool chunks;             // the chunk kernel is needed
+};
+Choice choose(int64_t tokens, int64_t batch, int64_t group, int64_t dim, bool may_chunk) {
+  constexpr int FEW = 16, MANY = 8, MOST = 256;
+  const int64_t rows = tokens * group, most = tokens < batch ? rows : (tokens - batch + 1) * group;
+  const bool usual = rows <= (dim == 64 ? 2 * FEW : FEW) * batch;
+  const bool narrow = rows <= FEW / 2 * batch || (!usual && group <= FEW / 2);
+  Choice c;
+  c.chunks = may_chunk && !(usual && (batch < MANY || most <= MOST));
+  c.few = !c.chunks ? std::numeric_limits<int>::max() : batch < MANY ? 0 : usual ? 2 * FEW : narrow ? FEW / 2 : FEW;
+  if (c.few < group) c.few = 0;            // (no sequence has so few)
+  c.tile_rows = c.few == 0 ? 0 : narrow ? FEW / 2 : FEW;
+  return c;
+}
+int64_t workspace_bytes_of(int64_t dim, bool chunks) {
+  return kPagedHeader + paged_rows_parts_bytes(dim) + (chunks ? paged_chunk_parts_bytes(dim) : 0);
+}
+
 template <typename T>
 int attend(const View3& q, const View4& k_cache, const View4& v_cache, const View2& table, const View1* offsets,
            const View1& lengths, const View3& out, int32_t scale_bits, int32_t window, void* workspace, int64_t workspace_bytes,
@@ -49,12 +84,6 @@ int attend(const View3& q, const View4& k_cache, const View4& v_cache, const Vie
     return cuda_status(cudaMemsetAsync(out.p, 0, size_t(tokens * heads * dim) * 2, stream));
   }
   if (!k_cache.p || !v_cache.p || !table.p) return INTENT_B200_ERR_NULL;
-  if (!workspace || workspace_bytes < intent_b200_paged_attention_workspace_bytes(dim, offsets ? 0 : 1))
-    return INTENT_B200_ERR_WORKSPACE;
-  if (!aligned16(workspace)) return INTENT_B200_ERR_LAYOUT;
-  const int sms = device_sms();
-  if (sms <= 0) return INTENT_B200_ERR_CUDA;
-
   PagedParams p = {};
   p.q = static_cast<const uint16_t*>(q.p);
   p.q_token = q.s0, p.q_head = q.s1;
@@ -68,53 +97,47 @@ int attend(const View3& q, const View4& k_cache, const View4& v_cache, const Vie
   while ((int64_t(1) << p.page_shift) < page) ++p.page_shift;
   p.window = window < p.capacity ? window : 0;   // (a query that sees as many tokens as there may be sees all)
   p.scale = scale * 1.44269504f;         // log2(e): the exponentials are powers of two
+  const Choice choice = choose(tokens, batch, p.group, dim, offsets && paged_chunk_takes(p));
+  p.few = choice.few;
+  if (!workspace || workspace_bytes < workspace_bytes_of(dim, choice.chunks)) return INTENT_B200_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return INTENT_B200_ERR_LAYOUT;
+  const int sms = device_sms();
+  if (sms <= 0) return INTENT_B200_ERR_CUDA;
+
   p.status = static_cast<int*>(workspace);
   p.joins = static_cast<unsigned char*>(workspace) + kPagedRowsJoins;
   p.parts = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + kPagedHeader);
-  // Which kernel takes a sequence goes by its rows (new tokens x query heads of a key head).  Those of one tile, up to sixteen
-  // rows, are bound by HBM in the rows kernel; with more rows it reads and multiplies the cache once for every tile.  us for 64
-  // sequences of up to 4000 tokens, 32 heads of 128 on 8 key heads, 1 / 4 / 8 / 16 new tokens each: rows 98 / 103 / 189 / 345, chunk
-  // 146 / 146 / 147 / 146; one sequence of 8000: rows 14 / 17 / 20 / 30, chunk 24 throughout.  With heads of 64 two tiles still are
-  // (64 heads on 8, 4 / 8 new tokens: rows 105 / 185, chunk 128 / 130).
-  // The host knows the number of all rows only, so a call may need both kernels, each for its sequences (`few`):
-  //  * more rows than one tile each on average: the chunk kernel, in calls of many sequences beside the rows kernel for those of
-  //    one tile (20 single tokens beside 4 chunks of up to 500: 169 -> 160 us, with tiles of eight 144; of few sequences the two
-  //    launches cost more than that: 3 prompts 120 -> 128);
-  //  * no more: the rows kernel, and the chunk kernel for those of more than two tiles.  768 tokens beside 255 single ones (up to
-  //    8192, as above): 1375 us by the rows kernel alone, 802 by both; 2000 beside 199 (16 heads on 16): 1175 and 618; 128 beside
-  //    64: 163 and 135.  Where no sequence turns out to have so many that costs a launch (64 of 4 tokens 111 and 118), so calls in
-  //    which none can have more than MOST rows, if each has a token, leave it out: 49 tokens beside 15 single ones 62 and 66 (but of
-  //    up to 16384 189 and 139), 16 of 4 tokens 40 and 47.
-  constexpr int FEW = 16, MANY = 8, MOST = 256;
   const WorkspaceTurn turn(workspace);
   const int grid = std::min(sms, kPagedCtas);
-  const int64_t rows = tokens * p.group, most = tokens < batch ? rows : (tokens - batch + 1) * p.group;
-  const bool usual = rows <= (dim == 64 ? 2 * FEW : FEW) * batch;
-  const bool narrow = rows <= FEW / 2 * batch || (!usual && p.group <= FEW / 2);
-  const bool chunks = offsets && paged_chunk_takes(p) && !(usual && (batch < MANY || most <= MOST));
-  p.few = !chunks ? std::numeric_limits<int>::max() : batch < MANY ? 0 : usual ? 2 * FEW : narrow ? FEW / 2 : FEW;
-  if (p.few < p.group) p.few = 0;          // (no sequence has so few)
-  const int tile_rows = p.few == 0 ? 0 : narrow ? FEW / 2 : FEW;
   PagedParams chunk = p;
-  if (tile_rows > 0) {
-    const int status = paged_rows<T>(p, dim, tile_rows, k_cache.p, v_cache.p, grid, stream);
+  if (choice.tile_rows > 0) {
+    const int status = paged_rows<T>(p, dim, choice.tile_rows, k_cache.p, v_cache.p, grid, stream);
     if (status != INTENT_B200_OK) return status;
   }
-  if (chunks) {
+  if (choice.chunks) {
     chunk.joins = static_cast<unsigned char*>(workspace) + kPagedChunkJoins;
     chunk.parts += paged_rows_parts_bytes(dim) / int64_t(sizeof(float));
     chunk.half_tokens = paged_chunk_half_tokens(p);
     const int status = paged_chunk<T>(chunk, dim, k_cache.p, v_cache.p, grid, stream);
     if (status != INTENT_B200_OK) return status;
   }
-  return paged_join<T>(p, tile_rows, chunk, chunks, dim, grid, stream);
+  return paged_join<T>(p, choice.tile_rows, chunk, choice.chunks, dim, grid, stream);
 }
 
 }  // namespace
 }  // namespace ib200
 
 extern "C" int64_t intent_b200_paged_attention_workspace_bytes(int64_t dim, int32_t single) {
-  return ib200::kPagedHeader + ib200::paged_rows_parts_bytes(dim) + (single ? 0 : ib200::paged_chunk_parts_bytes(dim));
+  return ib200::workspace_bytes_of(dim, !single);
+}
+// The same for one call of paged_attention: with few rows it needs as much as single tokens do.
+extern "C" int64_t intent_b200_paged_attention_call_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t k_heads,
+                                                                    int64_t dim) {
+  if (tokens <= 0 || batch <= 0 || k_heads <= 0 || q_heads < k_heads || q_heads > 4096) return 0;
+  const int64_t group = q_heads / k_heads;
+  ib200::PagedParams p = {};
+  p.tokens = p.q_heads = 1, p.group = int(group);      // (what its strides may rule out asks for less)
+  return ib200::workspace_bytes_of(dim, ib200::choose(tokens, batch, group, dim, ib200::paged_chunk_takes(p)).chunks);
 }
 
 // Reads the status word at the head of a workspace after synchronising `stream`, and clears it.

@@ -930,14 +930,20 @@ paged_kv_append = KernelDefinition(
 
 
 @cache
-def _paged_workspace_bytes(dim, single):
+def _paged_workspace_query(name, arguments):
     import ctypes
 
     from .runtime import native
 
-    query = native.library()["intent_b200_paged_attention_workspace_bytes"]
-    query.restype, query.argtypes = ctypes.c_int64, [ctypes.c_int64, ctypes.c_int32]
-    return int(query(dim, 1 if single else 0))
+    query = native.library()[f"intent_b200_paged_attention_{name}"]
+    query.restype, query.argtypes = ctypes.c_int64, [ctypes.c_int64] * arguments
+    return query
+
+
+def _paged_workspace_bytes(d, single):
+    if single:
+        return int(_paged_workspace_query("workspace_bytes", 2)(d["D"], 1))
+    return int(_paged_workspace_query("call_workspace_bytes", 5)(d["T"], d["B"], d["HQ"], d["HK"], d["D"]))
 
 
 def _lower_paged(c, device, *, single):
@@ -965,7 +971,7 @@ def _lower_paged(c, device, *, single):
     return NativeProgram(interface=PublicInterface(tuple(views), dimension_rules=rules), device=device,
                          entry_name=f"intent_b200_{stem}_{act.name}",
                          constants=(bits, window),
-                         workspace=lambda d: _paged_workspace_bytes(d["D"], single),
+                         workspace=lambda d: _paged_workspace_bytes(d, single),
                          empty=lambda d: d["B"] == 0 or (not single and d["T"] == 0),
                          workspace_status="intent_b200_paged_attention_workspace_status")
 

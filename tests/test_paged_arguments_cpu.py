@@ -48,3 +48,17 @@ def test_where_the_positions_of_a_step_end():
     assert store.step({"a": 20, "b": 3}).longest == 20
     assert store.step({"b": 1}).longest == 4
     assert store.step({"a": 0, "b": 2}).longest == 6 and store.step({"a": 0}).longest == 0
+
+
+def test_workspace_of_a_call():
+    """The parts of chunks, 40 MB with heads of 128, are asked for by calls that may have chunks only."""
+    query = ib.compile(ib.programs.paged_attention, resolve_target=False).runtime._workspace_spec
+    single = ib.compile(ib.programs.paged_decode_attention, resolve_target=False).runtime._workspace_spec
+    sizes = {"HQ": 32, "HK": 8, "D": 128}
+    few = single({**sizes, "B": 64})
+    assert few < 4 << 20
+    for T, B in ((1, 1), (64, 64), (4, 1), (64, 16), (100, 90)):
+        assert query({**sizes, "T": T, "B": B}) == few
+    for T, B in ((33, 1), (800, 64), (1023, 256), (4096, 1), (1 << 20, 1)):
+        assert query({**sizes, "T": T, "B": B}) > 40 << 20
+    assert query({"HQ": 130, "HK": 1, "D": 128, "T": 4096, "B": 1}) == few       # (heads that the chunk kernel does not take)
