@@ -385,7 +385,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       const int rows = min(1 << p.page_shift, STEP);                   // of a box
       const int boxes = STEP / rows;                                   // of 64 elements of a step
       const int cache_rows = (p.pages * p.k_heads) << p.page_shift;
-      uint32_t u = 0, parts = 0, odd = 0;                              // odd: keys asked for whose values were given up on
+      uint32_t u = 0, parts = 0, odd = 0;                     // odd: keys asked for whose values were given up on
       walk(p, at_first, end, [&](const Sequence& s, int b, int head, int tile, int step, int steps, int all, int at) {
         const uint32_t place = parts & 3;
         ok = mbar_wait_warp(part_empty + 8 * place, (parts / 4 & 1) ^ 1) && mbar_wait_warp(q_empty, (parts & 1) ^ 1);
@@ -443,8 +443,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       }
       // (also where another warp gave up: no load may be on its way to a CTA that is gone)
       if (parts > 0) mbar_wait_warp(q_full, (parts - 1) & 1);
-      const uint32_t loads = 2 * u + odd;
-      for (uint32_t i = loads > SLOTS ? loads - SLOTS : 0; i < loads; ++i) mbar_wait_warp(kv_full + 8 * (i % SLOTS), i / SLOTS & 1);
+      const uint32_t loads = 2 * u + odd, last = loads - 1 - lane;
+      if (lane < min(loads, uint32_t(SLOTS))) mbar_wait(kv_full + 8 * (last % SLOTS), last / SLOTS & 1, 1u << 12);
+      __syncwarp();
     } else if (warp == MMA_WARP) {
       // ------------------------------ products ------------------------------------
       constexpr uint32_t FORMAT = std::is_same<T, __half>::value ? 0 : 1;
