@@ -507,7 +507,7 @@ INTENT_B200_API int intent_b200_quantized_projection(INTENT_B200_VIEW3(a0), INTE
 
 /* ------------------------------------------------------------------------
  * Norms and rotation of queries and keys; append to a paged cache
- * (no counterpart in the reference: its examples stop at the projections).
+ * (an interface of its own; the reference's attention programs are not among those that this library stands in for).
  *   q [T, HQ, D], k and v [T, HK, D]   f16 | bf16, D 64 or 128; rows may lie at any strides that keep each on a
  *                                      16-byte boundary (slices of one projection's output), the last axis contiguous
  *   positions [T] i32, rotary [P, R] f32: row p holds the cosines of R / 2 angles, then their sines; R a multiple of
@@ -516,7 +516,8 @@ INTENT_B200_API int intent_b200_quantized_projection(INTENT_B200_VIEW3(a0), INTE
  *   pairs                              0 = (i, i + R/2), 1 = (2i, 2i + 1);  eps_bits: the f32 eps
  *   slots [T] i64                      page * PAGE + place in the page; outside the cache (-1): the token is not stored
  *   k_cache, v_cache [PAGES, HK, PAGE, D]   PAGE a power of two from 16 to 256
- * f32 arithmetic, one rounding.  A position outside the table gives NaN.  Two tokens with one slot: either is stored.
+ * f32 arithmetic, one rounding.  A position outside the table gives NaN.  Two tokens with one slot:
+ * which one's elements are stored is undefined, for every 8 bytes of keys and values.
  * ------------------------------------------------------------------------ */
 INTENT_B200_API int intent_b200_qk_rope_f16(INTENT_B200_VIEW3(q), INTENT_B200_VIEW3(k), INTENT_B200_VIEW1(positions),
                                          INTENT_B200_VIEW2(rotary), INTENT_B200_VIEW3(q_out), INTENT_B200_VIEW3(k_out),
@@ -556,15 +557,17 @@ INTENT_B200_API int intent_b200_paged_kv_append_norm_bf16(INTENT_B200_VIEW3(q), 
                                                       int32_t eps_bits, int32_t pairs, void* stream);
 
 /* ------------------------------------------------------------------------
- * Attention over a paged cache (no counterpart in the reference).
+ * Attention over a paged cache (an interface of its own, as above).
  *   q, out [T, HQ, D]                  q may be strided as above; HQ a multiple of HK
  *   k_cache, v_cache [PAGES, HK, PAGE, D]
  *   page_table [B, W] i32              token j of sequence b lies in page page_table[b, j / PAGE]
  *   query_offsets [B + 1] i32          rows of q of sequence b (paged_attention); row b (paged_decode_attention, T = B)
- *   kv_lengths [B] i32                 tokens of sequence b in the cache, the new ones among them
+ *   kv_lengths [B] i32                 tokens of sequence b in the cache, the new ones among them; more than W * PAGE count as
+ *                                      W * PAGE
  * Query i of n sees the tokens j <= kv_length - n + i, with window > 0 only the last `window` of them.  No such token: a row
  * of zeros; a row all of whose scores are -infinity, as one with a score of +infinity, is NaN.  Tokens behind kv_length, ahead of the window, in pages that the table does not name or whose number lies
- * outside the cache are not read, whatever the memory there holds.  Rows of q that no sequence has are left alone.
+ * outside the cache are not read, whatever the memory there holds.  Rows of out that no sequence has are
+ * left alone, but for a cache or a table of no pages, where all of out is zero.
  * Limits: T * HQ and W * PAGE up to 2^30, PAGES * HK * PAGE below 2^31 rows (any number of elements), HQ up to 4096.
  * scale_bits: the f32 factor of the scores (> 0; 0: 1 / sqrt(D)).  f32 statistics and sums.
  * workspace: at least ..._workspace_bytes(D, 0) bytes (paged_decode_attention: (D, 1); a call of paged_attention of few rows

@@ -8,7 +8,7 @@ stream; no step reads a device value back to the host.
 
     cache = PagedKVCache(layers=2, pages=1024, kv_heads=8, head_dim=128)
     layer = W4A16Attention(hidden=4096, heads=32, kv_heads=8, head_dim=128)
-    rotary = rotary_table(32768, 128)
+    rotary = rotary_table(32768, 128, device="cuda")
     step = cache.step({"a": 700, "b": 45})                  # two prompts: their tokens' rows in this order
     y = layer.forward(x, weights, rotary, *cache.layer(0), step)
     step = cache.step({"a": 1, "b": 1})                     # a token each
@@ -26,7 +26,8 @@ from .targets import B200Target
 
 
 def rotary_table(positions: int, rotary_dim: int, *, base: float = 10000.0, device=None):
-    """[positions, rotary_dim] f32: row p holds cos and then sin of p * base^(-2 i / rotary_dim), worked out in 64 bits."""
+    """[positions, rotary_dim] f32: row p holds cos and then sin of p * base^(-2 i / rotary_dim), worked out in 64 bits
+    (on the CPU where no device is given)."""
     import torch
 
     if positions <= 0 or rotary_dim <= 0 or rotary_dim % 16:

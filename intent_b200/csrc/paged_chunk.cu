@@ -18,7 +18,7 @@
 // Keys and values come through a ring of TMA boxes of one page's rows each (128B swizzle, one lane per box); boxes of tokens
 // that no query of the tile sees are asked for behind the cache's end, where TMA fills in zeros.
 //
-// Measured on one B200: 4096 tokens behind 12288, 32 heads of 128 on 8 key heads, bf16: 0.91 ms, 1.06 PFLOP/s of what the queries
+// Measured on one B200: 4096 tokens behind 12288, 32 heads of 128 on 8 key heads, bf16: 0.92 ms, 1.05 PFLOP/s of what the queries
 // see, at the power cap (1.6 GHz, 1000 W).  A step takes 3500 cycles there: the tensor core is busy for 58 % of them (a half's two
 // products take 1440, as both operands of S come through shared memory), the exponential unit for 59 %; the rest is the chain of
 // one half, scores to registers, exponentials (1450), weights back, which two halves do not hide altogether.  With the arithmetic
@@ -97,8 +97,8 @@ __device__ __forceinline__ int steps_of(const PagedParams& p, const Sequence& s,
   return (end + STEP - 1) / STEP - first_step(p, s, j);
 }
 
-// sum of floor((a j + b) / 128) over j < n, for n < 2^24: the whole parts of a / 128 and b / 128, then the same with the
-// remainder of a as the divisor
+// sum of floor((a j + b) / 128) over j < n, for n < 2^24, by Euclid's algorithm (the reciprocity of such sums: Graham, Knuth,
+// Patashnik, Concrete Mathematics, 3.5): the whole parts of a / 128 and b / 128, then the same with the remainder of a as the divisor
 __device__ __forceinline__ unsigned long long floor_sum(unsigned n, unsigned a, unsigned b) {
   static_assert(STEP == 128, "the divisor that it begins with");
   unsigned long long sum = (unsigned long long)(n * (n - 1ull) / 2) * (a >> 7) + (unsigned long long)n * (b >> 7);

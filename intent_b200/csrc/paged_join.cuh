@@ -1,4 +1,4 @@
-// Joins of attention over a paged cache: the parts of the tiles that CTA boundaries cut, added in the CTAs' order.
+// What the kernels of attention over a paged cache leave to the joins (paged_join.cu).
 #pragma once
 
 #include "common.cuh"

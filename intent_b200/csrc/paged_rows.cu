@@ -4,8 +4,8 @@
 // L tokens in the cache (p = L - n + i), over the tokens j with max(0, p - W + 1) <= j <= p (W = 0: no window)
 //   o = sum_j softmax_j(scale * x . k_j) * v_j,     zero where there is no such token, NaN where all scores are -infinity
 // Token j of sequence b lies in page page_table[b, j / PAGE]; the tokens of a page number outside the cache are not seen.
-// All statistics and sums are in f32; the weights of one product with V are rounded to the 16-bit type (relative to the
-// running maximum, so at most 1), as the tensor core takes them.
+// All statistics and sums are in f32; the weights of one product with V are rounded to the 16-bit type (relative to a maximum
+// that a score may exceed by SLACK before it is raised, so at most 2^8), as the tensor core takes them.
 //
 // Bound by HBM: a token's keys and values (4 D bytes per key head) are read once for the whole group of query heads that share
 // them.  What has to be right for that:
@@ -22,7 +22,7 @@
 //
 // Measured on one B200 (6530 GB/s copied): 64 histories of up to 8192 tokens, 32 heads of 128 on 8 key heads, bf16: 181 us, 6.24
 // TB/s; 4 of up to 131072 on 4 key heads: 108 us, 5.9 TB/s; 200 of up to 2048, 16 heads of 64: 149 us, 5.9 TB/s.  One history of
-// 1000 tokens, 7.3 us: the reads one after another of a launch (lengths, page numbers, keys, parts) and its join.
+// 1000 tokens, 7.9 us: the reads one after another of a launch (lengths, page numbers, keys, parts) and its join.
 #include <cstring>
 
 #include "common.cuh"

@@ -20,7 +20,7 @@
 //
 // Measured on one B200: append of 8192 tokens, 32 + 8 + 8 heads of 128, norm, bf16: 42.5 us, 4.8 TB/s (with the angles read for
 // every row 66; pieces of eight elements 45; two rows per group 45, eight 42); 6001 tokens, heads of 64, no norm, f16: 11.2 us.
-// One token, 5.9 us, is the host's time for a call.
+// One token, 6.4 us, is the host's time for a call.
 #include <cstring>
 
 #include "common.cuh"

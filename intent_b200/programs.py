@@ -921,12 +921,12 @@ def _lower_rotation(c, device, *, cache):
 _ROTATION_CONSTEXPRS = {"ACT_DTYPE": "bf16", "NORM": True, "EPS": 1e-6, "PAIRS": "halves"}
 qk_norm_rope = KernelDefinition(
     "qk_norm_rope", dict(_ROTATION_CONSTEXPRS), lambda c, d: _lower_rotation(c, d, cache=False),
-    "no counterpart in the reference (its examples stop at the projections)",
+    "an interface of its own (the reference's attention programs are not ported)",
     "q and k normalised per head (NORM) and rotated by position, f32 arithmetic, one rounding")
 paged_kv_append = KernelDefinition(
     "paged_kv_append", dict(_ROTATION_CONSTEXPRS), lambda c, d: _lower_rotation(c, d, cache=True),
-    "no counterpart in the reference (its examples stop at the projections)",
-    "as qk_norm_rope, the keys and with them the values stored in a paged cache at slots[t] (-1: not stored)")
+    "an interface of its own (the reference's attention programs are not ported)",
+    "as qk_norm_rope, the keys and with them the values stored in a paged cache at slots[t] (-1: not stored; every slot once)")
 
 
 @cache
@@ -979,11 +979,11 @@ def _lower_paged(c, device, *, single):
 _PAGED_CONSTEXPRS = {"ACT_DTYPE": "bf16", "SCALE": None, "WINDOW": 0}
 paged_attention = KernelDefinition(
     "paged_attention", dict(_PAGED_CONSTEXPRS), lambda c, d: _lower_paged(c, d, single=False),
-    "no counterpart in the reference (its examples stop at the projections)",
+    "an interface of its own (the reference's attention programs are not ported)",
     "causal attention of each sequence's new tokens over its pages, any number of them per sequence")
 paged_decode_attention = KernelDefinition(
     "paged_decode_attention", dict(_PAGED_CONSTEXPRS), lambda c, d: _lower_paged(c, d, single=True),
-    "no counterpart in the reference (its examples stop at the projections)",
+    "an interface of its own (the reference's attention programs are not ported)",
     "attention of one new token per sequence over its pages")
 
 ALL.update({d.name: d for d in (qk_norm_rope, paged_kv_append, paged_attention, paged_decode_attention)})
