@@ -571,7 +571,7 @@ INTENT_B200_API int intent_b200_paged_kv_append_norm_bf16(INTENT_B200_VIEW3(q), 
  * Limits: T * HQ and W * PAGE up to 2^30, PAGES * HK * PAGE below 2^31 rows (any number of elements), HQ up to 4096.
  * scale_bits: the f32 factor of the scores (> 0; 0: 1 / sqrt(D)).  f32 statistics and sums.
  * workspace: at least ..._workspace_bytes(D, 0) bytes (paged_decode_attention: (D, 1); a call of paged_attention of few rows
- * needs no more than that, which ..._call_workspace_bytes(T, B, HQ, HK, D) tells), 16-byte aligned, its first four zero
+ * needs no more than that, which ..._call_workspace_bytes(T, B, HQ, HK, D, W * PAGE, window) tells), 16-byte aligned, its first four zero
  * before the first launch.  Launches that may overlap need separate ones; host threads that call on one stream may share one.
  * Bytes 0..3: INTENT_B200_ERR_TIMEOUT of a bounded wait that gave up, INTENT_B200_ERR_SHAPE where a multiprocessor would
  * have 2^30 or more steps of 128 tokens to go through (many minutes; nothing is written then); ..._workspace_status reads and
@@ -597,7 +597,8 @@ INTENT_B200_API int intent_b200_paged_decode_attention_bf16(INTENT_B200_VIEW3(q)
                                                         int64_t workspace_bytes, void* stream);
 INTENT_B200_API int64_t intent_b200_paged_attention_workspace_bytes(int64_t dim, int32_t single);
 INTENT_B200_API int64_t intent_b200_paged_attention_call_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads,
-                                                                         int64_t k_heads, int64_t dim);
+                                                                         int64_t k_heads, int64_t dim, int64_t capacity,
+                                                                         int64_t window);
 INTENT_B200_API int intent_b200_paged_attention_workspace_status(void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------

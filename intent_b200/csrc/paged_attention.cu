@@ -30,22 +30,26 @@ int device_sms() {
 //    launches cost more than that: 3 prompts 120 -> 128);
 //  * no more: the rows kernel, and the chunk kernel for those of more than two tiles.  768 tokens beside 255 single ones (up to
 //    8192, as above): 1375 us by the rows kernel alone, 802 by both; 2000 beside 199 (16 heads on 16): 1175 and 618; 128 beside
-//    64: 163 and 135.  Where no sequence turns out to have so many that costs a launch (64 of 4 tokens 111 and 118), so calls in
-//    which none can have more than MOST rows, if each has a token, leave it out: 49 tokens beside 15 single ones 62 and 66 (but of
-//    up to 16384 189 and 139), 16 of 4 tokens 40 and 47.
+//    64: 163 and 135.  Where no sequence turns out to have so many, that costs a launch that finds nothing to do: 64 of 4 tokens 111
+//    and 118.  So it is left out where it can win little: the rows that one sequence may have, if each has a token, times the
+//    tokens that they may walk through, up to MOST.  us without and with it: 49 tokens beside 15 single ones of up to 4096 (0.8 M)
+//    62 and 66, of up to 16384 (3.2 M) 189 and 139; 60 beside 63 of up to 4096 (1.0 M) 132 and 128; 22 beside 6 of up to 65536
+//    (5.8 M) 306 and 212; and if there is no long one 16 of 4 tokens 40 and 47, 64 of 2 of up to 300 26 and 31, 4 of 4 of up to
+//    65536 105 and 113.
 struct Choice {
   int tile_rows;           // of the rows kernel; 0: it is not needed
   int few;                 // rows up to which a sequence is its
   bool chunks;             // the chunk kernel is needed
 };
-Choice choose(int64_t tokens, int64_t batch, int64_t group, int64_t dim, bool may_chunk) {
-  constexpr int FEW = 16, MANY = 8, MOST = 256;
+Choice choose(int64_t tokens, int64_t batch, int64_t group, int64_t dim, int64_t capacity, int64_t window, bool may_chunk) {
+  constexpr int FEW = 16, MANY = 8, MOST = 1 << 20;
   const int64_t rows = tokens * group, most = tokens < batch ? rows : (tokens - batch + 1) * group;
   const bool usual = rows <= (dim == 64 ? 2 * FEW : FEW) * batch;
   const bool narrow = rows <= FEW / 2 * batch || (!usual && group <= FEW / 2);
   Choice c;
-  c.chunks = may_chunk && !(usual && (batch < MANY || most <= MOST));
-  c.few = !c.chunks ? std::numeric_limits<int>::max() : batch < MANY ? 0 : usual ? 2 * FEW : narrow ? FEW / 2 : FEW;
+  const int64_t reach = window > 0 ? std::min(capacity, window + most / group) : capacity;   // tokens that its rows may walk through
+  c.chunks = may_chunk && !(usual && (most <= 2 * FEW || most * reach <= MOST));
+  c.few = !c.chunks ? std::numeric_limits<int>::max() : usual ? 2 * FEW : batch < MANY ? 0 : narrow ? FEW / 2 : FEW;
   if (c.few < group) c.few = 0;            // (no sequence has so few)
   c.tile_rows = c.few == 0 ? 0 : narrow ? FEW / 2 : FEW;
   return c;
@@ -97,7 +101,7 @@ int attend(const View3& q, const View4& k_cache, const View4& v_cache, const Vie
   while ((int64_t(1) << p.page_shift) < page) ++p.page_shift;
   p.window = window < p.capacity ? window : 0;   // (a query that sees as many tokens as there may be sees all)
   p.scale = scale * 1.44269504f;         // log2(e): the exponentials are powers of two
-  const Choice choice = choose(tokens, batch, p.group, dim, offsets && paged_chunk_takes(p));
+  const Choice choice = choose(tokens, batch, p.group, dim, p.capacity, p.window, offsets && paged_chunk_takes(p));
   p.few = choice.few;
   if (!workspace || workspace_bytes < workspace_bytes_of(dim, choice.chunks)) return INTENT_B200_ERR_WORKSPACE;
   if (!aligned16(workspace)) return INTENT_B200_ERR_LAYOUT;
@@ -132,12 +136,12 @@ extern "C" int64_t intent_b200_paged_attention_workspace_bytes(int64_t dim, int3
 }
 // The same for one call of paged_attention: with few rows it needs as much as single tokens do.
 extern "C" int64_t intent_b200_paged_attention_call_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t k_heads,
-                                                                    int64_t dim) {
-  if (tokens <= 0 || batch <= 0 || k_heads <= 0 || q_heads < k_heads || q_heads > 4096) return 0;
+                                                                    int64_t dim, int64_t capacity, int64_t window) {
+  if (tokens <= 0 || batch <= 0 || k_heads <= 0 || q_heads < k_heads || q_heads > 4096 || capacity < 0 || window < 0) return 0;
   const int64_t group = q_heads / k_heads;
   ib200::PagedParams p = {};
   p.tokens = p.q_heads = 1, p.group = int(group);      // (what its strides may rule out asks for less)
-  return ib200::workspace_bytes_of(dim, ib200::choose(tokens, batch, group, dim, ib200::paged_chunk_takes(p)).chunks);
+  return ib200::workspace_bytes_of(dim, ib200::choose(tokens, batch, group, dim, capacity, window, ib200::paged_chunk_takes(p)).chunks);
 }
 
 // Reads the status word at the head of a workspace after synchronising `stream`, and clears it.

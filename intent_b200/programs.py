@@ -940,10 +940,11 @@ def _paged_workspace_query(name, arguments):
     return query
 
 
-def _paged_workspace_bytes(d, single):
+def _paged_workspace_bytes(d, single, window):
     if single:
         return int(_paged_workspace_query("workspace_bytes", 2)(d["D"], 1))
-    return int(_paged_workspace_query("call_workspace_bytes", 5)(d["T"], d["B"], d["HQ"], d["HK"], d["D"]))
+    query = _paged_workspace_query("call_workspace_bytes", 7)
+    return int(query(d["T"], d["B"], d["HQ"], d["HK"], d["D"], d["W"] * d["PAGE"], window))
 
 
 def _lower_paged(c, device, *, single):
@@ -971,7 +972,7 @@ def _lower_paged(c, device, *, single):
     return NativeProgram(interface=PublicInterface(tuple(views), dimension_rules=rules), device=device,
                          entry_name=f"intent_b200_{stem}_{act.name}",
                          constants=(bits, window),
-                         workspace=lambda d: _paged_workspace_bytes(d, single),
+                         workspace=lambda d: _paged_workspace_bytes(d, single, window),
                          empty=lambda d: d["B"] == 0 or (not single and d["T"] == 0),
                          workspace_status="intent_b200_paged_attention_workspace_status")
 

@@ -54,11 +54,14 @@ def test_workspace_of_a_call():
     """The parts of chunks, 40 MB with heads of 128, are asked for by calls that may have chunks only."""
     query = ib.compile(ib.programs.paged_attention, resolve_target=False).runtime._workspace_spec
     single = ib.compile(ib.programs.paged_decode_attention, resolve_target=False).runtime._workspace_spec
-    sizes = {"HQ": 32, "HK": 8, "D": 128}
+    sizes = {"HQ": 32, "HK": 8, "D": 128, "PAGE": 64, "W": 512}
     few = single({**sizes, "B": 64})
     assert few < 4 << 20
-    for T, B in ((1, 1), (64, 64), (4, 1), (64, 16), (100, 90)):
+    for T, B in ((1, 1), (64, 64), (4, 1), (96, 89)):
         assert query({**sizes, "T": T, "B": B}) == few
-    for T, B in ((33, 1), (800, 64), (1023, 256), (4096, 1), (1 << 20, 1)):
+    for T, B in ((33, 1), (64, 16), (800, 64), (1023, 256), (4096, 1), (1 << 20, 1)):
         assert query({**sizes, "T": T, "B": B}) > 40 << 20
-    assert query({"HQ": 130, "HK": 1, "D": 128, "T": 4096, "B": 1}) == few       # (heads that the chunk kernel does not take)
+    assert query({**sizes, "T": 64, "B": 16, "W": 64}) == few                    # (histories that are short)
+    assert query({**sizes, "HQ": 130, "HK": 1, "T": 4096, "B": 1}) == few        # (heads that the chunk kernel does not take)
+    narrow = ib.compile(ib.programs.paged_attention, constexprs={"WINDOW": 100}, resolve_target=False).runtime._workspace_spec
+    assert narrow({**sizes, "T": 64, "B": 16}) == few

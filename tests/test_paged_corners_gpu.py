@@ -63,21 +63,38 @@ def lengths_of(counts, seed, most=150):
     ([1] * 50 + [90] + [1] * 49, 8, 2, 128, 3),                    # in tiles of eight
     ([8, 9, 70, 0, 1, 3, 33] + [1] * 80, 8, 2, 64, 3),             # sequences of up to four tiles, more than that, none
     ([300] + [1] * 40, 16, 1, 64, 3),
-    ([60] + [1] * 30, 4, 4, 64, 2),                                # so few that one kernel takes all
-    ([4] * 12, 4, 2, 128, 2),
+    ([31] + [1] * 30, 4, 4, 64, 2),                                # so few that one kernel takes all
+    ([60] + [1] * 30, 4, 4, 64, 3),
+    ([3] * 12, 4, 4, 128, 2),
     ([1] * 70, 32, 1, 64, 2),
     ([0] * 90 + [75] + [0] * 9, 8, 2, 64, 3),                      # (a step of a fixed number of places, most of them empty)
 ])
 def test_a_chunk_beside_many_single_tokens(cuda_device, counts, HQ, HK, D, launches):
-    """What takes a sequence goes by its own new tokens, whatever the others have on average."""
+    """What takes a sequence goes by its own new tokens, whatever the others have on average, where its history may be long: that
+    is what the page table has room for."""
     data = make(lengths_of(counts, len(counts)), counts, HQ, HK, D, 16, "bf16")
     expected, weight = oracle.paged_attention(*data)
+    table = torch.cat([data[3], torch.full((len(counts), 2048), -1, dtype=torch.int32)], 1)
+    data = (*data[:3], table, *data[4:])
     artifact = ib.compile(ib.programs.paged_attention)
     assert_close(run(artifact, cuda_device, *data, False), expected, weight, "bf16")
     before = native.launch_count()
     assert_close(run(artifact, cuda_device, *data, False), expected, weight, "bf16")
     assert native.launch_count() - before == launches
     artifact.check()
+
+
+def test_chunks_of_short_histories(cuda_device):
+    """One kernel takes a call whose page table has room for little, or whose window leaves little of it."""
+    counts = [150] + [1] * 59
+    q, k, v, table, offsets, n = make(lengths_of(counts, 3), counts, 8, 2, 128, 16, "bf16")
+    wide = torch.cat([table, torch.full((60, 2048), -1, dtype=torch.int32)], 1)
+    for pages, window, launches in ((table, 0, 2), (wide, 0, 3), (wide, 100, 2)):
+        expected, weight = oracle.paged_attention(q, k, v, table, offsets, n, window=window)
+        before = native.launch_count()
+        out = attend(cuda_device, (q, k, v, pages, offsets, n), kernel=ROWS, WINDOW=window)
+        assert native.launch_count() - before == launches
+        assert_close(out, expected, weight, "bf16")
 
 
 def test_heads_too_many_for_the_rows_kernel(cuda_device):
