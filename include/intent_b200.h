@@ -565,17 +565,18 @@ INTENT_B200_API int intent_b200_paged_kv_append_norm_bf16(INTENT_B200_VIEW3(q), 
  *   kv_lengths [B] i32                 tokens of sequence b in the cache, the new ones among them; more than W * PAGE count as
  *                                      W * PAGE
  * Query i of n sees the tokens j <= kv_length - n + i, with window > 0 only the last `window` of them.  No such token: a row
- * of zeros; a row all of whose scores are -infinity, as one with a score of +infinity, is NaN.  Tokens behind kv_length, ahead of the window, in pages that the table does not name or whose number lies
- * outside the cache are not read, whatever the memory there holds.  Rows of out that no sequence has are
- * left alone, but for a cache or a table of no pages, where all of out is zero.
+ * of zeros; a row all of whose scores are -infinity, as one with a score of +infinity, is NaN.  Tokens behind kv_length, ahead
+ * of the window, in pages that the table does not name or whose number lies outside the cache are not read, whatever the memory
+ * there holds.  Rows of out that no sequence has are left alone, but for a cache or a table of no pages, where all of out is
+ * zero.
  * Limits: T * HQ and W * PAGE up to 2^30, PAGES * HK * PAGE below 2^31 rows (any number of elements), HQ up to 4096.
  * scale_bits: the f32 factor of the scores (> 0; 0: 1 / sqrt(D)).  f32 statistics and sums.
  * workspace: at least ..._workspace_bytes(D, 0) bytes (paged_decode_attention: (D, 1); a call of paged_attention of few rows
- * needs no more than that, which ..._call_workspace_bytes(T, B, HQ, HK, D, W * PAGE, window) tells), 16-byte aligned, its first four zero
- * before the first launch.  Launches that may overlap need separate ones; host threads that call on one stream may share one.
- * Bytes 0..3: INTENT_B200_ERR_TIMEOUT of a bounded wait that gave up, INTENT_B200_ERR_SHAPE where a multiprocessor would
- * have 2^30 or more steps of 128 tokens to go through (many minutes; nothing is written then); ..._workspace_status reads and
- * clears it.  The same call gives the same bits.
+ * needs no more than that, which ..._call_workspace_bytes(T, B, HQ, HK, D, W * PAGE, window) tells), 16-byte aligned, its first
+ * four zero before the first launch.  Launches that may overlap need separate ones; host threads that call on one stream may
+ * share one.  Bytes 0..3: INTENT_B200_ERR_TIMEOUT of a bounded wait that gave up, INTENT_B200_ERR_SHAPE where a multiprocessor
+ * would have 2^30 or more steps of 128 tokens to go through (many minutes; the rows are not written then);
+ * ..._workspace_status reads and clears it.  The same call gives the same bits.
  * ------------------------------------------------------------------------ */
 INTENT_B200_API int intent_b200_paged_attention_f16(INTENT_B200_VIEW3(q), INTENT_B200_VIEW4(k_cache), INTENT_B200_VIEW4(v_cache),
                                                  INTENT_B200_VIEW2(page_table), INTENT_B200_VIEW1(query_offsets),
