@@ -557,6 +557,42 @@ INTENT_B200_API int intent_b200_paged_kv_append_norm_bf16(INTENT_B200_VIEW3(q), 
                                                       int32_t eps_bits, int32_t pairs, void* stream);
 
 /* ------------------------------------------------------------------------
+ * The same with a cache in 4 bits, and reading it back
+ *   k_codes, v_codes [PAGES, HK, PAGE, D / 2] u8    element 2i of a row in the low half of byte i, element 2i + 1 in the high half
+ *   k_scales, v_scales [PAGES, HK, PAGE, 2 D / group] f16 | bf16   scale s and minimum m, one after the other, of every `group`
+ *                                      (32, 64 or 128, up to D) consecutive elements: a code n stands for m + s * n
+ * append: rows as above; m = min and s = (max - min) / 15 of a group, rounded to the type, n = (x - m) / s rounded to the nearest
+ * (even) of 0 .. 15; n = 0 where s = 0.  Where m + 15 s would be beyond the type, s is the next lower number.  Keys are normalised and rotated in f32 and not rounded before.  A group with something that
+ * is no finite number (or a minimum or scale beyond the type) is stored as s = m = NaN.  Two tokens with one slot: what is stored is
+ * undefined.
+ * read: k, v [T, HK, D] of the tokens at slots [T] i64, m + s * n in f32 rounded to the type; zeros for a slot outside the cache.
+ * ------------------------------------------------------------------------ */
+INTENT_B200_API int intent_b200_paged_kv_append_int4_f16(
+    INTENT_B200_VIEW3(q), INTENT_B200_VIEW3(k), INTENT_B200_VIEW3(v), INTENT_B200_VIEW1(positions), INTENT_B200_VIEW1(slots),
+    INTENT_B200_VIEW2(rotary), INTENT_B200_VIEW4(k_codes), INTENT_B200_VIEW4(k_scales), INTENT_B200_VIEW4(v_codes),
+    INTENT_B200_VIEW4(v_scales), INTENT_B200_VIEW3(q_out), int32_t group, int32_t pairs, void* stream);
+INTENT_B200_API int intent_b200_paged_kv_append_norm_int4_f16(
+    INTENT_B200_VIEW3(q), INTENT_B200_VIEW3(k), INTENT_B200_VIEW3(v), INTENT_B200_VIEW1(positions), INTENT_B200_VIEW1(slots),
+    INTENT_B200_VIEW2(rotary), INTENT_B200_VIEW1(q_weight), INTENT_B200_VIEW1(k_weight), INTENT_B200_VIEW4(k_codes),
+    INTENT_B200_VIEW4(k_scales), INTENT_B200_VIEW4(v_codes), INTENT_B200_VIEW4(v_scales), INTENT_B200_VIEW3(q_out), int32_t group,
+    int32_t eps_bits, int32_t pairs, void* stream);
+INTENT_B200_API int intent_b200_paged_kv_read_int4_f16(
+    INTENT_B200_VIEW1(slots), INTENT_B200_VIEW4(k_codes), INTENT_B200_VIEW4(k_scales), INTENT_B200_VIEW4(v_codes),
+    INTENT_B200_VIEW4(v_scales), INTENT_B200_VIEW3(k), INTENT_B200_VIEW3(v), int32_t group, void* stream);
+INTENT_B200_API int intent_b200_paged_kv_append_int4_bf16(
+    INTENT_B200_VIEW3(q), INTENT_B200_VIEW3(k), INTENT_B200_VIEW3(v), INTENT_B200_VIEW1(positions), INTENT_B200_VIEW1(slots),
+    INTENT_B200_VIEW2(rotary), INTENT_B200_VIEW4(k_codes), INTENT_B200_VIEW4(k_scales), INTENT_B200_VIEW4(v_codes),
+    INTENT_B200_VIEW4(v_scales), INTENT_B200_VIEW3(q_out), int32_t group, int32_t pairs, void* stream);
+INTENT_B200_API int intent_b200_paged_kv_append_norm_int4_bf16(
+    INTENT_B200_VIEW3(q), INTENT_B200_VIEW3(k), INTENT_B200_VIEW3(v), INTENT_B200_VIEW1(positions), INTENT_B200_VIEW1(slots),
+    INTENT_B200_VIEW2(rotary), INTENT_B200_VIEW1(q_weight), INTENT_B200_VIEW1(k_weight), INTENT_B200_VIEW4(k_codes),
+    INTENT_B200_VIEW4(k_scales), INTENT_B200_VIEW4(v_codes), INTENT_B200_VIEW4(v_scales), INTENT_B200_VIEW3(q_out), int32_t group,
+    int32_t eps_bits, int32_t pairs, void* stream);
+INTENT_B200_API int intent_b200_paged_kv_read_int4_bf16(
+    INTENT_B200_VIEW1(slots), INTENT_B200_VIEW4(k_codes), INTENT_B200_VIEW4(k_scales), INTENT_B200_VIEW4(v_codes),
+    INTENT_B200_VIEW4(v_scales), INTENT_B200_VIEW3(k), INTENT_B200_VIEW3(v), int32_t group, void* stream);
+
+/* ------------------------------------------------------------------------
  * Attention over a paged cache (an interface of its own, as above).
  *   q, out [T, HQ, D]                  q may be strided as above; HQ a multiple of HK
  *   k_cache, v_cache [PAGES, HK, PAGE, D]
@@ -577,6 +613,8 @@ INTENT_B200_API int intent_b200_paged_kv_append_norm_bf16(INTENT_B200_VIEW3(q), 
  * share one.  Bytes 0..3: INTENT_B200_ERR_TIMEOUT of a bounded wait that gave up, INTENT_B200_ERR_SHAPE where a multiprocessor
  * would have 2^30 or more steps of 128 tokens to go through (many minutes; the rows are not written then);
  * ..._workspace_status reads and clears it.  The same call gives the same bits.
+ * _int4: over a cache in 4 bits as above, of the values m + s * n; the workspace is the same.  The factor of the scores is at most 2^50
+ * there, bf16 queries below 2^67 and scales of values below 2^55 in magnitude (beyond that a row may be NaN).
  * ------------------------------------------------------------------------ */
 INTENT_B200_API int intent_b200_paged_attention_f16(INTENT_B200_VIEW3(q), INTENT_B200_VIEW4(k_cache), INTENT_B200_VIEW4(v_cache),
                                                  INTENT_B200_VIEW2(page_table), INTENT_B200_VIEW1(query_offsets),
@@ -596,6 +634,22 @@ INTENT_B200_API int intent_b200_paged_decode_attention_bf16(INTENT_B200_VIEW3(q)
                                                         INTENT_B200_VIEW1(kv_lengths), INTENT_B200_VIEW3(out),
                                                         int32_t scale_bits, int32_t window, void* workspace,
                                                         int64_t workspace_bytes, void* stream);
+INTENT_B200_API int intent_b200_paged_attention_int4_f16(
+    INTENT_B200_VIEW3(q), INTENT_B200_VIEW4(k_codes), INTENT_B200_VIEW4(k_scales), INTENT_B200_VIEW4(v_codes),
+    INTENT_B200_VIEW4(v_scales), INTENT_B200_VIEW2(page_table), INTENT_B200_VIEW1(query_offsets), INTENT_B200_VIEW1(kv_lengths),
+    INTENT_B200_VIEW3(out), int32_t group, int32_t scale_bits, int32_t window, void* workspace, int64_t workspace_bytes, void* stream);
+INTENT_B200_API int intent_b200_paged_decode_attention_int4_f16(
+    INTENT_B200_VIEW3(q), INTENT_B200_VIEW4(k_codes), INTENT_B200_VIEW4(k_scales), INTENT_B200_VIEW4(v_codes),
+    INTENT_B200_VIEW4(v_scales), INTENT_B200_VIEW2(page_table), INTENT_B200_VIEW1(kv_lengths), INTENT_B200_VIEW3(out), int32_t group,
+    int32_t scale_bits, int32_t window, void* workspace, int64_t workspace_bytes, void* stream);
+INTENT_B200_API int intent_b200_paged_attention_int4_bf16(
+    INTENT_B200_VIEW3(q), INTENT_B200_VIEW4(k_codes), INTENT_B200_VIEW4(k_scales), INTENT_B200_VIEW4(v_codes),
+    INTENT_B200_VIEW4(v_scales), INTENT_B200_VIEW2(page_table), INTENT_B200_VIEW1(query_offsets), INTENT_B200_VIEW1(kv_lengths),
+    INTENT_B200_VIEW3(out), int32_t group, int32_t scale_bits, int32_t window, void* workspace, int64_t workspace_bytes, void* stream);
+INTENT_B200_API int intent_b200_paged_decode_attention_int4_bf16(
+    INTENT_B200_VIEW3(q), INTENT_B200_VIEW4(k_codes), INTENT_B200_VIEW4(k_scales), INTENT_B200_VIEW4(v_codes),
+    INTENT_B200_VIEW4(v_scales), INTENT_B200_VIEW2(page_table), INTENT_B200_VIEW1(kv_lengths), INTENT_B200_VIEW3(out), int32_t group,
+    int32_t scale_bits, int32_t window, void* workspace, int64_t workspace_bytes, void* stream);
 INTENT_B200_API int64_t intent_b200_paged_attention_workspace_bytes(int64_t dim, int32_t single);
 INTENT_B200_API int64_t intent_b200_paged_attention_call_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads,
                                                                          int64_t k_heads, int64_t dim, int64_t capacity,

@@ -68,12 +68,22 @@ const Row kRows[] = {
     IB200_PACKED(intent_b200_moe_scatter_routes),
     IB200_PACKED(intent_b200_paged_attention_bf16),
     IB200_PACKED(intent_b200_paged_attention_f16),
+    IB200_PACKED(intent_b200_paged_attention_int4_bf16),
+    IB200_PACKED(intent_b200_paged_attention_int4_f16),
     IB200_PACKED(intent_b200_paged_decode_attention_bf16),
     IB200_PACKED(intent_b200_paged_decode_attention_f16),
+    IB200_PACKED(intent_b200_paged_decode_attention_int4_bf16),
+    IB200_PACKED(intent_b200_paged_decode_attention_int4_f16),
     IB200_PACKED(intent_b200_paged_kv_append_bf16),
     IB200_PACKED(intent_b200_paged_kv_append_f16),
+    IB200_PACKED(intent_b200_paged_kv_append_int4_bf16),
+    IB200_PACKED(intent_b200_paged_kv_append_int4_f16),
     IB200_PACKED(intent_b200_paged_kv_append_norm_bf16),
     IB200_PACKED(intent_b200_paged_kv_append_norm_f16),
+    IB200_PACKED(intent_b200_paged_kv_append_norm_int4_bf16),
+    IB200_PACKED(intent_b200_paged_kv_append_norm_int4_f16),
+    IB200_PACKED(intent_b200_paged_kv_read_int4_bf16),
+    IB200_PACKED(intent_b200_paged_kv_read_int4_f16),
     IB200_PACKED(intent_b200_qk_norm_rope_bf16),
     IB200_PACKED(intent_b200_qk_norm_rope_f16),
     IB200_PACKED(intent_b200_qk_rope_bf16),

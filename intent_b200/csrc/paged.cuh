@@ -33,6 +33,22 @@ struct PagedParams {
                                      // are the chunk kernel's (either may get all: INT_MAX, 0)
 };
 
+// Checks of a cache in 4 bits: codes [PAGES, HK, PAGE, D / 2] of 8 bits, scales [PAGES, HK, PAGE, 2 D / GROUP] of the 16-bit type.
+inline int check_int4(const View4& k_codes, const View4& k_scales, const View4& v_codes, const View4& v_scales, int64_t heads,
+                      int64_t dim, int32_t group) {
+  if (group != 32 && group != 64 && group != 128) return INTENT_B200_ERR_UNSUPPORTED;
+  if (group > dim) return INTENT_B200_ERR_UNSUPPORTED;
+  const int64_t pages = k_codes.d0, page = k_codes.d2;
+  for (const View4* v : {&k_codes, &v_codes, &k_scales, &v_scales})
+    if (v->d0 != pages || pages < 0 || v->d1 != heads || v->d2 != page) return INTENT_B200_ERR_SHAPE;
+  if (k_codes.d3 * 2 != dim || v_codes.d3 * 2 != dim || k_scales.d3 * group != 2 * dim || v_scales.d3 * group != 2 * dim)
+    return INTENT_B200_ERR_SHAPE;
+  if (page < 16 || page > 256 || (page & (page - 1)) != 0 || pages > (int64_t(1) << 40) / page) return INTENT_B200_ERR_UNSUPPORTED;
+  for (const View4* v : {&k_codes, &v_codes, &k_scales, &v_scales})
+    if (!contiguous(*v) || !aligned16(v->p)) return INTENT_B200_ERR_LAYOUT;
+  return INTENT_B200_OK;
+}
+
 #ifdef __CUDACC__
 
 template <bool B>
@@ -95,6 +111,14 @@ int64_t paged_rows_parts_bytes(int64_t dim);
 template <typename T>
 int paged_rows(const PagedParams& p, int64_t dim, int tile_rows, const void* k_cache, const void* v_cache, int grid,
                cudaStream_t stream);
+
+// the same over a cache in 4 bits (paged_rows_int4.cu)
+struct Int4Cache {
+  const void *k_codes, *k_scales, *v_codes, *v_scales;
+  int group;
+};
+template <typename T>
+int paged_rows_int4(const PagedParams& p, int64_t dim, int tile_rows, const Int4Cache& cache, int grid, cudaStream_t stream);
 
 // chunks (paged_chunk.cu)
 int64_t paged_chunk_parts_bytes(int64_t dim);

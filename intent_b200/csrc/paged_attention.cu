@@ -9,6 +9,8 @@
 namespace ib200 {
 namespace {
 
+constexpr float kInt4Scale = 0x1p50f;     // (scores over a cache in 4 bits are in a unit of their own)
+
 int device_sms() {
   int device = 0, sms = 0;
   if (cudaGetDevice(&device) != cudaSuccess ||
@@ -58,25 +60,37 @@ int64_t workspace_bytes_of(int64_t dim, bool chunks) {
   return kPagedHeader + paged_rows_parts_bytes(dim) + (chunks ? paged_chunk_parts_bytes(dim) : 0);
 }
 
+// A cache of 16-bit elements, or in 4 bits (its scales and the elements of a group of them)
+struct CacheViews {
+  const View4 &k, &v;
+  const View4 *k_scales, *v_scales;
+  int32_t group;
+};
+
 template <typename T>
-int attend(const View3& q, const View4& k_cache, const View4& v_cache, const View2& table, const View1* offsets,
-           const View1& lengths, const View3& out, int32_t scale_bits, int32_t window, void* workspace, int64_t workspace_bytes,
-           cudaStream_t stream) {
+int attend(const View3& q, const CacheViews& cache, const View2& table, const View1* offsets, const View1& lengths, const View3& out,
+           int32_t scale_bits, int32_t window, void* workspace, int64_t workspace_bytes, cudaStream_t stream) {
+  const View4 &k_cache = cache.k, &v_cache = cache.v;
+  const bool int4 = cache.k_scales != nullptr;
   const int64_t tokens = q.d0, heads = q.d1, dim = q.d2, pages = k_cache.d0, k_heads = k_cache.d1, page = k_cache.d2;
   const int64_t batch = lengths.d0;
-  if (tokens < 0 || batch < 0 || heads <= 0 || k_heads <= 0 || heads % k_heads != 0 || k_cache.d3 != dim || v_cache.d0 != pages ||
-      v_cache.d1 != k_heads || v_cache.d2 != page || v_cache.d3 != dim || table.d0 != batch || out.d0 != tokens ||
+  if (tokens < 0 || batch < 0 || heads <= 0 || k_heads <= 0 || heads % k_heads != 0 || v_cache.d0 != pages ||
+      v_cache.d1 != k_heads || v_cache.d2 != page || (!int4 && (k_cache.d3 != dim || v_cache.d3 != dim)) || table.d0 != batch || out.d0 != tokens ||
       out.d1 != heads || out.d2 != dim || (offsets ? offsets->d0 != batch + 1 : tokens != batch))
     return INTENT_B200_ERR_SHAPE;
   if (dim != 64 && dim != 128) return INTENT_B200_ERR_UNSUPPORTED;
   if (page < 16 || page > 256 || (page & (page - 1)) != 0 || window < 0) return INTENT_B200_ERR_UNSUPPORTED;
+  if (int4) {
+    const int status = check_int4(k_cache, *cache.k_scales, v_cache, *cache.v_scales, k_heads, dim, cache.group);
+    if (status != INTENT_B200_OK) return status;
+  }
   constexpr int64_t kMost = (int64_t(1) << 31) - 1, kHalf = int64_t(1) << 30;   // (differences of positions are 32 bits, too)
   if (heads > 4096 || batch > (1 << 24) || tokens > kHalf / heads || pages > kMost / (k_heads * page) || table.d1 > kHalf / page)
     return INTENT_B200_ERR_UNSUPPORTED;
   float scale;
   std::memcpy(&scale, &scale_bits, sizeof(float));
   if (scale == 0.f) scale = 1.f / std::sqrt(float(dim));
-  if (!(scale > 0.f) || std::isinf(scale)) return INTENT_B200_ERR_UNSUPPORTED;
+  if (!(scale > 0.f) || std::isinf(scale) || (int4 && scale > kInt4Scale)) return INTENT_B200_ERR_UNSUPPORTED;
   if (!rows16(q) || !contiguous(k_cache) || !contiguous(v_cache) || !contiguous(table) || !contiguous(lengths) ||
       !contiguous(out) || (offsets && !contiguous(*offsets)) || !aligned16(q.p) || !aligned16(k_cache.p) ||
       !aligned16(v_cache.p) || !aligned16(out.p))
@@ -87,7 +101,7 @@ int attend(const View3& q, const View4& k_cache, const View4& v_cache, const Vie
     if (observe_sink()) return INTENT_B200_OK;
     return cuda_status(cudaMemsetAsync(out.p, 0, size_t(tokens * heads * dim) * 2, stream));
   }
-  if (!k_cache.p || !v_cache.p || !table.p) return INTENT_B200_ERR_NULL;
+  if (!k_cache.p || !v_cache.p || !table.p || (int4 && (!cache.k_scales->p || !cache.v_scales->p))) return INTENT_B200_ERR_NULL;
   PagedParams p = {};
   p.q = static_cast<const uint16_t*>(q.p);
   p.q_token = q.s0, p.q_head = q.s1;
@@ -101,7 +115,7 @@ int attend(const View3& q, const View4& k_cache, const View4& v_cache, const Vie
   while ((int64_t(1) << p.page_shift) < page) ++p.page_shift;
   p.window = window < p.capacity ? window : 0;   // (a query that sees as many tokens as there may be sees all)
   p.scale = scale * 1.44269504f;         // log2(e): the exponentials are powers of two
-  const Choice choice = choose(tokens, batch, p.group, dim, p.capacity, p.window, offsets && paged_chunk_takes(p));
+  const Choice choice = choose(tokens, batch, p.group, dim, p.capacity, p.window, offsets && !int4 && paged_chunk_takes(p));
   p.few = choice.few;
   if (!workspace || workspace_bytes < workspace_bytes_of(dim, choice.chunks)) return INTENT_B200_ERR_WORKSPACE;
   if (!aligned16(workspace)) return INTENT_B200_ERR_LAYOUT;
@@ -115,7 +129,9 @@ int attend(const View3& q, const View4& k_cache, const View4& v_cache, const Vie
   const int grid = std::min(sms, kPagedCtas);
   PagedParams chunk = p;
   if (choice.tile_rows > 0) {
-    const int status = paged_rows<T>(p, dim, choice.tile_rows, k_cache.p, v_cache.p, grid, stream);
+    const Int4Cache codes = {k_cache.p, int4 ? cache.k_scales->p : nullptr, v_cache.p, int4 ? cache.v_scales->p : nullptr, cache.group};
+    const int status = int4 ? paged_rows_int4<T>(p, dim, choice.tile_rows, codes, grid, stream)
+                            : paged_rows<T>(p, dim, choice.tile_rows, k_cache.p, v_cache.p, grid, stream);
     if (status != INTENT_B200_OK) return status;
   }
   if (choice.chunks) {
@@ -158,22 +174,43 @@ extern "C" int intent_b200_paged_attention_workspace_status(void* workspace, int
   return e == cudaSuccess ? value : ib200::cuda_status(e);
 }
 
+#define IB200_PAGED_TAIL int32_t window, void *workspace, int64_t workspace_bytes, void *stream
 #define IB200_PAGED_ENTRIES(NAME, TYPE)                                                                                    \
   extern "C" int intent_b200_paged_attention_##NAME(                                                                       \
       INTENT_B200_VIEW3(a0), INTENT_B200_VIEW4(a1), INTENT_B200_VIEW4(a2), INTENT_B200_VIEW2(a3), INTENT_B200_VIEW1(a4),   \
-      INTENT_B200_VIEW1(a5), INTENT_B200_VIEW3(a6), int32_t scale_bits, int32_t window, void* workspace,                   \
-      int64_t workspace_bytes, void* stream) {                                                                             \
+      INTENT_B200_VIEW1(a5), INTENT_B200_VIEW3(a6), int32_t scale_bits, IB200_PAGED_TAIL) {                                \
+    const ib200::View4 k = IB200_VIEW4_ARG(a1), v = IB200_VIEW4_ARG(a2);                                                   \
     const ib200::View1 offsets = IB200_VIEW1_ARG(a4);                                                                      \
-    return ib200::attend<TYPE>(IB200_VIEW3_ARG(a0), IB200_VIEW4_ARG(a1), IB200_VIEW4_ARG(a2), IB200_VIEW2_ARG(a3),         \
-                               &offsets, IB200_VIEW1_ARG(a5), IB200_VIEW3_ARG(a6), scale_bits, window, workspace,          \
-                               workspace_bytes, static_cast<cudaStream_t>(stream));                                        \
+    return ib200::attend<TYPE>(IB200_VIEW3_ARG(a0), {k, v, nullptr, nullptr, 0}, IB200_VIEW2_ARG(a3), &offsets,            \
+                               IB200_VIEW1_ARG(a5), IB200_VIEW3_ARG(a6), scale_bits, window, workspace, workspace_bytes,   \
+                               static_cast<cudaStream_t>(stream));                                                         \
   }                                                                                                                        \
   extern "C" int intent_b200_paged_decode_attention_##NAME(                                                                \
       INTENT_B200_VIEW3(a0), INTENT_B200_VIEW4(a1), INTENT_B200_VIEW4(a2), INTENT_B200_VIEW2(a3), INTENT_B200_VIEW1(a4),   \
-      INTENT_B200_VIEW3(a5), int32_t scale_bits, int32_t window, void* workspace, int64_t workspace_bytes, void* stream) { \
-    return ib200::attend<TYPE>(IB200_VIEW3_ARG(a0), IB200_VIEW4_ARG(a1), IB200_VIEW4_ARG(a2), IB200_VIEW2_ARG(a3),         \
-                               nullptr, IB200_VIEW1_ARG(a4), IB200_VIEW3_ARG(a5), scale_bits, window, workspace,           \
-                               workspace_bytes, static_cast<cudaStream_t>(stream));                                        \
+      INTENT_B200_VIEW3(a5), int32_t scale_bits, IB200_PAGED_TAIL) {                                                       \
+    const ib200::View4 k = IB200_VIEW4_ARG(a1), v = IB200_VIEW4_ARG(a2);                                                   \
+    return ib200::attend<TYPE>(IB200_VIEW3_ARG(a0), {k, v, nullptr, nullptr, 0}, IB200_VIEW2_ARG(a3), nullptr,             \
+                               IB200_VIEW1_ARG(a4), IB200_VIEW3_ARG(a5), scale_bits, window, workspace, workspace_bytes,   \
+                               static_cast<cudaStream_t>(stream));                                                         \
+  }                                                                                                                        \
+  extern "C" int intent_b200_paged_attention_int4_##NAME(                                                                  \
+      INTENT_B200_VIEW3(a0), INTENT_B200_VIEW4(a1), INTENT_B200_VIEW4(a2), INTENT_B200_VIEW4(a3), INTENT_B200_VIEW4(a4),   \
+      INTENT_B200_VIEW2(a5), INTENT_B200_VIEW1(a6), INTENT_B200_VIEW1(a7), INTENT_B200_VIEW3(a8), int32_t group,           \
+      int32_t scale_bits, IB200_PAGED_TAIL) {                                                                              \
+    const ib200::View4 k = IB200_VIEW4_ARG(a1), ks = IB200_VIEW4_ARG(a2), v = IB200_VIEW4_ARG(a3), vs = IB200_VIEW4_ARG(a4); \
+    const ib200::View1 offsets = IB200_VIEW1_ARG(a6);                                                                      \
+    return ib200::attend<TYPE>(IB200_VIEW3_ARG(a0), {k, v, &ks, &vs, group}, IB200_VIEW2_ARG(a5), &offsets,                \
+                               IB200_VIEW1_ARG(a7), IB200_VIEW3_ARG(a8), scale_bits, window, workspace, workspace_bytes,   \
+                               static_cast<cudaStream_t>(stream));                                                         \
+  }                                                                                                                        \
+  extern "C" int intent_b200_paged_decode_attention_int4_##NAME(                                                           \
+      INTENT_B200_VIEW3(a0), INTENT_B200_VIEW4(a1), INTENT_B200_VIEW4(a2), INTENT_B200_VIEW4(a3), INTENT_B200_VIEW4(a4),   \
+      INTENT_B200_VIEW2(a5), INTENT_B200_VIEW1(a6), INTENT_B200_VIEW3(a7), int32_t group, int32_t scale_bits,              \
+      IB200_PAGED_TAIL) {                                                                                                  \
+    const ib200::View4 k = IB200_VIEW4_ARG(a1), ks = IB200_VIEW4_ARG(a2), v = IB200_VIEW4_ARG(a3), vs = IB200_VIEW4_ARG(a4); \
+    return ib200::attend<TYPE>(IB200_VIEW3_ARG(a0), {k, v, &ks, &vs, group}, IB200_VIEW2_ARG(a5), nullptr,                 \
+                               IB200_VIEW1_ARG(a6), IB200_VIEW3_ARG(a7), scale_bits, window, workspace, workspace_bytes,   \
+                               static_cast<cudaStream_t>(stream));                                                         \
   }
 IB200_PAGED_ENTRIES(f16, __half)
 IB200_PAGED_ENTRIES(bf16, __nv_bfloat16)

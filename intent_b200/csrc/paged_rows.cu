@@ -28,13 +28,13 @@
 #include "common.cuh"
 #include "paged.cuh"
 #include "paged_join.cuh"
+#include "paged_rows.cuh"
 #include "tma.cuh"
 
 namespace ib200 {
 namespace {
 
 constexpr int UNIT = 32;                 // tokens of a ring slot
-constexpr float SLACK = 8.f;             // growth of a row's maximum (log2) that its weights are left to absorb
 
 template <int D>
 struct Ring {
@@ -66,74 +66,6 @@ constexpr int smem_bytes() {
 static_assert(smem_bytes<128, 2>() <= 227 * 1024 && smem_bytes<128, 1>() <= 227 * 1024 && smem_bytes<64, 2>() <= 227 * 1024,
               "shared memory of a CTA");
 
-// One sequence's share of the line of steps
-struct Sequence {
-  int rows;        // query rows of a key head: new tokens x group
-  int first_row;   // its first token among all
-  int length;      // tokens in the cache
-  int first;       // position of its first query
-  int low;         // first token that any of its queries sees
-  int begin;       // first step
-  int steps;       // of a row tile, one at least: a tile without tokens writes zeros
-  int tiles;       // row tiles of a key head
-};
-
-template <int STEP>
-__device__ __forceinline__ Sequence sequence_of(const PagedParams& p, int b, int tile_rows) {
-  Sequence s;
-  const TokenSpan span = span_of(p, b);
-  s.rows = span.count * p.group <= p.few ? span.count * p.group : 0;
-  s.first_row = span.begin;
-  s.length = min(max(__ldg(p.lengths + b), 0), p.capacity);
-  s.first = s.length - span.count;
-  s.low = p.window > 0 ? min(max(s.first - p.window + 1, 0), s.length) : 0;
-  s.begin = s.low / STEP;
-  s.steps = max((s.length + STEP - 1) / STEP - s.begin, 1);
-  s.tiles = (s.rows + tile_rows - 1) / tile_rows;
-  return s;
-}
-
-// Places of a sequence on the line
-template <int BEGIN>
-__device__ __forceinline__ long long places_of(const PagedParams& p, const Sequence& s) {
-  return (long long)s.tiles * p.k_heads * (s.steps + BEGIN);
-}
-
-// A step on the line
-template <int STEP, int BEGIN>
-struct Walk {
-  Sequence s;
-  int b, head, tile, step;
-  // how many places on the next one is
-  __device__ __forceinline__ int distance() const { return step + 1 < s.steps ? 1 : 1 + BEGIN; }
-  __device__ __forceinline__ void advance(const PagedParams& p, int tile_rows) {
-    if (++step < s.steps) return;
-    step = 0;
-    if (++tile < s.tiles) return;
-    tile = 0;
-    if (++head < p.k_heads) return;
-    head = 0;
-    do {
-      if (++b >= p.batch) return;
-      s = sequence_of<STEP>(p, b, tile_rows);
-    } while (s.tiles == 0);
-  }
-};
-
-__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
-}
-__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
-}
-__device__ __forceinline__ uint32_t movmatrix(uint32_t v) {
-  uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
-  return d;
-}
-
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(32 * Ring<D>::WARPS, 1)
 paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedParams p) {
@@ -163,63 +95,11 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   programmatic_wait();
 
   // ---- this CTA's part of the line
-  const int per_thread = (p.batch + THREADS - 1) / THREADS, mine = tid * per_thread;
-  long long sum = 0;
-  for (int b = mine; b < min(mine + per_thread, p.batch); ++b) {
-    const Sequence s = sequence_of<STEP>(p, b, ROWS);
-    sum += places_of<BEGIN>(p, s);
-  }
-  long long before = sum;
-#pragma unroll
-  for (int d = 1; d < 32; d *= 2) {
-    const long long v = __shfl_up_sync(0xffffffffu, before, d);
-    if (lane >= d) before += v;
-  }
-  if (lane == 31) warp_sums[warp] = before;
-  __syncthreads();
-  long long line = 0;
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
-    if (w < warp) before += warp_sums[w];
-    line += warp_sums[w];
-  }
-  before -= sum;
-  const int share = share_of(line), cta = blockIdx.x;
-  RowsJoin* entry = static_cast<RowsJoin*>(p.joins) + cta;
-  if (tid == 0) {
-    entry->last_cta = -1;
-    if (share < 0) atomicExch(p.status, INTENT_B200_ERR_SHAPE);
-  }
-  const long long begin = (long long)cta * share;
-  if (share <= 0 || begin >= line) return;
-  const int end = int(min((long long)share, line - begin));            // of this CTA's places, counted from its first one
-  if (begin >= before && begin < before + sum) {
-    int b = mine;
-    long long at = before;
-    for (;; ++b) {
-      const Sequence s = sequence_of<STEP>(p, b, ROWS);
-      const long long places = places_of<BEGIN>(p, s);
-      if (begin < at + places || b + 1 >= min(mine + per_thread, p.batch)) break;
-      at += places;
-    }
-    shared[0] = b;
-    *reinterpret_cast<long long*>(shared + 2) = begin - at;            // place in the sequence
-  }
-  __syncthreads();
-  Walk<STEP, BEGIN> load;
-  load.b = shared[0];
-  load.s = sequence_of<STEP>(p, load.b, ROWS);
-  {
-    const long long place = *reinterpret_cast<const long long*>(shared + 2);
-    const int item = divide(place, load.s.steps + BEGIN);
-    load.step = int(place - (long long)item * (load.s.steps + BEGIN)) - BEGIN;
-    load.head = item / load.s.tiles;
-    load.tile = item - load.head * load.s.tiles;
-  }
-  const int first_place = max(-load.step, 0);            // of a step
-  if (first_place >= end) return;
-  load.step = max(load.step, 0);
-  Walk<STEP, BEGIN> work = load;
+  RowsJoin* entry = static_cast<RowsJoin*>(p.joins) + blockIdx.x;
+  const Place<STEP, BEGIN> start = place_of<STEP, BEGIN, THREADS>(p, ROWS, shared, warp_sums, entry);
+  if (start.first >= start.end) return;
+  const int first_place = start.first, end = start.end;
+  Walk<STEP, BEGIN> load = start.at, work = load;
 
   const float infinity = __int_as_float(0x7f800000);
   int loading = first_place, slot_in = 0, slot_out = 0;
@@ -528,49 +408,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         begin_tile();                    // (its queries are on their way while this tile is put together)
       }
       __syncthreads();
-      const bool begins = item_begin >= 0, whole = begins && item_end <= share;
-      float* part = p.parts + size_t(2 * cta + begins) * (ROWS * (D + 2));
-      auto place = [&](int r) {
-        const int token = (tile_row + r) / p.group, of_group = tile_row + r - token * p.group;
-        return p.out + (int64_t(first_row + token) * p.q_heads + head * p.group + of_group) * D;
-      };
-      for (int w = tid; w < rows * (D / 8); w += THREADS) {
-        const int r = w / (D / 8), c = w - r * (D / 8);
-        float m = -infinity, l = 0.f, x[8] = {};
-#pragma unroll
-        for (int v = 0; v < WARPS; ++v) m = fmaxf(m, max_here[v * ROWS + r]);
-        const float origin = m == -infinity ? 0.f : m;
-#pragma unroll
-        for (int v = 0; v < WARPS; ++v) {
-          const float f = exp2_fast(max_here[v * ROWS + r] - origin);
-          l = fmaf(sum_here[v * ROWS + r], f, l);
-          const float* from = join_here + (v * ROWS + r) * PITCH + 8 * (c ^ (r >> 1 & 3));
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = fmaf(from[e], f, x[e]);
-        }
-        if (whole) {
-          const float inverse = l == 0.f ? of_nothing(p, sequence, first_row + (tile_row + r) / p.group) : 1.f / l;
-          *reinterpret_cast<uint4*>(place(r) + 8 * c) =
-              make_uint4(Elem<T>::pack2(x[0] * inverse, x[1] * inverse), Elem<T>::pack2(x[2] * inverse, x[3] * inverse),
-                         Elem<T>::pack2(x[4] * inverse, x[5] * inverse), Elem<T>::pack2(x[6] * inverse, x[7] * inverse));
-        } else {
-          float4* to = reinterpret_cast<float4*>(part + r * D + 8 * c);
-          to[0] = make_float4(x[0], x[1], x[2], x[3]);
-          to[1] = make_float4(x[4], x[5], x[6], x[7]);
-          if (c == 0) {
-            part[ROWS * D + r] = m;
-            part[ROWS * (D + 1) + r] = l;
-          }
-        }
-      }
-      if (tid == 0 && !whole && begins) {
-        entry->row = first_row;
-        entry->head = head;
-        entry->tile_row = tile_row;
-        entry->rows = rows;
-        entry->sequence = sequence;
-        entry->last_cta = cta + (item_end - 1) / share;
-      }
+      put_together<T, D, ROWS, WARPS>(p, start.share, join_here, max_here, sum_here, entry, tile_row, rows, head, first_row, sequence,
+                                      item_begin, item_end);
       if (JOINS == 1) __syncthreads();
     }
   }

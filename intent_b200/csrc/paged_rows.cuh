@@ -1,0 +1,208 @@
+// What the kernels for few rows of queries share: the line of steps, its cut into equal parts, and the end of a tile.
+#pragma once
+
+#include "common.cuh"
+#include "paged.cuh"
+#include "paged_join.cuh"
+
+namespace ib200 {
+
+#ifdef __CUDACC__
+
+constexpr float SLACK = 8.f;             // growth of a row's maximum (log2) that its weights are left to absorb
+
+// One sequence's share of the line of steps
+struct Sequence {
+  int rows;        // query rows of a key head: new tokens x group
+  int first_row;   // its first token among all
+  int length;      // tokens in the cache
+  int first;       // position of its first query
+  int low;         // first token that any of its queries sees
+  int begin;       // first step
+  int steps;       // of a row tile, one at least: a tile without tokens writes zeros
+  int tiles;       // row tiles of a key head
+};
+
+template <int STEP>
+__device__ __forceinline__ Sequence sequence_of(const PagedParams& p, int b, int tile_rows) {
+  Sequence s;
+  const TokenSpan span = span_of(p, b);
+  s.rows = span.count * p.group <= p.few ? span.count * p.group : 0;
+  s.first_row = span.begin;
+  s.length = min(max(__ldg(p.lengths + b), 0), p.capacity);
+  s.first = s.length - span.count;
+  s.low = p.window > 0 ? min(max(s.first - p.window + 1, 0), s.length) : 0;
+  s.begin = s.low / STEP;
+  s.steps = max((s.length + STEP - 1) / STEP - s.begin, 1);
+  s.tiles = (s.rows + tile_rows - 1) / tile_rows;
+  return s;
+}
+
+// Places of a sequence on the line
+template <int BEGIN>
+__device__ __forceinline__ long long places_of(const PagedParams& p, const Sequence& s) {
+  return (long long)s.tiles * p.k_heads * (s.steps + BEGIN);
+}
+
+// A step on the line
+template <int STEP, int BEGIN>
+struct Walk {
+  Sequence s;
+  int b, head, tile, step;
+  // how many places on the next one is
+  __device__ __forceinline__ int distance() const { return step + 1 < s.steps ? 1 : 1 + BEGIN; }
+  __device__ __forceinline__ void advance(const PagedParams& p, int tile_rows) {
+    if (++step < s.steps) return;
+    step = 0;
+    if (++tile < s.tiles) return;
+    tile = 0;
+    if (++head < p.k_heads) return;
+    head = 0;
+    do {
+      if (++b >= p.batch) return;
+      s = sequence_of<STEP>(p, b, tile_rows);
+    } while (s.tiles == 0);
+  }
+};
+
+// The part of the line that a CTA takes
+template <int STEP, int BEGIN>
+struct Place {
+  Walk<STEP, BEGIN> at;    // its first step
+  int first, end;          // its place and where the CTA's places end, counted from the CTA's first one (first >= end: none)
+  int share;               // places of every CTA
+};
+
+// To be called by all threads of a CTA; `shared` has room for a number and a 64-bit one behind it, `warp_sums` for one a warp.
+template <int STEP, int BEGIN, int THREADS>
+__device__ __forceinline__ Place<STEP, BEGIN> place_of(const PagedParams& p, int tile_rows, int* shared, long long* warp_sums,
+                                                       RowsJoin* entry) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  Place<STEP, BEGIN> place;
+  place.first = place.end = 0;
+  const int per_thread = (p.batch + THREADS - 1) / THREADS, mine = tid * per_thread;
+  long long sum = 0;
+  for (int b = mine; b < min(mine + per_thread, p.batch); ++b) {
+    const Sequence s = sequence_of<STEP>(p, b, tile_rows);
+    sum += places_of<BEGIN>(p, s);
+  }
+  long long before = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const long long v = __shfl_up_sync(0xffffffffu, before, d);
+    if (lane >= d) before += v;
+  }
+  if (lane == 31) warp_sums[warp] = before;
+  __syncthreads();
+  long long line = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += warp_sums[w];
+    line += warp_sums[w];
+  }
+  before -= sum;
+  place.share = share_of(line);
+  if (tid == 0) {
+    entry->last_cta = -1;
+    if (place.share < 0) atomicExch(p.status, INTENT_B200_ERR_SHAPE);
+  }
+  const long long begin = (long long)blockIdx.x * place.share;
+  if (place.share <= 0 || begin >= line) return place;
+  place.end = int(min((long long)place.share, line - begin));
+  if (begin >= before && begin < before + sum) {
+    int b = mine;
+    long long at = before;
+    for (;; ++b) {
+      const Sequence s = sequence_of<STEP>(p, b, tile_rows);
+      const long long places = places_of<BEGIN>(p, s);
+      if (begin < at + places || b + 1 >= min(mine + per_thread, p.batch)) break;
+      at += places;
+    }
+    shared[0] = b;
+    *reinterpret_cast<long long*>(shared + 2) = begin - at;            // place in the sequence
+  }
+  __syncthreads();
+  Walk<STEP, BEGIN>& first = place.at;
+  first.b = shared[0];
+  first.s = sequence_of<STEP>(p, first.b, tile_rows);
+  const long long of_sequence = *reinterpret_cast<const long long*>(shared + 2);
+  const int item = divide(of_sequence, first.s.steps + BEGIN);
+  first.step = int(of_sequence - (long long)item * (first.s.steps + BEGIN)) - BEGIN;
+  first.head = item / first.s.tiles;
+  first.tile = item - first.head * first.s.tiles;
+  place.first = max(-first.step, 0);                     // of a step
+  first.step = max(first.step, 0);
+  return place;
+}
+
+// The warps' parts of a tile, [WARPS][ROWS][D] with pieces of eight elements in the order that swaps them by row, their maxima and
+// sums: the result where the CTA has the whole tile, a part for the join where it has not.
+template <typename T, int D, int ROWS, int WARPS>
+__device__ __forceinline__ void put_together(const PagedParams& p, int share, const float* join_here, const float* max_here,
+                                             const float* sum_here, RowsJoin* entry, int tile_row, int rows, int head, int first_row,
+                                             int sequence, int item_begin, int item_end) {
+  constexpr int THREADS = 32 * WARPS;
+  const float infinity = __int_as_float(0x7f800000);
+  const int cta = blockIdx.x, tid = threadIdx.x;
+  const bool begins = item_begin >= 0, whole = begins && item_end <= share;
+  float* part = p.parts + size_t(2 * cta + begins) * (ROWS * (D + 2));
+  auto place = [&](int r) {
+    const int token = (tile_row + r) / p.group, of_group = tile_row + r - token * p.group;
+    return p.out + (int64_t(first_row + token) * p.q_heads + head * p.group + of_group) * D;
+  };
+  for (int w = tid; w < rows * (D / 8); w += THREADS) {
+    const int r = w / (D / 8), c = w - r * (D / 8);
+    float m = -infinity, l = 0.f, x[8] = {};
+#pragma unroll
+    for (int v = 0; v < WARPS; ++v) m = fmaxf(m, max_here[v * ROWS + r]);
+    const float origin = m == -infinity ? 0.f : m;
+#pragma unroll
+    for (int v = 0; v < WARPS; ++v) {
+      const float f = exp2_fast(max_here[v * ROWS + r] - origin);
+      l = fmaf(sum_here[v * ROWS + r], f, l);
+      const float* from = join_here + (v * ROWS + r) * D + 8 * (c ^ (r >> 1 & 3));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = fmaf(from[e], f, x[e]);
+    }
+    if (whole) {
+      const float inverse = l == 0.f ? of_nothing(p, sequence, first_row + (tile_row + r) / p.group) : 1.f / l;
+      *reinterpret_cast<uint4*>(place(r) + 8 * c) =
+          make_uint4(Elem<T>::pack2(x[0] * inverse, x[1] * inverse), Elem<T>::pack2(x[2] * inverse, x[3] * inverse),
+                     Elem<T>::pack2(x[4] * inverse, x[5] * inverse), Elem<T>::pack2(x[6] * inverse, x[7] * inverse));
+    } else {
+      float4* to = reinterpret_cast<float4*>(part + r * D + 8 * c);
+      to[0] = make_float4(x[0], x[1], x[2], x[3]);
+      to[1] = make_float4(x[4], x[5], x[6], x[7]);
+      if (c == 0) {
+        part[ROWS * D + r] = m;
+        part[ROWS * (D + 1) + r] = l;
+      }
+    }
+  }
+  if (tid == 0 && !whole && begins) {
+    entry->row = first_row;
+    entry->head = head;
+    entry->tile_row = tile_row;
+    entry->rows = rows;
+    entry->sequence = sequence;
+    entry->last_cta = cta + (item_end - 1) / share;
+  }
+}
+
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ uint32_t movmatrix(uint32_t v) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
+}
+
+#endif  // __CUDACC__
+
+}  // namespace ib200

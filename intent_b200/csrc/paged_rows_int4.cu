@@ -1,0 +1,556 @@
+// Attention over a paged cache in 4 bits for few rows of queries per sequence and key head (paged_decode_attention_int4, and
+// paged_attention_int4 for short chunks).  The program is that of paged_rows.cu with keys and values m + s n: of a code n (0 .. 15), and of
+// the scale s and the minimum m of its group of GROUP elements.
+//
+// Codes are multiplied as they are, and scales and minima go to the scores and the weights: with the sums over a group g
+//   x . k_j = sum_g s_jg (x_g . n_jg) + m_jg sum(x_g)            o = sum_j w_j v_j = sum_g (sum_j (w_j s_jg) n_jg + sum_j w_j m_jg)
+// Four bits become operands of the tensor core by being masked where they are: in the lowest or the next four bits of a 16-bit
+// word they are n or 16 n times the smallest bf16 (2^-133; an f16 too, 2^-24, in the lowest four), exact numbers for it.  The factor of
+// 16 is taken out of the queries (bf16) or the results ahead, so that eight codes cost five instructions; with a weight's
+// exponent 2^64 and a query's 2^60 larger no product comes near the ends of f32.  (Queries of 2^67 and more and scales of values
+// of 2^55 and more are out of that range.)
+//
+// All statistics and sums are in f32.  A weight times its scale is rounded to bf16 for the product with the codes, and the same
+// rounded numbers are added up for the middle of the codes (8), which is taken off again: the rounding is worth what it is for a
+// product with v_j.  For f16 results the product is made with what the rounding left over, too.
+//
+// A CTA's line of steps, its shares, and the parts of tiles that are cut are those of paged_rows.cu; a step is 64 tokens for each warp.
+#include <cstring>
+
+#include "common.cuh"
+#include "paged.cuh"
+#include "paged_join.cuh"
+#include "paged_rows.cuh"
+#include "tma.cuh"
+
+namespace ib200 {
+namespace {
+
+constexpr int UNIT = 64;                 // tokens of a ring slot
+constexpr int PARTS = UNIT / 16;         // pieces of it that lie in one page in any case
+
+template <int D, int GROUP>
+struct Ring {
+  static constexpr int WARPS = 8;
+  static constexpr int STAGES = D == 128 ? 2 : 3;
+  static constexpr int STEP = UNIT * WARPS;               // tokens of a CTA's step
+  static constexpr int GROUPS = D / GROUP;
+  static constexpr int ROW = D / 2;                       // bytes of a token's codes
+  static constexpr int CODES = UNIT * ROW, SCALES = UNIT * GROUPS * 4;   // of keys or values of a unit
+  static constexpr int SLOT = 2 * CODES, SCALE_SLOT = 2 * SCALES;
+  static constexpr int BYTES = WARPS * STAGES * (SLOT + SCALE_SLOT);
+  static constexpr int BEGIN = 1;                         // places on the line ahead of the steps of a tile
+};
+
+constexpr int SMEM_MOST = 227 * 1024;
+template <int D, int GROUP, int NT>
+constexpr int smem_bytes_with(int joins) {
+  using R = Ring<D, GROUP>;
+  return 1024 + R::BYTES + joins * R::WARPS * 8 * NT * (D * 4 + 8) + R::WARPS * R::STAGES * 8 + 16 + 8 * R::WARPS;
+}
+// Places for the warps' parts of a tile: two where there is room
+template <int D, int GROUP, int NT>
+constexpr int joins() {
+  return smem_bytes_with<D, GROUP, NT>(2) <= SMEM_MOST ? 2 : 1;
+}
+template <int D, int GROUP, int NT>
+constexpr int smem_bytes() {
+  static_assert(smem_bytes_with<D, GROUP, NT>(joins<D, GROUP, NT>()) <= SMEM_MOST, "shared memory of a CTA");
+  return smem_bytes_with<D, GROUP, NT>(joins<D, GROUP, NT>());
+}
+
+// bytes, a multiple of 16 at 16-byte boundaries, to shared memory
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+template <int N>
+struct Words {
+  uint32_t w[N];
+};
+template <int N>
+__device__ __forceinline__ Words<N> lds(uint32_t addr) {
+  Words<N> d;
+  if constexpr (N == 1) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(d.w[0]) : "r"(addr));
+  else if constexpr (N == 2) asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(d.w[0]), "=r"(d.w[1]) : "r"(addr));
+  else asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(d.w[0]), "=r"(d.w[1]), "=r"(d.w[2]), "=r"(d.w[3]) : "r"(addr));
+  return d;
+}
+
+using Wide = __nv_bfloat16;              // the type of the weights' product with the codes
+constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u;
+
+// What the scores of keys' codes are multiplied with
+template <typename T>
+struct Codes;
+template <>
+struct Codes<__nv_bfloat16> {
+  static constexpr float UNIT_OF_SCORES = 0x1p-73f;      // 2^60 * 2^-133
+  // the 16-bit pair as an operand for codes in the lowest four bits, and in the next
+  __device__ static __forceinline__ uint32_t low(uint32_t x) { return Elem<__nv_bfloat16>::mul2(x, 0x5d805d80u); }     // 2^60
+  __device__ static __forceinline__ uint32_t high(uint32_t x) { return Elem<__nv_bfloat16>::mul2(x, 0x5b805b80u); }    // 2^56
+  __device__ static __forceinline__ uint32_t odd(uint32_t codes) { return codes & HIGH; }
+};
+template <>
+struct Codes<__half> {
+  static constexpr float UNIT_OF_SCORES = 0x1p-24f;
+  __device__ static __forceinline__ uint32_t low(uint32_t x) { return x; }
+  __device__ static __forceinline__ uint32_t high(uint32_t x) { return x; }
+  // (an f16 query divided by 16 might lose bits)
+  __device__ static __forceinline__ uint32_t odd(uint32_t codes) { return (codes >> 4) & LOW; }
+};
+
+template <typename T, int D, int GROUP, int NT>
+__global__ void __launch_bounds__(32 * Ring<D, GROUP>::WARPS, 1)
+paged_rows_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const uint32_t* k_scales,
+                       const uint32_t* v_scales, const PagedParams p) {
+  using R = Ring<D, GROUP>;
+  constexpr int ROWS = 8 * NT, WARPS = R::WARPS, THREADS = 32 * WARPS, STEP = R::STEP, BEGIN = R::BEGIN, GROUPS = R::GROUPS;
+  constexpr int CHUNKS = D / 32, OF_GROUP = CHUNKS / GROUPS;            // 16 bytes of a token's codes
+  constexpr bool SPLIT = std::is_same<T, __half>::value;                // weights in two bf16 parts
+  extern __shared__ unsigned char smem_raw[];
+  programmatic_begin();
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&map_k);
+    prefetch_tensormap(&map_v);
+  }
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  unsigned char* base_ptr = smem_raw + (base - smem_u32(smem_raw));
+  constexpr int JOINS = joins<D, GROUP, NT>();
+  float* join = reinterpret_cast<float*>(base_ptr + R::BYTES);          // [JOINS][WARPS][ROWS][D]
+  float* join_max = join + JOINS * WARPS * ROWS * D;                    // [JOINS][WARPS][ROWS]
+  float* join_sum = join_max + JOINS * WARPS * ROWS;
+  int* shared = reinterpret_cast<int*>(join_sum + JOINS * WARPS * ROWS);   // a number, a 64-bit one, the warps' 64-bit sums
+  long long* warp_sums = reinterpret_cast<long long*>(shared + 4);
+  const uint32_t bars = smem_u32(warp_sums + WARPS);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t ring = base + warp * R::STAGES * R::SLOT, full = bars + warp * R::STAGES * 8;
+  const uint32_t scale_ring = base + WARPS * R::STAGES * R::SLOT + warp * R::STAGES * R::SCALE_SLOT;
+  if (lane == 0) {
+    for (int s = 0; s < R::STAGES; ++s) mbar_init(full + 8 * s, 1);
+    fence_mbar_init();
+  }
+  programmatic_wait();
+
+  // ---- this CTA's part of the line
+  RowsJoin* entry = static_cast<RowsJoin*>(p.joins) + blockIdx.x;
+  const Place<STEP, BEGIN> start = place_of<STEP, BEGIN, THREADS>(p, ROWS, shared, warp_sums, entry);
+  if (start.first >= start.end) return;
+  const int first_place = start.first, end = start.end;
+  Walk<STEP, BEGIN> load = start.at, work = load;
+
+  const float infinity = __int_as_float(0x7f800000);
+  int loading = first_place, slot_in = 0, slot_out = 0;
+  uint32_t parity = 0, present = 0;      // a bit per slot; PARTS bits per unit asked for, the oldest lowest
+  int queued = 0;
+  bool ok = true;
+  const int box = min(1 << p.page_shift, UNIT);          // tokens of a unit that lie in one page
+  int page;                              // of piece lane % PARTS of the unit at `load`, asked for one unit ahead; -1: not needed
+  auto look_up = [&] {
+    const int t = (load.s.begin + load.step) * STEP + warp * UNIT + (lane % PARTS) * 16;
+    page = -1;
+    if (t < load.s.length && t + 16 > load.s.low)
+      page = __ldg(p.page_table + int64_t(load.b) * p.table_width + (t >> p.page_shift));
+  };
+  // asks for the unit of this warp at `load`, and goes on
+  auto ask = [&] {
+    const int token = (load.s.begin + load.step) * STEP + warp * UNIT;
+    // (pieces of one page are one box, whichever of them is needed)
+    int number = page >= 0 && page < p.pages ? page : -1;
+    const uint32_t here = __ballot_sync(0xffffffffu, number >= 0) & ((1u << PARTS) - 1);
+    number = box >= 32 ? max(number, __shfl_xor_sync(0xffffffffu, number, 1)) : number;
+    number = box >= 64 ? max(number, __shfl_xor_sync(0xffffffffu, number, 2)) : number;
+    // lane: piece lane % PARTS of keys' codes, values' codes, keys' scales, values' scales
+    const int piece = lane % PARTS, what = lane / PARTS;
+    const bool mine = number >= 0 && piece * 16 % box == 0;
+    const uint32_t boxes = __ballot_sync(0xffffffffu, mine) & ((1u << PARTS) - 1);
+    if (here) {
+      const uint32_t bar = full + 8 * slot_in;
+      if (lane == 0) mbar_expect_tx(bar, uint32_t(__popc(boxes) * box * 2 * (R::ROW + 4 * GROUPS)));
+      __syncwarp();
+      if (mine && what < 4) {
+        const int t = token + piece * 16;
+        const int row = ((number * p.k_heads + load.head) << p.page_shift) + (t & ((1 << p.page_shift) - 1));
+        const uint32_t to = ring + slot_in * R::SLOT + piece * 16 * R::ROW;
+        const uint32_t to_scales = scale_ring + slot_in * R::SCALE_SLOT + piece * 16 * GROUPS * 4;
+        if (what < 2) tma_load_2d(to + what * R::CODES, what ? &map_v : &map_k, 0, row, bar);
+        else bulk_load(to_scales + (what - 2) * R::SCALES, (what == 3 ? v_scales : k_scales) + int64_t(row) * GROUPS,
+                       uint32_t(box * GROUPS * 4), bar);
+      }
+      slot_in = slot_in + 1 == R::STAGES ? 0 : slot_in + 1;
+    }
+    present |= here << (PARTS * queued);
+    ++queued;
+    loading += load.distance();
+    if (loading < end) {
+      load.advance(p, ROWS);
+      look_up();
+    }
+  };
+  uint32_t qf[NT][CHUNKS][4];            // queries as B fragments: elements 32 c + 8 (lane % 4) + {0, 4}, {1, 5}, {2, 6}, {3, 7}
+  float q_sum[NT][2][GROUPS];            // of this thread's rows, in the scores' unit
+  float o[NT][CHUNKS][2][4];             // sums of codes: elements 32 c + 4 (lane / 4) + 2 t (+ 1, times 16) of rows 2 (lane % 4) (+ 1)
+  float eights[NT][GROUPS][4];           // sums of the weights that the codes are multiplied with, of the same rows (twice)
+  float middle[NT][2][GROUPS];           // sums of weight times minimum (and 8 scales), of this thread's tokens
+  float top[NT][2], weight_sum[NT][2];
+  int position[NT][2];                   // of this thread's rows; -1 where there is none
+  int least = 0, most = 0;               // positions of the tile's first and last row
+  const float scale = p.scale / Codes<T>::UNIT_OF_SCORES;
+  // the queries of the tile at `work`
+  auto begin_tile = [&] {
+    const int tile_row = work.tile * ROWS, rows = min(ROWS, work.s.rows - tile_row);
+    least = work.s.first + tile_row / p.group;
+    most = work.s.first + (tile_row + rows - 1) / p.group;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = min(tile_row + nt * 8 + (lane >> 2), work.s.rows - 1), token = r / p.group;
+      const uint16_t* x = p.q + int64_t(work.s.first_row + token) * p.q_token +
+                          int64_t(work.head * p.group + r - token * p.group) * p.q_head + 8 * (lane & 3);
+      float sums[GROUPS] = {};
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(x + 32 * c));
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          sums[c / OF_GROUP] += Elem<T>::to_float(uint16_t(w[e])) + Elem<T>::to_float(uint16_t(w[e] >> 16));
+        qf[nt][c][0] = Codes<T>::low(prmt(v.x, v.z, 0x5410));
+        qf[nt][c][1] = Codes<T>::high(prmt(v.x, v.z, 0x7632));
+        qf[nt][c][2] = Codes<T>::low(prmt(v.y, v.w, 0x5410));
+        qf[nt][c][3] = Codes<T>::high(prmt(v.y, v.w, 0x7632));
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nt][c][t][e] = 0.f;
+      }
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
+        sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          q_sum[nt][e][g] = __shfl_sync(0xffffffffu, sums[g], 8 * (lane & 3) + 4 * e) * Codes<T>::UNIT_OF_SCORES;
+          middle[nt][e][g] = 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) eights[nt][g][e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int of_thread = tile_row + nt * 8 + 2 * (lane & 3) + e;
+        position[nt][e] = of_thread < work.s.rows ? work.s.first + of_thread / p.group : -1;
+        top[nt][e] = -infinity;
+        weight_sum[nt][e] = 0.f;
+      }
+    }
+  };
+  look_up();
+  begin_tile();
+  for (int i = 0; i < R::STAGES && loading < end; ++i) ask();
+  int turn = 0;                          // place of the join that is next
+  for (int at = first_place, next; at < end; at = next) {
+    const uint32_t pieces = present & ((1u << PARTS) - 1);
+    present >>= PARTS;
+    --queued;
+    if (pieces) {
+      const int token = (work.s.begin + work.step) * STEP + warp * UNIT;
+      const uint32_t keys = ring + slot_out * R::SLOT, values = keys + R::CODES;
+      const uint32_t of_keys = scale_ring + slot_out * R::SCALE_SLOT + (lane >> 2) * (GROUPS * 4), of_values = of_keys + R::SCALES;
+      if (ok) ok = mbar_wait_warp(full + 8 * slot_out, (parity >> slot_out) & 1);
+      parity ^= 1u << slot_out;
+      slot_out = slot_out + 1 == R::STAGES ? 0 : slot_out + 1;
+
+      float s[NT][PARTS][4];             // S^T: tokens 16 m + lane / 4 (+ 8), rows as in o
+#pragma unroll
+      for (int m = 0; m < PARTS; ++m) {
+        uint32_t codes[2][CHUNKS];       // of tokens 16 m + lane / 4 (+ 8): elements 32 c + 8 (lane % 4) ..
+        if constexpr (D == 128) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = 16 * m + 8 * h + (lane & 7), c = lane >> 3;
+            ldmatrix_x4(codes[h], keys + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+          }
+        } else {
+          const int r = 16 * m + 8 * (lane >> 4) + (lane & 7), c = (lane >> 3) & 1;
+          uint32_t all[4];
+          ldmatrix_x4(all, keys + r * 32 + ((c ^ ((r >> 2) & 1)) << 4));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) codes[e >> 1][e & 1] = all[e];
+        }
+        float x[NT][GROUPS][4] = {};
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+          for (int pair = 0; pair < 2; ++pair) {
+            const uint32_t a = codes[0][c] >> (8 * pair), b = codes[1][c] >> (8 * pair);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              Elem<T>::mma16816(x[nt][c / OF_GROUP], a & LOW, b & LOW, Codes<T>::odd(a), Codes<T>::odd(b), qf[nt][c][2 * pair],
+                                qf[nt][c][2 * pair + 1]);
+          }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const Words<GROUPS> w = lds<GROUPS>(of_keys + (16 * m + 8 * h) * (GROUPS * 4));
+#pragma unroll
+          for (int g = 0; g < GROUPS; ++g) {
+            const float by = Elem<T>::to_float(uint16_t(w.w[g])), from = Elem<T>::to_float(uint16_t(w.w[g] >> 16));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float sum = fmaf(from, q_sum[nt][e][g], g == 0 ? 0.f : s[nt][m][2 * h + e]);
+                s[nt][m][2 * h + e] = fmaf(by, x[nt][g][2 * h + e], sum);
+              }
+          }
+        }
+      }
+      const bool all = pieces == (1u << PARTS) - 1 && token + UNIT - 1 <= least && (p.window == 0 || token > most - p.window);
+      uint32_t hidden[NT] = {};          // bit 4 m + e: of s[nt][m][e]
+      if (!all) {
+#pragma unroll
+        for (int m = 0; m < PARTS; ++m) {
+          const bool there = (pieces >> m) & 1;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int t = token + 16 * m + (lane >> 2) + 8 * (e >> 1), at_row = position[nt][e & 1];
+              if (!there || t > at_row || (p.window > 0 && t <= at_row - p.window)) {
+                s[nt][m][e] = -infinity;
+                hidden[nt] |= 1u << (4 * m + e);
+              }
+            }
+        }
+      }
+      // A row's maximum is raised only when a score exceeds it by more than SLACK: until then no lane has to know the others'.
+      bool raise = false;
+      float here[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          here[nt][e] = fmaxf(s[nt][0][e], s[nt][0][e + 2]);
+#pragma unroll
+          for (int m = 1; m < PARTS; ++m) here[nt][e] = fmaxf(here[nt][e], fmaxf(s[nt][m][e], s[nt][m][e + 2]));
+          raise |= here[nt][e] * scale > top[nt][e] + SLACK;           // (from -inf: any)
+        }
+      if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float factor[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) here[nt][e] = fmaxf(here[nt][e], __shfl_xor_sync(0xffffffffu, here[nt][e], d));
+            const float now = fmaxf(top[nt][e], here[nt][e] * scale);
+            factor[e] = exp2_fast(top[nt][e] - (now == -infinity ? 0.f : now));
+            top[nt][e] = now;
+            weight_sum[nt][e] *= factor[e];
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) middle[nt][e][g] *= factor[e];
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+              for (int t = 0; t < 2; ++t) o[nt][c][t][e] *= factor[e & 1];
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) eights[nt][g][e] *= factor[e & 1];
+          }
+        }
+      }
+      // weights, 2^64 times what they are
+      float origin[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) origin[nt][e] = 64.f - (top[nt][e] == -infinity ? 0.f : top[nt][e]);
+      auto add_values = [&](auto whole) {
+#pragma unroll
+        for (int m = 0; m < PARTS; ++m) {
+          uint32_t pf[NT][GROUPS][2], rest[NT][GROUPS][2];             // (weights times scales)^T as B fragments
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float w = exp2_fast(fmaf(s[nt][m][e], scale, origin[nt][e & 1]));
+              s[nt][m][e] = w;
+              weight_sum[nt][e & 1] += w;
+            }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const Words<GROUPS> w = lds<GROUPS>(of_values + (16 * m + 8 * h) * (GROUPS * 4));
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) {
+              const float by = Elem<T>::to_float(uint16_t(w.w[g])), from = Elem<T>::to_float(uint16_t(w.w[g] >> 16));
+              const float centre = SPLIT ? from : fmaf(8.f, by, from);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                float scaled[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  // (what is hidden may be anything, and 0 * NaN is NaN)
+                  const bool seen = decltype(whole)::value || !(hidden[nt] >> (4 * m + 2 * h + e) & 1);
+                  scaled[e] = seen ? s[nt][m][2 * h + e] * by : 0.f;
+                  if (seen) middle[nt][e][g] = fmaf(s[nt][m][2 * h + e], centre, middle[nt][e][g]);
+                }
+                const uint32_t rounded = Elem<Wide>::pack2(scaled[0], scaled[1]);
+                pf[nt][g][h] = movmatrix(rounded);
+                if (SPLIT)
+                  rest[nt][g][h] = movmatrix(Elem<Wide>::pack2(scaled[0] - Elem<Wide>::to_float(uint16_t(rounded)),
+                                                               scaled[1] - Elem<Wide>::to_float(uint16_t(rounded >> 16))));
+              }
+            }
+          }
+          if (!SPLIT) {
+            constexpr uint32_t ONES = 0x3f803f80u;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int g = 0; g < GROUPS; ++g)
+                Elem<Wide>::mma16816(eights[nt][g], ONES, ONES, ONES, ONES, pf[nt][g][0], pf[nt][g][1]);
+          }
+#pragma unroll
+          for (int pair = 0; pair < CHUNKS / 2; ++pair) {
+            // codes of tokens 16 m + 2 (lane % 4) (+ 1; + 8): elements 32 c + 4 (lane / 4) .. of chunks 2 pair and 2 pair + 1
+            const int r = 16 * m + (lane & 15), c = 2 * pair + (lane >> 4);
+            uint32_t codes[4];
+            ldmatrix_x4_trans(codes, values + r * R::ROW + ((c ^ (D == 128 ? (r >> 1) & 3 : (r >> 2) & 1)) << 4));
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int t = 0; t < 2; ++t) {
+                const uint32_t a = codes[2 * i] >> (8 * t), b = codes[2 * i + 1] >> (8 * t);
+                const int at_chunk = 2 * pair + i;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  const uint32_t(&f)[2] = pf[nt][at_chunk / OF_GROUP];
+                  Elem<Wide>::mma16816(o[nt][at_chunk][t], a & LOW, a & HIGH, b & LOW, b & HIGH, f[0], f[1]);
+                  if (SPLIT) {
+                    const uint32_t(&left)[2] = rest[nt][at_chunk / OF_GROUP];
+                    Elem<Wide>::mma16816(o[nt][at_chunk][t], a & LOW, a & HIGH, b & LOW, b & HIGH, left[0], left[1]);
+                  }
+                }
+              }
+          }
+        }
+      };
+      if (all) add_values(Bool<true>{});
+      else add_values(Bool<false>{});
+      __syncwarp();                      // every lane is done with the slot
+    }
+    if (ok && loading < end) ask();      // (a slot that was given up on may still be on its way)
+
+    const bool last_step = work.step + 1 == work.s.steps;
+    next = at + work.distance();
+    if (!last_step && next < end) {
+      ++work.step;
+    } else {
+      // ---- the warps' parts, then the CTAs'.  There are two places for them in turn: when a warp writes to one of them again,
+      // all have passed the barrier of the tile between.
+      float* join_here = join + turn * (WARPS * ROWS * D);
+      float* max_here = join_max + turn * (WARPS * ROWS);
+      float* sum_here = join_sum + turn * (WARPS * ROWS);
+      turn ^= JOINS - 1;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = nt * 8 + 2 * (lane & 3) + e;
+          float sum_all = weight_sum[nt][e];
+#pragma unroll
+          for (int d = 4; d < 32; d *= 2) sum_all += __shfl_xor_sync(0xffffffffu, sum_all, d);
+          if (lane < 4) {
+            max_here[warp * ROWS + r] = top[nt][e];
+            sum_here[warp * ROWS + r] = sum_all * 0x1p-64f;
+          }
+          float constant[GROUPS];
+#pragma unroll
+          for (int g = 0; g < GROUPS; ++g) {
+            float m = middle[nt][e][g];
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) m += __shfl_xor_sync(0xffffffffu, m, d);
+            constant[g] = (SPLIT ? m : fmaf(-8.f, eights[nt][g][e], m)) * 0x1p-64f;
+          }
+#pragma unroll
+          for (int c = 0; c < CHUNKS; ++c) {
+            // (pieces change places with the row, so that a store meets 32 banks)
+            const float from = constant[c / OF_GROUP];
+            float* to = join_here + (warp * ROWS + r) * D + 4 * ((8 * c + (lane >> 2)) ^ (2 * (lane & 3)));
+            *reinterpret_cast<float4*>(to) = make_float4(fmaf(o[nt][c][0][e], 0x1p69f, from), fmaf(o[nt][c][0][e + 2], 0x1p65f, from),
+                                                         fmaf(o[nt][c][1][e], 0x1p69f, from), fmaf(o[nt][c][1][e + 2], 0x1p65f, from));
+          }
+        }
+      }
+      const int tile_row = work.tile * ROWS, rows = min(ROWS, work.s.rows - tile_row), head = work.head;
+      const int first_row = work.s.first_row, sequence = work.b;
+      const int item_begin = at - work.step, item_end = item_begin + work.s.steps;   // the tile's places, maybe of other CTAs
+      if (next < end) {
+        work.advance(p, ROWS);
+        begin_tile();                    // (its queries are on their way while this tile is put together)
+      }
+      __syncthreads();
+      put_together<T, D, ROWS, WARPS>(p, start.share, join_here, max_here, sum_here, entry, tile_row, rows, head, first_row, sequence,
+                                      item_begin, item_end);
+      if (JOINS == 1) __syncthreads();
+    }
+  }
+  if (!ok) {
+    // Nothing may be on its way to a CTA that is gone.  (Which phase a slot is in has not been counted since the wait that gave
+    // up: of the two parities the wait for one is for the current phase, the other is over.)
+    for (int s = 0; s < R::STAGES; ++s)
+      for (int of_phase = 0; of_phase < 2; ++of_phase) mbar_wait_warp(full + 8 * s, of_phase, 64);
+    if (lane == 0) atomicExch(p.status, INTENT_B200_ERR_TIMEOUT);
+  }
+}
+
+template <typename T, int D, int GROUP, int NT>
+int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, const Int4Cache& cache, const PagedParams& p, int grid,
+           cudaStream_t stream) {
+  auto kernel = paged_rows_int4_kernel<T, D, GROUP, NT>;
+  constexpr int smem = smem_bytes<D, GROUP, NT>(), threads = 32 * Ring<D, GROUP>::WARPS;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return cuda_status(e);
+  if (LaunchFacts* sink = observe_sink())
+    return record_launch(sink, reinterpret_cast<const void*>(kernel),
+                         NT == 1 ? "paged_rows_int4_kernel 8 rows" : "paged_rows_int4_kernel 16 rows", grid, threads, smem, 1);
+  e = launch_programmatic(kernel, dim3(unsigned(grid)), dim3(threads), smem, stream, 1, map_k, map_v,
+                          static_cast<const uint32_t*>(cache.k_scales), static_cast<const uint32_t*>(cache.v_scales), p);
+  if (e != cudaSuccess) return cuda_status(e);
+  note_launch();
+  return launch_status();
+}
+
+template <typename T, int D, int GROUP>
+int launch_rows(const CUtensorMap& map_k, const CUtensorMap& map_v, const Int4Cache& cache, const PagedParams& p, int tile_rows, int grid,
+                cudaStream_t stream) {
+  return tile_rows == 8 ? launch<T, D, GROUP, 1>(map_k, map_v, cache, p, grid, stream)
+                        : launch<T, D, GROUP, 2>(map_k, map_v, cache, p, grid, stream);
+}
+
+}  // namespace
+
+template <typename T>
+int paged_rows_int4(const PagedParams& p, int64_t dim, int tile_rows, const Int4Cache& cache, int grid, cudaStream_t stream) {
+  CUtensorMap map_k, map_v;
+  const uint64_t rows = uint64_t(p.pages) * uint64_t(p.k_heads) << p.page_shift;
+  const uint32_t box = (1 << p.page_shift) < UNIT ? 1u << p.page_shift : UNIT;
+  const auto swizzle = dim == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
+  const uint64_t row = uint64_t(dim) / 2;
+  if (!make_tensor_map_2d(&map_k, CU_TENSOR_MAP_DATA_TYPE_UINT8, cache.k_codes, rows, row, row, box, uint32_t(row), swizzle) ||
+      !make_tensor_map_2d(&map_v, CU_TENSOR_MAP_DATA_TYPE_UINT8, cache.v_codes, rows, row, row, box, uint32_t(row), swizzle))
+    return INTENT_B200_ERR_CUDA;
+  if (dim == 64)
+    return cache.group == 32 ? launch_rows<T, 64, 32>(map_k, map_v, cache, p, tile_rows, grid, stream)
+                             : launch_rows<T, 64, 64>(map_k, map_v, cache, p, tile_rows, grid, stream);
+  return cache.group == 32   ? launch_rows<T, 128, 32>(map_k, map_v, cache, p, tile_rows, grid, stream)
+         : cache.group == 64 ? launch_rows<T, 128, 64>(map_k, map_v, cache, p, tile_rows, grid, stream)
+                             : launch_rows<T, 128, 128>(map_k, map_v, cache, p, tile_rows, grid, stream);
+}
+template int paged_rows_int4<__half>(const PagedParams&, int64_t, int, const Int4Cache&, int, cudaStream_t);
+template int paged_rows_int4<__nv_bfloat16>(const PagedParams&, int64_t, int, const Int4Cache&, int, cudaStream_t);
+
+}  // namespace ib200

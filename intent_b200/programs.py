@@ -875,8 +875,31 @@ def _cache_rules():
                   lambda d: f"a page must hold a power of two from 16 to 256 tokens, got {d['PAGE']}"),)
 
 
-def _lower_rotation(c, device, *, cache):
+def _group_size(c):
+    group = c["GROUP_SIZE"]
+    if group not in (32, 64, 128):
+        raise CompilationStageError("provider_native_compilation", f"GROUP_SIZE {group} has no kernel specialisation")
+    return int(group)
+
+
+def _int4_cache(view, act, access):
+    """Keys and values in 4 bits: codes, two to a byte, and scale and minimum of every group."""
+    for name in ("k", "v"):
+        view(f"{name}_cache", dtypes.u8, ("PAGES", "HK", "PAGE", "C"), access)
+        view(f"{name}_scales", act, ("PAGES", "HK", "PAGE", "S"), access)
+
+
+def _int4_rules(group):
+    return _cache_rules() + (
+        _rule(lambda d: d["D"] == 2 * d["C"], lambda d: f"k_cache and v_cache must have {d['D'] // 2} bytes a row, got {d['C']}"),
+        _rule(lambda d: d["D"] % group == 0, lambda d: f"GROUP_SIZE {group} does not divide heads of {d['D']}"),
+        _rule(lambda d: d["S"] * group == 2 * d["D"],
+              lambda d: f"k_scales and v_scales must have {2 * d['D'] // group} numbers a row, got {d['S']}"))
+
+
+def _lower_rotation(c, device, *, cache, bits=16):
     act = _act_dtype(c)
+    group = _group_size(c) if bits == 4 else None
     pairs = _PAIRS.get(c["PAIRS"])
     if pairs is None:
         raise CompilationStageError("frontend_kir", "PAIRS must be 'halves' or 'neighbours'")
@@ -904,17 +927,22 @@ def _lower_rotation(c, device, *, cache):
         _rule(lambda d: d["R"] % 16 == 0 and 0 < d["R"] <= d["D"],
               lambda d: f"rotary.shape[1] must be a multiple of 16 up to {d['D']}, got {d['R']}"))
     if cache:
-        view("k_cache", act, ("PAGES", "HK", "PAGE", "D"), INOUT)
-        view("v_cache", act, ("PAGES", "HK", "PAGE", "D"), INOUT)
-        rules += _cache_rules()
-        stem = "paged_kv_append_norm" if c["NORM"] else "paged_kv_append"
+        if bits == 4:
+            _int4_cache(view, act, INOUT)
+            rules += _int4_rules(group)
+        else:
+            view("k_cache", act, ("PAGES", "HK", "PAGE", "D"), INOUT)
+            view("v_cache", act, ("PAGES", "HK", "PAGE", "D"), INOUT)
+            rules += _cache_rules()
+        stem = ("paged_kv_append_norm" if c["NORM"] else "paged_kv_append") + ("_int4" if bits == 4 else "")
     else:
         stem = "qk_norm_rope" if c["NORM"] else "qk_rope"
     view("q_out", act, ("T", "HQ", "D"), OUT)
     if not cache:
         view("k_out", act, ("T", "HK", "D"), OUT)
     return NativeProgram(interface=PublicInterface(tuple(views), dimension_rules=rules), device=device,
-                         entry_name=f"intent_b200_{stem}_{act.name}", constants=(eps, pairs) if c["NORM"] else (pairs,),
+                         entry_name=f"intent_b200_{stem}_{act.name}",
+                         constants=((group,) if bits == 4 else ()) + ((eps, pairs) if c["NORM"] else (pairs,)),
                          empty=lambda d: d["T"] == 0)
 
 
@@ -927,6 +955,39 @@ paged_kv_append = KernelDefinition(
     "paged_kv_append", dict(_ROTATION_CONSTEXPRS), lambda c, d: _lower_rotation(c, d, cache=True),
     "an interface of its own (the reference's attention programs are not ported)",
     "as qk_norm_rope, the keys and with them the values stored in a paged cache at slots[t] (-1: not stored; every slot once)")
+
+
+paged_kv_append_int4 = KernelDefinition(
+    "paged_kv_append_int4", dict(_ROTATION_CONSTEXPRS, GROUP_SIZE=64), lambda c, d: _lower_rotation(c, d, cache=True, bits=4),
+    "an interface of its own (the reference's attention programs are not ported)",
+    "as paged_kv_append, keys and values held in 4 bits: m + s n with a scale s and a minimum m for GROUP_SIZE elements")
+
+
+def _lower_read(c, device):
+    act, group = _act_dtype(c), _group_size(c)
+    views = []
+
+    def view(name, element, shape, access=IN, alignment=16):
+        views.append(ViewParameter(len(views), name, element, shape, access, alignment))
+
+    view("slots", dtypes.i64, ("T",), alignment=8)
+    _int4_cache(view, act, IN)
+    width = Derived("D", lambda d: 2 * d["C"])
+    view("k", act, ("T", "HK", width), OUT)
+    view("v", act, ("T", "HK", width), OUT)
+
+    def rules(d):
+        for check in _head_rules() + _int4_rules(group):
+            check({**d, "D": 2 * d["C"]})
+
+    return NativeProgram(interface=PublicInterface(tuple(views), dimension_rules=(rules,)), device=device,
+                         entry_name=f"intent_b200_paged_kv_read_int4_{act.name}", constants=(group,), empty=lambda d: d["T"] == 0)
+
+
+paged_kv_read_int4 = KernelDefinition(
+    "paged_kv_read_int4", {"ACT_DTYPE": "bf16", "GROUP_SIZE": 64}, _lower_read,
+    "an interface of its own (the reference's attention programs are not ported)",
+    "keys and values [T, HK, D] out of a paged cache in 4 bits at slots[t] (-1: zeros), f32 arithmetic, one rounding")
 
 
 @cache
@@ -947,31 +1008,42 @@ def _paged_workspace_bytes(d, single, window):
     return int(query(d["T"], d["B"], d["HQ"], d["HK"], d["D"], d["W"] * d["PAGE"], window))
 
 
-def _lower_paged(c, device, *, single):
+def _lower_paged(c, device, *, single, bits=16):
     act = _act_dtype(c)
+    group = _group_size(c) if bits == 4 else None
     scale, window = c["SCALE"], c["WINDOW"]
-    bits = _f32_bits(0 if scale is None else scale, "SCALE")
-    if scale is not None and not 0 < bits < 0x7f800000:      # (as the f32 that it becomes: 0 would stand for the default)
+    factor = _f32_bits(0 if scale is None else scale, "SCALE")
+    if scale is not None and not 0 < factor < 0x7f800000:      # (as the f32 that it becomes: 0 would stand for the default)
         raise CompilationStageError("frontend_kir", "SCALE must be a positive f32 number, or None for 1 / sqrt(D)")
     if not isinstance(window, int) or not 0 <= window < 1 << 31:
         raise CompilationStageError("frontend_kir", "WINDOW must be a number of tokens, 0 for all")
-    views = [ViewParameter(0, "q", act, ("B" if single else "T", "HQ", "D"), IN, layout="rows"),
-             ViewParameter(1, "k_cache", act, ("PAGES", "HK", "PAGE", "D"), IN),
-             ViewParameter(2, "v_cache", act, ("PAGES", "HK", "PAGE", "D"), IN),
-             ViewParameter(3, "page_table", dtypes.i32, ("B", "W"), IN, alignment=4)]
+    if group and scale is not None and scale > 2.0 ** 50:
+        raise CompilationStageError("provider_native_compilation", "SCALE must be at most 2^50 for a cache in 4 bits")
+    views = []
+
+    def view(name, element, shape, access=IN, alignment=16, layout="contiguous"):
+        views.append(ViewParameter(len(views), name, element, shape, access, alignment, layout))
+
+    view("q", act, ("B" if single else "T", "HQ", "D"), layout="rows")
+    if group:
+        _int4_cache(view, act, IN)
+    else:
+        view("k_cache", act, ("PAGES", "HK", "PAGE", "D"))
+        view("v_cache", act, ("PAGES", "HK", "PAGE", "D"))
+    view("page_table", dtypes.i32, ("B", "W"), alignment=4)
     if not single:
-        views.append(ViewParameter(4, "query_offsets", dtypes.i32, ("B_PLUS_1",), IN, alignment=4))
-    views.append(ViewParameter(len(views), "kv_lengths", dtypes.i32, ("B",), IN, alignment=4))
-    views.append(ViewParameter(len(views), "output", act, ("B" if single else "T", "HQ", "D"), OUT))
-    rules = _head_rules() + _cache_rules() + (
+        view("query_offsets", dtypes.i32, ("B_PLUS_1",), alignment=4)
+    view("kv_lengths", dtypes.i32, ("B",), alignment=4)
+    view("output", act, ("B" if single else "T", "HQ", "D"), OUT)
+    rules = _head_rules() + (_int4_rules(group) if group else _cache_rules()) + (
         _rule(lambda d: d["HK"] > 0 and d["HQ"] > 0 and d["HQ"] % d["HK"] == 0,
               lambda d: f"{d['HQ']} query heads do not share {d['HK']} key heads evenly"),)
     if not single:
         rules += (_rule(lambda d: d["B_PLUS_1"] == d["B"] + 1, "query_offsets must have B + 1 entries"),)
-    stem = "paged_decode_attention" if single else "paged_attention"
+    stem = ("paged_decode_attention" if single else "paged_attention") + ("_int4" if group else "")
     return NativeProgram(interface=PublicInterface(tuple(views), dimension_rules=rules), device=device,
                          entry_name=f"intent_b200_{stem}_{act.name}",
-                         constants=(bits, window),
+                         constants=((group,) if group else ()) + (factor, window),
                          workspace=lambda d: _paged_workspace_bytes(d, single, window),
                          empty=lambda d: d["B"] == 0 or (not single and d["T"] == 0),
                          workspace_status="intent_b200_paged_attention_workspace_status")
@@ -987,4 +1059,14 @@ paged_decode_attention = KernelDefinition(
     "an interface of its own (the reference's attention programs are not ported)",
     "attention of one new token per sequence over its pages")
 
-ALL.update({d.name: d for d in (qk_norm_rope, paged_kv_append, paged_attention, paged_decode_attention)})
+paged_attention_int4 = KernelDefinition(
+    "paged_attention_int4", dict(_PAGED_CONSTEXPRS, GROUP_SIZE=64), lambda c, d: _lower_paged(c, d, single=False, bits=4),
+    "an interface of its own (the reference's attention programs are not ported)",
+    "paged_attention over the cache that paged_kv_append_int4 writes")
+paged_decode_attention_int4 = KernelDefinition(
+    "paged_decode_attention_int4", dict(_PAGED_CONSTEXPRS, GROUP_SIZE=64), lambda c, d: _lower_paged(c, d, single=True, bits=4),
+    "an interface of its own (the reference's attention programs are not ported)",
+    "paged_decode_attention over the cache that paged_kv_append_int4 writes")
+
+ALL.update({d.name: d for d in (qk_norm_rope, paged_kv_append, paged_attention, paged_decode_attention, paged_kv_append_int4,
+                                paged_kv_read_int4, paged_attention_int4, paged_decode_attention_int4)})

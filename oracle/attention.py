@@ -60,3 +60,24 @@ def paged_attention(q, k_cache, v_cache, page_table, query_offsets, kv_lengths, 
             out[start + i] = torch.einsum("hgn,nhd->hgd", w, values).reshape(HQ, D)
             weight[start + i] = torch.einsum("hgn,nhd->hgd", w, values.abs()).reshape(HQ, D)
     return out, weight
+
+
+def quantise(x, group, dtype):
+    """Rows [..., D] -> (codes [..., D / 2] u8, scales [..., 2 D / group]): groups as m + s * n, in 64 bits."""
+    y = x.double().unflatten(-1, (-1, group))
+    m = y.amin(-1).to(dtype)
+    s = (y.amax(-1) / 15 - y.amin(-1) / 15).to(dtype)
+    beyond = ~(m.double() + 15 * s.double()).to(dtype).isfinite() & m.isfinite() & s.isfinite() & y.amax(-1).isfinite()
+    s = (s.view(torch.int16) - beyond.to(torch.int16)).view(dtype)       # the next lower number
+    bad = ~(m.isfinite() & s.isfinite())
+    s, m = s.masked_fill(bad, math.nan), m.masked_fill(bad, math.nan)
+    n = ((y - m.double()[..., None]) / s.double()[..., None]).nan_to_num(0, 0, 0).round().clamp(0, 15).to(torch.uint8)
+    n = n.flatten(-2)
+    return n[..., 0::2] + 16 * n[..., 1::2], torch.stack([s, m], -1).flatten(-2)
+
+
+def values(codes, scales, group):
+    """What a cache in 4 bits stands for, [..., D] in f64, and the same with 8 in the place of every code."""
+    n = torch.stack([codes % 16, codes // 16], -1).flatten(-2).double().unflatten(-1, (-1, group))
+    s, m = scales.double().unflatten(-1, (-1, 2)).split(1, -1)
+    return (m + s * n).flatten(-2), (m + s * 8).expand_as(n).flatten(-2)

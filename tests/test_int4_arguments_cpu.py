@@ -1,0 +1,89 @@
+"""What the programs of a cache in 4 bits refuse, in the compiler and at the C entries, without a GPU."""
+import ctypes
+import math
+
+import pytest
+
+import intent_b200 as ib
+from intent_b200.runtime import native
+
+PROGRAMS = ["paged_kv_append_int4", "paged_kv_read_int4", "paged_attention_int4", "paged_decode_attention_int4"]
+
+
+@pytest.mark.parametrize("name", PROGRAMS)
+@pytest.mark.parametrize("constexprs", [{"GROUP_SIZE": 16}, {"GROUP_SIZE": 48}, {"GROUP_SIZE": 256}, {"GROUP_SIZE": "64"},
+                                        {"GROUP_SIZE": None}, {"ACT_DTYPE": "f32"}, {"BITS": 4}])
+def test_constants(name, constexprs):
+    with pytest.raises(ib.CompilationStageError):
+        ib.compile(getattr(ib.programs, name), constexprs=constexprs, resolve_target=False)
+
+
+@pytest.mark.parametrize("name", PROGRAMS[2:])
+@pytest.mark.parametrize("scale", [0, -1.0, 1e-46, math.inf, math.nan, 2.0 ** 51, 3e38])
+def test_scales_of_scores(name, scale):
+    with pytest.raises(ib.CompilationStageError):
+        ib.compile(getattr(ib.programs, name), constexprs={"SCALE": scale}, resolve_target=False)
+
+
+@pytest.mark.parametrize("name", PROGRAMS)
+def test_saved_and_loaded(name, tmp_path):
+    artifact = ib.compile(getattr(ib.programs, name), constexprs={"GROUP_SIZE": 32}, resolve_target=False)
+    again = ib.load(artifact.save(tmp_path / "program"), resolve_target=False)
+    assert again.runtime.constants == artifact.runtime.constants and again.runtime.entry_name == artifact.runtime.entry_name
+
+
+def view(shape, pointer=0x10000, strides=None):
+    if strides is None:
+        strides = [math.prod(shape[i + 1:]) for i in range(len(shape))]
+    return [pointer, *shape, *strides]
+
+
+def status(name, views, *rest):
+    slots = [s for v in views for s in v]
+    carriers = ["ptr" if i == 0 else "i64" for v in views for i in range(len(v))]
+    return native.entry(f"intent_b200_{name}_bf16", (*carriers, *("i32" if r is not None else "ptr" for r in rest)))(*slots, *rest, None)
+
+
+OK, SHAPE, LAYOUT, UNSUPPORTED, WORKSPACE, NULL = 0, 1, 2, 3, 5, 6
+
+
+def cache(pages=4, heads=2, page=16, dim=128, group=64):
+    return [view([pages, heads, page, dim // 2]), view([pages, heads, page, 2 * dim // group])] * 2
+
+
+def read(slots=5, parts=None, heads=2, dim=128, group=64, **changes):
+    views = [view([slots]), *(parts or cache(heads=heads, dim=dim, group=group)), view([slots, heads, dim]), view([slots, heads, dim])]
+    for place, v in changes.items():
+        views[int(place[1:])] = v
+    return status("paged_kv_read_int4", views, group)
+
+
+def test_entry_of_reads():
+    assert read(slots=0) == OK
+    assert read(group=48) == read(dim=64, group=128) == read(dim=96, group=32) == UNSUPPORTED
+    assert read(parts=cache(page=24)) == read(parts=cache(page=8)) == UNSUPPORTED
+    assert read(parts=cache(heads=3)) == read(parts=cache(dim=64)) == read(parts=cache(group=32)) == SHAPE
+    assert read(_3=view([3, 2, 16, 64])) == read(_6=view([5, 2, 64])) == read(_5=view([4, 2, 128])) == SHAPE
+    assert read(_1=view([4, 2, 16, 64], 0x10008)) == read(_2=view([4, 2, 16, 4], strides=[128, 4, 8, 1])) == LAYOUT
+    assert read(_5=view([5, 2, 128], 0x10002)) == LAYOUT
+    assert read(_1=view([4, 2, 16, 64], 0)) == read(_0=view([5], 0)) == read(_4=view([4, 2, 16, 4], 0)) == NULL
+
+
+def attend(parts=None, group=64, scale=0, window=0, workspace=None, tokens=3, q=None, heads=4):
+    views = [q or view([tokens, heads, 128]), *(parts or cache()), view([tokens, 2]), view([tokens]), view([tokens, heads, 128])]
+    slots = [s for v in views for s in v]
+    carriers = ["ptr" if i == 0 else "i64" for v in views for i in range(len(v))]
+    entry = native.entry("intent_b200_paged_decode_attention_int4_bf16", (*carriers, "i32", "i32", "i32", "ptr", "i64"))
+    return entry(*slots, group, scale, window, workspace, 0, None)
+
+
+def test_entry_of_attention():
+    assert attend(tokens=0) == OK
+    assert attend() == WORKSPACE
+    assert attend(group=48) == attend(window=-1) == attend(parts=cache(page=512)) == UNSUPPORTED
+    assert attend(scale=0x59000000) == UNSUPPORTED          # 2^51
+    assert attend(scale=0x58800000) == WORKSPACE            # 2^50
+    assert attend(parts=cache(group=32)) == attend(parts=cache(heads=3)) == attend(parts=cache(dim=64)) == SHAPE
+    assert attend(parts=[*cache()[:3], view([4, 2, 16, 4], 0x10004)]) == LAYOUT
+    assert attend(parts=[*cache()[:3], view([4, 2, 16, 4], 0)]) == attend(q=view([3, 4, 128], 0)) == NULL
+    assert ctypes.sizeof(ctypes.c_void_p) == 8
