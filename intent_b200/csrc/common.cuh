@@ -260,6 +260,11 @@ struct Elem<__half> {
     asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
   }
+  __device__ static __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+  }
   __device__ static __forceinline__ float to_float(uint16_t bits) {
     return __half2float(__ushort_as_half(bits));
   }
@@ -301,6 +306,11 @@ struct Elem<__nv_bfloat16> {
   __device__ static __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
     uint32_t d;
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
+  __device__ static __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
     return d;
   }
   __device__ static __forceinline__ float to_float(uint16_t bits) {

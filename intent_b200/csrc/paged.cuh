@@ -126,6 +126,8 @@ bool paged_chunk_takes(const PagedParams& p);
 int paged_chunk_half_tokens(const PagedParams& p);
 template <typename T>
 int paged_chunk(const PagedParams& p, int64_t dim, const void* k_cache, const void* v_cache, int grid, cudaStream_t stream);
+template <typename T>
+int paged_chunk_int4(const PagedParams& p, int64_t dim, const Int4Cache& cache, int grid, cudaStream_t stream);
 
 // the parts that paged_rows (tile_rows > 0) and paged_chunk (`chunks`) leave (paged_join.cu)
 template <typename T>

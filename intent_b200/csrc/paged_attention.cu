@@ -115,7 +115,7 @@ int attend(const View3& q, const CacheViews& cache, const View2& table, const Vi
   while ((int64_t(1) << p.page_shift) < page) ++p.page_shift;
   p.window = window < p.capacity ? window : 0;   // (a query that sees as many tokens as there may be sees all)
   p.scale = scale * 1.44269504f;         // log2(e): the exponentials are powers of two
-  const Choice choice = choose(tokens, batch, p.group, dim, p.capacity, p.window, offsets && !int4 && paged_chunk_takes(p));
+  const Choice choice = choose(tokens, batch, p.group, dim, p.capacity, p.window, offsets && paged_chunk_takes(p));
   p.few = choice.few;
   if (!workspace || workspace_bytes < workspace_bytes_of(dim, choice.chunks)) return INTENT_B200_ERR_WORKSPACE;
   if (!aligned16(workspace)) return INTENT_B200_ERR_LAYOUT;
@@ -128,8 +128,8 @@ int attend(const View3& q, const CacheViews& cache, const View2& table, const Vi
   const WorkspaceTurn turn(workspace);
   const int grid = std::min(sms, kPagedCtas);
   PagedParams chunk = p;
+  const Int4Cache codes = {k_cache.p, int4 ? cache.k_scales->p : nullptr, v_cache.p, int4 ? cache.v_scales->p : nullptr, cache.group};
   if (choice.tile_rows > 0) {
-    const Int4Cache codes = {k_cache.p, int4 ? cache.k_scales->p : nullptr, v_cache.p, int4 ? cache.v_scales->p : nullptr, cache.group};
     const int status = int4 ? paged_rows_int4<T>(p, dim, choice.tile_rows, codes, grid, stream)
                             : paged_rows<T>(p, dim, choice.tile_rows, k_cache.p, v_cache.p, grid, stream);
     if (status != INTENT_B200_OK) return status;
@@ -138,7 +138,8 @@ int attend(const View3& q, const CacheViews& cache, const View2& table, const Vi
     chunk.joins = static_cast<unsigned char*>(workspace) + kPagedChunkJoins;
     chunk.parts += paged_rows_parts_bytes(dim) / int64_t(sizeof(float));
     chunk.half_tokens = paged_chunk_half_tokens(p);
-    const int status = paged_chunk<T>(chunk, dim, k_cache.p, v_cache.p, grid, stream);
+    const int status = int4 ? paged_chunk_int4<T>(chunk, dim, codes, grid, stream)
+                            : paged_chunk<T>(chunk, dim, k_cache.p, v_cache.p, grid, stream);
     if (status != INTENT_B200_OK) return status;
   }
   return paged_join<T>(p, choice.tile_rows, chunk, choice.chunks, dim, grid, stream);

@@ -48,7 +48,8 @@ namespace ib200 {
 namespace {
 
 constexpr int STEP = 128;                  // tokens of a step
-constexpr int LOAD_WARP = 9, MMA_WARP = 8, THREADS = 12 * 32;   // warps 0..3 and 4..7: a half's rows; 10 and 11 only lend registers
+// warps 0..3 and 4..7: a half's rows; 10 and 11 turn codes of a cache in 4 bits into operands, and else only lend registers
+constexpr int LOAD_WARP = 9, MMA_WARP = 8, THREADS = 12 * 32, CONVERT_WARPS = 2;
 // Registers of a thread: the launch's, then those of a row's thread (128 scores and more) and of the others.
 constexpr int LAUNCH_REGISTERS = 168, ROW_REGISTERS = 224, OTHER_REGISTERS = 56;
 static_assert(2 * ROW_REGISTERS + OTHER_REGISTERS <= 3 * LAUNCH_REGISTERS, "three warpgroups share the launch's registers");
@@ -59,13 +60,24 @@ constexpr int BEGIN = 2;
 constexpr int EARLY = 96;                  // tokens of a step whose weights the products begin with
 constexpr float SLACK = 8.f;               // growth of a row's maximum (log2) that its weights are left to absorb
 
-template <int D>
+// GROUP: elements of a group of a cache in 4 bits, 0 for one of 16-bit elements
+template <int D, int GROUP>
 struct Room {
   static constexpr int BOX = STEP * 128;                 // 64 elements of 128 rows
   static constexpr int OPERAND = BOX * (D / 64);
-  static constexpr int SLOTS = D == 128 ? 5 : 10;
-  static constexpr int BYTES = (2 + SLOTS) * OPERAND;
+  static constexpr int SLOTS = GROUP ? (D == 128 ? 4 : 8) : D == 128 ? 5 : 10;
+  // codes of a step's keys or values, and their scales, on their way to a slot
+  static constexpr int GROUPS = GROUP ? D / (GROUP ? GROUP : D) : 0, ROW = D / 2;
+  static constexpr int STAGES = GROUP ? (D == 128 ? 3 : 4) : 0, CODES = STEP * ROW, STAGE = CODES + STEP * GROUPS * 4;
+  static constexpr int OPERANDS = (2 + SLOTS) * OPERAND, BYTES = OPERANDS + STAGES * STAGE;
 };
+
+// Column of an element among eight: values of a cache in 4 bits are put down as they come out of a word, one of its lower four
+// codes beside one of its upper.
+template <int GROUP>
+__host__ __device__ constexpr int column_of(int element) {
+  return GROUP == 0 ? element : (element & ~7) + 2 * (element & 3) + (element >> 2 & 1);
+}
 
 // ---- the line of steps -----------------------------------------------------------------------------------------------
 struct Sequence {
@@ -245,11 +257,21 @@ __device__ __forceinline__ void weigh(const uint32_t (&v)[32], uint64_t scale, u
   }
 }
 
+// Eight codes as numbers m + s * n of the type, rounded once: elements 0 and 4, 1 and 5, 2 and 6, 3 and 7
+template <typename T>
+__device__ __forceinline__ void numbers_of(uint32_t codes, uint32_t s, uint32_t m, uint32_t (&w)[4]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    constexpr uint32_t ZERO = Elem<T>::kMagic2;
+    w[e] = Elem<T>::fma2(Elem<T>::sub2(lop3_and_or(codes >> (4 * e), 0x000f000fu, Elem<T>::kMagic2), ZERO), s, m);
+  }
+}
+
 // What lies behind the operands in shared memory
 template <int SLOTS>
 struct Shared {
   uint64_t q_full, q_empty, kv_full[SLOTS], kv_empty[SLOTS], s_full[2], p_full[2][2], o_full[2], vote_full[2], part_full[4],
-      part_empty[4], products_over;
+      part_empty[4], products_over, stage_full[4], stage_empty[4];
   long long warp_sums[THREADS / 32];
   Part parts[4];
   long long start, start_head;             // this CTA's first place, counted in the sequence; places of a key head of it
@@ -258,13 +280,14 @@ struct Shared {
   volatile int skip[2];                    // this half's step has been added to O by its threads
   volatile uint32_t vote[2];               // step + 1 in which a warp of the half asked for that
   volatile uint32_t missing[8];            // per step, boxes of pages outside the cache
+  volatile uint32_t absent[8];             // and of those, with boxes that no query sees, that were not asked for (4 bits)
 };
 
-template <typename T, int D>
+template <typename T, int D, int GROUP>
 __global__ void __launch_bounds__(THREADS, 1)
 paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                   const __grid_constant__ CUtensorMap map_v, const PagedParams p) {
-  using R = Room<D>;
+                   const __grid_constant__ CUtensorMap map_v, const Int4Cache cache, const PagedParams p) {
+  using R = Room<D, GROUP>;
   constexpr int SLOTS = R::SLOTS, BOXES = D / 64;
   extern __shared__ unsigned char smem_raw[];
   programmatic_begin();
@@ -278,17 +301,21 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                  s_full = bars + offsetof(Shared<SLOTS>, s_full), p_full = bars + offsetof(Shared<SLOTS>, p_full),
                  o_full = bars + offsetof(Shared<SLOTS>, o_full), vote_full = bars + offsetof(Shared<SLOTS>, vote_full),
                  part_full = bars + offsetof(Shared<SLOTS>, part_full), part_empty = bars + offsetof(Shared<SLOTS>, part_empty),
-                 products_over = bars + offsetof(Shared<SLOTS>, products_over);
+                 products_over = bars + offsetof(Shared<SLOTS>, products_over),
+                 stage_full = bars + offsetof(Shared<SLOTS>, stage_full), stage_empty = bars + offsetof(Shared<SLOTS>, stage_empty);
+  const uint32_t stages = base + R::OPERANDS;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     prefetch_tensormap(&map_q);
-    prefetch_tensormap(&map_k);
-    prefetch_tensormap(&map_v);
+    if (GROUP == 0) {
+      prefetch_tensormap(&map_k);
+      prefetch_tensormap(&map_v);
+    }
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
     for (int i = 0; i < SLOTS; ++i) {
-      mbar_init(kv_full + 8 * i, 1);
+      mbar_init(kv_full + 8 * i, GROUP ? CONVERT_WARPS : 1);
       mbar_init(kv_empty + 8 * i, 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -302,8 +329,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     mbar_init(products_over, 1);
     for (int i = 0; i < 4; ++i) {
       mbar_init(part_full + 8 * i, 1);
-      mbar_init(part_empty + 8 * i, 9);      // the warps of both halves and the products'
+      mbar_init(part_empty + 8 * i, GROUP ? 9 + CONVERT_WARPS : 9);      // the warps of both halves and the products'
     }
+    if (GROUP)
+      for (int i = 0; i < R::STAGES; ++i) {
+        mbar_init(stage_full + 8 * i, 1);
+        mbar_init(stage_empty + 8 * i, CONVERT_WARPS);
+      }
     fence_mbar_init();
   }
   if (warp == MMA_WARP) tmem_alloc(bars + offsetof(Shared<SLOTS>, tmem), 512);
@@ -415,23 +447,50 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
           const bool there = page >= 0 && page < p.pages;
           const int row = there ? ((page * p.k_heads + head) << p.page_shift) + (token & ((1 << p.page_shift) - 1)) : cache_rows;
           const uint32_t missing = __ballot_sync(0xffffffffu, wanted && !there && column == 0);
+          if constexpr (GROUP > 0) {
+            // codes by the lanes of column 0, scales by those of column 1, each one run of bytes
+            const uint32_t absent = __ballot_sync(0xffffffffu, !there && column == 0);
+            const uint32_t bytes = uint32_t((boxes - __popc(absent)) * rows * (R::ROW + 4 * R::GROUPS));
 #pragma unroll
-          for (int operand = 0; operand < 2; ++operand) {
-            const uint32_t slot = (2 * u + operand) % SLOTS, turn = (2 * u + operand) / SLOTS;
-            ok = mbar_wait_warp(kv_empty + 8 * slot, (turn & 1) ^ 1);
-            if (!ok) {
-              odd = operand;
-              return false;
+            for (int operand = 0; operand < 2; ++operand) {
+              const uint32_t stage = (2 * u + operand) % R::STAGES, turn = (2 * u + operand) / R::STAGES;
+              ok = mbar_wait_warp(stage_empty + 8 * stage, (turn & 1) ^ 1);
+              if (!ok) {
+                odd = operand;
+                return false;
+              }
+              if (lane == 0) {
+                if (operand == 0) sh.missing[u & 7] = missing, sh.absent[u & 7] = absent;
+                mbar_expect_tx(stage_full + 8 * stage, bytes);
+              }
+              __syncwarp();
+              if (there && column < 2) {
+                const uint32_t size = column ? 4 * R::GROUPS : R::ROW;                 // bytes of a token
+                const void* from = operand == 0 ? (column ? cache.k_scales : cache.k_codes) : (column ? cache.v_scales : cache.v_codes);
+                bulk_load(stages + stage * R::STAGE + column * R::CODES + box * rows * size,
+                          static_cast<const unsigned char*>(from) + int64_t(row) * size, rows * size, stage_full + 8 * stage);
+              }
+              __syncwarp();
             }
-            if (lane == 0) {
-              if (operand == 0) sh.missing[u & 7] = missing;
-              mbar_expect_tx(kv_full + 8 * slot, R::OPERAND);
+          } else {
+#pragma unroll
+            for (int operand = 0; operand < 2; ++operand) {
+              const uint32_t slot = (2 * u + operand) % SLOTS, turn = (2 * u + operand) / SLOTS;
+              ok = mbar_wait_warp(kv_empty + 8 * slot, (turn & 1) ^ 1);
+              if (!ok) {
+                odd = operand;
+                return false;
+              }
+              if (lane == 0) {
+                if (operand == 0) sh.missing[u & 7] = missing;
+                mbar_expect_tx(kv_full + 8 * slot, R::OPERAND);
+              }
+              __syncwarp();
+              if (column < BOXES)
+                tma_load_2d(ring + slot * R::OPERAND + column * R::BOX + box * rows * 128, operand == 0 ? &map_k : &map_v, 64 * column,
+                            row, kv_full + 8 * slot);
+              __syncwarp();
             }
-            __syncwarp();
-            if (column < BOXES)
-              tma_load_2d(ring + slot * R::OPERAND + column * R::BOX + box * rows * 128, operand == 0 ? &map_k : &map_v, 64 * column,
-                          row, kv_full + 8 * slot);
-            __syncwarp();
           }
         }
         return true;
@@ -444,8 +503,67 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       // (also where another warp gave up: no load may be on its way to a CTA that is gone)
       if (parts > 0) mbar_wait_warp(q_full, (parts - 1) & 1);
       const uint32_t loads = 2 * u + odd, last = loads - 1 - lane;
-      if (lane < min(loads, uint32_t(SLOTS))) mbar_wait(kv_full + 8 * (last % SLOTS), last / SLOTS & 1, 1u << 12);
+      constexpr uint32_t PLACES = GROUP ? R::STAGES : SLOTS;
+      if (lane < min(loads, PLACES)) mbar_wait((GROUP ? stage_full : kv_full) + 8 * (last % PLACES), last / PLACES & 1, 1u << 12);
       __syncwarp();
+    } else if (GROUP > 0 && warp > LOAD_WARP) {
+      // ------------------------------ codes to numbers ----------------------------
+      // A lane turns 32 codes (16 bytes of a row) into four pieces of eight numbers where the products expect them, in an order in
+      // which eight lanes meet 32 banks.  Keys' elements lie as the queries' do, values' by column_of.
+      if constexpr (GROUP > 0) {
+        constexpr int PER_ROW = D / 32, ROWS_AT_ONCE = 32 / PER_ROW, ROWS = STEP / CONVERT_WARPS;
+        const int k = lane % PER_ROW, first_row = (warp - LOAD_WARP - 1) * ROWS + lane / PER_ROW;
+        const bool swapped = (k & 2) != 0;
+        const int shift = min(p.page_shift, 7);
+        uint32_t parts = 0, n = 0;                                     // n: operands
+        while (ok) {
+          const uint32_t place = parts & 3;
+          ok = mbar_wait_warp(part_full + 8 * place, parts / 4 & 1);
+          if (!ok || sh.parts[place].steps == 0) break;
+          const int steps = sh.parts[place].steps;
+          ++parts;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(part_empty + 8 * place);
+          for (int i = 0; i < 2 * steps; ++i, ++n) {
+            const uint32_t stage = n % R::STAGES, slot = n % SLOTS;
+            ok = mbar_wait_warp(stage_full + 8 * stage, n / R::STAGES & 1) && mbar_wait_warp(kv_empty + 8 * slot, (n / SLOTS & 1) ^ 1);
+            if (!ok) break;
+            const uint32_t absent = sh.absent[(n / 2) & 7];
+            const uint32_t codes = stages + stage * R::STAGE, scales = codes + R::CODES + (k * 32 / GROUP) * 4;
+            unsigned char* to = base_ptr + (ring - base) + slot * R::OPERAND + (k >> 1) * R::BOX;
+            auto convert = [&](auto values) {
+#pragma unroll 2
+              for (int r = first_row; r < first_row + ROWS; r += ROWS_AT_ONCE) {
+                const uint4 v = lds128(codes + r * R::ROW + 16 * k);
+                uint32_t pair;
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(pair) : "r"(scales + r * (4 * R::GROUPS)));
+                if (absent >> (r >> shift) & 1) pair = 0;              // (what is there was left by others)
+                const uint32_t s = prmt(pair, pair, 0x1010), m = prmt(pair, pair, 0x3232);
+                const uint32_t words[4] = {swapped ? v.z : v.x, swapped ? v.w : v.y, swapped ? v.x : v.z, swapped ? v.y : v.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  uint32_t w[4];
+                  numbers_of<T>(words[j], s, m, w);
+                  const uint4 out = decltype(values)::value
+                                        ? make_uint4(w[0], w[1], w[2], w[3])
+                                        : make_uint4(prmt(w[0], w[1], 0x5410), prmt(w[2], w[3], 0x5410), prmt(w[0], w[1], 0x7632),
+                                                     prmt(w[2], w[3], 0x7632));
+                  const int piece = 4 * (k & 1) + (swapped ? j ^ 2 : j);
+                  *reinterpret_cast<uint4*>(to + r * 128 + ((piece ^ (r & 7)) << 4)) = out;
+                }
+              }
+            };
+            if (i & 1) convert(Bool<true>{});
+            else convert(Bool<false>{});
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(kv_full + 8 * slot);
+              mbar_arrive(stage_empty + 8 * stage);
+            }
+          }
+        }
+      }
     } else if (warp == MMA_WARP) {
       // ------------------------------ products ------------------------------------
       constexpr uint32_t FORMAT = std::is_same<T, __half>::value ? 0 : 1;
@@ -763,7 +881,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             uint32_t x[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              x[j] = Elem<T>::pack2(__uint_as_float(o[e + 2 * j]) * inverse, __uint_as_float(o[e + 2 * j + 1]) * inverse);
+              x[j] = Elem<T>::pack2(__uint_as_float(o[column_of<GROUP>(e + 2 * j)]) * inverse,
+                                    __uint_as_float(o[column_of<GROUP>(e + 2 * j + 1)]) * inverse);
             *reinterpret_cast<uint4*>(to + 32 * c + e) = make_uint4(x[0], x[1], x[2], x[3]);
           }
         } else if (real) {
@@ -771,7 +890,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
             *reinterpret_cast<uint4*>(to_part + ((8 * c + e / 4) * 2 * HALF_ROWS + h * HALF_ROWS + row) * 4) =
-                make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                make_uint4(o[column_of<GROUP>(e)], o[column_of<GROUP>(e + 1)], o[column_of<GROUP>(e + 2)], o[column_of<GROUP>(e + 3)]);
         }
         __syncwarp();
       }
@@ -790,11 +909,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
 }
 
-template <typename T, int D>
-int launch(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v, const PagedParams& p, int grid,
-           cudaStream_t stream) {
-  auto kernel = paged_chunk_kernel<T, D>;
-  constexpr int smem = 1024 + Room<D>::BYTES + int(sizeof(Shared<Room<D>::SLOTS>));
+template <typename T, int D, int GROUP>
+int launch(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v, const Int4Cache& cache,
+           const PagedParams& p, int grid, cudaStream_t stream) {
+  auto kernel = paged_chunk_kernel<T, D, GROUP>;
+  constexpr int smem = 1024 + Room<D, GROUP>::BYTES + int(sizeof(Shared<Room<D, GROUP>::SLOTS>));
   static_assert(smem <= 227 * 1024, "shared memory of a CTA");
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return cuda_status(e);
@@ -808,9 +927,10 @@ int launch(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap
   }
   if (registers.load(std::memory_order_relaxed) != LAUNCH_REGISTERS) return INTENT_B200_ERR_UNSUPPORTED;
   if (LaunchFacts* sink = observe_sink())
-    return record_launch(sink, reinterpret_cast<const void*>(kernel), "paged_chunk_kernel 2 x 128 rows, parts joined", grid,
+    return record_launch(sink, reinterpret_cast<const void*>(kernel), GROUP ? "paged_chunk_kernel int4 2 x 128 rows, parts joined"
+                                                                                  : "paged_chunk_kernel 2 x 128 rows, parts joined", grid,
                          THREADS, smem, 1);
-  e = launch_programmatic(kernel, dim3(unsigned(grid)), dim3(THREADS), smem, stream, 1, map_q, map_k, map_v, p);
+  e = launch_programmatic(kernel, dim3(unsigned(grid)), dim3(THREADS), smem, stream, 1, map_q, map_k, map_v, cache, p);
   if (e != cudaSuccess) return cuda_status(e);
   note_launch();
   return launch_status();
@@ -828,26 +948,53 @@ bool paged_chunk_takes(const PagedParams& p) {
 
 int paged_chunk_half_tokens(const PagedParams& p) { return HALF_ROWS / p.group; }
 
+namespace {
+
+// 64 elements of the queries of half a tile
 template <typename T>
-int paged_chunk(const PagedParams& p, int64_t dim, const void* k_cache, const void* v_cache, int grid, cudaStream_t stream) {
+bool map_queries(CUtensorMap* map, const PagedParams& p, int64_t dim) {
   EncodeTiledFn encode = encode_tiled_fn();
-  if (!encode) return INTENT_B200_ERR_CUDA;
-  CUtensorMap map_q, map_k, map_v;
-  const uint64_t rows = uint64_t(p.pages) * uint64_t(p.k_heads) << p.page_shift;
   constexpr auto type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const uint32_t box = uint32_t(std::min(1 << p.page_shift, STEP));
   const cuuint64_t dims[3] = {cuuint64_t(dim), cuuint64_t(p.q_heads), cuuint64_t(p.tokens)};
   const cuuint64_t strides[2] = {cuuint64_t(p.q_heads > 1 ? p.q_head : dim) * 2,
                                  cuuint64_t(p.tokens > 1 ? p.q_token : p.q_heads * dim) * 2};
   const cuuint32_t sizes[3] = {64, cuuint32_t(p.group), cuuint32_t(p.half_tokens)}, ones[3] = {1, 1, 1};
-  if (encode(&map_q, type, 3, const_cast<uint16_t*>(p.q), dims, strides, sizes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS ||
+  return encode && encode(map, type, 3, const_cast<uint16_t*>(p.q), dims, strides, sizes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace
+
+template <typename T>
+int paged_chunk(const PagedParams& p, int64_t dim, const void* k_cache, const void* v_cache, int grid, cudaStream_t stream) {
+  CUtensorMap map_q, map_k, map_v;
+  const uint64_t rows = uint64_t(p.pages) * uint64_t(p.k_heads) << p.page_shift;
+  constexpr auto type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const uint32_t box = uint32_t(std::min(1 << p.page_shift, STEP));
+  if (!map_queries<T>(&map_q, p, dim) ||
       !make_tensor_map_2d(&map_k, type, k_cache, rows, uint64_t(dim), uint64_t(dim) * 2, box, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
       !make_tensor_map_2d(&map_v, type, v_cache, rows, uint64_t(dim), uint64_t(dim) * 2, box, 64, CU_TENSOR_MAP_SWIZZLE_128B))
     return INTENT_B200_ERR_CUDA;
-  return dim == 128 ? launch<T, 128>(map_q, map_k, map_v, p, grid, stream) : launch<T, 64>(map_q, map_k, map_v, p, grid, stream);
+  const Int4Cache none = {};
+  return dim == 128 ? launch<T, 128, 0>(map_q, map_k, map_v, none, p, grid, stream)
+                    : launch<T, 64, 0>(map_q, map_k, map_v, none, p, grid, stream);
 }
 template int paged_chunk<__half>(const PagedParams&, int64_t, const void*, const void*, int, cudaStream_t);
 template int paged_chunk<__nv_bfloat16>(const PagedParams&, int64_t, const void*, const void*, int, cudaStream_t);
+
+template <typename T>
+int paged_chunk_int4(const PagedParams& p, int64_t dim, const Int4Cache& cache, int grid, cudaStream_t stream) {
+  CUtensorMap map;
+  if (!map_queries<T>(&map, p, dim)) return INTENT_B200_ERR_CUDA;
+  if (dim == 64)
+    return cache.group == 32 ? launch<T, 64, 32>(map, map, map, cache, p, grid, stream)
+                             : launch<T, 64, 64>(map, map, map, cache, p, grid, stream);
+  return cache.group == 32   ? launch<T, 128, 32>(map, map, map, cache, p, grid, stream)
+         : cache.group == 64 ? launch<T, 128, 64>(map, map, map, cache, p, grid, stream)
+                             : launch<T, 128, 128>(map, map, map, cache, p, grid, stream);
+}
+template int paged_chunk_int4<__half>(const PagedParams&, int64_t, const Int4Cache&, int, cudaStream_t);
+template int paged_chunk_int4<__nv_bfloat16>(const PagedParams&, int64_t, const Int4Cache&, int, cudaStream_t);
 
 }  // namespace ib200

@@ -59,13 +59,6 @@ constexpr int smem_bytes() {
   return smem_bytes_with<D, GROUP, NT>(joins<D, GROUP, NT>());
 }
 
-// bytes, a multiple of 16 at 16-byte boundaries, to shared memory
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
-}
-
 template <int N>
 struct Words {
   uint32_t w[N];
