@@ -87,3 +87,40 @@ def test_entry_of_attention():
     assert attend(parts=[*cache()[:3], view([4, 2, 16, 4], 0x10004)]) == LAYOUT
     assert attend(parts=[*cache()[:3], view([4, 2, 16, 4], 0)]) == attend(q=view([3, 4, 128], 0)) == NULL
     assert ctypes.sizeof(ctypes.c_void_p) == 8
+
+
+def test_pages_in_4_bits():
+    from intent_b200.attention import PagedKVCache, QuantisedPages, W4A16Attention
+
+    sizes = {"layers": 2, "pages": 8, "kv_heads": 2, "head_dim": 128, "page_size": 16, "device": "cpu"}
+    store = PagedKVCache(bits=4, group_size=32, **sizes)
+    for part in store.layer(1):
+        assert isinstance(part, QuantisedPages)
+        assert part.codes.shape == (8, 2, 16, 64) and part.scales.shape == (8, 2, 16, 8)
+    step = store.step({"a": 20, "b": 3})
+    assert step.kv_lengths.tolist() == [20, 3] and store.free_pages == 5
+    for name, start, stop, error in (("c", 0, None, KeyError), ("a", 0, 21, ValueError), ("a", 5, 4, ValueError), ("a", -1, 4, ValueError)):
+        with pytest.raises(error):
+            store.read(0, name, start, stop)
+    for wrong in ({"bits": 8}, {"bits": 4, "group_size": 16}, {"bits": 4, "group_size": 256}):
+        with pytest.raises(ValueError):
+            PagedKVCache(**{**sizes, **wrong})
+    with pytest.raises(ValueError):
+        PagedKVCache(**{**sizes, "head_dim": 64}, bits=4, group_size=128)
+    with pytest.raises(ValueError):
+        W4A16Attention(hidden=256, heads=4, kv_heads=2, head_dim=64, cache_bits=8)
+
+
+def test_reading_pages_of_16_bits():
+    import torch
+
+    from intent_b200.attention import PagedKVCache
+
+    store = PagedKVCache(layers=2, pages=8, kv_heads=2, head_dim=64, page_size=16, device="cpu")
+    store.k.copy_(torch.randn(store.k.shape)), store.v.copy_(torch.randn(store.v.shape))
+    store.step({"x": 20})
+    step = store.step({"a": 40})
+    for got, whole in zip(store.read(1, "a", 3, 39), (store.k[1], store.v[1])):
+        flat = whole.transpose(1, 2).flatten(0, 1)
+        assert torch.equal(got, flat[step.slots[3:39]])
+    assert store.read(0, "a", 40)[0].shape == (0, 2, 64)
