@@ -1,0 +1,321 @@
+// Append of keys and values to a paged cache in 4 bits, with the norms and the rotation of queries and keys (paged_kv_append_int4).
+//
+// Queries are those of paged_kv_append (rotate.cuh).  A group of GROUP consecutive elements x of a head's key, after its norm and
+// rotation and not rounded before, or of its value, is held as
+//   m = min x,   s = (max x - min x) / 15, both rounded to the 16-bit type,   n = nearest((x - m) / s), the even one of two, in 0 .. 15
+// (s the next lower number where m + 15 s would be beyond the type; a group with something that is no finite number is NaN).
+//
+// A code is off by one as soon as a number next to a half is off by a little, and then by a whole step.  So keys are worked out in 64
+// bits: in f32 three of a million codes were others, now they are those of the definition.  Values have no arithmetic before
+// and 16 bits, and f32 holds their differences; quotients are rounded as a division rounds them, so that halves, common among
+// 16-bit numbers, are halves.
+//
+// A lane has eight neighbouring elements of a row.  The partners of a key's elements in pairs (i, i + R/2) are another lane's; it reads
+// them once more from the first-level cache and works out its own half of each pair.  Blocks have keys, values or queries; in
+// calls of many rows four rows of a token share what does not depend on the row.
+#include "common.cuh"
+#include "paged.cuh"
+#include "rotate.cuh"
+
+namespace ib200 {
+namespace {
+
+constexpr int THREADS = ROTATE_THREADS;
+
+template <typename F>
+__device__ __forceinline__ F least_of(F a, F b) {
+  return a < b ? a : b;
+}
+template <typename F>
+__device__ __forceinline__ F largest_of(F a, F b) {
+  return a > b ? a : b;
+}
+
+// The quotients of eight numbers by a scale s, rounded to whole numbers from 0 to 15.  The product with the rounded reciprocal gets its
+// remainder added, which makes it the quotient as a division rounds it (P. Markstein, Computation of elementary functions on the
+// IBM RISC System/6000 processor, 1990).  Added to 1.5 times 2 to the mantissa's length a number is rounded in the lowest bits.
+template <typename T>
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float s, float m) {
+  // (powers of two that keep the reciprocal a normal number)
+  const float by = std::is_same<T, __half>::value ? 1.f : s < 0x1p-60f ? 0x1p64f : s > 0x1p60f ? 0x1p-64f : 1.f;
+  const float divisor = s * by, inverse = s > 0.f ? __frcp_rn(divisor) : 0.f, origin = -m * by;
+  uint32_t codes = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float d = fmaf(x[e], by, origin), q = d * inverse;
+    const float n = fminf(fmaxf(fmaf(fmaf(-q, divisor, d), inverse, q), 0.f), 15.f);
+    codes += (__float_as_uint(n + 12582912.f) - 0x4b400000u) << (4 * e);
+  }
+  return codes;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t codes_of(const double (&x)[8], float scale, float minimum) {
+  const double s = scale, m = minimum, inverse = scale > 0.f ? __drcp_rn(s) : 0.;
+  uint32_t codes = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const double d = x[e] - m, q = d * inverse;
+    const int n = __double2loint(fma(fma(-q, s, d), inverse, q) + 6755399441055744.);
+    codes |= uint32_t(min(max(n, 0), 15)) << (4 * e);
+  }
+  return codes;
+}
+
+// Eight neighbouring elements of a row as codes; `scales`: scale | minimum of their group, which all of its lanes know
+template <typename T, int GROUP, typename F>
+__device__ __forceinline__ uint32_t quantise(const F (&x)[8], uint32_t& scales) {
+  const float infinity = __int_as_float(0x7f800000);
+  F low = x[0], high = x[0];
+  bool finite = true;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    low = least_of(x[e], low), high = largest_of(x[e], high);
+    finite &= fabsf(float(x[e])) < infinity;
+  }
+#pragma unroll
+  for (int d = 1; d < GROUP / 8; d *= 2) {
+    low = least_of(__shfl_xor_sync(0xffffffffu, low, d), low);
+    high = largest_of(__shfl_xor_sync(0xffffffffu, high, d), high);
+  }
+  constexpr uint32_t LANES = (1u << (GROUP / 8)) - 1;
+  const uint32_t odd = __ballot_sync(0xffffffffu, !finite) >> (threadIdx.x & 31 & ~(GROUP / 8 - 1));
+  // (in 64 bits, in which the scale's rounding is that of the exact quotient)
+  scales = Elem<T>::pack2(float((double(high) - double(low)) * (1. / 15.)), float(low));
+  const float m = Elem<T>::to_float(uint16_t(scales >> 16));
+  float s = Elem<T>::to_float(uint16_t(scales));
+  if ((odd & LANES) || !(s < infinity) || !(fabsf(m) < infinity)) {
+    scales = 0x7fff7fffu;
+    return 0;
+  }
+  if (!(Elem<T>::to_float(Elem<T>::from_float(fmaf(15.f, s, m))) < infinity)) s = Elem<T>::to_float(uint16_t(--scales));
+  return codes_of<T>(x, s, m);
+}
+
+// A group of lanes and its rows of one kind of one token
+template <int D, int ROWS>
+struct Group {
+  uint32_t token, first;               // its first head
+  int rows;                            // 0: there is none
+  int64_t place;                       // of the first row in the cache, in rows
+  bool kept;
+  __device__ __forceinline__ Group(const RotateParams& p, uint32_t block) {
+    const uint32_t groups = (p.k_heads + ROWS - 1) / ROWS, at = block * uint32_t(THREADS / (D / 8)) + threadIdx.x / (D / 8);
+    const bool live = at < p.tokens * groups;
+    token = live ? at / groups : 0;
+    first = (at - token * groups) * ROWS;
+    rows = live ? int(min(p.k_heads - first, uint32_t(ROWS))) : 0;
+  }
+  __device__ __forceinline__ void find(const RotateParams& p) {
+    const int64_t slot = __ldg(p.slots + token);
+    kept = rows > 0 && slot >= 0 && slot < p.slot_count;
+    place = kept ? (((slot >> p.page_shift) * p.k_heads + first) << p.page_shift) + (slot & ((int64_t(1) << p.page_shift) - 1)) : 0;
+  }
+  template <int GROUP>
+  __device__ __forceinline__ void store(const RotateParams& p, int i, int j, uint32_t* codes_to, uint32_t* scales_to, uint32_t codes,
+                                        uint32_t scales) const {
+    if (!kept || i >= rows) return;
+    const int64_t row = place + (int64_t(i) << p.page_shift);
+    codes_to[row * (D / 8) + j] = codes;
+    if (j % (GROUP / 8) == 0) scales_to[row * (D / GROUP) + j / (GROUP / 8)] = scales;
+  }
+};
+
+template <typename T, int D, int ROWS, int GROUP>
+__device__ __forceinline__ void value_rows(const RotateParams& p, uint32_t block) {
+  const int j = threadIdx.x % (D / 8);
+  Group<D, ROWS> group(p, block);
+  const uint16_t* from = p.v + group.token * p.v_token + group.first * p.v_head + 8 * j;
+  programmatic_wait();
+  uint4 raw[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) raw[i] = i < group.rows ? ldg_stream_v4(from + i * p.v_head) : make_uint4(0, 0, 0, 0);
+  group.find(p);
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = Elem<T>::to_float(uint16_t(w[e / 2] >> (16 * (e & 1))));
+    uint32_t scales;
+    const uint32_t codes = quantise<T, GROUP>(x, scales);
+    group.template store<GROUP>(p, i, j, p.v_codes, p.v_scales, codes, scales);
+  }
+}
+
+template <typename T, int D, bool NORM, bool NEIGHBOURS, int ROWS, int GROUP>
+__device__ __forceinline__ void key_rows(const RotateParams& p, uint32_t block) {
+  constexpr int LANES = D / 8;
+  const int j = threadIdx.x % LANES, half = p.rotary_dim / 2;
+  const bool turned = 8 * j < p.rotary_dim, upper = 8 * j >= half;
+  const int mate = NEIGHBOURS || !turned ? 8 * j : upper ? 8 * j - half : 8 * j + half;    // first of the partners
+  Group<D, ROWS> group(p, block);
+  const uint16_t* from = p.k + group.token * p.k_token + group.first * p.k_head;
+  programmatic_wait();
+  uint4 raw[ROWS], partners[NEIGHBOURS ? 1 : ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const bool there = i < group.rows;
+    raw[i] = there ? __ldg(reinterpret_cast<const uint4*>(from + i * p.k_head + 8 * j)) : make_uint4(0, 0, 0, 0);
+    if (!NEIGHBOURS)
+      partners[i] = there && turned ? __ldg(reinterpret_cast<const uint4*>(from + i * p.k_head + mate)) : make_uint4(0, 0, 0, 0);
+  }
+  const int64_t position = __ldg(p.positions + group.token);
+  const bool known = position >= 0 && position < p.table_rows;
+  group.find(p);
+
+  // What an element is multiplied with, and what its partner is for it: weight times cosine, weight times (minus) sine.
+  double own[8], cross[8];
+  {
+    constexpr int ANGLES = NEIGHBOURS ? 4 : 8;
+    float c[ANGLES], s[ANGLES];
+#pragma unroll
+    for (int e = 0; e < ANGLES; ++e) c[e] = known ? 1.f : __int_as_float(0x7fc00000), s[e] = 0.f;
+    if (known && turned) {
+      const float* angles = p.rotary + position * p.rotary_dim + (NEIGHBOURS ? 4 * j : upper ? 8 * j - half : 8 * j);
+#pragma unroll
+      for (int e = 0; e < ANGLES; e += 4) {
+        const float4 cosine = __ldg(reinterpret_cast<const float4*>(angles + e));
+        const float4 sine = __ldg(reinterpret_cast<const float4*>(angles + half + e));
+        c[e] = cosine.x, c[e + 1] = cosine.y, c[e + 2] = cosine.z, c[e + 3] = cosine.w;
+        s[e] = sine.x, s[e + 1] = sine.y, s[e + 2] = sine.z, s[e + 3] = sine.w;
+      }
+    }
+    uint4 weight = make_uint4(0, 0, 0, 0), partner_weight = weight;
+    if (NORM) {
+      weight = __ldg(reinterpret_cast<const uint4*>(p.k_weight + 8 * j));
+      if (!NEIGHBOURS) partner_weight = __ldg(reinterpret_cast<const uint4*>(p.k_weight + mate));
+    }
+    const uint32_t w[4] = {weight.x, weight.y, weight.z, weight.w};
+    const uint32_t v[4] = {partner_weight.x, partner_weight.y, partner_weight.z, partner_weight.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int pair = NEIGHBOURS ? e / 2 : e;
+      const double cosine = c[pair], sine = (NEIGHBOURS ? e & 1 : upper) ? s[pair] : -s[pair];
+      own[e] = NORM ? cosine * double(Elem<T>::to_float(uint16_t(w[e / 2] >> (16 * (e & 1))))) : cosine;
+      const uint32_t of_partner = NEIGHBOURS ? w[e / 2] >> (16 * (1 - (e & 1))) : v[e / 2] >> (16 * (e & 1));
+      cross[e] = NORM ? sine * double(Elem<T>::to_float(uint16_t(of_partner))) : sine;
+    }
+  }
+
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+    double x[8], y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = Elem<T>::to_float(uint16_t(w[e / 2] >> (16 * (e & 1))));
+    double scale = 1.;
+    if (NORM) {
+      double sum = x[0] * x[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) sum = fma(x[e], x[e], sum);
+#pragma unroll
+      for (int d = LANES / 2; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      scale = rsqrt(sum * (1. / D) + double(p.eps));
+    }
+    if (NEIGHBOURS) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = turned ? fma(x[e], own[e], x[e ^ 1] * cross[e]) : x[e] * own[e];
+    } else {
+      const uint32_t v[4] = {partners[i].x, partners[i].y, partners[i].z, partners[i].w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        y[e] = fma(x[e], own[e], double(Elem<T>::to_float(uint16_t(v[e / 2] >> (16 * (e & 1))))) * cross[e]);
+    }
+    if (NORM)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] *= scale;
+    uint32_t scales;
+    const uint32_t codes = quantise<T, GROUP>(y, scales);
+    group.template store<GROUP>(p, i, j, p.k_codes, p.k_scales, codes, scales);
+  }
+}
+
+// k_blocks blocks of keys, as many of values, the others of queries (p.k_heads is 0 in `queries`)
+template <typename T, int D, bool NORM, bool NEIGHBOURS, int ROWS, int GROUP>
+__global__ void __launch_bounds__(THREADS) append_int4_kernel(const RotateParams p, const RotateParams queries, uint32_t k_blocks) {
+  programmatic_begin();
+  const uint32_t block = blockIdx.x;
+  if (block < k_blocks) key_rows<T, D, NORM, NEIGHBOURS, ROWS, GROUP>(p, block);
+  else if (block < 2 * k_blocks) value_rows<T, D, ROWS, GROUP>(p, block - k_blocks);
+  else rotate_rows<T, D, NORM, NEIGHBOURS, false, ROWS>(queries, block - 2 * k_blocks);
+}
+
+template <typename T, int D, bool NORM, int ROWS, int GROUP>
+int launch(const RotateParams& p, bool neighbours, cudaStream_t stream) {
+  auto kernel = neighbours ? append_int4_kernel<T, D, NORM, true, ROWS, GROUP> : append_int4_kernel<T, D, NORM, false, ROWS, GROUP>;
+  constexpr uint32_t PER_CTA = THREADS / (D / 8);
+  static_assert(D / 8 == D / (2 * PIECE_OF), "lanes of a row of queries");
+  const uint32_t k_blocks = (p.tokens * ((p.k_heads + ROWS - 1) / ROWS) + PER_CTA - 1) / PER_CTA;
+  const uint32_t q_blocks = (p.tokens * ((p.q_heads + ROWS - 1) / ROWS) + PER_CTA - 1) / PER_CTA, grid = 2 * k_blocks + q_blocks;
+  RotateParams queries = p;
+  queries.k_heads = 0;
+  if (LaunchFacts* sink = observe_sink())
+    return record_launch(sink, reinterpret_cast<const void*>(kernel),
+                         ROWS == 1 ? "append_int4_kernel a row per group" : "append_int4_kernel several rows per group", int(grid), THREADS,
+                         0, 1);
+  const cudaError_t e = launch_programmatic(kernel, dim3(grid), dim3(THREADS), 0, stream, 1, p, queries, k_blocks);
+  if (e != cudaSuccess) return cuda_status(e);
+  note_launch();
+  return launch_status();
+}
+
+template <typename T, int D, int GROUP>
+int choose(const RotateParams& p, bool neighbours, cudaStream_t stream) {
+  const bool many = p.tokens * (p.q_heads + 2 * p.k_heads) >= MANY;
+  if (p.q_weight) return many ? launch<T, D, true, SHARED_ROWS, GROUP>(p, neighbours, stream)
+                              : launch<T, D, true, 1, GROUP>(p, neighbours, stream);
+  return many ? launch<T, D, false, SHARED_ROWS, GROUP>(p, neighbours, stream) : launch<T, D, false, 1, GROUP>(p, neighbours, stream);
+}
+
+template <typename T>
+int append(const View3& q, const View3& k, const View3& v, const View1& positions, const View1& slots, const View2& rotary,
+           const View1* q_weight, const View1* k_weight, const View4& k_codes, const View4& k_scales, const View4& v_codes,
+           const View4& v_scales, const View3& q_out, int32_t group, int32_t eps_bits, int32_t pairs, cudaStream_t stream) {
+  RotateParams p = {};
+  int status = rotate_prepare(p, q, k, positions, rotary, q_out, q_weight, k_weight, eps_bits, pairs);
+  if (status != INTENT_B200_OK) return status;
+  if (v.d0 != k.d0 || v.d1 != k.d1 || v.d2 != k.d2 || slots.d0 != q.d0) return INTENT_B200_ERR_SHAPE;
+  status = check_int4(k_codes, k_scales, v_codes, v_scales, k.d1, k.d2, group);
+  if (status != INTENT_B200_OK) return status;
+  if (!rows16(v) || !contiguous(slots) || !aligned16(v.p)) return INTENT_B200_ERR_LAYOUT;
+  if ((status = rotate_set_rows(p, q.d0, q.d1 + 2 * k.d1)) != INTENT_B200_OK) return status;
+  if (p.tokens == 0) return INTENT_B200_OK;
+  if (!v.p || !slots.p || (k_codes.d0 > 0 && (!k_codes.p || !v_codes.p || !k_scales.p || !v_scales.p))) return INTENT_B200_ERR_NULL;
+  p.v = static_cast<const uint16_t*>(v.p);
+  p.v_token = v.s0, p.v_head = v.s1;
+  p.slots = static_cast<const int64_t*>(slots.p);
+  p.k_codes = static_cast<uint32_t*>(k_codes.p), p.v_codes = static_cast<uint32_t*>(v_codes.p);
+  p.k_scales = static_cast<uint32_t*>(k_scales.p), p.v_scales = static_cast<uint32_t*>(v_scales.p);
+  p.slot_count = k_codes.d0 * k_codes.d2;
+  while ((int64_t(1) << p.page_shift) < k_codes.d2) ++p.page_shift;
+  if (q.d2 == 64) return group == 32 ? choose<T, 64, 32>(p, pairs, stream) : choose<T, 64, 64>(p, pairs, stream);
+  return group == 32   ? choose<T, 128, 32>(p, pairs, stream)
+         : group == 64 ? choose<T, 128, 64>(p, pairs, stream) : choose<T, 128, 128>(p, pairs, stream);
+}
+
+}  // namespace
+}  // namespace ib200
+
+#define IB200_APPEND_INT4_ENTRIES(NAME, TYPE)                                                                              \
+  extern "C" int intent_b200_paged_kv_append_int4_##NAME(                                                                  \
+      INTENT_B200_VIEW3(a0), INTENT_B200_VIEW3(a1), INTENT_B200_VIEW3(a2), INTENT_B200_VIEW1(a3), INTENT_B200_VIEW1(a4),   \
+      INTENT_B200_VIEW2(a5), INTENT_B200_VIEW4(a6), INTENT_B200_VIEW4(a7), INTENT_B200_VIEW4(a8), INTENT_B200_VIEW4(a9),   \
+      INTENT_B200_VIEW3(a10), int32_t group, int32_t pairs, void* stream) {                                                \
+    return ib200::append<TYPE>(IB200_VIEW3_ARG(a0), IB200_VIEW3_ARG(a1), IB200_VIEW3_ARG(a2), IB200_VIEW1_ARG(a3),         \
+                               IB200_VIEW1_ARG(a4), IB200_VIEW2_ARG(a5), nullptr, nullptr, IB200_VIEW4_ARG(a6),            \
+                               IB200_VIEW4_ARG(a7), IB200_VIEW4_ARG(a8), IB200_VIEW4_ARG(a9), IB200_VIEW3_ARG(a10),        \
+                               group, 0, pairs, static_cast<cudaStream_t>(stream));                                        \
+  }                                                                                                                        \
+  extern "C" int intent_b200_paged_kv_append_norm_int4_##NAME(                                                             \
+      INTENT_B200_VIEW3(a0), INTENT_B200_VIEW3(a1), INTENT_B200_VIEW3(a2), INTENT_B200_VIEW1(a3), INTENT_B200_VIEW1(a4),   \
+      INTENT_B200_VIEW2(a5), INTENT_B200_VIEW1(a6), INTENT_B200_VIEW1(a7), INTENT_B200_VIEW4(a8), INTENT_B200_VIEW4(a9),   \
+      INTENT_B200_VIEW4(a10), INTENT_B200_VIEW4(a11), INTENT_B200_VIEW3(a12), int32_t group, int32_t eps_bits,             \
+      int32_t pairs, void* stream) {                                                                                       \
+    const ib200::View1 qw = IB200_VIEW1_ARG(a6), kw = IB200_VIEW1_ARG(a7);                                                 \
+    return ib200::append<TYPE>(IB200_VIEW3_ARG(a0), IB200_VIEW3_ARG(a1), IB200_VIEW3_ARG(a2), IB200_VIEW1_ARG(a3),         \
+                               IB200_VIEW1_ARG(a4), IB200_VIEW2_ARG(a5), &qw, &kw, IB200_VIEW4_ARG(a8),                    \
+                               IB200_VIEW4_ARG(a9), IB200_VIEW4_ARG(a10), IB200_VIEW4_ARG(a11), IB200_VIEW3_ARG(a12),      \
+                               group, eps_bits, pairs, static_cast<cudaStream_t>(stream));                                 \
+  }
+IB200_APPEND_INT4_ENTRIES(f16, __half)
+IB200_APPEND_INT4_ENTRIES(bf16, __nv_bfloat16)
