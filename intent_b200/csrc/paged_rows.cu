@@ -83,8 +83,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   float* join = reinterpret_cast<float*>(base_ptr + R::BYTES);          // [JOINS][WARPS][ROWS][PITCH]
   float* join_max = join + JOINS * WARPS * ROWS * PITCH;                // [JOINS][WARPS][ROWS]
   float* join_sum = join_max + JOINS * WARPS * ROWS;
-  int* shared = reinterpret_cast<int*>(join_sum + JOINS * WARPS * ROWS);   // a number, a 64-bit one, the warps' 64-bit sums
-  long long* warp_sums = reinterpret_cast<long long*>(shared + 4);
+  long long* starts = reinterpret_cast<long long*>(join_sum + JOINS * WARPS * ROWS);   // two numbers, the warps' sums
+  long long* warp_sums = starts + 2;
   const uint32_t bars = smem_u32(warp_sums + WARPS);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t ring = base + warp * R::STAGES * R::SLOT, full = bars + warp * R::STAGES * 8;
@@ -96,7 +96,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 
   // ---- this CTA's part of the line
   RowsJoin* entry = static_cast<RowsJoin*>(p.joins) + blockIdx.x;
-  const Place<STEP, BEGIN> start = place_of<STEP, BEGIN, THREADS>(p, ROWS, shared, warp_sums, entry);
+  const Place<STEP, BEGIN> start = place_of<STEP, BEGIN, THREADS, 1>(p, ROWS, starts, warp_sums, entry);
   if (start.first >= start.end) return;
   const int first_place = start.first, end = start.end;
   Walk<STEP, BEGIN> load = start.at, work = load;

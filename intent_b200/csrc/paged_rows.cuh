@@ -65,19 +65,29 @@ struct Walk {
   }
 };
 
-// The part of the line that a CTA takes
+// The part of the line that a CTA, or one of its warps, takes
 template <int STEP, int BEGIN>
 struct Place {
   Walk<STEP, BEGIN> at;    // its first step
-  int first, end;          // its place and where the CTA's places end, counted from the CTA's first one (first >= end: none)
-  int share;               // places of every CTA
+  int first, end;          // its place and where the part's places end, counted from the part's first one (first >= end: none)
+  int share;               // places of every part
 };
 
-// To be called by all threads of a CTA; `shared` has room for a number and a 64-bit one behind it, `warp_sums` for one a warp.
-template <int STEP, int BEGIN, int THREADS>
-__device__ __forceinline__ Place<STEP, BEGIN> place_of(const PagedParams& p, int tile_rows, int* shared, long long* warp_sums,
+// The parts of a line of so many places that WORKERS of every CTA take, one behind the other; negative as in share_of
+template <int WORKERS>
+__device__ __forceinline__ int share_of_workers(long long line) {
+  if (WORKERS == 1) return share_of(line);
+  constexpr int MOST = 0x3fffffff / WORKERS;             // (a CTA's places are counted in 32 bits)
+  const long long workers = (long long)gridDim.x * WORKERS, share = (line + workers - 1) / workers;
+  return share <= MOST ? int(share) : -1;
+}
+
+// To be called by all threads of a CTA.  `starts` has room for two 64-bit numbers of every worker (the CTA, or each of its warps),
+// `warp_sums` for one a warp.
+template <int STEP, int BEGIN, int THREADS, int WORKERS>
+__device__ __forceinline__ Place<STEP, BEGIN> place_of(const PagedParams& p, int tile_rows, long long* starts, long long* warp_sums,
                                                        RowsJoin* entry) {
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, worker = WORKERS == 1 ? 0 : warp;
   Place<STEP, BEGIN> place;
   place.first = place.end = 0;
   const int per_thread = (p.batch + THREADS - 1) / THREADS, mine = tid * per_thread;
@@ -101,31 +111,37 @@ __device__ __forceinline__ Place<STEP, BEGIN> place_of(const PagedParams& p, int
     line += warp_sums[w];
   }
   before -= sum;
-  place.share = share_of(line);
+  place.share = share_of_workers<WORKERS>(line);
   if (tid == 0) {
     entry->last_cta = -1;
     if (place.share < 0) atomicExch(p.status, INTENT_B200_ERR_SHAPE);
   }
-  const long long begin = (long long)blockIdx.x * place.share;
-  if (place.share <= 0 || begin >= line) return place;
-  place.end = int(min((long long)place.share, line - begin));
-  if (begin >= before && begin < before + sum) {
-    int b = mine;
-    long long at = before;
-    for (;; ++b) {
-      const Sequence s = sequence_of<STEP>(p, b, tile_rows);
-      const long long places = places_of<BEGIN>(p, s);
-      if (begin < at + places || b + 1 >= min(mine + per_thread, p.batch)) break;
-      at += places;
+  const long long first_of_cta = (long long)blockIdx.x * WORKERS * place.share;
+  if (place.share <= 0 || first_of_cta >= line) return place;
+#pragma unroll 1
+  for (int i = 0; i < WORKERS; ++i) {
+    const long long begin = first_of_cta + (long long)i * place.share;
+    if (begin >= before && begin < before + sum) {
+      int b = mine;
+      long long at = before;
+      for (; per_thread > 1; ++b) {
+        const Sequence s = sequence_of<STEP>(p, b, tile_rows);
+        const long long places = places_of<BEGIN>(p, s);
+        if (begin < at + places || b + 1 >= min(mine + per_thread, p.batch)) break;
+        at += places;
+      }
+      starts[2 * i] = b;
+      starts[2 * i + 1] = begin - at;                    // place in the sequence
     }
-    shared[0] = b;
-    *reinterpret_cast<long long*>(shared + 2) = begin - at;            // place in the sequence
   }
   __syncthreads();
+  const long long begin = first_of_cta + (long long)worker * place.share;
+  if (begin >= line) return place;
+  place.end = int(min((long long)place.share, line - begin));
   Walk<STEP, BEGIN>& first = place.at;
-  first.b = shared[0];
+  first.b = int(starts[2 * worker]);
   first.s = sequence_of<STEP>(p, first.b, tile_rows);
-  const long long of_sequence = *reinterpret_cast<const long long*>(shared + 2);
+  const long long of_sequence = starts[2 * worker + 1];
   const int item = divide(of_sequence, first.s.steps + BEGIN);
   first.step = int(of_sequence - (long long)item * (first.s.steps + BEGIN)) - BEGIN;
   first.head = item / first.s.tiles;

@@ -14,7 +14,11 @@
 // rounded numbers are added up for the middle of the codes (8), which is taken off again: the rounding is worth what it is for a
 // product with v_j.  For f16 results the product is made with what the rounding left over, too.
 //
-// A CTA's line of steps, its shares, and the parts of tiles that are cut are those of paged_rows.cu; a step is 64 tokens for each warp.
+// With a quarter of the bytes of 16-bit elements there is a quarter of the time, and what all warps of a CTA have to wait for costs
+// four times as much.  So the line of steps (as in paged_rows.cu, but of UNIT tokens each) is cut into a share for every warp,
+// which goes through its tiles on its own, with a ring of its own, and writes the results of those that it has whole.  Tiles that are
+// cut leave at most two parts per warp in shared memory, which are put together once, at the end: the results, or one part of the
+// CTA for the join.
 #include <cstring>
 
 #include "common.cuh"
@@ -26,37 +30,35 @@
 namespace ib200 {
 namespace {
 
-constexpr int UNIT = 64;                 // tokens of a ring slot
-constexpr int PARTS = UNIT / 16;         // pieces of it that lie in one page in any case
-
-template <int D, int GROUP>
+template <int D, int GROUP, int NT>
 struct Ring {
+  static constexpr int UNIT = 64;                         // tokens of a ring slot, a step
+  static constexpr int PARTS = UNIT / 16;                 // pieces of it that lie in one page in any case
   static constexpr int WARPS = 8;
-  static constexpr int STAGES = D == 128 ? 2 : 3;
-  static constexpr int STEP = UNIT * WARPS;               // tokens of a CTA's step
+  static constexpr int STAGES = 2;
   static constexpr int GROUPS = D / GROUP;
   static constexpr int ROW = D / 2;                       // bytes of a token's codes
   static constexpr int CODES = UNIT * ROW, SCALES = UNIT * GROUPS * 4;   // of keys or values of a unit
   static constexpr int SLOT = 2 * CODES, SCALE_SLOT = 2 * SCALES;
-  static constexpr int BYTES = WARPS * STAGES * (SLOT + SCALE_SLOT);
+  static constexpr int OF_WARP = STAGES * SLOT, BYTES = WARPS * STAGES * (SLOT + SCALE_SLOT);
   static constexpr int BEGIN = 1;                         // places on the line ahead of the steps of a tile
+  static constexpr int PIECE = 8 * NT * (D + 2) * 4;      // a part of a tile: results, maxima, sums
+  static_assert(PIECE <= OF_WARP, "a warp's last part lies in its ring");
 };
 
-constexpr int SMEM_MOST = 227 * 1024;
-template <int D, int GROUP, int NT>
-constexpr int smem_bytes_with(int joins) {
-  using R = Ring<D, GROUP>;
-  return 1024 + R::BYTES + joins * R::WARPS * 8 * NT * (D * 4 + 8) + R::WARPS * R::STAGES * 8 + 16 + 8 * R::WARPS;
-}
-// Places for the warps' parts of a tile: two where there is room
-template <int D, int GROUP, int NT>
-constexpr int joins() {
-  return smem_bytes_with<D, GROUP, NT>(2) <= SMEM_MOST ? 2 : 1;
-}
+// What a warp leaves of a tile that it does not have whole
+struct Left {
+  int there;
+  int begin, end;          // the tile's places, counted from the CTA's first one
+  int row, head, tile_row, rows, sequence;      // as in RowsJoin
+};
+
 template <int D, int GROUP, int NT>
 constexpr int smem_bytes() {
-  static_assert(smem_bytes_with<D, GROUP, NT>(joins<D, GROUP, NT>()) <= SMEM_MOST, "shared memory of a CTA");
-  return smem_bytes_with<D, GROUP, NT>(joins<D, GROUP, NT>());
+  using R = Ring<D, GROUP, NT>;
+  constexpr int bytes = 1024 + R::BYTES + R::WARPS * (R::PIECE + 2 * int(sizeof(Left)) + R::STAGES * 8 + 8 + 16);
+  static_assert(bytes <= 227 * 1024, "shared memory of a CTA");
+  return bytes;
 }
 
 template <int N>
@@ -96,11 +98,11 @@ struct Codes<__half> {
 };
 
 template <typename T, int D, int GROUP, int NT>
-__global__ void __launch_bounds__(32 * Ring<D, GROUP>::WARPS, 1)
+__global__ void __launch_bounds__(32 * Ring<D, GROUP, NT>::WARPS, 1)
 paged_rows_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const uint32_t* k_scales,
                        const uint32_t* v_scales, const PagedParams p) {
-  using R = Ring<D, GROUP>;
-  constexpr int ROWS = 8 * NT, WARPS = R::WARPS, THREADS = 32 * WARPS, STEP = R::STEP, BEGIN = R::BEGIN, GROUPS = R::GROUPS;
+  using R = Ring<D, GROUP, NT>;
+  constexpr int ROWS = 8 * NT, WARPS = R::WARPS, THREADS = 32 * WARPS, UNIT = R::UNIT, PARTS = R::PARTS, STEP = UNIT, BEGIN = R::BEGIN, GROUPS = R::GROUPS;
   constexpr int CHUNKS = D / 32, OF_GROUP = CHUNKS / GROUPS;            // 16 bytes of a token's codes
   constexpr bool SPLIT = std::is_same<T, __half>::value;                // weights in two bf16 parts
   extern __shared__ unsigned char smem_raw[];
@@ -111,28 +113,30 @@ paged_rows_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   }
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* base_ptr = smem_raw + (base - smem_u32(smem_raw));
-  constexpr int JOINS = joins<D, GROUP, NT>();
-  float* join = reinterpret_cast<float*>(base_ptr + R::BYTES);          // [JOINS][WARPS][ROWS][D]
-  float* join_max = join + JOINS * WARPS * ROWS * D;                    // [JOINS][WARPS][ROWS]
-  float* join_sum = join_max + JOINS * WARPS * ROWS;
-  int* shared = reinterpret_cast<int*>(join_sum + JOINS * WARPS * ROWS);   // a number, a 64-bit one, the warps' 64-bit sums
-  long long* warp_sums = reinterpret_cast<long long*>(shared + 4);
+  // a warp's part of the tile that its share begins in; then of the tile that it ends in, in its ring
+  float* first_parts = reinterpret_cast<float*>(base_ptr + R::BYTES);
+  auto part_of = [&](int w, int which) {
+    return which == 0 ? first_parts + w * (R::PIECE / 4) : reinterpret_cast<float*>(base_ptr + w * R::OF_WARP);
+  };
+  Left* left = reinterpret_cast<Left*>(base_ptr + R::BYTES + WARPS * R::PIECE);          // [WARPS][2]
+  long long* starts = reinterpret_cast<long long*>(left + 2 * WARPS);                    // [WARPS][2]: sequence, place in it
+  long long* warp_sums = starts + 2 * WARPS;
   const uint32_t bars = smem_u32(warp_sums + WARPS);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t ring = base + warp * R::STAGES * R::SLOT, full = bars + warp * R::STAGES * 8;
-  const uint32_t scale_ring = base + WARPS * R::STAGES * R::SLOT + warp * R::STAGES * R::SCALE_SLOT;
+  const uint32_t ring = base + warp * R::OF_WARP, full = bars + warp * R::STAGES * 8;
+  const uint32_t scale_ring = base + WARPS * R::OF_WARP + warp * R::STAGES * R::SCALE_SLOT;
   if (lane == 0) {
     for (int s = 0; s < R::STAGES; ++s) mbar_init(full + 8 * s, 1);
     fence_mbar_init();
   }
   programmatic_wait();
 
-  // ---- this CTA's part of the line
+  // ---- this warp's part of the line
   RowsJoin* entry = static_cast<RowsJoin*>(p.joins) + blockIdx.x;
-  const Place<STEP, BEGIN> start = place_of<STEP, BEGIN, THREADS>(p, ROWS, shared, warp_sums, entry);
-  if (start.first >= start.end) return;
-  const int first_place = start.first, end = start.end;
+  const Place<STEP, BEGIN> start = place_of<STEP, BEGIN, THREADS, WARPS>(p, ROWS, starts, warp_sums, entry);
+  const int first_place = start.first, end = start.end, origin = warp * start.share;     // origin: the warp's first of the CTA's
   Walk<STEP, BEGIN> load = start.at, work = load;
+  if (lane < 2) left[2 * warp + lane].there = 0;
 
   const float infinity = __int_as_float(0x7f800000);
   int loading = first_place, slot_in = 0, slot_out = 0;
@@ -142,19 +146,19 @@ paged_rows_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   const int box = min(1 << p.page_shift, UNIT);          // tokens of a unit that lie in one page
   int page;                              // of piece lane % PARTS of the unit at `load`, asked for one unit ahead; -1: not needed
   auto look_up = [&] {
-    const int t = (load.s.begin + load.step) * STEP + warp * UNIT + (lane % PARTS) * 16;
+    const int t = (load.s.begin + load.step) * UNIT + (lane % PARTS) * 16;
     page = -1;
     if (t < load.s.length && t + 16 > load.s.low)
       page = __ldg(p.page_table + int64_t(load.b) * p.table_width + (t >> p.page_shift));
   };
   // asks for the unit of this warp at `load`, and goes on
   auto ask = [&] {
-    const int token = (load.s.begin + load.step) * STEP + warp * UNIT;
+    const int token = (load.s.begin + load.step) * UNIT;
     // (pieces of one page are one box, whichever of them is needed)
     int number = page >= 0 && page < p.pages ? page : -1;
     const uint32_t here = __ballot_sync(0xffffffffu, number >= 0) & ((1u << PARTS) - 1);
     number = box >= 32 ? max(number, __shfl_xor_sync(0xffffffffu, number, 1)) : number;
-    number = box >= 64 ? max(number, __shfl_xor_sync(0xffffffffu, number, 2)) : number;
+    number = UNIT >= 64 && box >= 64 ? max(number, __shfl_xor_sync(0xffffffffu, number, 2)) : number;
     // lane: piece lane % PARTS of keys' codes, values' codes, keys' scales, values' scales
     const int piece = lane % PARTS, what = lane / PARTS;
     const bool mine = number >= 0 && piece * 16 % box == 0;
@@ -239,16 +243,17 @@ paged_rows_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       }
     }
   };
-  look_up();
-  begin_tile();
+  if (first_place < end) {
+    look_up();
+    begin_tile();
+  }
   for (int i = 0; i < R::STAGES && loading < end; ++i) ask();
-  int turn = 0;                          // place of the join that is next
   for (int at = first_place, next; at < end; at = next) {
     const uint32_t pieces = present & ((1u << PARTS) - 1);
     present >>= PARTS;
     --queued;
     if (pieces) {
-      const int token = (work.s.begin + work.step) * STEP + warp * UNIT;
+      const int token = (work.s.begin + work.step) * UNIT;
       const uint32_t keys = ring + slot_out * R::SLOT, values = keys + R::CODES;
       const uint32_t of_keys = scale_ring + slot_out * R::SCALE_SLOT + (lane >> 2) * (GROUPS * 4), of_values = of_keys + R::SCALES;
       if (ok) ok = mbar_wait_warp(full + 8 * slot_out, (parity >> slot_out) & 1);
@@ -442,12 +447,12 @@ paged_rows_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     if (!last_step && next < end) {
       ++work.step;
     } else {
-      // ---- the warps' parts, then the CTAs'.  There are two places for them in turn: when a warp writes to one of them again,
-      // all have passed the barrier of the tile between.
-      float* join_here = join + turn * (WARPS * ROWS * D);
-      float* max_here = join_max + turn * (WARPS * ROWS);
-      float* sum_here = join_sum + turn * (WARPS * ROWS);
-      turn ^= JOINS - 1;
+      // ---- the tile's end, or the share's
+      const int tile_row = work.tile * ROWS, rows = min(ROWS, work.s.rows - tile_row);
+      const int item_begin = at - work.step, item_end = item_begin + work.s.steps;       // the tile's places, maybe of other warps
+      const bool begins = item_begin >= 0, whole = begins && last_step;
+      float* part = part_of(warp, begins);
+      // (a last part lies in the ring, which nothing is on its way to any more)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -456,10 +461,7 @@ paged_rows_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
           float sum_all = weight_sum[nt][e];
 #pragma unroll
           for (int d = 4; d < 32; d *= 2) sum_all += __shfl_xor_sync(0xffffffffu, sum_all, d);
-          if (lane < 4) {
-            max_here[warp * ROWS + r] = top[nt][e];
-            sum_here[warp * ROWS + r] = sum_all * 0x1p-64f;
-          }
+          sum_all *= 0x1p-64f;
           float constant[GROUPS];
 #pragma unroll
           for (int g = 0; g < GROUPS; ++g) {
@@ -468,27 +470,41 @@ paged_rows_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             for (int d = 4; d < 32; d *= 2) m += __shfl_xor_sync(0xffffffffu, m, d);
             constant[g] = (SPLIT ? m : fmaf(-8.f, eights[nt][g][e], m)) * 0x1p-64f;
           }
+          const int token = (tile_row + min(r, rows - 1)) / p.group, of_group = tile_row + min(r, rows - 1) - token * p.group;
+          uint16_t* to = p.out + (int64_t(work.s.first_row + token) * p.q_heads + work.head * p.group + of_group) * D + 4 * (lane >> 2);
+          float inverse = 1.f;
+          if (whole && r < rows) inverse = sum_all == 0.f ? of_nothing(p, work.b, work.s.first_row + token) : 1.f / sum_all;
 #pragma unroll
           for (int c = 0; c < CHUNKS; ++c) {
-            // (pieces change places with the row, so that a store meets 32 banks)
             const float from = constant[c / OF_GROUP];
-            float* to = join_here + (warp * ROWS + r) * D + 4 * ((8 * c + (lane >> 2)) ^ (2 * (lane & 3)));
-            *reinterpret_cast<float4*>(to) = make_float4(fmaf(o[nt][c][0][e], 0x1p69f, from), fmaf(o[nt][c][0][e + 2], 0x1p65f, from),
-                                                         fmaf(o[nt][c][1][e], 0x1p69f, from), fmaf(o[nt][c][1][e + 2], 0x1p65f, from));
+            const float x[4] = {fmaf(o[nt][c][0][e], 0x1p69f, from), fmaf(o[nt][c][0][e + 2], 0x1p65f, from),
+                                fmaf(o[nt][c][1][e], 0x1p69f, from), fmaf(o[nt][c][1][e + 2], 0x1p65f, from)};
+            if (whole) {
+              if (r < rows)
+                *reinterpret_cast<uint2*>(to + 32 * c) =
+                    make_uint2(Elem<T>::pack2(x[0] * inverse, x[1] * inverse), Elem<T>::pack2(x[2] * inverse, x[3] * inverse));
+            } else {
+              // (pieces change places with the row, so that a store meets 32 banks)
+              *reinterpret_cast<float4*>(part + r * D + 4 * ((8 * c + (lane >> 2)) ^ (2 * (lane & 3)))) =
+                  make_float4(x[0], x[1], x[2], x[3]);
+            }
+          }
+          if (!whole && lane < 4) {
+            part[ROWS * D + r] = top[nt][e];
+            part[ROWS * (D + 1) + r] = sum_all;
           }
         }
       }
-      const int tile_row = work.tile * ROWS, rows = min(ROWS, work.s.rows - tile_row), head = work.head;
-      const int first_row = work.s.first_row, sequence = work.b;
-      const int item_begin = at - work.step, item_end = item_begin + work.s.steps;   // the tile's places, maybe of other CTAs
+      if (!whole && lane == 0) {
+        Left& mine = left[2 * warp + begins];
+        mine.there = 1;
+        mine.begin = origin + item_begin, mine.end = origin + item_end;
+        mine.row = work.s.first_row, mine.head = work.head, mine.tile_row = tile_row, mine.rows = rows, mine.sequence = work.b;
+      }
       if (next < end) {
         work.advance(p, ROWS);
-        begin_tile();                    // (its queries are on their way while this tile is put together)
+        begin_tile();
       }
-      __syncthreads();
-      put_together<T, D, ROWS, WARPS>(p, start.share, join_here, max_here, sum_here, entry, tile_row, rows, head, first_row, sequence,
-                                      item_begin, item_end);
-      if (JOINS == 1) __syncthreads();
     }
   }
   if (!ok) {
@@ -498,13 +514,78 @@ paged_rows_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       for (int of_phase = 0; of_phase < 2; ++of_phase) mbar_wait_warp(full + 8 * s, of_phase, 64);
     if (lane == 0) atomicExch(p.status, INTENT_B200_ERR_TIMEOUT);
   }
+
+  // ---- the warps' parts, then the CTAs': of every tile that was cut in this CTA, a thread per row and eight elements
+  __syncthreads();
+  const int of_cta = WARPS * start.share;
+  // Where they begin: with a warp's last part, or the CTA's very first (the first part of another warp goes on with one before).
+  uint32_t tiles = __ballot_sync(0xffffffffu, lane < 2 * WARPS && (lane % 2 == 1 || lane == 0) && left[lane].there);
+  constexpr int OF_TILE = ROWS * (D / 8);
+  for (int at = tid, before = 0; tiles; tiles &= tiles - 1, before += OF_TILE) {
+    if (at >= before + OF_TILE) continue;
+    const int from = __ffs(tiles) - 1, first = from / 2, w = at - before, r = w / (D / 8), c = w - r * (D / 8);
+    at += THREADS;
+    const Left item = left[from];
+    const bool begins = item.begin >= 0, whole = begins && item.end <= of_cta;
+    int count = 1;                       // warps that have a part of it
+    while (first + count < WARPS && left[2 * (first + count)].there && left[2 * (first + count)].begin == item.begin) ++count;
+    if (r >= item.rows) continue;
+    auto part = [&](int v) { return part_of(first + v, v == 0 ? from % 2 : 0); };
+    float maxima[WARPS], m = -infinity, l = 0.f, x[8] = {};
+#pragma unroll
+    for (int v = 0; v < WARPS; ++v) maxima[v] = v < count ? part(v)[ROWS * D + r] : -infinity;
+#pragma unroll
+    for (int v = 0; v < WARPS; ++v) m = fmaxf(m, maxima[v]);
+    const float top_here = m == -infinity ? 0.f : m;
+#pragma unroll
+    for (int v = 0; v < WARPS; ++v) {
+      if (v >= count) break;
+      const float f = exp2_fast(maxima[v] - top_here);
+      l = fmaf(part(v)[ROWS * (D + 1) + r], f, l);
+      const float4* of_row = reinterpret_cast<const float4*>(part(v) + r * D + 8 * (c ^ (r >> 1 & 3)));
+      const float4 low = of_row[0], high = of_row[1];
+      x[0] = fmaf(low.x, f, x[0]), x[1] = fmaf(low.y, f, x[1]), x[2] = fmaf(low.z, f, x[2]), x[3] = fmaf(low.w, f, x[3]);
+      x[4] = fmaf(high.x, f, x[4]), x[5] = fmaf(high.y, f, x[5]), x[6] = fmaf(high.z, f, x[6]), x[7] = fmaf(high.w, f, x[7]);
+    }
+    if (whole) {
+      const int token = (item.tile_row + r) / p.group, of_group = item.tile_row + r - token * p.group;
+      const float inverse = l == 0.f ? of_nothing(p, item.sequence, item.row + token) : 1.f / l;
+      *reinterpret_cast<uint4*>(p.out + (int64_t(item.row + token) * p.q_heads + item.head * p.group + of_group) * D + 8 * c) =
+          make_uint4(Elem<T>::pack2(x[0] * inverse, x[1] * inverse), Elem<T>::pack2(x[2] * inverse, x[3] * inverse),
+                     Elem<T>::pack2(x[4] * inverse, x[5] * inverse), Elem<T>::pack2(x[6] * inverse, x[7] * inverse));
+    } else {
+      float* to_part = p.parts + size_t(2 * blockIdx.x + begins) * (ROWS * (D + 2));
+      float4* to = reinterpret_cast<float4*>(to_part + r * D + 8 * c);
+      to[0] = make_float4(x[0], x[1], x[2], x[3]);
+      to[1] = make_float4(x[4], x[5], x[6], x[7]);
+      if (c == 0) {
+        to_part[ROWS * D + r] = m;
+        to_part[ROWS * (D + 1) + r] = l;
+      }
+      if (w == 0 && begins) {
+        entry->row = item.row;
+        entry->head = item.head;
+        entry->tile_row = item.tile_row;
+        entry->rows = item.rows;
+        entry->sequence = item.sequence;
+        entry->last_cta = blockIdx.x + (item.end - 1) / of_cta;
+      }
+    }
+  }
 }
 
 template <typename T, int D, int GROUP, int NT>
-int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, const Int4Cache& cache, const PagedParams& p, int grid,
-           cudaStream_t stream) {
+int launch(const Int4Cache& cache, const PagedParams& p, int grid, cudaStream_t stream) {
+  CUtensorMap map_k, map_v;
+  constexpr int UNIT = Ring<D, GROUP, NT>::UNIT, ROW = Ring<D, GROUP, NT>::ROW;
+  const uint64_t rows = uint64_t(p.pages) * uint64_t(p.k_heads) << p.page_shift;
+  const uint32_t box = (1 << p.page_shift) < UNIT ? 1u << p.page_shift : UNIT;
+  constexpr auto swizzle = D == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
+  if (!make_tensor_map_2d(&map_k, CU_TENSOR_MAP_DATA_TYPE_UINT8, cache.k_codes, rows, ROW, ROW, box, ROW, swizzle) ||
+      !make_tensor_map_2d(&map_v, CU_TENSOR_MAP_DATA_TYPE_UINT8, cache.v_codes, rows, ROW, ROW, box, ROW, swizzle))
+    return INTENT_B200_ERR_CUDA;
   auto kernel = paged_rows_int4_kernel<T, D, GROUP, NT>;
-  constexpr int smem = smem_bytes<D, GROUP, NT>(), threads = 32 * Ring<D, GROUP>::WARPS;
+  constexpr int smem = smem_bytes<D, GROUP, NT>(), threads = 32 * Ring<D, GROUP, NT>::WARPS;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return cuda_status(e);
   if (LaunchFacts* sink = observe_sink())
@@ -518,30 +599,20 @@ int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, const Int4Cache& 
 }
 
 template <typename T, int D, int GROUP>
-int launch_rows(const CUtensorMap& map_k, const CUtensorMap& map_v, const Int4Cache& cache, const PagedParams& p, int tile_rows, int grid,
-                cudaStream_t stream) {
-  return tile_rows == 8 ? launch<T, D, GROUP, 1>(map_k, map_v, cache, p, grid, stream)
-                        : launch<T, D, GROUP, 2>(map_k, map_v, cache, p, grid, stream);
+int launch_rows(const Int4Cache& cache, const PagedParams& p, int tile_rows, int grid, cudaStream_t stream) {
+  return tile_rows == 8 ? launch<T, D, GROUP, 1>(cache, p, grid, stream) : launch<T, D, GROUP, 2>(cache, p, grid, stream);
 }
 
 }  // namespace
 
 template <typename T>
 int paged_rows_int4(const PagedParams& p, int64_t dim, int tile_rows, const Int4Cache& cache, int grid, cudaStream_t stream) {
-  CUtensorMap map_k, map_v;
-  const uint64_t rows = uint64_t(p.pages) * uint64_t(p.k_heads) << p.page_shift;
-  const uint32_t box = (1 << p.page_shift) < UNIT ? 1u << p.page_shift : UNIT;
-  const auto swizzle = dim == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
-  const uint64_t row = uint64_t(dim) / 2;
-  if (!make_tensor_map_2d(&map_k, CU_TENSOR_MAP_DATA_TYPE_UINT8, cache.k_codes, rows, row, row, box, uint32_t(row), swizzle) ||
-      !make_tensor_map_2d(&map_v, CU_TENSOR_MAP_DATA_TYPE_UINT8, cache.v_codes, rows, row, row, box, uint32_t(row), swizzle))
-    return INTENT_B200_ERR_CUDA;
   if (dim == 64)
-    return cache.group == 32 ? launch_rows<T, 64, 32>(map_k, map_v, cache, p, tile_rows, grid, stream)
-                             : launch_rows<T, 64, 64>(map_k, map_v, cache, p, tile_rows, grid, stream);
-  return cache.group == 32   ? launch_rows<T, 128, 32>(map_k, map_v, cache, p, tile_rows, grid, stream)
-         : cache.group == 64 ? launch_rows<T, 128, 64>(map_k, map_v, cache, p, tile_rows, grid, stream)
-                             : launch_rows<T, 128, 128>(map_k, map_v, cache, p, tile_rows, grid, stream);
+    return cache.group == 32 ? launch_rows<T, 64, 32>(cache, p, tile_rows, grid, stream)
+                             : launch_rows<T, 64, 64>(cache, p, tile_rows, grid, stream);
+  return cache.group == 32   ? launch_rows<T, 128, 32>(cache, p, tile_rows, grid, stream)
+         : cache.group == 64 ? launch_rows<T, 128, 64>(cache, p, tile_rows, grid, stream)
+                             : launch_rows<T, 128, 128>(cache, p, tile_rows, grid, stream);
 }
 template int paged_rows_int4<__half>(const PagedParams&, int64_t, int, const Int4Cache&, int, cudaStream_t);
 template int paged_rows_int4<__nv_bfloat16>(const PagedParams&, int64_t, int, const Int4Cache&, int, cudaStream_t);
