@@ -34,13 +34,13 @@ template <int D, int GROUP, int NT>
 struct Ring {
   static constexpr int UNIT = 64;                         // tokens of a ring slot, a step
   static constexpr int PARTS = UNIT / 16;                 // pieces of it that lie in one page in any case
-  static constexpr int WARPS = 8;
+  static constexpr int WARPS = NT == 1 && D == 64 ? 16 : 8;
   static constexpr int STAGES = 2;
   static constexpr int GROUPS = D / GROUP;
   static constexpr int ROW = D / 2;                       // bytes of a token's codes
   static constexpr int CODES = UNIT * ROW, SCALES = UNIT * GROUPS * 4;   // of keys or values of a unit
-  static constexpr int SLOT = 2 * CODES, SCALE_SLOT = 2 * SCALES;
-  static constexpr int OF_WARP = STAGES * SLOT, BYTES = WARPS * STAGES * (SLOT + SCALE_SLOT);
+  static constexpr int SLOT = 2 * (CODES + SCALES);       // keys' codes, values' codes, keys' scales, values' scales
+  static constexpr int OF_WARP = STAGES * SLOT, BYTES = WARPS * OF_WARP;
   static constexpr int BEGIN = 1;                         // places on the line ahead of the steps of a tile
   static constexpr int PIECE = 8 * NT * (D + 2) * 4;      // a part of a tile: results, maxima, sums
   static_assert(PIECE <= OF_WARP, "a warp's last part lies in its ring");
@@ -56,9 +56,25 @@ struct Left {
 template <int D, int GROUP, int NT>
 constexpr int smem_bytes() {
   using R = Ring<D, GROUP, NT>;
-  constexpr int bytes = 1024 + R::BYTES + R::WARPS * (R::PIECE + 2 * int(sizeof(Left)) + R::STAGES * 8 + 8 + 16);
+  constexpr int bytes = 128 + R::BYTES + R::WARPS * (R::PIECE + 2 * int(sizeof(Left)) + 8 + 16);
   static_assert(bytes <= 227 * 1024, "shared memory of a CTA");
   return bytes;
+}
+
+// 16 bytes to shared memory, past the first-level cache; copies are waited for in groups, in order
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
+// What the number of a 16-byte chunk of a row of codes is changed by: rows of 64 or 32 bytes, eight of which fill 32 banks
+template <int D>
+__device__ __forceinline__ int swizzle_of(int row) {
+  return D == 128 ? (row >> 1) & 3 : (row >> 2) & 1;
 }
 
 template <int N>
@@ -99,19 +115,14 @@ struct Codes<__half> {
 
 template <typename T, int D, int GROUP, int NT>
 __global__ void __launch_bounds__(32 * Ring<D, GROUP, NT>::WARPS, 1)
-paged_rows_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const uint32_t* k_scales,
-                       const uint32_t* v_scales, const PagedParams p) {
+paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
   using R = Ring<D, GROUP, NT>;
   constexpr int ROWS = 8 * NT, WARPS = R::WARPS, THREADS = 32 * WARPS, UNIT = R::UNIT, PARTS = R::PARTS, STEP = UNIT, BEGIN = R::BEGIN, GROUPS = R::GROUPS;
   constexpr int CHUNKS = D / 32, OF_GROUP = CHUNKS / GROUPS;            // 16 bytes of a token's codes
   constexpr bool SPLIT = std::is_same<T, __half>::value;                // weights in two bf16 parts
   extern __shared__ unsigned char smem_raw[];
   programmatic_begin();
-  if (threadIdx.x == 0) {
-    prefetch_tensormap(&map_k);
-    prefetch_tensormap(&map_v);
-  }
-  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t base = (smem_u32(smem_raw) + 127u) & ~127u;
   unsigned char* base_ptr = smem_raw + (base - smem_u32(smem_raw));
   // a warp's part of the tile that its share begins in; then of the tile that it ends in, in its ring
   float* first_parts = reinterpret_cast<float*>(base_ptr + R::BYTES);
@@ -121,14 +132,8 @@ paged_rows_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   Left* left = reinterpret_cast<Left*>(base_ptr + R::BYTES + WARPS * R::PIECE);          // [WARPS][2]
   long long* starts = reinterpret_cast<long long*>(left + 2 * WARPS);                    // [WARPS][2]: sequence, place in it
   long long* warp_sums = starts + 2 * WARPS;
-  const uint32_t bars = smem_u32(warp_sums + WARPS);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t ring = base + warp * R::OF_WARP, full = bars + warp * R::STAGES * 8;
-  const uint32_t scale_ring = base + WARPS * R::OF_WARP + warp * R::STAGES * R::SCALE_SLOT;
-  if (lane == 0) {
-    for (int s = 0; s < R::STAGES; ++s) mbar_init(full + 8 * s, 1);
-    fence_mbar_init();
-  }
+  const uint32_t ring = base + warp * R::OF_WARP;
   programmatic_wait();
 
   // ---- this warp's part of the line
@@ -140,9 +145,8 @@ paged_rows_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 
   const float infinity = __int_as_float(0x7f800000);
   int loading = first_place, slot_in = 0, slot_out = 0;
-  uint32_t parity = 0, present = 0;      // a bit per slot; PARTS bits per unit asked for, the oldest lowest
+  uint32_t present = 0;                  // PARTS bits per unit asked for, the oldest lowest
   int queued = 0;
-  bool ok = true;
   const int box = min(1 << p.page_shift, UNIT);          // tokens of a unit that lie in one page
   int page;                              // of piece lane % PARTS of the unit at `load`, asked for one unit ahead; -1: not needed
   auto look_up = [&] {
@@ -151,33 +155,55 @@ paged_rows_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     if (t < load.s.length && t + 16 > load.s.low)
       page = __ldg(p.page_table + int64_t(load.b) * p.table_width + (t >> p.page_shift));
   };
+  // A lane copies 16 bytes at a time of the 512 that a warp does, rows of codes in an order in which eight of them meet 32 banks.
+  constexpr int CHUNKS_OF_ROW = R::ROW / 16;
+  const int copied_row = lane / CHUNKS_OF_ROW, copied_chunk = lane % CHUNKS_OF_ROW;
+  const uint32_t copied = copied_row * R::ROW + ((copied_chunk ^ swizzle_of<D>(copied_row)) << 4);
+  const unsigned char *k_codes = static_cast<const unsigned char*>(cache.k_codes) + 16 * lane,
+                      *v_codes = static_cast<const unsigned char*>(cache.v_codes) + 16 * lane;
   // asks for the unit of this warp at `load`, and goes on
   auto ask = [&] {
-    const int token = (load.s.begin + load.step) * UNIT;
-    // (pieces of one page are one box, whichever of them is needed)
-    int number = page >= 0 && page < p.pages ? page : -1;
+    const int number = page >= 0 && page < p.pages ? page : -1;
     const uint32_t here = __ballot_sync(0xffffffffu, number >= 0) & ((1u << PARTS) - 1);
-    number = box >= 32 ? max(number, __shfl_xor_sync(0xffffffffu, number, 1)) : number;
-    number = UNIT >= 64 && box >= 64 ? max(number, __shfl_xor_sync(0xffffffffu, number, 2)) : number;
-    // lane: piece lane % PARTS of keys' codes, values' codes, keys' scales, values' scales
-    const int piece = lane % PARTS, what = lane / PARTS;
-    const bool mine = number >= 0 && piece * 16 % box == 0;
-    const uint32_t boxes = __ballot_sync(0xffffffffu, mine) & ((1u << PARTS) - 1);
-    if (here) {
-      const uint32_t bar = full + 8 * slot_in;
-      if (lane == 0) mbar_expect_tx(bar, uint32_t(__popc(boxes) * box * 2 * (R::ROW + 4 * GROUPS)));
-      __syncwarp();
-      if (mine && what < 4) {
-        const int t = token + piece * 16;
-        const int row = ((number * p.k_heads + load.head) << p.page_shift) + (t & ((1 << p.page_shift) - 1));
-        const uint32_t to = ring + slot_in * R::SLOT + piece * 16 * R::ROW;
-        const uint32_t to_scales = scale_ring + slot_in * R::SCALE_SLOT + piece * 16 * GROUPS * 4;
-        if (what < 2) tma_load_2d(to + what * R::CODES, what ? &map_v : &map_k, 0, row, bar);
-        else bulk_load(to_scales + (what - 2) * R::SCALES, (what == 3 ? v_scales : k_scales) + int64_t(row) * GROUPS,
-                       uint32_t(box * GROUPS * 4), bar);
+    const int first = ((load.s.begin + load.step) * UNIT) & ((1 << p.page_shift) - 1);     // in its page
+    const uint32_t to = ring + slot_in * R::SLOT;
+    if (box == UNIT) {
+      // (the pieces that are needed have the same page)
+      if (here) {
+        const int row = ((__shfl_sync(0xffffffffu, number, __ffs(here) - 1) * p.k_heads + load.head) << p.page_shift) + first;
+        const int64_t code = int64_t(row) * R::ROW, scale = int64_t(row) * (GROUPS * 4);
+#pragma unroll
+        for (int i = 0; i < R::CODES / 512; ++i) {
+          copy16(to + copied + 512 * i, k_codes + code + 512 * i);
+          copy16(to + R::CODES + copied + 512 * i, v_codes + code + 512 * i);
+        }
+#pragma unroll
+        for (int i = 0; i < (2 * R::SCALES + 511) / 512; ++i) {
+          const int at = 512 * i + 16 * lane;            // keys' scales, then values'
+          const unsigned char* from = static_cast<const unsigned char*>(at < R::SCALES ? cache.k_scales : cache.v_scales);
+          if (at < 2 * R::SCALES) copy16(to + 2 * R::CODES + at, from + scale + (at < R::SCALES ? at : at - R::SCALES));
+        }
       }
-      slot_in = slot_in + 1 == R::STAGES ? 0 : slot_in + 1;
+    } else {
+#pragma unroll
+      for (int piece = 0; piece < PARTS; ++piece) {
+        const int of_piece = __shfl_sync(0xffffffffu, number, piece);
+        if (of_piece < 0) continue;
+        const int row = ((of_piece * p.k_heads + load.head) << p.page_shift) + ((first + 16 * piece) & ((1 << p.page_shift) - 1));
+        const int64_t code = int64_t(row) * R::ROW, scale = int64_t(row) * (GROUPS * 4);
+#pragma unroll
+        for (int i = 0; i < 16 * R::ROW / 512; ++i) {
+          const uint32_t there = to + copied + 16 * piece * R::ROW + 512 * i;
+          copy16(there, k_codes + code + 512 * i);
+          copy16(there + R::CODES, v_codes + code + 512 * i);
+        }
+        const unsigned char* from = static_cast<const unsigned char*>(lane < 16 ? cache.k_scales : cache.v_scales) + 16 * (lane % 16);
+        if (lane % 16 < 4 * GROUPS)
+          copy16(to + 2 * R::CODES + (lane < 16 ? 0 : R::SCALES) + 64 * GROUPS * piece + 16 * (lane % 16), from + scale);
+      }
     }
+    copies_commit();
+    slot_in = slot_in + 1 == R::STAGES ? 0 : slot_in + 1;
     present |= here << (PARTS * queued);
     ++queued;
     loading += load.distance();
@@ -247,18 +273,23 @@ paged_rows_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     look_up();
     begin_tile();
   }
-  for (int i = 0; i < R::STAGES && loading < end; ++i) ask();
+#pragma unroll
+  for (int i = 0; i < R::STAGES; ++i) {
+    if (loading < end) ask();
+    else copies_commit();                // (every unit of the ring has a group of copies, be it empty)
+  }
   for (int at = first_place, next; at < end; at = next) {
     const uint32_t pieces = present & ((1u << PARTS) - 1);
     present >>= PARTS;
     --queued;
+    copies_wait<R::STAGES - 1>();
+    __syncwarp();
+    const uint32_t slot = ring + slot_out * R::SLOT;
+    slot_out = slot_out + 1 == R::STAGES ? 0 : slot_out + 1;
     if (pieces) {
       const int token = (work.s.begin + work.step) * UNIT;
-      const uint32_t keys = ring + slot_out * R::SLOT, values = keys + R::CODES;
-      const uint32_t of_keys = scale_ring + slot_out * R::SCALE_SLOT + (lane >> 2) * (GROUPS * 4), of_values = of_keys + R::SCALES;
-      if (ok) ok = mbar_wait_warp(full + 8 * slot_out, (parity >> slot_out) & 1);
-      parity ^= 1u << slot_out;
-      slot_out = slot_out + 1 == R::STAGES ? 0 : slot_out + 1;
+      const uint32_t keys = slot, values = keys + R::CODES;
+      const uint32_t of_keys = slot + 2 * R::CODES + (lane >> 2) * (GROUPS * 4), of_values = of_keys + R::SCALES;
 
       float s[NT][PARTS][4];             // S^T: tokens 16 m + lane / 4 (+ 8), rows as in o
 #pragma unroll
@@ -268,12 +299,12 @@ paged_rows_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int r = 16 * m + 8 * h + (lane & 7), c = lane >> 3;
-            ldmatrix_x4(codes[h], keys + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+            ldmatrix_x4(codes[h], keys + r * 64 + ((c ^ swizzle_of<D>(lane & 7)) << 4));
           }
         } else {
           const int r = 16 * m + 8 * (lane >> 4) + (lane & 7), c = (lane >> 3) & 1;
           uint32_t all[4];
-          ldmatrix_x4(all, keys + r * 32 + ((c ^ ((r >> 2) & 1)) << 4));
+          ldmatrix_x4(all, keys + r * 32 + ((c ^ swizzle_of<D>(lane & 7)) << 4));
 #pragma unroll
           for (int e = 0; e < 4; ++e) codes[e >> 1][e & 1] = all[e];
         }
@@ -416,7 +447,7 @@ paged_rows_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             // codes of tokens 16 m + 2 (lane % 4) (+ 1; + 8): elements 32 c + 4 (lane / 4) .. of chunks 2 pair and 2 pair + 1
             const int r = 16 * m + (lane & 15), c = 2 * pair + (lane >> 4);
             uint32_t codes[4];
-            ldmatrix_x4_trans(codes, values + r * R::ROW + ((c ^ (D == 128 ? (r >> 1) & 3 : (r >> 2) & 1)) << 4));
+            ldmatrix_x4_trans(codes, values + r * R::ROW + ((c ^ swizzle_of<D>(lane & 7)) << 4));
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -440,7 +471,8 @@ paged_rows_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       else add_values(Bool<false>{});
       __syncwarp();                      // every lane is done with the slot
     }
-    if (ok && loading < end) ask();      // (a slot that was given up on may still be on its way)
+    if (loading < end) ask();
+    else copies_commit();
 
     const bool last_step = work.step + 1 == work.s.steps;
     next = at + work.distance();
@@ -507,14 +539,6 @@ paged_rows_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       }
     }
   }
-  if (!ok) {
-    // Nothing may be on its way to a CTA that is gone.  (Which phase a slot is in has not been counted since the wait that gave
-    // up: of the two parities the wait for one is for the current phase, the other is over.)
-    for (int s = 0; s < R::STAGES; ++s)
-      for (int of_phase = 0; of_phase < 2; ++of_phase) mbar_wait_warp(full + 8 * s, of_phase, 64);
-    if (lane == 0) atomicExch(p.status, INTENT_B200_ERR_TIMEOUT);
-  }
-
   // ---- the warps' parts, then the CTAs': of every tile that was cut in this CTA, a thread per row and eight elements
   __syncthreads();
   const int of_cta = WARPS * start.share;
@@ -576,14 +600,6 @@ paged_rows_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 
 template <typename T, int D, int GROUP, int NT>
 int launch(const Int4Cache& cache, const PagedParams& p, int grid, cudaStream_t stream) {
-  CUtensorMap map_k, map_v;
-  constexpr int UNIT = Ring<D, GROUP, NT>::UNIT, ROW = Ring<D, GROUP, NT>::ROW;
-  const uint64_t rows = uint64_t(p.pages) * uint64_t(p.k_heads) << p.page_shift;
-  const uint32_t box = (1 << p.page_shift) < UNIT ? 1u << p.page_shift : UNIT;
-  constexpr auto swizzle = D == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
-  if (!make_tensor_map_2d(&map_k, CU_TENSOR_MAP_DATA_TYPE_UINT8, cache.k_codes, rows, ROW, ROW, box, ROW, swizzle) ||
-      !make_tensor_map_2d(&map_v, CU_TENSOR_MAP_DATA_TYPE_UINT8, cache.v_codes, rows, ROW, ROW, box, ROW, swizzle))
-    return INTENT_B200_ERR_CUDA;
   auto kernel = paged_rows_int4_kernel<T, D, GROUP, NT>;
   constexpr int smem = smem_bytes<D, GROUP, NT>(), threads = 32 * Ring<D, GROUP, NT>::WARPS;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -591,8 +607,7 @@ int launch(const Int4Cache& cache, const PagedParams& p, int grid, cudaStream_t 
   if (LaunchFacts* sink = observe_sink())
     return record_launch(sink, reinterpret_cast<const void*>(kernel),
                          NT == 1 ? "paged_rows_int4_kernel 8 rows" : "paged_rows_int4_kernel 16 rows", grid, threads, smem, 1);
-  e = launch_programmatic(kernel, dim3(unsigned(grid)), dim3(threads), smem, stream, 1, map_k, map_v,
-                          static_cast<const uint32_t*>(cache.k_scales), static_cast<const uint32_t*>(cache.v_scales), p);
+  e = launch_programmatic(kernel, dim3(unsigned(grid)), dim3(threads), smem, stream, 1, cache, p);
   if (e != cudaSuccess) return cuda_status(e);
   note_launch();
   return launch_status();
