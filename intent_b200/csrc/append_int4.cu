@@ -21,6 +21,7 @@ namespace ib200 {
 namespace {
 
 constexpr int THREADS = ROTATE_THREADS;
+constexpr int CACHE_ROWS = 2;           // keys or values of a group in calls of many rows
 
 template <typename F>
 __device__ __forceinline__ F least_of(F a, F b) {
@@ -232,11 +233,12 @@ __device__ __forceinline__ void key_rows(const RotateParams& p, uint32_t block) 
 
 // k_blocks blocks of keys, as many of values, the others of queries (p.k_heads is 0 in `queries`)
 template <typename T, int D, bool NORM, bool NEIGHBOURS, int ROWS, int GROUP>
-__global__ void __launch_bounds__(THREADS) append_int4_kernel(const RotateParams p, const RotateParams queries, uint32_t k_blocks) {
+__global__ void __launch_bounds__(THREADS, 4) append_int4_kernel(const RotateParams p, const RotateParams queries, uint32_t k_blocks) {
+  constexpr int K_ROWS = ROWS == 1 ? 1 : CACHE_ROWS;
   programmatic_begin();
   const uint32_t block = blockIdx.x;
-  if (block < k_blocks) key_rows<T, D, NORM, NEIGHBOURS, ROWS, GROUP>(p, block);
-  else if (block < 2 * k_blocks) value_rows<T, D, ROWS, GROUP>(p, block - k_blocks);
+  if (block < k_blocks) key_rows<T, D, NORM, NEIGHBOURS, K_ROWS, GROUP>(p, block);
+  else if (block < 2 * k_blocks) value_rows<T, D, K_ROWS, GROUP>(p, block - k_blocks);
   else rotate_rows<T, D, NORM, NEIGHBOURS, false, ROWS>(queries, block - 2 * k_blocks);
 }
 
@@ -245,7 +247,8 @@ int launch(const RotateParams& p, bool neighbours, cudaStream_t stream) {
   auto kernel = neighbours ? append_int4_kernel<T, D, NORM, true, ROWS, GROUP> : append_int4_kernel<T, D, NORM, false, ROWS, GROUP>;
   constexpr uint32_t PER_CTA = THREADS / (D / 8);
   static_assert(D / 8 == D / (2 * PIECE_OF), "lanes of a row of queries");
-  const uint32_t k_blocks = (p.tokens * ((p.k_heads + ROWS - 1) / ROWS) + PER_CTA - 1) / PER_CTA;
+  constexpr uint32_t K_ROWS = ROWS == 1 ? 1 : CACHE_ROWS;
+  const uint32_t k_blocks = (p.tokens * ((p.k_heads + K_ROWS - 1) / K_ROWS) + PER_CTA - 1) / PER_CTA;
   const uint32_t q_blocks = (p.tokens * ((p.q_heads + ROWS - 1) / ROWS) + PER_CTA - 1) / PER_CTA, grid = 2 * k_blocks + q_blocks;
   RotateParams queries = p;
   queries.k_heads = 0;

@@ -11,6 +11,7 @@ namespace ib200 {
 namespace {
 
 constexpr int THREADS = 256;
+constexpr int ROWS = 2;                  // of a thread
 
 struct ReadParams {
   const int64_t* slots;
@@ -21,13 +22,17 @@ struct ReadParams {
   int page_shift;
 };
 
+// (2^23 + n has n in its lowest bits: no conversion)
 template <typename T>
 __device__ __forceinline__ uint4 values_of(uint32_t codes, uint32_t scales) {
   const float s = Elem<T>::to_float(uint16_t(scales)), m = Elem<T>::to_float(uint16_t(scales >> 16));
   uint32_t w[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    w[e] = Elem<T>::pack2(fmaf(float(codes >> (8 * e) & 15), s, m), fmaf(float(codes >> (8 * e + 4) & 15), s, m));
+  for (int e = 0; e < 4; ++e) {
+    const float low = __uint_as_float(lop3_and_or(codes >> (8 * e), 15u, 0x4b000000u)) - 8388608.f;
+    const float high = __uint_as_float(lop3_and_or(codes >> (8 * e + 4), 15u, 0x4b000000u)) - 8388608.f;
+    w[e] = Elem<T>::pack2(fmaf(low, s, m), fmaf(high, s, m));
+  }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
@@ -35,28 +40,37 @@ template <typename T, int D, int GROUP>
 __global__ void __launch_bounds__(THREADS) read_kernel(const ReadParams p) {
   constexpr uint32_t PIECES = D / 8;
   programmatic_begin();
-  const uint64_t at = uint64_t(blockIdx.x) * THREADS + threadIdx.x, row = at / PIECES;
-  const uint32_t piece = uint32_t(at % PIECES);
+  const uint32_t lane_piece = threadIdx.x % PIECES, rows = p.tokens * p.heads;
+  const uint32_t first = blockIdx.x * (THREADS / PIECES * ROWS) + threadIdx.x / PIECES;
   programmatic_wait();
-  if (row >= uint64_t(p.tokens) * p.heads) return;
-  const uint32_t token = uint32_t(row) / p.heads, head = uint32_t(row) - token * p.heads;
-  const int64_t slot = __ldg(p.slots + token);
-  uint4 k = make_uint4(0, 0, 0, 0), v = k;
-  if (slot >= 0 && slot < p.slot_count) {
+  uint32_t codes[ROWS][2], scales[ROWS][2];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const uint32_t row = first + i * (THREADS / PIECES);
+    codes[i][0] = codes[i][1] = scales[i][0] = scales[i][1] = 0;
+    if (row >= rows) continue;
+    const uint32_t token = row / p.heads, head = row - token * p.heads;
+    const int64_t slot = __ldg(p.slots + token);
+    if (slot < 0 || slot >= p.slot_count) continue;
     const int64_t place = (((slot >> p.page_shift) * p.heads + head) << p.page_shift) + (slot & ((int64_t(1) << p.page_shift) - 1));
-    const int64_t code = place * PIECES + piece, scale = place * (D / GROUP) + piece / (GROUP / 8);
-    const uint32_t a = __ldg(p.k_codes + code), b = __ldg(p.k_scales + scale), c = __ldg(p.v_codes + code), d = __ldg(p.v_scales + scale);
-    k = values_of<T>(a, b);
-    v = values_of<T>(c, d);
+    const int64_t code = place * PIECES + lane_piece, scale = place * (D / GROUP) + lane_piece / (GROUP / 8);
+    codes[i][0] = __ldg(p.k_codes + code), scales[i][0] = __ldg(p.k_scales + scale);
+    codes[i][1] = __ldg(p.v_codes + code), scales[i][1] = __ldg(p.v_scales + scale);
   }
-  p.k[at] = k;
-  p.v[at] = v;
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const uint32_t row = first + i * (THREADS / PIECES);
+    if (row >= rows) continue;
+    __stcs(p.k + size_t(row) * PIECES + lane_piece, values_of<T>(codes[i][0], scales[i][0]));
+    __stcs(p.v + size_t(row) * PIECES + lane_piece, values_of<T>(codes[i][1], scales[i][1]));
+  }
 }
 
 template <typename T, int D, int GROUP>
 int launch(const ReadParams& p, cudaStream_t stream) {
   auto kernel = read_kernel<T, D, GROUP>;
-  const uint32_t grid = uint32_t((uint64_t(p.tokens) * p.heads * (D / 8) + THREADS - 1) / THREADS);
+  constexpr uint32_t PER_CTA = THREADS / (D / 8) * ROWS;
+  const uint32_t grid = (p.tokens * p.heads + PER_CTA - 1) / PER_CTA;
   if (LaunchFacts* sink = observe_sink())
     return record_launch(sink, reinterpret_cast<const void*>(kernel), "read_kernel", int(grid), THREADS, 0, 1);
   const cudaError_t e = launch_programmatic(kernel, dim3(grid), dim3(THREADS), 0, stream, 1, p);
