@@ -23,19 +23,25 @@ namespace {
 constexpr int THREADS = ROTATE_THREADS;
 constexpr int CACHE_ROWS = 2;           // keys or values of a group in calls of many rows
 
-template <typename F>
-__device__ __forceinline__ F least_of(F a, F b) {
-  return a < b ? a : b;
+// The smaller and the larger of two; NaN if one is (f32), which is looked for apart (f64)
+__device__ __forceinline__ float least_of(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
 }
-template <typename F>
-__device__ __forceinline__ F largest_of(F a, F b) {
-  return a > b ? a : b;
+__device__ __forceinline__ float largest_of(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
 }
+__device__ __forceinline__ double least_of(double a, double b) { return a < b ? a : b; }
+__device__ __forceinline__ double largest_of(double a, double b) { return a > b ? a : b; }
 
 // The quotients of eight numbers by a scale s, rounded to whole numbers from 0 to 15.  The product with the rounded reciprocal gets its
 // remainder added, which makes it the quotient as a division rounds it (P. Markstein, Computation of elementary functions on the
-// IBM RISC System/6000 processor, 1990).  Added to 1.5 times 2 to the mantissa's length a number is rounded in the lowest bits.
-template <typename T>
+// IBM RISC System/6000 processor, 1990).  HALVES: whether quotients may lie in the middle between two numbers; those of keys that
+// were normalised do not, and need no such care.  Added to 1.5 times 2 to the mantissa's length a number is rounded in the lowest bits.
+template <typename T, bool HALVES>
 __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float s, float m) {
   // (powers of two that keep the reciprocal a normal number)
   const float by = std::is_same<T, __half>::value ? 1.f : s < 0x1p-60f ? 0x1p64f : s > 0x1p60f ? 0x1p-64f : 1.f;
@@ -49,47 +55,55 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float s, float
   }
   return codes;
 }
-template <typename T>
+template <typename T, bool HALVES>
 __device__ __forceinline__ uint32_t codes_of(const double (&x)[8], float scale, float minimum) {
-  const double s = scale, m = minimum, inverse = scale > 0.f ? __drcp_rn(s) : 0.;
+  const double s = scale, m = minimum, inverse = scale > 0.f ? __drcp_rn(s) : 0., origin = -m * inverse;
   uint32_t codes = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const double d = x[e] - m, q = d * inverse;
-    const int n = __double2loint(fma(fma(-q, s, d), inverse, q) + 6755399441055744.);
+    double quotient;
+    if (HALVES) {
+      const double d = x[e] - m, q = d * inverse;
+      quotient = fma(fma(-q, s, d), inverse, q);
+    } else {
+      quotient = fma(x[e], inverse, origin);
+    }
+    const int n = __double2loint(quotient + 6755399441055744.);
     codes |= uint32_t(min(max(n, 0), 15)) << (4 * e);
   }
   return codes;
 }
 
 // Eight neighbouring elements of a row as codes; `scales`: scale | minimum of their group, which all of its lanes know
-template <typename T, int GROUP, typename F>
+template <typename T, int GROUP, bool HALVES, typename F>
 __device__ __forceinline__ uint32_t quantise(const F (&x)[8], uint32_t& scales) {
   const float infinity = __int_as_float(0x7f800000);
   F low = x[0], high = x[0];
-  bool finite = true;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    low = least_of(x[e], low), high = largest_of(x[e], high);
-    finite &= fabsf(float(x[e])) < infinity;
-  }
+  for (int e = 1; e < 8; ++e) low = least_of(x[e], low), high = largest_of(x[e], high);
 #pragma unroll
   for (int d = 1; d < GROUP / 8; d *= 2) {
     low = least_of(__shfl_xor_sync(0xffffffffu, low, d), low);
     high = largest_of(__shfl_xor_sync(0xffffffffu, high, d), high);
   }
-  constexpr uint32_t LANES = (1u << (GROUP / 8)) - 1;
-  const uint32_t odd = __ballot_sync(0xffffffffu, !finite) >> (threadIdx.x & 31 & ~(GROUP / 8 - 1));
+  bool odd = false;                    // something of the group is no number
+  if (std::is_same<F, double>::value) {
+    F nothing = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) nothing = fma(x[e], F(0), nothing);
+    constexpr uint32_t LANES = (1u << (GROUP / 8)) - 1;
+    odd = __ballot_sync(0xffffffffu, nothing != 0) >> (threadIdx.x & 31 & ~(GROUP / 8 - 1)) & LANES;
+  }
   // (in 64 bits, in which the scale's rounding is that of the exact quotient)
   scales = Elem<T>::pack2(float((double(high) - double(low)) * (1. / 15.)), float(low));
   const float m = Elem<T>::to_float(uint16_t(scales >> 16));
   float s = Elem<T>::to_float(uint16_t(scales));
-  if ((odd & LANES) || !(s < infinity) || !(fabsf(m) < infinity)) {
+  if (odd || !(s < infinity) || !(fabsf(m) < infinity)) {
     scales = 0x7fff7fffu;
     return 0;
   }
   if (!(Elem<T>::to_float(Elem<T>::from_float(fmaf(15.f, s, m))) < infinity)) s = Elem<T>::to_float(uint16_t(--scales));
-  return codes_of<T>(x, s, m);
+  return codes_of<T, HALVES>(x, s, m);
 }
 
 // A group of lanes and its rows of one kind of one token
@@ -138,7 +152,7 @@ __device__ __forceinline__ void value_rows(const RotateParams& p, uint32_t block
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = Elem<T>::to_float(uint16_t(w[e / 2] >> (16 * (e & 1))));
     uint32_t scales;
-    const uint32_t codes = quantise<T, GROUP>(x, scales);
+    const uint32_t codes = quantise<T, GROUP, true>(x, scales);
     group.template store<GROUP>(p, i, j, p.v_codes, p.v_scales, codes, scales);
   }
 }
@@ -226,7 +240,7 @@ __device__ __forceinline__ void key_rows(const RotateParams& p, uint32_t block) 
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] *= scale;
     uint32_t scales;
-    const uint32_t codes = quantise<T, GROUP>(y, scales);
+    const uint32_t codes = quantise<T, GROUP, !NORM>(y, scales);
     group.template store<GROUP>(p, i, j, p.k_codes, p.k_scales, codes, scales);
   }
 }
