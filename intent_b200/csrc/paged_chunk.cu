@@ -48,11 +48,17 @@ namespace ib200 {
 namespace {
 
 constexpr int STEP = 128;                  // tokens of a step
-// warps 0..3 and 4..7: a half's rows; 10 and 11 turn codes of a cache in 4 bits into operands, and else only lend registers
-constexpr int LOAD_WARP = 9, MMA_WARP = 8, THREADS = 12 * 32, CONVERT_WARPS = 2;
+// Warps 0..3 and 4..7: a half's rows; 10 .. 13 turn codes of a cache in 4 bits into operands.  What is left only lends registers.
+constexpr int LOAD_WARP = 9, MMA_WARP = 8, CONVERT_WARPS = 4;
 // Registers of a thread: the launch's, then those of a row's thread (128 scores and more) and of the others.
-constexpr int LAUNCH_REGISTERS = 168, ROW_REGISTERS = 224, OTHER_REGISTERS = 56;
-static_assert(2 * ROW_REGISTERS + OTHER_REGISTERS <= 3 * LAUNCH_REGISTERS, "three warpgroups share the launch's registers");
+struct Split {
+  int threads, launch, row, other;
+};
+// (with two warps for the codes, on two of the four schedulers, 4096 tokens behind 12288 took 1129 us, with four 1014)
+constexpr Split WIDE = {12 * 32, 168, 224, 56}, INT4 = {16 * 32, 128, 208, 48};
+constexpr bool shared_out(const Split& s) { return 256 * s.row + (s.threads - 256) * s.other <= s.threads * s.launch; }
+static_assert(shared_out(WIDE) && shared_out(INT4), "the warpgroups share the launch's registers");
+constexpr Split split_of(int group) { return group ? INT4 : WIDE; }
 // Places on the line ahead of the steps of a tile, for what it costs beside them (four chunks of up to 500 tokens beside 20 single
 // ones, 16-bit heads of 128: 149 us without, 142 with one, 137 with two, 136 with three, 137 with four; 33 tokens behind 7967:
 // 28.2 without, 26.1 with two; long chunks alike).
@@ -257,18 +263,47 @@ __device__ __forceinline__ void weigh(const uint32_t (&v)[32], uint64_t scale, u
   }
 }
 
-// Eight codes as numbers m + s * n of the type, rounded once: elements 0 and 4, 1 and 5, 2 and 6, 3 and 7
+// Codes, masked where they are, as numbers m + s * n of the type, rounded once.  A pair of 16-bit words has a code each in its lowest
+// four bits (which = 0), in the next (1), or in one word in these and in the other in those (2).
+//   bf16  such bits are n or 16 n times the smallest number; a product makes n / 64 of them.  (Scales of 2^122 and more would not do.)
+//   f16   beside the bits of 1024 they are 1024 + n or 1024 + 16 n, of which a product and a difference make n.
 template <typename T>
-__device__ __forceinline__ void numbers_of(uint32_t codes, uint32_t s, uint32_t m, uint32_t (&w)[4]) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    constexpr uint32_t ZERO = Elem<T>::kMagic2;
-    w[e] = Elem<T>::fma2(Elem<T>::sub2(lop3_and_or(codes >> (4 * e), 0x000f000fu, Elem<T>::kMagic2), ZERO), s, m);
+struct Codes;
+template <>
+struct Codes<__nv_bfloat16> {
+  __device__ static __forceinline__ uint32_t scale(uint32_t s) { return Elem<__nv_bfloat16>::mul2(s, 0x42804280u); }
+  template <int WHICH>
+  __device__ static __forceinline__ uint32_t number(uint32_t codes, uint32_t s, uint32_t m) {
+    constexpr uint32_t MASK = WHICH == 0 ? 0x000f000fu : WHICH == 1 ? 0x00f000f0u : 0x00f0000fu;
+    constexpr uint32_t BY = WHICH == 0 ? 0x7f007f00u : WHICH == 1 ? 0x7d007d00u : 0x7d007f00u;       // 2^127, 2^123
+    return Elem<__nv_bfloat16>::fma2(Elem<__nv_bfloat16>::mul2(codes & MASK, BY), s, m);
   }
+};
+template <>
+struct Codes<__half> {
+  __device__ static __forceinline__ uint32_t scale(uint32_t s) { return s; }
+  template <int WHICH>
+  __device__ static __forceinline__ uint32_t number(uint32_t codes, uint32_t s, uint32_t m) {
+    constexpr uint32_t MASK = WHICH == 0 ? 0x000f000fu : WHICH == 1 ? 0x00f000f0u : 0x00f0000fu;
+    constexpr uint32_t BY = WHICH == 0 ? 0x3c003c00u : WHICH == 1 ? 0x2c002c00u : 0x2c003c00u;       // 1, 1 / 16
+    constexpr uint32_t LESS = WHICH == 0 ? 0xe400e400u : WHICH == 1 ? 0xd400d400u : 0xd400e400u;     // 1024, 64
+    return Elem<__half>::fma2(Elem<__half>::fma2(lop3_and_or(codes, MASK, 0x64006400u), BY, LESS), s, m);
+  }
+};
+// eight of them in their order, and by column_of
+template <typename T>
+__device__ __forceinline__ uint4 numbers_in_order(uint32_t codes, uint32_t s, uint32_t m) {
+  return make_uint4(Codes<T>::template number<2>(prmt(codes, 0u, 0x4040), s, m), Codes<T>::template number<2>(prmt(codes, 0u, 0x4141), s, m),
+                    Codes<T>::template number<2>(prmt(codes, 0u, 0x4242), s, m), Codes<T>::template number<2>(prmt(codes, 0u, 0x4343), s, m));
+}
+template <typename T>
+__device__ __forceinline__ uint4 numbers_by_column(uint32_t codes, uint32_t s, uint32_t m) {
+  return make_uint4(Codes<T>::template number<0>(codes, s, m), Codes<T>::template number<1>(codes, s, m),
+                    Codes<T>::template number<0>(codes >> 8, s, m), Codes<T>::template number<1>(codes >> 8, s, m));
 }
 
 // What lies behind the operands in shared memory
-template <int SLOTS>
+template <int SLOTS, int THREADS>
 struct Shared {
   uint64_t q_full, q_empty, kv_full[SLOTS], kv_empty[SLOTS], s_full[2], p_full[2][2], o_full[2], vote_full[2], part_full[4],
       part_empty[4], products_over, stage_full[4], stage_empty[4];
@@ -284,25 +319,26 @@ struct Shared {
 };
 
 template <typename T, int D, int GROUP>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(split_of(GROUP).threads, 1)
 paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                    const __grid_constant__ CUtensorMap map_v, const Int4Cache cache, const PagedParams p) {
   using R = Room<D, GROUP>;
-  constexpr int SLOTS = R::SLOTS, BOXES = D / 64;
+  constexpr int SLOTS = R::SLOTS, BOXES = D / 64, THREADS = split_of(GROUP).threads;
+  using Behind = Shared<SLOTS, THREADS>;
   extern __shared__ unsigned char smem_raw[];
   programmatic_begin();
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* base_ptr = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t queries = base, ring = base + 2 * R::OPERAND;
-  Shared<SLOTS>& sh = *reinterpret_cast<Shared<SLOTS>*>(base_ptr + R::BYTES);
+  Behind& sh = *reinterpret_cast<Behind*>(base_ptr + R::BYTES);
   const uint32_t bars = base + R::BYTES;
-  const uint32_t q_full = bars + offsetof(Shared<SLOTS>, q_full), q_empty = bars + offsetof(Shared<SLOTS>, q_empty),
-                 kv_full = bars + offsetof(Shared<SLOTS>, kv_full), kv_empty = bars + offsetof(Shared<SLOTS>, kv_empty),
-                 s_full = bars + offsetof(Shared<SLOTS>, s_full), p_full = bars + offsetof(Shared<SLOTS>, p_full),
-                 o_full = bars + offsetof(Shared<SLOTS>, o_full), vote_full = bars + offsetof(Shared<SLOTS>, vote_full),
-                 part_full = bars + offsetof(Shared<SLOTS>, part_full), part_empty = bars + offsetof(Shared<SLOTS>, part_empty),
-                 products_over = bars + offsetof(Shared<SLOTS>, products_over),
-                 stage_full = bars + offsetof(Shared<SLOTS>, stage_full), stage_empty = bars + offsetof(Shared<SLOTS>, stage_empty);
+  const uint32_t q_full = bars + offsetof(Behind, q_full), q_empty = bars + offsetof(Behind, q_empty),
+                 kv_full = bars + offsetof(Behind, kv_full), kv_empty = bars + offsetof(Behind, kv_empty),
+                 s_full = bars + offsetof(Behind, s_full), p_full = bars + offsetof(Behind, p_full),
+                 o_full = bars + offsetof(Behind, o_full), vote_full = bars + offsetof(Behind, vote_full),
+                 part_full = bars + offsetof(Behind, part_full), part_empty = bars + offsetof(Behind, part_empty),
+                 products_over = bars + offsetof(Behind, products_over),
+                 stage_full = bars + offsetof(Behind, stage_full), stage_empty = bars + offsetof(Behind, stage_empty);
   const uint32_t stages = base + R::OPERANDS;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -338,7 +374,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       }
     fence_mbar_init();
   }
-  if (warp == MMA_WARP) tmem_alloc(bars + offsetof(Shared<SLOTS>, tmem), 512);
+  if (warp == MMA_WARP) tmem_alloc(bars + offsetof(Behind, tmem), 512);
   programmatic_wait();
 
   // ---- this CTA's part of the line
@@ -395,7 +431,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   if (end == 0) {
     // nothing to do
   } else if (warp >= MMA_WARP) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGISTERS));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(split_of(GROUP).other));
     if (warp == LOAD_WARP) {
       // ------------------------------ loads ---------------------------------------
       Start at_first;
@@ -506,7 +542,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       constexpr uint32_t PLACES = GROUP ? R::STAGES : SLOTS;
       if (lane < min(loads, PLACES)) mbar_wait((GROUP ? stage_full : kv_full) + 8 * (last % PLACES), last / PLACES & 1, 1u << 12);
       __syncwarp();
-    } else if (GROUP > 0 && warp > LOAD_WARP) {
+    } else if (GROUP > 0 && warp > LOAD_WARP && warp <= LOAD_WARP + CONVERT_WARPS) {
       // ------------------------------ codes to numbers ----------------------------
       // A lane turns 32 codes (16 bytes of a row) into four pieces of eight numbers where the products expect them, in an order in
       // which eight lanes meet 32 banks.  Keys' elements lie as the queries' do, values' by column_of.
@@ -532,22 +568,17 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             const uint32_t codes = stages + stage * R::STAGE, scales = codes + R::CODES + (k * 32 / GROUP) * 4;
             unsigned char* to = base_ptr + (ring - base) + slot * R::OPERAND + (k >> 1) * R::BOX;
             auto convert = [&](auto values) {
-#pragma unroll 2
+#pragma unroll 1                            // (two rows at a time do not fit the registers: 1014 -> 1100 us)
               for (int r = first_row; r < first_row + ROWS; r += ROWS_AT_ONCE) {
                 const uint4 v = lds128(codes + r * R::ROW + 16 * k);
                 uint32_t pair;
                 asm volatile("ld.shared.u32 %0, [%1];" : "=r"(pair) : "r"(scales + r * (4 * R::GROUPS)));
                 if (absent >> (r >> shift) & 1) pair = 0;              // (what is there was left by others)
-                const uint32_t s = prmt(pair, pair, 0x1010), m = prmt(pair, pair, 0x3232);
+                const uint32_t s = Codes<T>::scale(prmt(pair, pair, 0x1010)), m = prmt(pair, pair, 0x3232);
                 const uint32_t words[4] = {swapped ? v.z : v.x, swapped ? v.w : v.y, swapped ? v.x : v.z, swapped ? v.y : v.w};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                  uint32_t w[4];
-                  numbers_of<T>(words[j], s, m, w);
-                  const uint4 out = decltype(values)::value
-                                        ? make_uint4(w[0], w[1], w[2], w[3])
-                                        : make_uint4(prmt(w[0], w[1], 0x5410), prmt(w[2], w[3], 0x5410), prmt(w[0], w[1], 0x7632),
-                                                     prmt(w[2], w[3], 0x7632));
+                  const uint4 out = decltype(values)::value ? numbers_by_column<T>(words[j], s, m) : numbers_in_order<T>(words[j], s, m);
                   const int piece = 4 * (k & 1) + (swapped ? j ^ 2 : j);
                   *reinterpret_cast<uint4*>(to + r * 128 + ((piece ^ (r & 7)) << 4)) = out;
                 }
@@ -666,7 +697,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     }
   } else {
     // ------------------------------ weights and results --------------------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(ROW_REGISTERS));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(split_of(GROUP).row));
     const int h = warp >> 2, quadrant = warp & 3, row = quadrant * 32 + lane;
     const uint32_t lanes = uint32_t(quadrant * 32) << 16;
     const uint32_t at_s = tmem_s + h * STEP + lanes, at_o = tmem_o + h * 128 + lanes;
@@ -912,8 +943,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
 template <typename T, int D, int GROUP>
 int launch(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v, const Int4Cache& cache,
            const PagedParams& p, int grid, cudaStream_t stream) {
+  constexpr int THREADS = split_of(GROUP).threads;
   auto kernel = paged_chunk_kernel<T, D, GROUP>;
-  constexpr int smem = 1024 + Room<D, GROUP>::BYTES + int(sizeof(Shared<Room<D, GROUP>::SLOTS>));
+  constexpr int smem = 1024 + Room<D, GROUP>::BYTES + int(sizeof(Shared<Room<D, GROUP>::SLOTS, split_of(GROUP).threads>));
   static_assert(smem <= 227 * 1024, "shared memory of a CTA");
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return cuda_status(e);
@@ -925,7 +957,7 @@ int launch(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap
     if (e != cudaSuccess) return cuda_status(e);
     registers.store(attributes.numRegs, std::memory_order_relaxed);
   }
-  if (registers.load(std::memory_order_relaxed) != LAUNCH_REGISTERS) return INTENT_B200_ERR_UNSUPPORTED;
+  if (registers.load(std::memory_order_relaxed) != split_of(GROUP).launch) return INTENT_B200_ERR_UNSUPPORTED;
   if (LaunchFacts* sink = observe_sink())
     return record_launch(sink, reinterpret_cast<const void*>(kernel), GROUP ? "paged_chunk_kernel int4 2 x 128 rows, parts joined"
                                                                                   : "paged_chunk_kernel 2 x 128 rows, parts joined", grid,
