@@ -38,20 +38,27 @@ int device_sms() {
 //    62 and 66, of up to 16384 (3.2 M) 189 and 139; 60 beside 63 of up to 4096 (1.0 M) 132 and 128; 22 beside 6 of up to 65536
 //    (5.8 M) 306 and 212; and if there is no long one 16 of 4 tokens 40 and 47, 64 of 2 of up to 300 26 and 31, 4 of 4 of up to
 //    65536 105 and 113.
+// A cache in 4 bits is read four times as fast, and more of the time goes to what both kernels do with its codes: the rows kernel's
+// tiles are worth it for more rows.  us for the 64 sequences of up to 4000 tokens, 1 / 4 / 8 / 16 new ones each, groups of 64:
+// rows 41 / 67 / 116 / 211, chunk 146 / 147 / 149 / 148; heads of 64 28 / 39 / 69 / 114, chunk 130 throughout; 8 of up to 16000, 4 / 8
+// / 16: rows 41 / 71 / 122, chunk 82.  The launch that may find nothing to do costs 12 us there (64 of 4 tokens: 67 and 79).
 struct Choice {
   int tile_rows;           // of the rows kernel; 0: it is not needed
   int few;                 // rows up to which a sequence is its
   bool chunks;             // the chunk kernel is needed
 };
-Choice choose(int64_t tokens, int64_t batch, int64_t group, int64_t dim, int64_t capacity, int64_t window, bool may_chunk) {
+Choice choose(int64_t tokens, int64_t batch, int64_t group, int64_t dim, int64_t capacity, int64_t window, bool may_chunk, bool int4) {
   constexpr int FEW = 16, MANY = 8, MOST = 1 << 20;
+  // rows per sequence, on average, up to which a call is the rows kernel's; a sequence's rows up to which it is beside others
+  const int all_few = int4 ? (dim == 64 ? 4 * FEW : 2 * FEW) : dim == 64 ? 2 * FEW : FEW;
+  const int one_few = int4 ? (dim == 64 ? 4 * FEW : 3 * FEW) : 2 * FEW;
   const int64_t rows = tokens * group, most = tokens < batch ? rows : (tokens - batch + 1) * group;
-  const bool usual = rows <= (dim == 64 ? 2 * FEW : FEW) * batch;
+  const bool usual = rows <= all_few * batch;
   const bool narrow = rows <= FEW / 2 * batch || (!usual && group <= FEW / 2);
   Choice c;
   const int64_t reach = window > 0 ? std::min(capacity, window + most / group) : capacity;   // tokens that its rows may walk through
-  c.chunks = may_chunk && !(usual && (most <= 2 * FEW || most * reach <= MOST));
-  c.few = !c.chunks ? std::numeric_limits<int>::max() : usual ? 2 * FEW : batch < MANY ? 0 : narrow ? FEW / 2 : FEW;
+  c.chunks = may_chunk && !(usual && (most <= one_few || most * reach <= MOST));
+  c.few = !c.chunks ? std::numeric_limits<int>::max() : usual ? one_few : batch < MANY ? 0 : narrow ? FEW / 2 : FEW;
   if (c.few < group) c.few = 0;            // (no sequence has so few)
   c.tile_rows = c.few == 0 ? 0 : narrow ? FEW / 2 : FEW;
   return c;
@@ -115,7 +122,7 @@ int attend(const View3& q, const CacheViews& cache, const View2& table, const Vi
   while ((int64_t(1) << p.page_shift) < page) ++p.page_shift;
   p.window = window < p.capacity ? window : 0;   // (a query that sees as many tokens as there may be sees all)
   p.scale = scale * 1.44269504f;         // log2(e): the exponentials are powers of two
-  const Choice choice = choose(tokens, batch, p.group, dim, p.capacity, p.window, offsets && paged_chunk_takes(p));
+  const Choice choice = choose(tokens, batch, p.group, dim, p.capacity, p.window, offsets && paged_chunk_takes(p), int4);
   p.few = choice.few;
   if (!workspace || workspace_bytes < workspace_bytes_of(dim, choice.chunks)) return INTENT_B200_ERR_WORKSPACE;
   if (!aligned16(workspace)) return INTENT_B200_ERR_LAYOUT;
@@ -151,14 +158,27 @@ int attend(const View3& q, const CacheViews& cache, const View2& table, const Vi
 extern "C" int64_t intent_b200_paged_attention_workspace_bytes(int64_t dim, int32_t single) {
   return ib200::workspace_bytes_of(dim, !single);
 }
-// The same for one call of paged_attention: with few rows it needs as much as single tokens do.
-extern "C" int64_t intent_b200_paged_attention_call_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t k_heads,
-                                                                    int64_t dim, int64_t capacity, int64_t window) {
+namespace ib200 {
+namespace {
+int64_t call_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t k_heads, int64_t dim, int64_t capacity,
+                             int64_t window, bool int4) {
   if (tokens <= 0 || batch <= 0 || k_heads <= 0 || q_heads < k_heads || q_heads > 4096 || capacity < 0 || window < 0) return 0;
   const int64_t group = q_heads / k_heads;
-  ib200::PagedParams p = {};
+  PagedParams p = {};
   p.tokens = p.q_heads = 1, p.group = int(group);      // (what its strides may rule out asks for less)
-  return ib200::workspace_bytes_of(dim, ib200::choose(tokens, batch, group, dim, capacity, window, ib200::paged_chunk_takes(p)).chunks);
+  return workspace_bytes_of(dim, choose(tokens, batch, group, dim, capacity, window, paged_chunk_takes(p), int4).chunks);
+}
+}  // namespace
+}  // namespace ib200
+
+// The same for one call of paged_attention (of paged_attention_int4): with few rows it needs as much as single tokens do.
+extern "C" int64_t intent_b200_paged_attention_call_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t k_heads,
+                                                                    int64_t dim, int64_t capacity, int64_t window) {
+  return ib200::call_workspace_bytes(tokens, batch, q_heads, k_heads, dim, capacity, window, false);
+}
+extern "C" int64_t intent_b200_paged_attention_int4_call_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t k_heads,
+                                                                         int64_t dim, int64_t capacity, int64_t window) {
+  return ib200::call_workspace_bytes(tokens, batch, q_heads, k_heads, dim, capacity, window, true);
 }
 
 // Reads the status word at the head of a workspace after synchronising `stream`, and clears it.

@@ -996,15 +996,15 @@ def _paged_workspace_query(name, arguments):
 
     from .runtime import native
 
-    query = native.library()[f"intent_b200_paged_attention_{name}"]
+    query = native.library()[f"intent_b200_{name}"]
     query.restype, query.argtypes = ctypes.c_int64, [ctypes.c_int64] * arguments
     return query
 
 
-def _paged_workspace_bytes(d, single, window):
+def _paged_workspace_bytes(d, single, window, stem):
     if single:
-        return int(_paged_workspace_query("workspace_bytes", 2)(d["D"], 1))
-    query = _paged_workspace_query("call_workspace_bytes", 7)
+        return int(_paged_workspace_query("paged_attention_workspace_bytes", 2)(d["D"], 1))
+    query = _paged_workspace_query(f"{stem}_call_workspace_bytes", 7)
     return int(query(d["T"], d["B"], d["HQ"], d["HK"], d["D"], d["W"] * d["PAGE"], window))
 
 
@@ -1044,7 +1044,7 @@ def _lower_paged(c, device, *, single, bits=16):
     return NativeProgram(interface=PublicInterface(tuple(views), dimension_rules=rules), device=device,
                          entry_name=f"intent_b200_{stem}_{act.name}",
                          constants=((group,) if group else ()) + (factor, window),
-                         workspace=lambda d: _paged_workspace_bytes(d, single, window),
+                         workspace=lambda d: _paged_workspace_bytes(d, single, window, stem),
                          empty=lambda d: d["B"] == 0 or (not single and d["T"] == 0),
                          workspace_status="intent_b200_paged_attention_workspace_status")
 
