@@ -213,11 +213,16 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
     }
   };
   uint32_t qf[NT][CHUNKS][4];            // queries as B fragments: elements 32 c + 8 (lane % 4) + {0, 4}, {1, 5}, {2, 6}, {3, 7}
-  float q_sum[NT][2][GROUPS];            // of this thread's rows, in the scores' unit
+  // Sums of a group's queries in the scores' unit, which its minimum is multiplied with: of this thread's rows (f16), or in two
+  // bf16 parts as a B fragment, elements 0 .. GROUPS - 1 the rounded sums and the next ones what that left over.
+  constexpr bool BY_PRODUCT = std::is_same<T, __nv_bfloat16>::value;
+  float q_sum[NT][2][GROUPS];
+  uint32_t q_parts[NT];
   float o[NT][CHUNKS][2][4];             // sums of codes: elements 32 c + 4 (lane / 4) + 2 t (+ 1, times 16) of rows 2 (lane % 4) (+ 1)
   float eights[NT][GROUPS][4];           // sums of the weights that the codes are multiplied with, of the same rows (twice)
   float middle[NT][2][GROUPS];           // sums of weight times minimum (and 8 scales), of this thread's tokens
-  float top[NT][2], weight_sum[NT][2];
+  float top[NT][2];
+  uint64_t weight_sum[NT];               // of both rows
   int position[NT][2];                   // of this thread's rows; -1 where there is none
   int least = 0, most = 0;               // positions of the tile's first and last row
   const float scale = p.scale / Codes<T>::UNIT_OF_SCORES;
@@ -252,21 +257,34 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
       for (int g = 0; g < GROUPS; ++g) {
         sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
         sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
+        sums[g] *= Codes<T>::UNIT_OF_SCORES;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          q_sum[nt][e][g] = __shfl_sync(0xffffffffu, sums[g], 8 * (lane & 3) + 4 * e) * Codes<T>::UNIT_OF_SCORES;
+          if (!BY_PRODUCT) q_sum[nt][e][g] = __shfl_sync(0xffffffffu, sums[g], 8 * (lane & 3) + 4 * e);
           middle[nt][e][g] = 0.f;
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) eights[nt][g][e] = 0.f;
+      }
+      if (BY_PRODUCT) {
+        uint32_t parts[2 * GROUPS];
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+          parts[g] = Elem<Wide>::from_float(sums[g]);
+          parts[GROUPS + g] = Elem<Wide>::from_float(sums[g] - Elem<Wide>::to_float(uint16_t(parts[g])));
+        }
+        q_parts[nt] = 0;
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i)
+          if ((lane & 3) == i) q_parts[nt] = parts[2 * i] | (parts[2 * i + 1] << 16);
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int of_thread = tile_row + nt * 8 + 2 * (lane & 3) + e;
         position[nt][e] = of_thread < work.s.rows ? work.s.first + of_thread / p.group : -1;
         top[nt][e] = -infinity;
-        weight_sum[nt][e] = 0.f;
       }
+      weight_sum[nt] = 0;
     }
   };
   if (first_place < end) {
@@ -319,18 +337,37 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
               Elem<T>::mma16816(x[nt][c / OF_GROUP], a & LOW, b & LOW, Codes<T>::odd(a), Codes<T>::odd(b), qf[nt][c][2 * pair],
                                 qf[nt][c][2 * pair + 1]);
           }
+        Words<GROUPS> w[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) w[h] = lds<GROUPS>(of_keys + (16 * m + 8 * h) * (GROUPS * 4));
+        if (BY_PRODUCT) {
+          // minima of tokens 16 m + lane / 4 (+ 8): elements 2 (lane % 4) (+ 1) are groups, in turn
+          uint32_t minima[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            minima[h] = GROUPS == 1   ? prmt(w[h].w[0], w[h].w[0], 0x3232)
+                        : GROUPS == 2 ? prmt(w[h].w[0], w[h].w[GROUPS > 1], 0x7632)
+                                      : (lane & 1) ? prmt(w[h].w[GROUPS / 2], w[h].w[GROUPS - 1], 0x7632)
+                                                   : prmt(w[h].w[0], w[h].w[GROUPS > 1], 0x7632);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[nt][m][e] = 0.f;
+            Elem<T>::mma16816(s[nt][m], minima[0], minima[1], 0u, 0u, q_parts[nt], 0u);
+          }
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const Words<GROUPS> w = lds<GROUPS>(of_keys + (16 * m + 8 * h) * (GROUPS * 4));
 #pragma unroll
           for (int g = 0; g < GROUPS; ++g) {
-            const float by = Elem<T>::to_float(uint16_t(w.w[g])), from = Elem<T>::to_float(uint16_t(w.w[g] >> 16));
+            const float by = Elem<T>::to_float(uint16_t(w[h].w[g])), from = Elem<T>::to_float(uint16_t(w[h].w[g] >> 16));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                const float sum = fmaf(from, q_sum[nt][e][g], g == 0 ? 0.f : s[nt][m][2 * h + e]);
-                s[nt][m][2 * h + e] = fmaf(by, x[nt][g][2 * h + e], sum);
+                float& sum = s[nt][m][2 * h + e];
+                if (!BY_PRODUCT) sum = fmaf(from, q_sum[nt][e][g], g == 0 ? 0.f : sum);
+                sum = fmaf(by, x[nt][g][2 * h + e], sum);
               }
           }
         }
@@ -376,10 +413,10 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
             const float now = fmaxf(top[nt][e], here[nt][e] * scale);
             factor[e] = exp2_fast(top[nt][e] - (now == -infinity ? 0.f : now));
             top[nt][e] = now;
-            weight_sum[nt][e] *= factor[e];
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) middle[nt][e][g] *= factor[e];
           }
+          weight_sum[nt] = mul_two(weight_sum[nt], two(factor[0], factor[1]));
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
 #pragma unroll
@@ -392,11 +429,11 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
         }
       }
       // weights, 2^64 times what they are
-      float origin[NT][2];
+      const uint64_t scales = two(scale, scale);
+      uint64_t origins[NT];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) origin[nt][e] = 64.f - (top[nt][e] == -infinity ? 0.f : top[nt][e]);
+        origins[nt] = two(64.f - (top[nt][0] == -infinity ? 0.f : top[nt][0]), 64.f - (top[nt][1] == -infinity ? 0.f : top[nt][1]));
       auto add_values = [&](auto whole) {
 #pragma unroll
         for (int m = 0; m < PARTS; ++m) {
@@ -404,10 +441,10 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float w = exp2_fast(fmaf(s[nt][m][e], scale, origin[nt][e & 1]));
-              s[nt][m][e] = w;
-              weight_sum[nt][e & 1] += w;
+            for (int e = 0; e < 4; e += 2) {
+              const float2 power = apart(fma_two(two(s[nt][m][e], s[nt][m][e + 1]), scales, origins[nt]));
+              s[nt][m][e] = exp2_fast(power.x), s[nt][m][e + 1] = exp2_fast(power.y);
+              weight_sum[nt] = add_two(weight_sum[nt], two(s[nt][m][e], s[nt][m][e + 1]));
             }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -490,7 +527,7 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int r = nt * 8 + 2 * (lane & 3) + e;
-          float sum_all = weight_sum[nt][e];
+          float sum_all = e ? apart(weight_sum[nt]).y : apart(weight_sum[nt]).x;
 #pragma unroll
           for (int d = 4; d < 32; d *= 2) sum_all += __shfl_xor_sync(0xffffffffu, sum_all, d);
           sum_all *= 0x1p-64f;
