@@ -245,15 +245,16 @@ __device__ __forceinline__ void key_rows(const RotateParams& p, uint32_t block) 
   }
 }
 
-// k_blocks blocks of keys, as many of values, the others of queries (p.k_heads is 0 in `queries`)
+// Blocks of keys and as many of values, in turn, spread evenly among those of queries (p.k_heads is 0 in `queries`): keys are bound by
+// instructions, queries by HBM.  `share`: of the blocks, keys' and values', in 2^-32, rounded up.
 template <typename T, int D, bool NORM, bool NEIGHBOURS, int ROWS, int GROUP>
-__global__ void __launch_bounds__(THREADS, 4) append_int4_kernel(const RotateParams p, const RotateParams queries, uint32_t k_blocks) {
-  constexpr int K_ROWS = ROWS == 1 ? 1 : CACHE_ROWS;
+__global__ void __launch_bounds__(THREADS, 4) append_int4_kernel(const RotateParams p, const RotateParams queries, uint32_t share) {
+  constexpr int OF_CACHE = ROWS == 1 ? 1 : CACHE_ROWS;
   programmatic_begin();
-  const uint32_t block = blockIdx.x;
-  if (block < k_blocks) key_rows<T, D, NORM, NEIGHBOURS, K_ROWS, GROUP>(p, block);
-  else if (block < 2 * k_blocks) value_rows<T, D, K_ROWS, GROUP>(p, block - k_blocks);
-  else rotate_rows<T, D, NORM, NEIGHBOURS, false, ROWS>(queries, block - 2 * k_blocks);
+  const uint32_t before = __umulhi(blockIdx.x, share);             // keys' and values' blocks ahead of this one
+  if (__umulhi(blockIdx.x + 1, share) == before) rotate_rows<T, D, NORM, NEIGHBOURS, false, ROWS>(queries, blockIdx.x - before);
+  else if (before % 2 == 0) key_rows<T, D, NORM, NEIGHBOURS, OF_CACHE, GROUP>(p, before / 2);
+  else value_rows<T, D, OF_CACHE, GROUP>(p, before / 2);
 }
 
 template <typename T, int D, bool NORM, int ROWS, int GROUP>
@@ -261,16 +262,17 @@ int launch(const RotateParams& p, bool neighbours, cudaStream_t stream) {
   auto kernel = neighbours ? append_int4_kernel<T, D, NORM, true, ROWS, GROUP> : append_int4_kernel<T, D, NORM, false, ROWS, GROUP>;
   constexpr uint32_t PER_CTA = THREADS / (D / 8);
   static_assert(D / 8 == D / (2 * PIECE_OF), "lanes of a row of queries");
-  constexpr uint32_t K_ROWS = ROWS == 1 ? 1 : CACHE_ROWS;
-  const uint32_t k_blocks = (p.tokens * ((p.k_heads + K_ROWS - 1) / K_ROWS) + PER_CTA - 1) / PER_CTA;
+  constexpr uint32_t OF_CACHE = ROWS == 1 ? 1 : CACHE_ROWS;
+  const uint32_t k_blocks = (p.tokens * ((p.k_heads + OF_CACHE - 1) / OF_CACHE) + PER_CTA - 1) / PER_CTA;
   const uint32_t q_blocks = (p.tokens * ((p.q_heads + ROWS - 1) / ROWS) + PER_CTA - 1) / PER_CTA, grid = 2 * k_blocks + q_blocks;
+  const uint32_t share = uint32_t((uint64_t(2 * k_blocks) << 32) / grid) + 1;
   RotateParams queries = p;
   queries.k_heads = 0;
   if (LaunchFacts* sink = observe_sink())
     return record_launch(sink, reinterpret_cast<const void*>(kernel),
                          ROWS == 1 ? "append_int4_kernel a row per group" : "append_int4_kernel several rows per group", int(grid), THREADS,
                          0, 1);
-  const cudaError_t e = launch_programmatic(kernel, dim3(grid), dim3(THREADS), 0, stream, 1, p, queries, k_blocks);
+  const cudaError_t e = launch_programmatic(kernel, dim3(grid), dim3(THREADS), 0, stream, 1, p, queries, share);
   if (e != cudaSuccess) return cuda_status(e);
   note_launch();
   return launch_status();
