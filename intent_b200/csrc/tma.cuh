@@ -23,7 +23,12 @@ inline EncodeTiledFn encode_tiled_fn() {
       p = nullptr;
     return reinterpret_cast<EncodeTiledFn>(p);
   }();
-  return fn;
+  // A map is encoded in the calling thread's context, which a thread has not before its first call that needs one.
+  thread_local const bool bound = [] {
+    int device = 0;
+    return cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess;
+  }();
+  return bound ? fn : nullptr;
 }
 
 // Row-major 2-D tensor [rows][cols]; `pitch_bytes` between rows (multiple of 16);
