@@ -124,3 +124,39 @@ def test_reading_pages_of_16_bits():
         flat = whole.transpose(1, 2).flatten(0, 1)
         assert torch.equal(got, flat[step.slots[3:39]])
     assert store.read(0, "a", 40)[0].shape == (0, 2, 64)
+
+
+def test_shapes_are_inferred_without_a_device():
+    """What fake tensors go through."""
+    import torch
+
+    def empty(*shape, dtype=torch.bfloat16):
+        return torch.empty(shape, dtype=dtype, device="meta")
+
+    caches = [empty(7, 2, 16, 64, dtype=torch.uint8), empty(7, 2, 16, 4)] * 2
+    caches = [c.clone() for c in caches]
+    program = {name: ib.compile(getattr(ib.programs, name), resolve_target=False).runtime for name in PROGRAMS}
+    ints = [empty(n, dtype=torch.int32) for n in (5, 4, 3)]
+    slots = empty(5, dtype=torch.int64)
+    keys, values = program["paged_kv_read_int4"].infer_outputs((slots, *caches))
+    assert keys.shape == values.shape == (5, 2, 128) and keys.dtype == torch.bfloat16
+    q, k = empty(5, 8, 128), empty(5, 2, 128)
+    out = program["paged_kv_append_int4"].infer_outputs((q, k, k.clone(), ints[0], slots, empty(9, 64, dtype=torch.float32), empty(128),
+                                                         empty(128), *caches))
+    assert out.shape == (5, 8, 128)
+    pages = empty(3, 4, dtype=torch.int32)
+    assert program["paged_attention_int4"].infer_outputs((q, *caches, pages, ints[1], ints[2])).shape == (5, 8, 128)
+    assert program["paged_decode_attention_int4"].infer_outputs((q[:3], *caches, pages, ints[2])).shape == (3, 8, 128)
+
+
+def test_workspace_of_a_call():
+    """As of a cache of 16 bits: the parts of chunks are asked for by calls that may have chunks only."""
+    query = ib.compile(ib.programs.paged_attention_int4, resolve_target=False).runtime._workspace_spec
+    single = ib.compile(ib.programs.paged_decode_attention_int4, resolve_target=False).runtime._workspace_spec
+    sizes = {"HQ": 32, "HK": 8, "D": 128, "PAGE": 64, "W": 512}
+    few = single({**sizes, "B": 64})
+    assert few < 4 << 20
+    for T, B in ((1, 1), (64, 64), (8, 1), (75, 64)):
+        assert query({**sizes, "T": T, "B": B}) == few
+    for T, B in ((33, 1), (1000, 64), (4096, 1), (1 << 20, 1)):
+        assert query({**sizes, "T": T, "B": B}) > 40 << 20
