@@ -137,7 +137,8 @@ int attend(const View3& q, const CacheViews& cache, const View2& table, const Vi
   PagedParams chunk = p;
   const Int4Cache codes = {k_cache.p, int4 ? cache.k_scales->p : nullptr, v_cache.p, int4 ? cache.v_scales->p : nullptr, cache.group};
   if (choice.tile_rows > 0) {
-    const int status = int4 ? paged_rows_int4<T>(p, dim, choice.tile_rows, codes, grid, stream)
+    const int four = tokens * p.group <= 4 * batch ? 4 : choice.tile_rows;     // (rows of a tile; its parts are laid out as of eight)
+    const int status = int4 ? paged_rows_int4<T>(p, dim, four, codes, grid, stream)
                             : paged_rows<T>(p, dim, choice.tile_rows, k_cache.p, v_cache.p, grid, stream);
     if (status != INTENT_B200_OK) return status;
   }
