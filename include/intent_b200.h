@@ -613,8 +613,10 @@ INTENT_B200_API int intent_b200_paged_kv_read_int4_bf16(
  * share one.  Bytes 0..3: INTENT_B200_ERR_TIMEOUT of a bounded wait that gave up, INTENT_B200_ERR_SHAPE where a multiprocessor
  * would have 2^30 or more steps of 128 tokens to go through (many minutes; the rows are not written then);
  * ..._workspace_status reads and clears it.  The same call gives the same bits.
- * _int4: over a cache in 4 bits as above, of the values m + s * n; the workspace is the same (..._int4_call_workspace_bytes).  The factor of the scores is at most 2^50
- * there, bf16 queries below 2^67 and scales of values below 2^55 in magnitude (beyond that a row may be NaN).
+ * _int4: over a cache in 4 bits as above, of the values m + s * n; the workspace is the same (..._int4_call_workspace_bytes).  Chunks of
+ * many rows take these values rounded to the type, as reading them back gives them; single tokens and few rows take them as they
+ * are.  The factor of the scores is at most 2^50 there, bf16 queries are below 2^67 and scales of values below 2^55 in magnitude
+ * (beyond that a row may be NaN).  A group whose scale or minimum is no number makes the rows that see its token NaN, and no others.
  * ------------------------------------------------------------------------ */
 INTENT_B200_API int intent_b200_paged_attention_f16(INTENT_B200_VIEW3(q), INTENT_B200_VIEW4(k_cache), INTENT_B200_VIEW4(v_cache),
                                                  INTENT_B200_VIEW2(page_table), INTENT_B200_VIEW1(query_offsets),

@@ -12,7 +12,11 @@
 //
 // A lane has eight neighbouring elements of a row.  The partners of a key's elements in pairs (i, i + R/2) are another lane's; it reads
 // them once more from the first-level cache and works out its own half of each pair.  Blocks have keys, values or queries; in
-// calls of many rows four rows of a token share what does not depend on the row.
+// calls of many rows two rows of keys or values, and four of queries, share what does not depend on the row.
+//
+// Measured on one B200: 8192 tokens, 32 + 8 + 8 heads of 128, norm, bf16, with paged_kv_read_int4 of them 59 us (floor 33), of which the
+// read is 9, queries take 24 alone, keys 18 and values 8: bound by instructions, two thirds of the issue slots.  With four rows
+// of keys and 102 registers 76; keys' blocks ahead of the others 63.  (Keys in f32 took as long.)
 #include "common.cuh"
 #include "paged.cuh"
 #include "rotate.cuh"
