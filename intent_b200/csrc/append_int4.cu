@@ -41,6 +41,12 @@ __device__ __forceinline__ float largest_of(float a, float b) {
 __device__ __forceinline__ double least_of(double a, double b) { return a < b ? a : b; }
 __device__ __forceinline__ double largest_of(double a, double b) { return a > b ? a : b; }
 
+// A number added to this is rounded to a whole one in the lowest bits, from which code_of takes it, cut to 0 .. 15
+constexpr float WHOLE = 12582912.f;
+__device__ __forceinline__ uint32_t code_of(float sum) {
+  return uint32_t(__viaddmin_s32_relu(__float_as_int(sum), -__float_as_int(WHOLE), 15));
+}
+
 // The quotients of eight numbers by a scale s, rounded to whole numbers from 0 to 15.  The product with the rounded reciprocal gets its
 // remainder added, which makes it the quotient as a division rounds it (P. Markstein, Computation of elementary functions on the
 // IBM RISC System/6000 processor, 1990).  HALVES: whether quotients may lie in the middle between two numbers; those of keys that
@@ -54,8 +60,7 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float s, float
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const float d = fmaf(x[e], by, origin), q = d * inverse;
-    const float n = fminf(fmaxf(fmaf(fmaf(-q, divisor, d), inverse, q), 0.f), 15.f);
-    codes += (__float_as_uint(n + 12582912.f) - 0x4b400000u) << (4 * e);
+    codes |= code_of(fmaf(fmaf(-q, divisor, d), inverse, q) + WHOLE) << (4 * e);
   }
   return codes;
 }
@@ -72,8 +77,8 @@ __device__ __forceinline__ uint32_t codes_of(const double (&x)[8], float scale, 
     } else {
       quotient = fma(x[e], inverse, origin);
     }
-    const int n = __double2loint(quotient + 6755399441055744.);
-    codes |= uint32_t(min(max(n, 0), 15)) << (4 * e);
+    quotient = quotient < 0. ? 0. : quotient > 15. ? 15. : quotient;     // (where a minimum's rounding is many scales, it may be far out)
+    codes |= uint32_t(__double2loint(quotient + 6755399441055744.)) << (4 * e);
   }
   return codes;
 }
@@ -161,30 +166,18 @@ __device__ __forceinline__ void value_rows(const RotateParams& p, uint32_t block
   }
 }
 
-template <typename T, int D, bool NORM, bool NEIGHBOURS, int ROWS, int GROUP>
-__device__ __forceinline__ void key_rows(const RotateParams& p, uint32_t block) {
-  constexpr int LANES = D / 8;
-  const int j = threadIdx.x % LANES, half = p.rotary_dim / 2;
-  const bool turned = 8 * j < p.rotary_dim, upper = 8 * j >= half;
-  const int mate = NEIGHBOURS || !turned ? 8 * j : upper ? 8 * j - half : 8 * j + half;    // first of the partners
-  Group<D, ROWS> group(p, block);
-  const uint16_t* from = p.k + group.token * p.k_token + group.first * p.k_head;
-  programmatic_wait();
-  uint4 raw[ROWS], partners[NEIGHBOURS ? 1 : ROWS];
-#pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    const bool there = i < group.rows;
-    raw[i] = there ? __ldg(reinterpret_cast<const uint4*>(from + i * p.k_head + 8 * j)) : make_uint4(0, 0, 0, 0);
-    if (!NEIGHBOURS)
-      partners[i] = there && turned ? __ldg(reinterpret_cast<const uint4*>(from + i * p.k_head + mate)) : make_uint4(0, 0, 0, 0);
-  }
-  const int64_t position = __ldg(p.positions + group.token);
-  const bool known = position >= 0 && position < p.table_rows;
-  group.find(p);
-
-  // What an element is multiplied with, and what its partner is for it: weight times cosine, weight times (minus) sine.
-  double own[8], cross[8];
-  {
+// What a lane's eight elements of a key are multiplied with, and what their partners are for them: weight times cosine, weight times
+// (minus) sine.
+template <typename T, int D, bool NORM, bool NEIGHBOURS, typename F>
+struct Turn {
+  F own[8], cross[8];
+  int mate;                            // first of the partners
+  bool turned;
+  __device__ __forceinline__ Turn(const RotateParams& p, int j, int64_t position) {
+    const int half = p.rotary_dim / 2;
+    const bool upper = 8 * j >= half, known = position >= 0 && position < p.table_rows;
+    turned = 8 * j < p.rotary_dim;
+    mate = NEIGHBOURS || !turned ? 8 * j : upper ? 8 * j - half : 8 * j + half;
     constexpr int ANGLES = NEIGHBOURS ? 4 : 8;
     float c[ANGLES], s[ANGLES];
 #pragma unroll
@@ -209,42 +202,133 @@ __device__ __forceinline__ void key_rows(const RotateParams& p, uint32_t block) 
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int pair = NEIGHBOURS ? e / 2 : e;
-      const double cosine = c[pair], sine = (NEIGHBOURS ? e & 1 : upper) ? s[pair] : -s[pair];
-      own[e] = NORM ? cosine * double(Elem<T>::to_float(uint16_t(w[e / 2] >> (16 * (e & 1))))) : cosine;
+      const F cosine = c[pair], sine = (NEIGHBOURS ? e & 1 : upper) ? s[pair] : -s[pair];
+      own[e] = NORM ? cosine * F(Elem<T>::to_float(uint16_t(w[e / 2] >> (16 * (e & 1))))) : cosine;
       const uint32_t of_partner = NEIGHBOURS ? w[e / 2] >> (16 * (1 - (e & 1))) : v[e / 2] >> (16 * (e & 1));
-      cross[e] = NORM ? sine * double(Elem<T>::to_float(uint16_t(of_partner))) : sine;
+      cross[e] = NORM ? sine * F(Elem<T>::to_float(uint16_t(of_partner))) : sine;
     }
   }
+  // the elements of a row before its norm's factor, and their partners
+  __device__ __forceinline__ void elements(const uint4& raw, const uint4& partners, F (&x)[8], F (&y)[8]) const {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w}, v[4] = {partners.x, partners.y, partners.z, partners.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = Elem<T>::to_float(uint16_t(w[e / 2] >> (16 * (e & 1))));
+      y[e] = Elem<T>::to_float(uint16_t(NEIGHBOURS ? w[e / 2] >> (16 * (1 - (e & 1))) : v[e / 2] >> (16 * (e & 1))));
+      if (NEIGHBOURS && !turned) y[e] = 0;           // (what is not rotated has none, and may be infinite)
+    }
+  }
+};
+
+__device__ __forceinline__ uint4 load_eight(const uint16_t* from, bool there) {
+  return there ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0, 0, 0, 0);
+}
+
+// A lane's part of a key in 64 bits, from its row in memory: codes in the lower half, scales in the upper.  (Few rows come here, so
+// it is a function of its own.)
+template <typename T, int D, bool NORM, bool NEIGHBOURS, int GROUP>
+__device__ __noinline__ uint64_t key_in_64_bits(const RotateParams& p, const uint16_t* row, bool there, int64_t position) {
+  constexpr int LANES = D / 8;
+  const int j = threadIdx.x % LANES;
+  const Turn<T, D, NORM, NEIGHBOURS, double> turn(p, j, position);
+  double x[8], y[8];
+  turn.elements(load_eight(row + 8 * j, there), load_eight(row + turn.mate, there && turn.turned && !NEIGHBOURS), x, y);
+  double scale = 1.;
+  if (NORM) {
+    double sum = x[0] * x[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) sum = fma(x[e], x[e], sum);
+#pragma unroll
+    for (int d = LANES / 2; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    scale = rsqrt(sum * (1. / D) + double(p.eps));
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = fma(x[e], turn.own[e], y[e] * turn.cross[e]) * scale;
+  uint32_t scales;
+  const uint32_t codes = quantise<T, GROUP, !NORM>(y, scales);
+  return codes | uint64_t(scales) << 32;
+}
+
+// Keys in f32 first.  An element is then off by at most DELTA = 2^-20 of |x own| + |partner cross|, times the norm's factor r (the
+// sum of squares and r up to 2^-21, four roundings of 2^-24), which is at most (largest |own| + |cross|) times sqrt(D), as r |x| is no more
+// than that, or times the row's largest |x| where there is no norm.  Where the minimum's or the scale's rounding, or a code's, could
+// be another within that, the warp's rows are worked out in 64 bits; so are those with something that is no number, with equal
+// elements, and near the ends of the type.
+template <typename T, int D, bool NORM, bool NEIGHBOURS, int ROWS, int GROUP>
+__device__ __forceinline__ void key_rows(const RotateParams& p, uint32_t block) {
+  constexpr int LANES = D / 8;
+  const int j = threadIdx.x % LANES;
+  Group<D, ROWS> group(p, block);
+  const uint16_t* from = p.k + group.token * p.k_token + group.first * p.k_head;
+  programmatic_wait();
+  const int64_t position = __ldg(p.positions + group.token);
+  const Turn<T, D, NORM, NEIGHBOURS, float> turn(p, j, position);
+  uint4 raw[ROWS], partners[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    raw[i] = load_eight(from + i * p.k_head + 8 * j, i < group.rows);
+    partners[i] = load_eight(from + i * p.k_head + turn.mate, i < group.rows && turn.turned && !NEIGHBOURS);
+  }
+  group.find(p);
+  float most = 0.f;                    // of |own| + |cross|, in the row
+#pragma unroll
+  for (int e = 0; e < 8; ++e) most = largest_of(most, fabsf(turn.own[e]) + fabsf(turn.cross[e]));
+#pragma unroll
+  for (int d = 1; d < LANES; d *= 2) most = largest_of(most, __shfl_xor_sync(0xffffffffu, most, d));
+  const float of_row = most * (NORM ? (D == 128 ? 11.4f : 8.1f) * 0x1p-20f : 0x1p-20f);
 
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
-    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-    double x[8], y[8];
+    float x[8], y[8], delta = of_row;
+    turn.elements(raw[i], partners[i], x, y);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = Elem<T>::to_float(uint16_t(w[e / 2] >> (16 * (e & 1))));
-    double scale = 1.;
+    for (int e = 0; e < 8; ++e) y[e] = fmaf(x[e], turn.own[e], y[e] * turn.cross[e]);
     if (NORM) {
-      double sum = x[0] * x[0];
+      float sum = x[0] * x[0];
 #pragma unroll
-      for (int e = 1; e < 8; ++e) sum = fma(x[e], x[e], sum);
+      for (int e = 1; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
 #pragma unroll
       for (int d = LANES / 2; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      scale = rsqrt(sum * (1. / D) + double(p.eps));
-    }
-    if (NEIGHBOURS) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = turned ? fma(x[e], own[e], x[e ^ 1] * cross[e]) : x[e] * own[e];
-    } else {
-      const uint32_t v[4] = {partners[i].x, partners[i].y, partners[i].z, partners[i].w};
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        y[e] = fma(x[e], own[e], double(Elem<T>::to_float(uint16_t(v[e / 2] >> (16 * (e & 1))))) * cross[e]);
-    }
-    if (NORM)
+      const float scale = rsqrtf(sum * (1.f / D) + p.eps);
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] *= scale;
-    uint32_t scales;
-    const uint32_t codes = quantise<T, GROUP, !NORM>(y, scales);
+    } else {
+      float size = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) size = largest_of(size, fabsf(x[e]));
+#pragma unroll
+      for (int d = 1; d < LANES; d *= 2) size = largest_of(size, __shfl_xor_sync(0xffffffffu, size, d));
+      delta *= size;
+    }
+    float low = y[0], high = y[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) low = least_of(y[e], low), high = largest_of(y[e], high);
+#pragma unroll
+    for (int d = 1; d < GROUP / 8; d *= 2) {
+      low = least_of(low, __shfl_xor_sync(0xffffffffu, low, d));
+      high = largest_of(high, __shfl_xor_sync(0xffffffffu, high, d));
+    }
+    const float step = (high - low) * (1.f / 15.f), of_step = fmaf(delta, 2.1f / 15.f, step * 0x1p-21f);
+    uint32_t scales = Elem<T>::pack2(step - of_step, low - delta);
+    const float s = Elem<T>::to_float(uint16_t(scales)), m = Elem<T>::to_float(uint16_t(scales >> 16));
+    bool sure = scales == Elem<T>::pack2(step + of_step, low + delta) && s > 0x1p-60f && s < 0x1p60f &&
+                Elem<T>::to_float(Elem<T>::from_float(fmaf(15.f, s, m))) < __int_as_float(0x7f800000);
+    // (a quotient is off by DELTA's share and a few roundings of numbers up to 16)
+    const float inverse = __fdividef(1.f, s), most_off = 0.5f - fmaf(delta, inverse, 0x1p-17f);
+    float off = 0.f;                   // farthest from a whole number
+    uint32_t codes = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float q = (y[e] - m) * inverse, sum = q + WHOLE;
+      off = largest_of(off, fabsf(q - (sum - WHOLE)));
+      codes |= code_of(sum) << (4 * e);
+    }
+    // (and none is so far out, by the minimum's rounding, that its whole number is)
+    sure = sure && off < most_off && fabsf(low - m) < 1024.f * s && high - m < 1024.f * s;
+    if (__any_sync(0xffffffffu, !sure && group.kept && i < group.rows)) {
+      const uint64_t both = key_in_64_bits<T, D, NORM, NEIGHBOURS, GROUP>(p, from + i * p.k_head, i < group.rows, position);
+      codes = uint32_t(both), scales = uint32_t(both >> 32);
+    }
     group.template store<GROUP>(p, i, j, p.k_codes, p.k_scales, codes, scales);
   }
 }
@@ -252,7 +336,7 @@ __device__ __forceinline__ void key_rows(const RotateParams& p, uint32_t block) 
 // Blocks of keys and as many of values, in turn, spread evenly among those of queries (p.k_heads is 0 in `queries`): keys are bound by
 // instructions, queries by HBM.  `share`: of the blocks, keys' and values', in 2^-32, rounded up.
 template <typename T, int D, bool NORM, bool NEIGHBOURS, int ROWS, int GROUP>
-__global__ void __launch_bounds__(THREADS, 4) append_int4_kernel(const RotateParams p, const RotateParams queries, uint32_t share) {
+__global__ void __launch_bounds__(THREADS, 4) append_int4_kernel(const __grid_constant__ RotateParams p, const __grid_constant__ RotateParams queries, uint32_t share) {
   constexpr int OF_CACHE = ROWS == 1 ? 1 : CACHE_ROWS;
   programmatic_begin();
   const uint32_t before = __umulhi(blockIdx.x, share);             // keys' and values' blocks ahead of this one

@@ -279,3 +279,46 @@ def test_refusals(cuda_device):
         read.run(args[4], *(c.transpose(1, 2).contiguous().transpose(1, 2) for c in cache))
     with pytest.raises(TypeError):
         read.run(args[4].int(), *cache)
+
+
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("dtype,D,R,group,pairs", [("bf16", 128, 128, 64, "halves"), ("f16", 128, 128, 32, "halves"), ("bf16", 128, 64, 128, "neighbours"),
+                                                   ("f16", 64, 32, 64, "halves"), ("bf16", 64, 64, 32, "neighbours")])
+def test_codes_of_keys_are_the_definitions(cuda_device, norm, dtype, D, R, group, pairs):
+    """Also next to a border: of half a million elements none may be off by a step.  What decides is then at least 2^-40 away from
+    equal (64 bits: a dozen operations of 2^-53 on numbers up to 2^4 of a step)."""
+    T, HK = 1000, 4
+    (q, k, v), weights = inputs(T, 2, HK, D, dtype, False, seed=5)
+    rotary, positions = table(2000, R), torch.arange(T, dtype=torch.int32) * 2
+    cache = empty_cache(-(-T // 64), HK, 64, D, group, dtype, cuda_device)
+    slots = torch.arange(T)
+    append = ib.compile(ib.programs.paged_kv_append_int4,
+                        constexprs={"ACT_DTYPE": dtype, "NORM": norm, "PAIRS": pairs, "GROUP_SIZE": group})
+    append.run(*(t.to(cuda_device) for t in (q, k, v, positions, slots, rotary, *(weights if norm else ()))), *cache)
+    keys = oracle.rotate(k, positions, rotary, weights[1] if norm else None, pairs=pairs, eps=float(torch.tensor(1e-6)))
+    codes, scales = oracle.quantise(keys, group, DTYPES[dtype])
+    held = [rows(c, slots) for c in cache[:2]]
+    assert torch.equal(held[1], scales)
+    n, m = (torch.stack([c % 16, c // 16], -1).flatten(-2).int() for c in (held[0], codes))
+    if norm:
+        assert torch.equal(n, m)
+    else:       # (halves of whole steps, where 64 bits round the quotient before it is rounded to a whole number)
+        by, least = scales.double().unflatten(-1, (-1, 2)).split(1, -1)
+        exact = ((keys.unflatten(-1, (-1, group)) - least) / by).flatten(-2)
+        assert ((n == m) | (((exact % 1) - 0.5).abs() < 2.0 ** -40)).all()
+
+
+def test_keys_that_are_nearly_equal(cuda_device):
+    """A group whose range is far below the rounding of its minimum: codes are cut, whichever way."""
+    k = torch.full((4, 1, 64), 1000.0, dtype=torch.bfloat16)
+    rotary = torch.zeros((4, 32))
+    rotary[:, :16] = torch.tensor([1.0, 1.003, 1 + 2.0 ** -20, 1 + 2.0 ** -23])[:, None]
+    rotary[:, 0] += 2.0 ** -22
+    cache = empty_cache(1, 1, 16, 64, 64, "bf16", cuda_device)
+    slots = torch.arange(4)
+    ib.compile(ib.programs.paged_kv_append_int4, constexprs={"NORM": False}).run(
+        *(t.to(cuda_device) for t in (k, k, k, slots.int(), slots, rotary)), *cache)
+    keys = oracle.rotate(k, slots, rotary)
+    codes, scales = oracle.quantise(keys, 64, torch.bfloat16)
+    held = [rows(c, slots) for c in cache[:2]]
+    assert torch.equal(held[0], codes) and torch.equal(held[1], scales)
