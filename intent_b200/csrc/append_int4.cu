@@ -6,17 +6,17 @@
 // (s the next lower number where m + 15 s would be beyond the type; a group with something that is no finite number is NaN).
 //
 // A code is off by one as soon as a number next to a half is off by a little, and then by a whole step.  So keys are worked out in 64
-// bits: in f32 three of a million codes were others, now they are those of the definition.  Values have no arithmetic before
-// and 16 bits, and f32 holds their differences; quotients are rounded as a division rounds them, so that halves, common among
-// 16-bit numbers, are halves.
+// bits where f32 does not decide (in f32 alone three of a million codes were others, now they are those of the definition).
+// Values have no arithmetic before and 16 bits, and f32 holds their differences; quotients are rounded as a division rounds
+// them, so that halves, common among 16-bit numbers, are halves.
 //
 // A lane has eight neighbouring elements of a row.  The partners of a key's elements in pairs (i, i + R/2) are another lane's; it reads
 // them once more from the first-level cache and works out its own half of each pair.  Blocks have keys, values or queries; in
 // calls of many rows two rows of keys or values, and four of queries, share what does not depend on the row.
 //
-// Measured on one B200: 8192 tokens, 32 + 8 + 8 heads of 128, norm, bf16, with paged_kv_read_int4 of them 59 us (floor 33), of which the
-// read is 9, queries take 24 alone, keys 18 and values 8: bound by instructions, two thirds of the issue slots.  With four rows
-// of keys and 102 registers 76; keys' blocks ahead of the others 63.  (Keys in f32 took as long.)
+// Measured on one B200: 8192 tokens, 32 + 8 + 8 heads of 128, norm, bf16, with paged_kv_read_int4 of them 54 us (floor 33), of which the
+// read is 9, queries take 20 alone, keys 12 and values 5: bound by instructions, two thirds of the issue slots.  All keys in 64
+// bits 59; keys' blocks ahead of the others 63; with four rows of keys and 102 registers 76.
 #include "common.cuh"
 #include "paged.cuh"
 #include "rotate.cuh"
@@ -250,8 +250,8 @@ __device__ __noinline__ uint64_t key_in_64_bits(const RotateParams& p, const uin
 }
 
 // Keys in f32 first.  An element is then off by at most DELTA = 2^-20 of |x own| + |partner cross|, times the norm's factor r (the
-// sum of squares and r up to 2^-21, four roundings of 2^-24), which is at most (largest |own| + |cross|) times sqrt(D), as r |x| is no more
-// than that, or times the row's largest |x| where there is no norm.  Where the minimum's or the scale's rounding, or a code's, could
+// sum of squares and r up to 2^-21, five roundings of 2^-24), which is at most the row's largest |own| + |cross| times its largest r |x|.
+// (With sqrt(D) in the place of that, which r |x| cannot exceed, four times as many rows were worked out twice: 6 us of 57.)  Where the minimum's or the scale's rounding, or a code's, could
 // be another within that, the warp's rows are worked out in 64 bits; so are those with something that is no number, with equal
 // elements, and near the ends of the type.
 template <typename T, int D, bool NORM, bool NEIGHBOURS, int ROWS, int GROUP>
@@ -275,12 +275,18 @@ __device__ __forceinline__ void key_rows(const RotateParams& p, uint32_t block) 
   for (int e = 0; e < 8; ++e) most = largest_of(most, fabsf(turn.own[e]) + fabsf(turn.cross[e]));
 #pragma unroll
   for (int d = 1; d < LANES; d *= 2) most = largest_of(most, __shfl_xor_sync(0xffffffffu, most, d));
-  const float of_row = most * (NORM ? (D == 128 ? 11.4f : 8.1f) * 0x1p-20f : 0x1p-20f);
+  most *= 0x1.001p-20f;                // (and what these products are rounded by)
+  uint32_t open = 0;                   // the rows that have to be worked out in 64 bits
 
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
-    float x[8], y[8], delta = of_row;
+    float x[8], y[8], size = 0.f;
     turn.elements(raw[i], partners[i], x, y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) size = largest_of(size, fabsf(x[e]));
+#pragma unroll
+    for (int d = 1; d < LANES; d *= 2) size = largest_of(size, __shfl_xor_sync(0xffffffffu, size, d));
+    float delta = most * size;
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = fmaf(x[e], turn.own[e], y[e] * turn.cross[e]);
     if (NORM) {
@@ -292,13 +298,7 @@ __device__ __forceinline__ void key_rows(const RotateParams& p, uint32_t block) 
       const float scale = rsqrtf(sum * (1.f / D) + p.eps);
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] *= scale;
-    } else {
-      float size = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) size = largest_of(size, fabsf(x[e]));
-#pragma unroll
-      for (int d = 1; d < LANES; d *= 2) size = largest_of(size, __shfl_xor_sync(0xffffffffu, size, d));
-      delta *= size;
+      delta *= scale;
     }
     float low = y[0], high = y[0];
 #pragma unroll
@@ -325,22 +325,26 @@ __device__ __forceinline__ void key_rows(const RotateParams& p, uint32_t block) 
     }
     // (and none is so far out, by the minimum's rounding, that its whole number is)
     sure = sure && off < most_off && fabsf(low - m) < 1024.f * s && high - m < 1024.f * s;
-    if (__any_sync(0xffffffffu, !sure && group.kept && i < group.rows)) {
-      const uint64_t both = key_in_64_bits<T, D, NORM, NEIGHBOURS, GROUP>(p, from + i * p.k_head, i < group.rows, position);
-      codes = uint32_t(both), scales = uint32_t(both >> 32);
-    }
+    if (__any_sync(0xffffffffu, !sure && group.kept && i < group.rows)) open |= 1u << i;
     group.template store<GROUP>(p, i, j, p.k_codes, p.k_scales, codes, scales);
+  }
+  // (behind the loop, where little has to be kept across the call: 57 -> 56 us)
+#pragma unroll 1
+  for (int i = 0; open; ++i, open >>= 1) {
+    if (!(open & 1)) continue;
+    const uint64_t both = key_in_64_bits<T, D, NORM, NEIGHBOURS, GROUP>(p, from + i * p.k_head, i < group.rows, position);
+    group.template store<GROUP>(p, i, j, p.k_codes, p.k_scales, uint32_t(both), uint32_t(both >> 32));
   }
 }
 
-// Blocks of keys and as many of values, in turn, spread evenly among those of queries (p.k_heads is 0 in `queries`): keys are bound by
+// Blocks of keys and as many of values, in turn, spread evenly among those of queries: keys are bound by
 // instructions, queries by HBM.  `share`: of the blocks, keys' and values', in 2^-32, rounded up.
 template <typename T, int D, bool NORM, bool NEIGHBOURS, int ROWS, int GROUP>
-__global__ void __launch_bounds__(THREADS, 4) append_int4_kernel(const __grid_constant__ RotateParams p, const __grid_constant__ RotateParams queries, uint32_t share) {
+__global__ void __launch_bounds__(THREADS, 4) append_int4_kernel(const __grid_constant__ RotateParams p, uint32_t share) {
   constexpr int OF_CACHE = ROWS == 1 ? 1 : CACHE_ROWS;
   programmatic_begin();
   const uint32_t before = __umulhi(blockIdx.x, share);             // keys' and values' blocks ahead of this one
-  if (__umulhi(blockIdx.x + 1, share) == before) rotate_rows<T, D, NORM, NEIGHBOURS, false, ROWS>(queries, blockIdx.x - before);
+  if (__umulhi(blockIdx.x + 1, share) == before) rotate_rows<T, D, NORM, NEIGHBOURS, false, ROWS, true>(p, blockIdx.x - before);
   else if (before % 2 == 0) key_rows<T, D, NORM, NEIGHBOURS, OF_CACHE, GROUP>(p, before / 2);
   else value_rows<T, D, OF_CACHE, GROUP>(p, before / 2);
 }
@@ -354,13 +358,11 @@ int launch(const RotateParams& p, bool neighbours, cudaStream_t stream) {
   const uint32_t k_blocks = (p.tokens * ((p.k_heads + OF_CACHE - 1) / OF_CACHE) + PER_CTA - 1) / PER_CTA;
   const uint32_t q_blocks = (p.tokens * ((p.q_heads + ROWS - 1) / ROWS) + PER_CTA - 1) / PER_CTA, grid = 2 * k_blocks + q_blocks;
   const uint32_t share = uint32_t((uint64_t(2 * k_blocks) << 32) / grid) + 1;
-  RotateParams queries = p;
-  queries.k_heads = 0;
   if (LaunchFacts* sink = observe_sink())
     return record_launch(sink, reinterpret_cast<const void*>(kernel),
                          ROWS == 1 ? "append_int4_kernel a row per group" : "append_int4_kernel several rows per group", int(grid), THREADS,
                          0, 1);
-  const cudaError_t e = launch_programmatic(kernel, dim3(grid), dim3(THREADS), 0, stream, 1, p, queries, share);
+  const cudaError_t e = launch_programmatic(kernel, dim3(grid), dim3(THREADS), 0, stream, 1, p, share);
   if (e != cudaSuccess) return cuda_status(e);
   note_launch();
   return launch_status();

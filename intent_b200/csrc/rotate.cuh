@@ -94,18 +94,18 @@ __device__ __forceinline__ void store_piece(uint16_t* to, const Piece<PIECE>& v)
   else *reinterpret_cast<uint2*>(to) = make_uint2(v.w[0], v.w[1]);
 }
 
-// The rows of one block of ROTATE_THREADS
-template <typename T, int D, bool NORM, bool NEIGHBOURS, bool CACHE, int ROWS>
+// The rows of one block of ROTATE_THREADS.  QUERIES: there are no others.
+template <typename T, int D, bool NORM, bool NEIGHBOURS, bool CACHE, int ROWS, bool QUERIES = false>
 __device__ __forceinline__ void rotate_rows(const RotateParams& p, uint32_t block) {
   constexpr int PIECE = PIECE_OF, PAIRS = PIECE / 2, LANES = D / (2 * PIECE);   // lanes of a row
   const int lane = threadIdx.x & 31, j = lane % LANES;
   // groups of a token: of its queries, its keys, its values
   const uint32_t q_groups = (p.q_heads + ROWS - 1) / ROWS, k_groups = (p.k_heads + ROWS - 1) / ROWS;
-  const uint32_t groups = q_groups + (CACHE ? 2 : 1) * k_groups;
+  const uint32_t groups = QUERIES ? q_groups : q_groups + (CACHE ? 2 : 1) * k_groups;
   const uint32_t at = block * uint32_t(ROTATE_THREADS / LANES) + threadIdx.x / LANES;
   const bool live = at < p.tokens * groups;          // (all lanes stay for the norms' sums)
   const uint32_t token = live ? at / groups : 0, group = at - token * groups;
-  const bool is_q = group < q_groups, is_v = CACHE && group >= q_groups + k_groups;
+  const bool is_q = QUERIES || group < q_groups, is_v = CACHE && group >= q_groups + k_groups;
   const uint32_t first = (is_q ? group : group - q_groups - (is_v ? k_groups : 0)) * ROWS;
   const uint32_t rows = live ? min((is_q ? p.q_heads : p.k_heads) - first, uint32_t(ROWS)) : 0;
   const int half = p.rotary_dim / 2;
