@@ -562,8 +562,9 @@ INTENT_B200_API int intent_b200_paged_kv_append_norm_bf16(INTENT_B200_VIEW3(q), 
  *   k_scales, v_scales [PAGES, HK, PAGE, 2 D / group] f16 | bf16   scale s and minimum m, one after the other, of every `group`
  *                                      (32, 64 or 128, up to D) consecutive elements: a code n stands for m + s * n
  * append: rows as above; m = min and s = (max - min) / 15 of a group, rounded to the type, n = (x - m) / s rounded to the nearest
- * (even) of 0 .. 15; n = 0 where s = 0.  Where m + 15 s would be beyond the type, s is the next lower number.  Keys are normalised and rotated in f32 and not rounded before.  A group with something that
- * is no finite number (or a minimum or scale beyond the type) is stored as s = m = NaN.  Two tokens with one slot: what is stored is
+ * (even) of 0 .. 15; n = 0 where s = 0.  Where m + 15 s would be beyond the type, s is the next lower number.  Keys are not rounded
+ * between their norm and rotation and this: minima, scales and codes are those of 64-bit arithmetic.  A group with something that is
+ * no finite number (or a minimum or scale beyond the type) is stored as s = m = NaN.  Two tokens with one slot: what is stored is
  * undefined.
  * read: k, v [T, HK, D] of the tokens at slots [T] i64, m + s * n in f32 rounded to the type; zeros for a slot outside the cache.
  * ------------------------------------------------------------------------ */
@@ -616,7 +617,8 @@ INTENT_B200_API int intent_b200_paged_kv_read_int4_bf16(
  * _int4: over a cache in 4 bits as above, of the values m + s * n; the workspace is the same (..._int4_call_workspace_bytes).  Chunks of
  * many rows take these values rounded to the type, as reading them back gives them; single tokens and few rows take them as they
  * are.  The factor of the scores is at most 2^50 there, bf16 queries are below 2^67 and scales of values below 2^55 in magnitude
- * (beyond that a row may be NaN).  A group whose scale or minimum is no number makes the rows that see its token NaN, and no others.
+ * (beyond that a row may be NaN); a code's part s * n of a value may be off by 2^-57 and its product with a query by 2^-53, which
+ * matters for values and queries of 10^-14 and less.  A group whose scale or minimum is no number makes the rows that see its token NaN, and no others.
  * ------------------------------------------------------------------------ */
 INTENT_B200_API int intent_b200_paged_attention_f16(INTENT_B200_VIEW3(q), INTENT_B200_VIEW4(k_cache), INTENT_B200_VIEW4(v_cache),
                                                  INTENT_B200_VIEW2(page_table), INTENT_B200_VIEW1(query_offsets),

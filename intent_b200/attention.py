@@ -1,10 +1,10 @@
 """The attention half of a transformer layer for serving, on a paged cache.
 
-``PagedKVCache`` keeps the keys and values of many sequences in pages, of 16-bit elements or in 4 bits, and makes, for every step of new tokens, the tensors
-that the attention programs take.  ``W4A16Attention`` chains the int4 projection to queries, keys and values, the norms and
-the rotation with the append (``paged_kv_append``), the attention over the pages (``paged_decode_attention`` where every
-sequence has one new token, ``paged_attention`` otherwise) and the int4 output projection; with ``cache_bits=4`` the programs for a
-cache in 4 bits take their places.  Everything runs on the current
+``PagedKVCache`` keeps the keys and values of many sequences in pages, of 16-bit elements or in 4 bits, and makes, for every step
+of new tokens, the tensors that the attention programs take.  ``W4A16Attention`` chains the int4 projection to queries, keys
+and values, the norms and the rotation with the append (``paged_kv_append``), the attention over the pages
+(``paged_decode_attention`` where every sequence has one new token, ``paged_attention`` otherwise) and the int4 output
+projection; with ``cache_bits=4`` the programs for a cache in 4 bits take their places.  Everything runs on the current
 stream; no step reads a device value back to the host.
 
     cache = PagedKVCache(layers=2, pages=1024, kv_heads=8, head_dim=128)

@@ -251,9 +251,9 @@ __device__ __noinline__ uint64_t key_in_64_bits(const RotateParams& p, const uin
 
 // Keys in f32 first.  An element is then off by at most DELTA = 2^-20 of |x own| + |partner cross|, times the norm's factor r (the
 // sum of squares and r up to 2^-21, five roundings of 2^-24), which is at most the row's largest |own| + |cross| times its largest r |x|.
-// (With sqrt(D) in the place of that, which r |x| cannot exceed, four times as many rows were worked out twice: 6 us of 57.)  Where the minimum's or the scale's rounding, or a code's, could
-// be another within that, the warp's rows are worked out in 64 bits; so are those with something that is no number, with equal
-// elements, and near the ends of the type.
+// (With sqrt(D) in the place of that, which r |x| cannot exceed, four times as many rows were worked out twice: 6 us of 57.)  Where the
+// minimum's or the scale's rounding, or a code's, could be another within that, the warp's rows are worked out in 64 bits; so are
+// those with something that is no number, with equal elements, and near the ends of the type.
 template <typename T, int D, bool NORM, bool NEIGHBOURS, int ROWS, int GROUP>
 __device__ __forceinline__ void key_rows(const RotateParams& p, uint32_t block) {
   constexpr int LANES = D / 8;

@@ -82,8 +82,8 @@ int attend(const View3& q, const CacheViews& cache, const View2& table, const Vi
   const int64_t tokens = q.d0, heads = q.d1, dim = q.d2, pages = k_cache.d0, k_heads = k_cache.d1, page = k_cache.d2;
   const int64_t batch = lengths.d0;
   if (tokens < 0 || batch < 0 || heads <= 0 || k_heads <= 0 || heads % k_heads != 0 || v_cache.d0 != pages ||
-      v_cache.d1 != k_heads || v_cache.d2 != page || (!int4 && (k_cache.d3 != dim || v_cache.d3 != dim)) || table.d0 != batch || out.d0 != tokens ||
-      out.d1 != heads || out.d2 != dim || (offsets ? offsets->d0 != batch + 1 : tokens != batch))
+      v_cache.d1 != k_heads || v_cache.d2 != page || (!int4 && (k_cache.d3 != dim || v_cache.d3 != dim)) || table.d0 != batch ||
+      out.d0 != tokens || out.d1 != heads || out.d2 != dim || (offsets ? offsets->d0 != batch + 1 : tokens != batch))
     return INTENT_B200_ERR_SHAPE;
   if (dim != 64 && dim != 128) return INTENT_B200_ERR_UNSUPPORTED;
   if (page < 16 || page > 256 || (page & (page - 1)) != 0 || window < 0) return INTENT_B200_ERR_UNSUPPORTED;

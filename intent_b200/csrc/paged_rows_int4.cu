@@ -8,7 +8,7 @@
 // word they are n or 16 n times the smallest bf16 (2^-133; an f16 too, 2^-24, in the lowest four), exact numbers for it.  The factor of
 // 16 is taken out of the queries (bf16) or the results ahead, so that eight codes cost five instructions; with a weight's
 // exponent 2^64 and a query's 2^60 larger no product comes near the ends of f32.  (Queries of 2^67 and more and scales of values
-// of 2^55 and more are out of that range.)
+// of 2^55 and more are out of that range, and below f32's smallest normal number, 2^-126, are 2^-57 of s n and 2^-53 of x n.)
 //
 // All statistics and sums are in f32.  A weight times its scale is rounded to bf16 for the product with the codes, and the same
 // rounded numbers are added up for the middle of the codes (8), which is taken off again: the rounding is worth what it is for a
@@ -29,7 +29,8 @@
 // reads one after another of two launches.  Bound by what a step of 64 tokens costs beside its bytes, 900 instructions on two
 // warps per scheduler, of which the ALU's are the masks (256 of 64 tokens' codes).
 // Tried and not kept: twelve warps with keys and values in slots of their own (more instructions issued, and more of them: 72 us where
-// eight warps took 70), steps of 32 or 48 tokens for sixteen or twelve (80, 76), codes asked for in the second-level cache a step
+// eight warps took 70), steps of 32 or 48 tokens for sixteen or twelve (80, 76), of 32 for tiles of
+// sixteen rows (64 sequences of 16 heads of 64 on one: 151 us, 122 with 64), codes asked for in the second-level cache a step
 // ahead (73), shifts as products (77), parts joined by the CTA that is done last in place of a launch (70, and 88 for 79 with four
 // tokens each).
 #include <cstring>
@@ -133,7 +134,8 @@ template <typename T, int D, int GROUP, int TILE>
 __global__ void __launch_bounds__(32 * Ring<D, GROUP, TILE>::WARPS, 1)
 paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
   using R = Ring<D, GROUP, TILE>;
-  constexpr int NT = R::NT, ROWS = 8 * NT, WARPS = R::WARPS, THREADS = 32 * WARPS, UNIT = R::UNIT, PARTS = R::PARTS, STEP = UNIT, BEGIN = R::BEGIN, GROUPS = R::GROUPS;
+  constexpr int NT = R::NT, ROWS = 8 * NT, WARPS = R::WARPS, THREADS = 32 * WARPS, UNIT = R::UNIT, PARTS = R::PARTS, STEP = UNIT,
+                BEGIN = R::BEGIN, GROUPS = R::GROUPS;
   constexpr int CHUNKS = D / 32, OF_GROUP = CHUNKS / GROUPS;            // 16 bytes of a token's codes
   // Columns of a product are the tile's rows, or these twice: then the upper half of the columns has the upper half of the groups.
   constexpr int COPIES = TILE == 4 && GROUPS > 1 ? 2 : 1, COLUMNS = ROWS / COPIES, SETS = GROUPS / COPIES;

@@ -217,6 +217,24 @@ def test_scales_of_nothing_and_of_much(cuda_device):
     assert_close(run(artifact, cuda_device, data, True), reference(data, 32))
 
 
+@pytest.mark.parametrize("single", [True, False])
+@pytest.mark.parametrize("power", [-30, 40])
+def test_powers_of_two(cuda_device, single, power):
+    """Values 2^power times as large give a result as many times as large; keys so many times as large and queries as many times as
+    small the same one.  All roundings are alike; what is too small for f32 is a product's 2^-57 at most (of values at 2^-30: 200
+    tokens' 2^-27 each, below 2^-19)."""
+    data = make([200, 50], [1, 1] if single else [3, 2], 4, 2, 64, 16, 32, "bf16")
+    q, cache, table, offsets, n = data
+    artifact = ib.compile(ib.programs.paged_decode_attention_int4 if single else ib.programs.paged_attention_int4,
+                          constexprs={"GROUP_SIZE": 32})
+    expected = run(artifact, cuda_device, data, single).cpu().double()
+    by = 2.0 ** power
+    values = run(artifact, cuda_device, (q, [*cache[:3], cache[3] * by], table, offsets, n), single).cpu().double() / by
+    keys = run(artifact, cuda_device, (q / by, [cache[0], cache[1] * by, *cache[2:]], table, offsets, n), single).cpu().double()
+    for actual in (values, keys):
+        assert ((actual - expected).abs() <= 2.0 ** -7 * expected.abs() + 2.0 ** -19).all()
+
+
 def test_f16_values_of_every_size(cuda_device):
     """Scales from the smallest f16 to thousands: weights times scales do not run out of range."""
     data = make([300, 120, 40], [1, 1, 1], 4, 1, 128, 32, 64, "f16")
