@@ -116,7 +116,6 @@ class PagedKVCache:
     def read(self, index: int, sequence, start: int = 0, stop: int | None = None):
         """Keys and values of one layer of a sequence's tokens from ``start`` to ``stop`` (its end), [tokens, kv_heads, head_dim]
         each, in 16 bits."""
-        import numpy as np
         import torch
 
         if sequence not in self._lengths:
@@ -125,8 +124,8 @@ class PagedKVCache:
         stop = length if stop is None else stop
         if not 0 <= start <= stop <= length:
             raise ValueError(f"the sequence has {length} tokens, not those from {start} to {stop}")
-        place, size = np.arange(start, stop), self.page_size
-        slots = torch.from_numpy(np.asarray(self._pages[sequence], dtype=np.int64)[place // size] * size + place % size)
+        place, size = torch.arange(start, stop, device="cpu"), self.page_size
+        slots = torch.tensor(self._pages[sequence], dtype=torch.int64, device="cpu")[place // size] * size + place % size
         device = self.k.device
         if device.type == "cuda":
             slots = slots.pin_memory().to(device, non_blocking=True)

@@ -78,6 +78,16 @@ def test_what_is_refused(cuda_device):
     assert layer.forward(x, w, table, *small.layer(0), small.step({"b": 3})).isfinite().all()
 
 
+@pytest.mark.parametrize("bits", [4, 16])
+def test_reading_no_tokens(cuda_device, bits):
+    cache = PagedKVCache(layers=1, pages=2, kv_heads=2, head_dim=64, page_size=16, device=cuda_device, bits=bits)
+    cache.step({"a": 20})
+    for start, stop in ((20, None), (3, 3), (0, 0)):
+        assert [tuple(t.shape) for t in cache.read(0, "a", start, stop)] == [(0, 2, 64)] * 2
+    with pytest.raises(ValueError):
+        cache.read(0, "a", 21)
+
+
 def test_a_step_in_a_graph(cuda_device):
     """A decode step of a layer, captured and replayed, is the step itself."""
     layer = W4A16Attention(hidden=HIDDEN, heads=HEADS, kv_heads=KV_HEADS, head_dim=DIM, cache_bits=4)
