@@ -23,7 +23,7 @@
 // Copies are made by the warps that read them (cp.async): a TMA copy needs a lane of its own, and with four of them per step they
 // were a quarter of a step's instructions (74 -> 70 us below).
 //
-// Measured on one B200 (6540 GB/s copied; bf16, 32 heads of 128 on 8, groups of 64): 64 histories of up to 8192 tokens 65 us, 4.9
+// Measured on one B200 (6540 GB/s copied; bf16, 32 heads of 128 on 8, groups of 64): 64 histories of up to 8192 tokens 66 us, 4.8
 // TB/s (floor 49; copies alone 58, arithmetic alone 61 before four rows stood twice); groups of 32 71 us; 4 of up to 131072, 4 key
 // heads, groups of 128 42 us, 4.0 TB/s; 200 of up to 2048, 16 heads of 64, f16, groups of 32 79 us, 3.5 TB/s; one of 2000 10.1 us, the
 // reads one after another of two launches.  Bound by what a step of 64 tokens costs beside its bytes, 900 instructions on two
