@@ -49,9 +49,9 @@ __device__ __forceinline__ uint32_t code_of(float sum) {
 
 // The quotients of eight numbers by a scale s, rounded to whole numbers from 0 to 15.  The product with the rounded reciprocal gets its
 // remainder added, which makes it the quotient as a division rounds it (P. Markstein, Computation of elementary functions on the
-// IBM RISC System/6000 processor, 1990).  HALVES: whether quotients may lie in the middle between two numbers; those of keys that
-// were normalised do not, and need no such care.  Added to 1.5 times 2 to the mantissa's length a number is rounded in the lowest bits.
-template <typename T, bool HALVES>
+// IBM RISC System/6000 processor, 1990).  Keys' elements may lie in the middle between two codes, too: what is zero stays zero, and
+// -m / s is a quotient of 16-bit numbers.  Added to 1.5 times 2 to the mantissa's length a number is rounded in the lowest bits.
+template <typename T>
 __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float s, float m) {
   // (powers of two that keep the reciprocal a normal number)
   const float by = std::is_same<T, __half>::value ? 1.f : s < 0x1p-60f ? 0x1p64f : s > 0x1p60f ? 0x1p-64f : 1.f;
@@ -64,19 +64,14 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float s, float
   }
   return codes;
 }
-template <typename T, bool HALVES>
+template <typename T>
 __device__ __forceinline__ uint32_t codes_of(const double (&x)[8], float scale, float minimum) {
-  const double s = scale, m = minimum, inverse = scale > 0.f ? __drcp_rn(s) : 0., origin = -m * inverse;
+  const double s = scale, m = minimum, inverse = scale > 0.f ? __drcp_rn(s) : 0.;
   uint32_t codes = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    double quotient;
-    if (HALVES) {
-      const double d = x[e] - m, q = d * inverse;
-      quotient = fma(fma(-q, s, d), inverse, q);
-    } else {
-      quotient = fma(x[e], inverse, origin);
-    }
+    const double d = x[e] - m, q = d * inverse;
+    double quotient = fma(fma(-q, s, d), inverse, q);
     quotient = quotient < 0. ? 0. : quotient > 15. ? 15. : quotient;     // (where a minimum's rounding is many scales, it may be far out)
     codes |= uint32_t(__double2loint(quotient + 6755399441055744.)) << (4 * e);
   }
@@ -84,7 +79,7 @@ __device__ __forceinline__ uint32_t codes_of(const double (&x)[8], float scale, 
 }
 
 // Eight neighbouring elements of a row as codes; `scales`: scale | minimum of their group, which all of its lanes know
-template <typename T, int GROUP, bool HALVES, typename F>
+template <typename T, int GROUP, typename F>
 __device__ __forceinline__ uint32_t quantise(const F (&x)[8], uint32_t& scales) {
   const float infinity = __int_as_float(0x7f800000);
   F low = x[0], high = x[0];
@@ -112,7 +107,7 @@ __device__ __forceinline__ uint32_t quantise(const F (&x)[8], uint32_t& scales) 
     return 0;
   }
   if (!(Elem<T>::to_float(Elem<T>::from_float(fmaf(15.f, s, m))) < infinity)) s = Elem<T>::to_float(uint16_t(--scales));
-  return codes_of<T, HALVES>(x, s, m);
+  return codes_of<T>(x, s, m);
 }
 
 // A group of lanes and its rows of one kind of one token
@@ -161,7 +156,7 @@ __device__ __forceinline__ void value_rows(const RotateParams& p, uint32_t block
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = Elem<T>::to_float(uint16_t(w[e / 2] >> (16 * (e & 1))));
     uint32_t scales;
-    const uint32_t codes = quantise<T, GROUP, true>(x, scales);
+    const uint32_t codes = quantise<T, GROUP>(x, scales);
     group.template store<GROUP>(p, i, j, p.v_codes, p.v_scales, codes, scales);
   }
 }
@@ -245,7 +240,7 @@ __device__ __noinline__ uint64_t key_in_64_bits(const RotateParams& p, const uin
 #pragma unroll
   for (int e = 0; e < 8; ++e) y[e] = fma(x[e], turn.own[e], y[e] * turn.cross[e]) * scale;
   uint32_t scales;
-  const uint32_t codes = quantise<T, GROUP, !NORM>(y, scales);
+  const uint32_t codes = quantise<T, GROUP>(y, scales);
   return codes | uint64_t(scales) << 32;
 }
 

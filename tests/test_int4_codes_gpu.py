@@ -1,0 +1,58 @@
+"""paged_kv_append_int4: codes next to a border between two are those of the definition in 64 bits."""
+import pytest
+import torch
+
+import intent_b200 as ib
+from oracle import attention as oracle
+from test_int4_cache_gpu import empty_cache, rows
+from test_rope_append_gpu import DTYPES, table
+
+pytestmark = pytest.mark.gpu
+
+
+def append(device, k, v, group, dtype, weight=None, pairs="halves", rotary=None):
+    """(codes, scales) of keys and of values, [T, HK, ...]; every token at position 0."""
+    T, HK, D = k.shape
+    cache = empty_cache(-(-T // 64), HK, 64, D, group, dtype, device)
+    slots, positions = torch.arange(T), torch.zeros(T, dtype=torch.int32)
+    norms = [] if weight is None else [weight.to(device)] * 2
+    ib.compile(ib.programs.paged_kv_append_int4,
+               constexprs={"ACT_DTYPE": dtype, "NORM": weight is not None, "PAIRS": pairs, "GROUP_SIZE": group}).run(
+        *(t.to(device) for t in (k, k, v, positions, slots, table(1, 16) if rotary is None else rotary)), *norms, *cache)
+    return [rows(c, slots) for c in cache]
+
+
+# Multiples k + 1/2 of a scale s that are 16-bit numbers, as s is, and whose product with the rounded 1 / s in 64 bits lies on the
+# other side of the half.
+TIES = {"f16": [(1288, 3), (1456, 6), (1568, 7), (1576, 1), (1648, 5), (1680, 2), (1712, 7), (1816, 2), (1872, 4), (1896, 3), (1916, 1),
+                (1968, 6), (2024, 3)],
+        "bf16": [(196, 1)]}
+
+
+@pytest.mark.parametrize("pairs", ["halves", "neighbours"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_zeros_of_normalised_keys(cuda_device, dtype, pairs):
+    """A key's element that is zero stays zero, and -m / s of the 16-bit m and s may lie in the middle between two codes.  Each row has
+    two numbers whose weights make them such a minimum and maximum, and a third, of weight zero, that sets the norm."""
+    D, eps = 128, float(torch.tensor(1e-6))
+    ties = TIES[dtype] * 8 if dtype == "bf16" else TIES[dtype]
+    k, weight = torch.zeros((len(ties), 1, D), dtype=DTYPES[dtype]), torch.zeros(D, dtype=DTYPES[dtype])
+    for i, (s, multiple) in enumerate(ties):
+        s = s * 2.0 ** (-10 - i // len(TIES[dtype]))
+        minimum = (multiple + 0.5) * s
+        low, high = 16 + 2 * i, 17 + 2 * i                    # (rotated are elements 0 to 15)
+        norm = torch.linspace(0.5, 1.0, 20001).to(DTYPES[dtype]).unique()
+        row = torch.zeros((len(norm), D), dtype=torch.float64)
+        row[:, low], row[:, high], row[:, -1] = -1, 1, norm.double()
+        factor = float((128 / 2.56) ** 0.5)
+        weight[low], weight[high] = minimum / factor, (15 * s - minimum) / factor
+        y = row / torch.sqrt((row * row).mean(-1, keepdim=True) + eps) * weight.double()
+        _, scales = oracle.quantise(y, D, DTYPES[dtype])
+        fits = ((scales[:, 0].double() == s) & (scales[:, 1].double() == -minimum)).nonzero().flatten()
+        assert len(fits), (s, multiple)
+        k[i, 0] = row[fits[0]].to(DTYPES[dtype])
+    codes, scales, _, _ = append(cuda_device, k, k, D, dtype, weight, pairs)
+    keys = oracle.rotate(k, torch.zeros(len(k), dtype=torch.int64), table(1, 16), weight, pairs=pairs, eps=eps)
+    expected, expected_scales = oracle.quantise(keys, D, DTYPES[dtype])
+    assert torch.equal(scales, expected_scales)
+    assert torch.equal(codes, expected)
