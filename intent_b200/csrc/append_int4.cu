@@ -53,8 +53,8 @@ __device__ __forceinline__ uint32_t code_of(float sum) {
 // -m / s is a quotient of 16-bit numbers.  Added to 1.5 times 2 to the mantissa's length a number is rounded in the lowest bits.
 template <typename T>
 __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float s, float m) {
-  // (powers of two that keep the reciprocal a normal number)
-  const float by = std::is_same<T, __half>::value ? 1.f : s < 0x1p-60f ? 0x1p64f : s > 0x1p60f ? 0x1p-64f : 1.f;
+  // (powers of two that keep the reciprocal a normal number; a scale of zero has none, and equal numbers of any size are its codes 0)
+  const float by = std::is_same<T, __half>::value || s == 0.f ? 1.f : s < 0x1p-60f ? 0x1p64f : s > 0x1p60f ? 0x1p-64f : 1.f;
   const float divisor = s * by, inverse = s > 0.f ? __frcp_rn(divisor) : 0.f, origin = -m * by;
   uint32_t codes = 0;
 #pragma unroll

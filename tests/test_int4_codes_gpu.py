@@ -56,3 +56,16 @@ def test_zeros_of_normalised_keys(cuda_device, dtype, pairs):
     expected, expected_scales = oracle.quantise(keys, D, DTYPES[dtype])
     assert torch.equal(scales, expected_scales)
     assert torch.equal(codes, expected)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("D,group", [(64, 32), (128, 128)])
+def test_equal_numbers_of_every_size(cuda_device, dtype, D, group):
+    """A group of equal numbers has the scale 0 and codes 0."""
+    top = torch.finfo(DTYPES[dtype]).max
+    x = torch.tensor([1.0, 2.0 ** -24, 60000.0] + ([2.0 ** 63, 2.0 ** 64, 2.0 ** 100, 2.0 ** -120] if dtype == "bf16" else []) + [top])
+    x = torch.cat([x, -x]).to(DTYPES[dtype])[:, None, None].expand(-1, 1, D).contiguous()
+    held = append(cuda_device, x, x, group, dtype)
+    for codes, scales in (held[:2], held[2:]):
+        assert not codes.any()
+        assert not scales[..., ::2].any() and torch.equal(scales[..., 1::2], x[..., ::group])
