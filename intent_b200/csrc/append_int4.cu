@@ -7,15 +7,15 @@
 //
 // A code is off by one as soon as a number next to a half is off by a little, and then by a whole step.  So keys are worked out in 64
 // bits where f32 does not decide (in f32 alone three of a million codes were others, now they are those of the definition).
-// Values have no arithmetic before and 16 bits, and f32 holds their differences; quotients are rounded as a division rounds
-// them, so that halves, common among 16-bit numbers, are halves.
+// Values have no arithmetic before: their minima are exact, their codes' quotients are in 64 bits (55.2 us below; with f32, in which
+// the difference to a minimum 2^16 times as large or as small is rounded, 54.4).
 //
 // A lane has eight neighbouring elements of a row.  The partners of a key's elements in pairs (i, i + R/2) are another lane's; it reads
 // them once more from the first-level cache and works out its own half of each pair.  Blocks have keys, values or queries; in
 // calls of many rows two rows of keys or values, and four of queries, share what does not depend on the row.
 //
-// Measured on one B200: 8192 tokens, 32 + 8 + 8 heads of 128, norm, bf16, with paged_kv_read_int4 of them 54 us (floor 33), of which the
-// read is 9, queries take 20 alone, keys 12 and values 5: bound by instructions, two thirds of the issue slots.  All keys in 64
+// Measured on one B200: 8192 tokens, 32 + 8 + 8 heads of 128, norm, bf16, with paged_kv_read_int4 of them 55 us (floor 33), of which the
+// read is 9, queries take 20 alone, keys 12 and values 6: bound by instructions, two thirds of the issue slots.  All keys in 64
 // bits 59; keys' blocks ahead of the others 63; with four rows of keys and 102 registers 76.
 #include "common.cuh"
 #include "paged.cuh"
@@ -41,39 +41,22 @@ __device__ __forceinline__ float largest_of(float a, float b) {
 __device__ __forceinline__ double least_of(double a, double b) { return a < b ? a : b; }
 __device__ __forceinline__ double largest_of(double a, double b) { return a > b ? a : b; }
 
-// A number added to this is rounded to a whole one in the lowest bits, from which code_of takes it, cut to 0 .. 15
-constexpr float WHOLE = 12582912.f;
-__device__ __forceinline__ uint32_t code_of(float sum) {
-  return uint32_t(__viaddmin_s32_relu(__float_as_int(sum), -__float_as_int(WHOLE), 15));
-}
-
-// The quotients of eight numbers by a scale s, rounded to whole numbers from 0 to 15.  The product with the rounded reciprocal gets its
-// remainder added, which makes it the quotient as a division rounds it (P. Markstein, Computation of elementary functions on the
-// IBM RISC System/6000 processor, 1990).  Keys' elements may lie in the middle between two codes, too: what is zero stays zero, and
-// -m / s is a quotient of 16-bit numbers.  Added to 1.5 times 2 to the mantissa's length a number is rounded in the lowest bits.
-template <typename T>
-__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float s, float m) {
-  // (powers of two that keep the reciprocal a normal number; a scale of zero has none, and equal numbers of any size are its codes 0)
-  const float by = std::is_same<T, __half>::value || s == 0.f ? 1.f : s < 0x1p-60f ? 0x1p64f : s > 0x1p60f ? 0x1p-64f : 1.f;
-  const float divisor = s * by, inverse = s > 0.f ? __frcp_rn(divisor) : 0.f, origin = -m * by;
-  uint32_t codes = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float d = fmaf(x[e], by, origin), q = d * inverse;
-    codes |= code_of(fmaf(fmaf(-q, divisor, d), inverse, q) + WHOLE) << (4 * e);
-  }
-  return codes;
-}
-template <typename T>
-__device__ __forceinline__ uint32_t codes_of(const double (&x)[8], float scale, float minimum) {
+// The quotients of eight numbers by a scale s, rounded to whole numbers from 0 to 15, in 64 bits: the difference to the minimum of two
+// 16-bit numbers can have more bits than f32 has, and a half and a little is not a half.  The product with the rounded reciprocal gets
+// its remainder added, which makes it the quotient as a division rounds it (P. Markstein, Computation of elementary functions on the
+// IBM RISC System/6000 processor, 1990): halves, common among 16-bit numbers, are halves.  So are those of keys: what is zero stays
+// zero, and -m / s is a quotient of 16-bit numbers.  Added to 1.5 * 2^52 a number is rounded in the lowest bits.
+template <typename F>
+__device__ __forceinline__ uint32_t codes_of(const F (&x)[8], float scale, float minimum) {
   const double s = scale, m = minimum, inverse = scale > 0.f ? __drcp_rn(s) : 0.;
   uint32_t codes = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const double d = x[e] - m, q = d * inverse;
+    const double d = double(x[e]) - m, q = d * inverse;
     double quotient = fma(fma(-q, s, d), inverse, q);
-    quotient = quotient < 0. ? 0. : quotient > 15. ? 15. : quotient;     // (where a minimum's rounding is many scales, it may be far out)
-    codes |= uint32_t(__double2loint(quotient + 6755399441055744.)) << (4 * e);
+    // (where the rounding of a key's minimum is many scales, it may be far out; a value's minimum is not rounded)
+    if (std::is_same<F, double>::value) quotient = quotient < 0. ? 0. : quotient > 15. ? 15. : quotient;
+    codes |= uint32_t(min(__double2loint(quotient + 6755399441055744.), 15)) << (4 * e);
   }
   return codes;
 }
@@ -98,7 +81,7 @@ __device__ __forceinline__ uint32_t quantise(const F (&x)[8], uint32_t& scales) 
     constexpr uint32_t LANES = (1u << (GROUP / 8)) - 1;
     odd = __ballot_sync(0xffffffffu, nothing != 0) >> (threadIdx.x & 31 & ~(GROUP / 8 - 1)) & LANES;
   }
-  // (in 64 bits, in which the scale's rounding is that of the exact quotient)
+  // (in 64 bits; rounded to the type by way of f32, so that within 2^-25 of the middle between two numbers it may be either)
   scales = Elem<T>::pack2(float((double(high) - double(low)) * (1. / 15.)), float(low));
   const float m = Elem<T>::to_float(uint16_t(scales >> 16));
   float s = Elem<T>::to_float(uint16_t(scales));
@@ -107,7 +90,7 @@ __device__ __forceinline__ uint32_t quantise(const F (&x)[8], uint32_t& scales) 
     return 0;
   }
   if (!(Elem<T>::to_float(Elem<T>::from_float(fmaf(15.f, s, m))) < infinity)) s = Elem<T>::to_float(uint16_t(--scales));
-  return codes_of<T>(x, s, m);
+  return codes_of(x, s, m);
 }
 
 // A group of lanes and its rows of one kind of one token
@@ -242,6 +225,12 @@ __device__ __noinline__ uint64_t key_in_64_bits(const RotateParams& p, const uin
   uint32_t scales;
   const uint32_t codes = quantise<T, GROUP>(y, scales);
   return codes | uint64_t(scales) << 32;
+}
+
+// A number added to this is rounded to a whole one in the lowest bits, from which code_of takes it, cut to 0 .. 15
+constexpr float WHOLE = 12582912.f;
+__device__ __forceinline__ uint32_t code_of(float sum) {
+  return uint32_t(__viaddmin_s32_relu(__float_as_int(sum), -__float_as_int(WHOLE), 15));
 }
 
 // Keys in f32 first.  An element is then off by at most DELTA = 2^-20 of |x own| + |partner cross|, times the norm's factor r (the

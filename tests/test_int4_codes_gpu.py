@@ -58,6 +58,37 @@ def test_zeros_of_normalised_keys(cuda_device, dtype, pairs):
     assert torch.equal(codes, expected)
 
 
+def next_to_halves(dtype, group):
+    """Rows of a group whose quotients are a half and a little more or less, and rows of numbers of every size."""
+    little = [2.0 ** -24, 2.0 ** -20] if dtype == "f16" else [2.0 ** -40, 2.0 ** -30, 2.0 ** -24, 2.0 ** -20]
+    out = []
+    for e in little:
+        for sign in (1, -1):
+            row = torch.arange(group).remainder(15) + 0.5     # multiples k + 1/2 of 1, less than nothing or more below them
+            row[0], row[1] = sign * e, 15
+            out.append(row)
+            for multiple in range(0, 15, 2):                  # and of 2 from a minimum that is one
+                row = torch.zeros(group)
+                row[0], row[1], row[2::2] = -(2 * multiple + 1), 29 - 2 * multiple, sign * e
+                out.append(row)
+    g = torch.Generator().manual_seed(group)
+    sizes = 2.0 ** torch.randint(-20, 1, (400, group), generator=g)
+    out += list(torch.randn((400, group), generator=g) * sizes)
+    return torch.stack(out).to(DTYPES[dtype])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("D,group", [(64, 32), (128, 64), (128, 128)])
+def test_values_next_to_halves(cuda_device, dtype, D, group):
+    """Their difference to the minimum can have more bits than f32 has: it is 64 bits' (in which all of these are exact)."""
+    x = next_to_halves(dtype, group).repeat(1, D // group)[:, None]
+    held = append(cuda_device, x, x, group, dtype)
+    expected, scales = oracle.quantise(x, group, DTYPES[dtype])
+    for i in (0, 2):                                          # keys, which position 0 turns by nothing, and values
+        assert torch.equal(held[i + 1], scales)
+        assert torch.equal(held[i], expected)
+
+
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("D,group", [(64, 32), (128, 128)])
 def test_equal_numbers_of_every_size(cuda_device, dtype, D, group):
