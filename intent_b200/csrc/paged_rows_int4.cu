@@ -10,7 +10,7 @@
 // exponent 2^64 and a query's 2^60 larger no product comes near the ends of f32.  (Queries of 2^67 and more and scales of values
 // of 2^55 and more are out of that range, and below f32's smallest normal number, 2^-126, are 2^-57 of s n and 2^-53 of x n.)
 //
-// All statistics and sums are in f32.  A weight times its scale is rounded to bf16 for the product with the codes, and the same
+// All statistics and sums are in f32, or in three bf16 parts that have its bits.  A weight times its scale is rounded to bf16 for the product with the codes, and the same
 // rounded numbers are added up for the middle of the codes (8), which is taken off again: the rounding is worth what it is for a
 // product with v_j.  For f16 results the product is made with what the rounding left over, too.
 //
@@ -233,11 +233,13 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
     }
   };
   uint32_t qf[NT][CHUNKS][4];            // queries as B fragments: elements 32 c + 8 (lane % 4) + {0, 4}, {1, 5}, {2, 6}, {3, 7}
-  // Sums of a group's queries in the scores' unit, which its minimum is multiplied with: of this thread's rows (f16), or in two
-  // bf16 parts as a B fragment, elements 0 .. GROUPS - 1 the rounded sums and the next ones what that left over.
+  // Sums of a group's queries in the scores' unit, which its minimum is multiplied with: of this thread's rows (f16), or in three
+  // bf16 parts, which have the bits of f32, as a B fragment: elements 0 .. GROUPS - 1 the rounded sums, the next ones what that left
+  // over, and from the eighth on what both left.  (With two parts a score is off by 2^-17 of minimum times sum, which can be many
+  // times the score where keys have a common offset.)
   constexpr bool BY_PRODUCT = std::is_same<T, __nv_bfloat16>::value;
   float q_sum[NT][2][GROUPS];
-  uint32_t q_parts[NT];
+  uint32_t q_parts[NT][2];
   float o[NT][CHUNKS][2][4];             // sums of codes: elements 32 c + 4 (lane / 4) + 2 t (+ 1, times 16) of rows 2 (lane % 4) (+ 1)
   const int upper = COPIES == 2 ? (lane & 3) >> 1 : 0;   // this thread's half of the groups
   float eights[NT][SETS][4];             // sums of the weights that the codes are multiplied with, of the same rows (twice)
@@ -291,16 +293,21 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
         for (int e = 0; e < 4; ++e) eights[nt][i][e] = 0.f;
       }
       if (BY_PRODUCT) {
-        uint32_t parts[2 * GROUPS];
+        uint32_t parts[2][2 * GROUPS] = {};
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
-          parts[g] = Elem<Wide>::from_float(sums[g]);
-          parts[GROUPS + g] = Elem<Wide>::from_float(sums[g] - Elem<Wide>::to_float(uint16_t(parts[g])));
+          parts[0][g] = Elem<Wide>::from_float(sums[g]);
+          const float rest = sums[g] - Elem<Wide>::to_float(uint16_t(parts[0][g]));
+          parts[0][GROUPS + g] = Elem<Wide>::from_float(rest);
+          parts[1][g] = Elem<Wide>::from_float(rest - Elem<Wide>::to_float(uint16_t(parts[0][GROUPS + g])));
         }
-        q_parts[nt] = 0;
 #pragma unroll
-        for (int i = 0; i < GROUPS; ++i)
-          if ((lane & 3) == i) q_parts[nt] = parts[2 * i] | (parts[2 * i + 1] << 16);
+        for (int h = 0; h < 2; ++h) {
+          q_parts[nt][h] = 0;
+#pragma unroll
+          for (int i = 0; i < GROUPS; ++i)
+            if ((lane & 3) == i) q_parts[nt][h] = parts[h][2 * i] | (parts[h][2 * i + 1] << 16);
+        }
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -377,7 +384,7 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
           for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[nt][m][e] = 0.f;
-            Elem<T>::mma16816(s[nt][m], minima[0], minima[1], 0u, 0u, q_parts[nt], 0u);
+            Elem<T>::mma16816(s[nt][m], minima[0], minima[1], minima[0], minima[1], q_parts[nt][0], q_parts[nt][1]);
           }
         }
 #pragma unroll

@@ -1,0 +1,51 @@
+"""Attention over a cache in 4 bits where sums of queries, minima or scales are large, or a history is long."""
+import math
+
+import pytest
+import torch
+
+import intent_b200 as ib
+from oracle import attention as oracle
+from test_int4_attention_gpu import assert_close, make, reference, run
+
+pytestmark = pytest.mark.gpu
+
+
+def opposite_minima(seed):
+    """Single tokens of two sequences, heads of 128 in two groups whose minima are a and -a, thousands, and queries whose sums over both
+    groups are nearly the same and take 20 bits: what a score is comes from the last of them."""
+    q, cache, table, offsets, n = make([24, 9], [1, 1], 4, 2, 128, 16, 64, "bf16", seed=seed)
+    g = torch.Generator().manual_seed(seed)
+    a = (4000 * torch.randn(cache[1].shape[:-1], generator=g)).bfloat16()
+    unused = cache[1][..., 1].isnan()
+    cache[1][..., 1], cache[1][..., 3] = torch.where(unused, math.nan, a), torch.where(unused, math.nan, -a)
+    x = torch.where(torch.rand((2, 4, 64), generator=g) < 0.5, 3 + torch.randn((2, 4, 64), generator=g), 0)
+    x += (x == 0) * torch.randint(1, 128, x.shape, generator=g) * 2.0 ** -14
+    x = (x.bfloat16() * 2.0 ** 14).round() * 2.0 ** -14            # (sums of such numbers are exact in f32)
+    other = x.clone()
+    other[..., 0] = 5 * 2.0 ** -8 + torch.randint(0, 32, x.shape[:2], generator=g) * 2.0 ** -14
+    x[..., 0] = 2.0 ** -6
+    return torch.cat([x, other], -1).bfloat16(), cache, table, offsets, n
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_sums_of_queries_beside_large_minima(cuda_device, seed):
+    """A score is the difference of two products of a minimum and a sum, each of which may be rounded sixteen times as an f32 sum is: that
+    changes a row by its weights' share of what they are off by, times their values' distance from the row."""
+    data = opposite_minima(seed)
+    q, (k_codes, k_scales, v_codes, v_scales), table, offsets, n = data
+    out, bound = reference(data, 64)
+    sums = q.double().unflatten(-1, (2, 64)).sum(-1)
+    values, _ = oracle.values(v_codes, v_scales, 64)
+    keys, _ = oracle.values(k_codes, k_scales, 64)
+    for b in range(2):
+        j = torch.arange(int(n[b]))
+        at = table[b, j // 16].long(), j % 16
+        for h in range(4):
+            head = h // 2
+            w = torch.softmax((keys[at[0], head, at[1]] @ q[b, h].double()) / 128 ** 0.5, 0)
+            minima = k_scales[at[0], head, at[1]].double()[:, 1::2].abs()
+            off = 16 * 2.0 ** -24 * (minima @ sums[b, h].abs()) / 128 ** 0.5
+            bound[b, h] += ((w * off.expm1())[:, None] * (values[at[0], head, at[1]] - out[b, h]).abs()).sum(0)
+    artifact = ib.compile(ib.programs.paged_decode_attention_int4, constexprs={"ACT_DTYPE": "bf16", "GROUP_SIZE": 64})
+    assert_close(run(artifact, cuda_device, data, True), (out, bound))
