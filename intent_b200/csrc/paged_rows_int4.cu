@@ -242,8 +242,10 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
   uint32_t q_parts[NT][2];
   float o[NT][CHUNKS][2][4];             // sums of codes: elements 32 c + 4 (lane / 4) + 2 t (+ 1, times 16) of rows 2 (lane % 4) (+ 1)
   const int upper = COPIES == 2 ? (lane & 3) >> 1 : 0;   // this thread's half of the groups
-  float eights[NT][SETS][4];             // sums of the weights that the codes are multiplied with, of the same rows (twice)
-  float middle[NT][2][SETS];             // sums of weight times minimum (and 8 scales), of this thread's tokens
+  // Sums of the weights that the codes are multiplied with, of the same rows (twice), and of weight times minimum (and 8 scales), of this
+  // thread's tokens: without the weights' 2^64, which large scales and minima of many tokens would take beyond f32.
+  float eights[NT][SETS][4];
+  float middle[NT][2][SETS];
   float top[NT][2];
   uint64_t weight_sum[NT];               // of both rows
   int position[NT][2];                   // of this thread's rows; -1 where there is none
@@ -483,7 +485,7 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
 #pragma unroll
             for (int g = 0; g < SETS; ++g) {
               const float by = Elem<T>::to_float(uint16_t(w.w[g])), from = Elem<T>::to_float(uint16_t(w.w[g] >> 16));
-              const float centre = SPLIT ? from : fmaf(8.f, by, from);
+              const float centre = (SPLIT ? from : fmaf(8.f, by, from)) * 0x1p-64f;
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
                 float scaled[2];
@@ -503,7 +505,7 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
             }
           }
           if (!SPLIT) {
-            constexpr uint32_t ONES = 0x3f803f80u;
+            constexpr uint32_t ONES = 0x1f801f80u;       // 2^-64
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -568,7 +570,7 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
             float m = middle[nt][e][g];
 #pragma unroll
             for (int d = 4; d < 32; d *= 2) m += __shfl_xor_sync(0xffffffffu, m, d);
-            constant[g] = (SPLIT ? m : fmaf(-8.f, eights[nt][g][e], m)) * 0x1p-64f;
+            constant[g] = SPLIT ? m : fmaf(-8.f, eights[nt][g][e], m);
           }
           const int token = (tile_row + min(r, rows - 1)) / p.group, of_group = tile_row + min(r, rows - 1) - token * p.group;
           uint16_t* to = p.out + (int64_t(work.s.first_row + token) * p.q_heads + work.head * p.group + of_group) * D + 4 * (lane >> 2);

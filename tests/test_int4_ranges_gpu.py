@@ -6,7 +6,7 @@ import torch
 
 import intent_b200 as ib
 from oracle import attention as oracle
-from test_int4_attention_gpu import assert_close, make, reference, run
+from test_int4_attention_gpu import assert_close, make, of_rounded, reference, run
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +49,31 @@ def test_sums_of_queries_beside_large_minima(cuda_device, seed):
             bound[b, h] += ((w * off.expm1())[:, None] * (values[at[0], head, at[1]] - out[b, h]).abs()).sum(0)
     artifact = ib.compile(ib.programs.paged_decode_attention_int4, constexprs={"ACT_DTYPE": "bf16", "GROUP_SIZE": 64})
     assert_close(run(artifact, cuda_device, data, True), (out, bound))
+
+
+@pytest.mark.parametrize("single", [True, False])
+@pytest.mark.parametrize("power", [60, 64, 100])
+@pytest.mark.parametrize("HQ,D,group", [(4, 128, 64), (16, 64, 32), (32, 128, 128)])
+def test_values_with_large_minima(cuda_device, single, power, HQ, D, group):
+    """Groups of equal numbers (their scale is 0), thousands of them as large as the type allows beside a weight."""
+    data = make([2500, 3], [1, 1] if single else [2, 3], HQ, 2, D, 32, group, "bf16")
+    q, cache, table, offsets, n = data
+    cache[3] = cache[3].unflatten(-1, (-1, 2)).mul(torch.tensor([0.0, 2.0 ** power])).flatten(-2).bfloat16()
+    cache[3].masked_fill_(cache[1].isnan(), math.nan)
+    program = ib.programs.paged_decode_attention_int4 if single else ib.programs.paged_attention_int4
+    artifact = ib.compile(program, constexprs={"GROUP_SIZE": group})
+    assert_close(run(artifact, cuda_device, data, single), reference(data, group), of_rounded(data, group))
+
+
+@pytest.mark.parametrize("HQ,D,group", [(4, 128, 64), (8, 64, 32), (16, 128, 128)])
+def test_values_with_large_scales(cuda_device, HQ, D, group):
+    """Scales up to 2^55, thousands of them with weights alike, in so many sequences that one warp has a whole one."""
+    L, B = 3000, 2400
+    q, cache, table, _, n = make([L], [1], HQ, 1, D, 64, group, "bf16")
+    cache[3] = cache[3] * 2.0 ** 54 / cache[3][..., ::2].nan_to_num().max()
+    q = 0.01 * q.repeat(4, 1, 1) * torch.tensor([1.0, -1.0, 2.0, 0.0])[:, None, None].bfloat16()
+    artifact = ib.compile(ib.programs.paged_decode_attention_int4, constexprs={"GROUP_SIZE": group})
+    out = artifact.run(*(t.to(cuda_device) for t in (q.repeat(B // 4, 1, 1), *cache, table.repeat(B, 1), n.repeat(B))))
+    expected = reference((q, cache, table.repeat(4, 1), torch.arange(5, dtype=torch.int32), n.repeat(4)), group)
+    for part in out.split(4)[::50]:
+        assert_close(part, expected)
