@@ -10,9 +10,15 @@
 // exponent 2^64 and a query's 2^60 larger no product comes near the ends of f32.  (Queries of 2^67 and more and scales of values
 // of 2^55 and more are out of that range, and below f32's smallest normal number, 2^-126, are 2^-57 of s n and 2^-53 of x n.)
 //
-// All statistics and sums are in f32, or in three bf16 parts that have its bits.  A weight times its scale is rounded to bf16 for the product with the codes, and the same
-// rounded numbers are added up for the middle of the codes (8), which is taken off again: the rounding is worth what it is for a
-// product with v_j.  For f16 results the product is made with what the rounding left over, too.
+// All statistics and sums are in f32, or in three bf16 parts that have its bits.  A weight times its scale is rounded to bf16 for the
+// product with the codes.  The same rounded numbers times the middle of the codes (8 and 7 in turn) are taken off, and the middle's
+// share is added up apart: the rounding is worth what it is for a product with v_j.  For f16 results the product is made with what
+// the rounding left over, too.
+//
+// A product adds to its sum by cutting, not by rounding, which one way or the other makes a sum of codes, which only grows, too
+// small: after 65536 tokens of a row in one warp by more than a tenth of the result.  So the middle is taken off in every step, and
+// in every LEVEL-th (or where a maximum is raised) what the sums of a row's group have in common goes to the middle's sum: what is
+// cut is a part of what is left then (2.5 10^-4 of the result where f16's rounding is worth 2 10^-4).
 //
 // With a quarter of the bytes of 16-bit elements there is a quarter of the time, and what all warps of a CTA have to wait for costs
 // four times as much.  So the line of steps (as in paged_rows.cu, but of UNIT tokens each) is cut into a share for every warp,
@@ -23,11 +29,11 @@
 // Copies are made by the warps that read them (cp.async): a TMA copy needs a lane of its own, and with four of them per step they
 // were a quarter of a step's instructions (74 -> 70 us below).
 //
-// Measured on one B200 (6540 GB/s copied; bf16, 32 heads of 128 on 8, groups of 64): 64 histories of up to 8192 tokens 66 us, 4.8
-// TB/s (floor 49; copies alone 58, arithmetic alone 61 before four rows stood twice); groups of 32 71 us; 4 of up to 131072, 4 key
-// heads, groups of 128 42 us, 4.0 TB/s; 200 of up to 2048, 16 heads of 64, f16, groups of 32 79 us, 3.5 TB/s; one of 2000 10.1 us, the
-// reads one after another of two launches.  Bound by what a step of 64 tokens costs beside its bytes, 900 instructions on two
-// warps per scheduler, of which the ALU's are the masks (256 of 64 tokens' codes).
+// Measured on one B200 (6540 GB/s copied; bf16, 32 heads of 128 on 8, groups of 64): 64 histories of up to 8192 tokens 68 - 71 us, 4.6
+// TB/s (floor 49); 4 of up to 131072, 4 key heads, groups of 128 43 us, 3.9 TB/s; 200 of up to 2048, 16 heads of 64, f16, groups of 32
+// 86 us, 3.2 TB/s; one of 2000 10.4 us, the reads one after another of two launches.  Bound by what a step of 64 tokens costs beside
+// its bytes, 900 instructions on two warps per scheduler, of which the ALU's are the masks (256 of 64 tokens' codes).  Tiles of sixteen
+// rows of heads of 128 are out of registers and spill (36 to 530 bytes; f16 with groups of 32 most).
 // Tried and not kept: twelve warps with keys and values in slots of their own (more instructions issued, and more of them: 72 us where
 // eight warps took 70), steps of 32 or 48 tokens for sixteen or twelve (80, 76), of 32 for tiles of
 // sixteen rows (64 sequences of 16 heads of 64 on one: 151 us, 122 with 64), codes asked for in the second-level cache a step
@@ -109,6 +115,9 @@ __device__ __forceinline__ Words<N> lds(uint32_t addr) {
 
 using Wide = __nv_bfloat16;              // the type of the weights' product with the codes
 constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u;
+// The middle of the codes of an even token and of the odd one behind it, 8 and 7, negative, in the same places
+constexpr uint32_t LOW_CENTRE = 0x80078008u, HIGH_CENTRE = 0x80708080u;
+constexpr int LEVEL = 16;                // steps after which sums of codes are brought back to nothing on average
 
 // What the scores of keys' codes are multiplied with
 template <typename T>
@@ -140,6 +149,7 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
   // Columns of a product are the tile's rows, or these twice: then the upper half of the columns has the upper half of the groups.
   constexpr int COPIES = TILE == 4 && GROUPS > 1 ? 2 : 1, COLUMNS = ROWS / COPIES, SETS = GROUPS / COPIES;
   constexpr bool SPLIT = std::is_same<T, __half>::value;                // weights in two bf16 parts
+  constexpr float WEIGHT = SPLIT ? 1.f : 0x1p-64f;                      // what weights, 2^64 times what they are, come with in `middle`
   extern __shared__ unsigned char smem_raw[];
   programmatic_begin();
   const uint32_t base = (smem_u32(smem_raw) + 127u) & ~127u;
@@ -241,10 +251,11 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
   float q_sum[NT][2][GROUPS];
   uint32_t q_parts[NT][2];
   float o[NT][CHUNKS][2][4];             // sums of codes: elements 32 c + 4 (lane / 4) + 2 t (+ 1, times 16) of rows 2 (lane % 4) (+ 1)
+  const float centre = lane & 4 ? 7.f : 8.f;             // of the codes of this thread's tokens, which are odd or even
   const int upper = COPIES == 2 ? (lane & 3) >> 1 : 0;   // this thread's half of the groups
-  // Sums of the weights that the codes are multiplied with, of the same rows (twice), and of weight times minimum (and 8 scales), of this
-  // thread's tokens: without the weights' 2^64, which large scales and minima of many tokens would take beyond f32.
-  float eights[NT][SETS][4];
+  // Sums of weight times the middle of the codes (f16: times the minimum, and of what stands for weight times scale in the product,
+  // times the middle code), of this thread's tokens.  For bf16 without the weights' 2^64, which large minima of many tokens would
+  // take beyond f32.
   float middle[NT][2][SETS];
   float top[NT][2];
   uint64_t weight_sum[NT];               // of both rows
@@ -289,11 +300,7 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
         }
       }
 #pragma unroll
-      for (int i = 0; i < SETS; ++i) {
-        middle[nt][0][i] = middle[nt][1][i] = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) eights[nt][i][e] = 0.f;
-      }
+      for (int i = 0; i < SETS; ++i) middle[nt][0][i] = middle[nt][1][i] = 0.f;
       if (BY_PRODUCT) {
         uint32_t parts[2][2 * GROUPS] = {};
 #pragma unroll
@@ -435,7 +442,7 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
           for (int m = 1; m < PARTS; ++m) here[nt][e] = fmaxf(here[nt][e], fmaxf(s[nt][m][e], s[nt][m][e + 2]));
           raise |= here[nt][e] * scale > top[nt][e] + SLACK;           // (from -inf: any)
         }
-      if (__any_sync(0xffffffffu, raise)) {
+      if (__any_sync(0xffffffffu, raise || work.step % LEVEL == LEVEL - 1)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float factor[2];
@@ -451,15 +458,37 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
           }
           weight_sum[nt] = mul_two(weight_sum[nt], two(factor[0], factor[1]));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
+          for (int e = 0; e < 4; ++e)
 #pragma unroll
             for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
               for (int t = 0; t < 2; ++t) o[nt][c][t][e] *= factor[e & 1];
-#pragma unroll
-            for (int i = 0; i < SETS; ++i) eights[nt][i][e] *= factor[e & 1];
-          }
         }
+        // What the elements of a row's group have in common goes to its middle.
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int g = 0; g < SETS; ++g)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float mean = 0.f;          // of this thread's four elements of a chunk, as codes in the lowest four bits
+#pragma unroll
+              for (int c = 0; c < CHUNKS; ++c) {
+                if (c / OF_GROUP % SETS != g || (COPIES == 2 && c / OF_GROUP / SETS != upper)) continue;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) mean += fmaf(o[nt][c][t][e + 2], 0x1p-4f, o[nt][c][t][e]);
+              }
+#pragma unroll
+              for (int d = 4; d < 32; d *= 2) mean += __shfl_xor_sync(0xffffffffu, mean, d);
+              mean *= 1.f / GROUP;
+              middle[nt][e][g] = fmaf(mean * 0x1p66f, 0x1p64f * WEIGHT, middle[nt][e][g]);          // (an eighth of 2^69 in each of eight lanes)
+#pragma unroll
+              for (int c = 0; c < CHUNKS; ++c) {
+                if (c / OF_GROUP % SETS != g) continue;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) o[nt][c][t][e] -= mean, o[nt][c][t][e + 2] = fmaf(mean, -16.f, o[nt][c][t][e + 2]);
+              }
+            }
       }
       // weights, 2^64 times what they are
       const uint64_t scales = two(scale, scale);
@@ -468,6 +497,7 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
       for (int nt = 0; nt < NT; ++nt)
         origins[nt] = two(64.f - (top[nt][0] == -infinity ? 0.f : top[nt][0]), 64.f - (top[nt][1] == -infinity ? 0.f : top[nt][1]));
       auto add_values = [&](auto whole) {
+        float centres[NT][SETS][4] = {}; // minus the centre's part of what this step adds to o, in its places
 #pragma unroll
         for (int m = 0; m < PARTS; ++m) {
           uint32_t pf[NT][SETS][2], rest[NT][SETS][2];                 // (weights times scales)^T as B fragments
@@ -485,7 +515,7 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
 #pragma unroll
             for (int g = 0; g < SETS; ++g) {
               const float by = Elem<T>::to_float(uint16_t(w.w[g])), from = Elem<T>::to_float(uint16_t(w.w[g] >> 16));
-              const float centre = (SPLIT ? from : fmaf(8.f, by, from)) * 0x1p-64f;
+              const float middle_here = SPLIT ? from : fmaf(centre, by, from) * WEIGHT;
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
                 float scaled[2];
@@ -494,24 +524,26 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
                   // (what is hidden may be anything, and 0 * NaN is NaN)
                   const bool seen = decltype(whole)::value || !(hidden[nt] >> (4 * m + 2 * h + e) & 1);
                   scaled[e] = seen ? s[nt][m][2 * h + e] * by : 0.f;
-                  if (seen) middle[nt][e][g] = fmaf(s[nt][m][2 * h + e], centre, middle[nt][e][g]);
+                  if (seen) middle[nt][e][g] = fmaf(s[nt][m][2 * h + e], middle_here, middle[nt][e][g]);
                 }
                 const uint32_t rounded = Elem<Wide>::pack2(scaled[0], scaled[1]);
                 pf[nt][g][h] = movmatrix(rounded);
-                if (SPLIT)
-                  rest[nt][g][h] = movmatrix(Elem<Wide>::pack2(scaled[0] - Elem<Wide>::to_float(uint16_t(rounded)),
-                                                               scaled[1] - Elem<Wide>::to_float(uint16_t(rounded >> 16))));
+                if (SPLIT) {
+                  const float a = Elem<Wide>::to_float(uint16_t(rounded)), b = Elem<Wide>::to_float(uint16_t(rounded >> 16));
+                  rest[nt][g][h] = movmatrix(Elem<Wide>::pack2(scaled[0] - a, scaled[1] - b));
+                  middle[nt][0][g] = fmaf(a, centre, middle[nt][0][g]);
+                  middle[nt][1][g] = fmaf(b, centre, middle[nt][1][g]);
+                }
               }
             }
           }
-          if (!SPLIT) {
-            constexpr uint32_t ONES = 0x1f801f80u;       // 2^-64
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int g = 0; g < SETS; ++g)
-                Elem<Wide>::mma16816(eights[nt][g], ONES, ONES, ONES, ONES, pf[nt][g][0], pf[nt][g][1]);
-          }
+            for (int g = 0; g < SETS; ++g) {
+              const uint32_t(&f)[2] = pf[nt][g];
+              Elem<Wide>::mma16816(centres[nt][g], LOW_CENTRE, HIGH_CENTRE, LOW_CENTRE, HIGH_CENTRE, f[0], f[1]);
+            }
 #pragma unroll
           for (int pair = 0; pair < CHUNKS / 2; ++pair) {
             // codes of tokens 16 m + 2 (lane % 4) (+ 1; + 8): elements 32 c + 4 (lane / 4) .. of chunks 2 pair and 2 pair + 1
@@ -536,6 +568,14 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
               }
           }
         }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[nt][c][t][e] += centres[nt][c / OF_GROUP % SETS][e];
       };
       if (all) add_values(Bool<true>{});
       else add_values(Bool<false>{});
@@ -570,7 +610,7 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
             float m = middle[nt][e][g];
 #pragma unroll
             for (int d = 4; d < 32; d *= 2) m += __shfl_xor_sync(0xffffffffu, m, d);
-            constant[g] = SPLIT ? m : fmaf(-8.f, eights[nt][g][e], m);
+            constant[g] = m * (0x1p-64f / WEIGHT);
           }
           const int token = (tile_row + min(r, rows - 1)) / p.group, of_group = tile_row + min(r, rows - 1) - token * p.group;
           uint16_t* to = p.out + (int64_t(work.s.first_row + token) * p.q_heads + work.head * p.group + of_group) * D + 4 * (lane >> 2);

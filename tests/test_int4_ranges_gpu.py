@@ -6,7 +6,7 @@ import torch
 
 import intent_b200 as ib
 from oracle import attention as oracle
-from test_int4_attention_gpu import assert_close, make, of_rounded, reference, run
+from test_int4_attention_gpu import DTYPES, HALF_UNIT, assert_close, make, of_rounded, reference, run
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +77,35 @@ def test_values_with_large_scales(cuda_device, HQ, D, group):
     expected = reference((q, cache, table.repeat(4, 1), torch.arange(5, dtype=torch.int32), n.repeat(4)), group)
     for part in out.split(4)[::50]:
         assert_close(part, expected)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("skew", [False, True])
+@pytest.mark.parametrize("HQ,D,group", [(4, 128, 64), (8, 64, 32), (16, 128, 128)])
+def test_sums_over_long_histories(cuda_device, dtype, skew, HQ, D, group):
+    """So many sequences that one warp has a whole one of 65536 tokens, of which its sums must not lose what is below their last bits.
+    For a step of 64 tokens four products (f16: eight) are added to a sum of codes, and as many to what is taken off it for the
+    middle of the codes.  An addition may cut the sum, by 2^-23 of it, which is at most what sixteen steps leave between them (7.5
+    scales a weight) and one puts on top (15).  Whatever else is rounded goes either way: the mean of the results is four of its
+    deviations from that at most."""
+    L, B = 65536, 2400
+    q, cache, table, _, n = make([L], [1], HQ, 1, D, 64, group, dtype)
+    g = torch.Generator().manual_seed(1)
+    q = torch.randn((4, HQ, D), generator=g).to(DTYPES[dtype])
+    if skew:                             # (most codes are low ones)
+        unused = cache[3].isnan()
+        x = torch.empty((*cache[2].shape[:-1], D)).exponential_(generator=g) - 1
+        cache[2], cache[3] = oracle.quantise(x, group, DTYPES[dtype])
+        cache[3].masked_fill_(unused, math.nan)
+    artifact = ib.compile(ib.programs.paged_decode_attention_int4, constexprs={"ACT_DTYPE": dtype, "GROUP_SIZE": group})
+    out = artifact.run(*(t.to(cuda_device) for t in (q.repeat(B // 4, 1, 1), *cache, table.repeat(B, 1), n.repeat(B)))).cpu()
+    once = q, cache, table.repeat(4, 1), torch.arange(5, dtype=torch.int32), n.repeat(4)
+    expected, bound = reference(once, group)
+    for part in out.split(4)[::50]:
+        assert_close(part, (expected, bound))
+    cut = 8 * (16 * 7.5 + 15) * 2.0 ** -23 * float(cache[3][..., ::2].double().nanmean())
+    # (deviation of an element: half a unit of the result, and of 5 scales' weights over the root of their number)
+    half, size = HALF_UNIT[dtype], float(expected.square().mean().sqrt()) + 5 * 2.0 ** -8
+    off = float((out[:4].double() - expected).mean())
+    print("off by %.2g, %.2g of the result" % (off, off / float(expected.square().mean().sqrt())))
+    assert abs(off) <= cut + 4 * half * size / expected.numel() ** 0.5, (off, cut)
