@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace ib200 {
 
 // ---- host: tensor maps -----------------------------------------------------
@@ -14,21 +16,36 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
+// A function of the driver; null where there is none (asked for until there is: a call that fails does not decide for those after it)
+template <typename Fn>
+inline Fn driver_fn(std::atomic<Fn>& found, const char* name) {
+  Fn fn = found.load(std::memory_order_relaxed);
+  if (fn) return fn;
+  void* p = nullptr;
+  cudaDriverEntryPointQueryResult query;
+  if (cudaGetDriverEntryPoint(name, &p, cudaEnableDefault, &query) != cudaSuccess) {
+    cudaGetLastError();
+    return nullptr;
+  }
+  fn = query == cudaDriverEntryPointSuccess ? reinterpret_cast<Fn>(p) : nullptr;
+  if (fn) found.store(fn, std::memory_order_relaxed);
+  return fn;
+}
+
 inline EncodeTiledFn encode_tiled_fn() {
-  static EncodeTiledFn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult query;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &query) != cudaSuccess ||
-        query != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return reinterpret_cast<EncodeTiledFn>(p);
-  }();
+  static std::atomic<EncodeTiledFn> encode{nullptr};
+  static std::atomic<CUresult (*)(CUcontext*)> current{nullptr};
   // A map is encoded in the calling thread's context, which a thread has not before its first call that needs one.
-  thread_local const bool bound = [] {
+  CUcontext context = nullptr;
+  const auto get = driver_fn(current, "cuCtxGetCurrent");
+  if (!get || get(&context) != CUDA_SUCCESS || !context) {
     int device = 0;
-    return cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess;
-  }();
-  return bound ? fn : nullptr;
+    if (cudaGetDevice(&device) != cudaSuccess || cudaSetDevice(device) != cudaSuccess) {
+      cudaGetLastError();
+      return nullptr;
+    }
+  }
+  return driver_fn(encode, "cuTensorMapEncodeTiled");
 }
 
 // Row-major 2-D tensor [rows][cols]; `pitch_bytes` between rows (multiple of 16);
