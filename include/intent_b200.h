@@ -562,10 +562,11 @@ INTENT_B200_API int intent_b200_paged_kv_append_norm_bf16(INTENT_B200_VIEW3(q), 
  *   k_scales, v_scales [PAGES, HK, PAGE, 2 D / group] f16 | bf16   scale s and minimum m, one after the other, of every `group`
  *                                      (32, 64 or 128, up to D) consecutive elements: a code n stands for m + s * n
  * append: rows as above; m = min and s = (max - min) / 15 of a group, rounded to the type, n = (x - m) / s rounded to the nearest
- * (even) of 0 .. 15; n = 0 where s = 0.  Where m + 15 s would be beyond the type, s is the next lower number.  Keys are not rounded
- * between their norm and rotation and this.  Minima, scales and codes of both are those of 64-bit arithmetic.  A group with something that is
- * no finite number (or a minimum or scale beyond the type) is stored as s = m = NaN.  Two tokens with one slot: what is stored is
- * undefined.
+ * (even) of 0 .. 15; n = 0 where s = 0.  Where m + 15 s would be beyond the type, s is the next lower number: enough for elements
+ * within the type; a key beyond it is held where its group's m and s are numbers, and read as an infinity.  Keys are not rounded
+ * between their norm and rotation and this.  Minima, scales and codes are those of 64-bit arithmetic (minima and scales rounded to
+ * the type by way of f32).  A group with something that is no finite number (or a minimum or scale beyond the type) is stored as
+ * s = m = NaN.  Two tokens with one slot: what is stored is undefined.
  * read: k, v [T, HK, D] of the tokens at slots [T] i64, m + s * n in f32 rounded to the type; zeros for a slot outside the cache.
  * ------------------------------------------------------------------------ */
 INTENT_B200_API int intent_b200_paged_kv_append_int4_f16(

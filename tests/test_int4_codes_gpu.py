@@ -100,3 +100,28 @@ def test_equal_numbers_of_every_size(cuda_device, dtype, D, group):
     for codes, scales in (held[:2], held[2:]):
         assert not codes.any()
         assert not scales[..., ::2].any() and torch.equal(scales[..., 1::2], x[..., ::group])
+
+
+def test_keys_beyond_the_type(cuda_device):
+    """A key that the rotation takes beyond f16 is held as long as its group's minimum and scale are numbers; what it stands for is
+    infinite when read in f16, as such a key is in a 16-bit cache."""
+    g = torch.Generator().manual_seed(0)
+    k = (20000 * torch.randn((5, 1, 64), generator=g)).clamp(-40000, 40000).half()
+    k[:, 0, 0], k[:, 0, 1] = 60000, -50000
+    k[4, 0, 2] = -60000                                     # (its minimum is beyond the type, too)
+    rotary = torch.zeros((1, 64))
+    rotary[:, :32] = 1.2
+    held = append(cuda_device, k, k, 64, "f16", rotary=rotary)
+    keys = oracle.rotate(k, torch.zeros(5, dtype=torch.int64), rotary)
+    codes, scales = oracle.quantise(keys, 64, torch.float16)
+    assert torch.equal(held[0], codes) and torch.equal(held[1].nan_to_num(-1.0), scales.nan_to_num(-1.0))
+    assert scales[:4].isfinite().all() and scales[4].isnan().all()
+    value, _ = oracle.values(codes[:4], scales[:4], 64)
+    cache = empty_cache(1, 1, 16, 64, 64, "f16", cuda_device)
+    slots = torch.arange(5)
+    for to, part in zip(cache, held):
+        to[0, :, :5] = part.transpose(0, 1).to(cuda_device)
+    out = ib.compile(ib.programs.paged_kv_read_int4, constexprs={"ACT_DTYPE": "f16", "GROUP_SIZE": 64}).run(slots.to(cuda_device), *cache)
+    read = out[0].cpu()
+    assert torch.equal(read[:4], value.half()) and read[4].isnan().all()
+    assert (read[:4, 0, 0] == torch.inf).all() and read[:4].isfinite().float().mean() > 0.9
