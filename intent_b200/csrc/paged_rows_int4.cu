@@ -6,19 +6,19 @@
 //   x . k_j = sum_g s_jg (x_g . n_jg) + m_jg sum(x_g)            o = sum_j w_j v_j = sum_g (sum_j (w_j s_jg) n_jg + sum_j w_j m_jg)
 // Four bits become operands of the tensor core by being masked where they are: in the lowest or the next four bits of a 16-bit
 // word they are n or 16 n times the smallest bf16 (2^-133; an f16 too, 2^-24, in the lowest four), exact numbers for it.  The factor of
-// 16 is taken out of the queries (bf16) or the results ahead, so that eight codes cost five instructions; with a weight's
-// exponent 2^64 and a query's 2^60 larger no product comes near the ends of f32.  (Queries of 2^67 and more and scales of values
-// of 2^55 and more are out of that range, and below f32's smallest normal number, 2^-126, are 2^-57 of s n and 2^-53 of x n.)
+// 16 is taken out of the queries (bf16) or the results ahead, so that eight codes cost five instructions; with 2^64 on weight times
+// scale and 2^60 on a query no product comes near the ends of f32.  (Queries of 2^67 and more and scales of values of 2^55 and more
+// are out of that range, and below f32's smallest normal number, 2^-126, are 2^-57 of s n and 2^-53 of x n.)
 //
 // All statistics and sums are in f32, or in three bf16 parts that have its bits.  A weight times its scale is rounded to bf16 for the
 // product with the codes.  The same rounded numbers times the middle of the codes (8 and 7 in turn) are taken off, and the middle's
 // share is added up apart: the rounding is worth what it is for a product with v_j.  For f16 results the product is made with what
 // the rounding left over, too.
 //
-// A product adds to its sum by cutting, not by rounding, which one way or the other makes a sum of codes, which only grows, too
-// small: after 65536 tokens of a row in one warp by more than a tenth of the result.  So the middle is taken off in every step, and
-// in every LEVEL-th (or where a maximum is raised) what the sums of a row's group have in common goes to the middle's sum: what is
-// cut is a part of what is left then (2.5 10^-4 of the result where f16's rounding is worth 2 10^-4).
+// A product cuts, instead of rounding, what it adds to, and a sum of codes only grows: after 131072 tokens of a row in one warp it
+// was too small by a fifth of the result.  So the middle is taken off in every step, and in every LEVEL-th (or where a maximum is
+// raised) what the sums of a row's group have in common goes to the middle's sum.  What is cut is a part of what is left then
+// (131072 tokens, f16: results off by 2.5 10^-4, of which 2.1 are their own rounding; skewed values 3.1).
 //
 // With a quarter of the bytes of 16-bit elements there is a quarter of the time, and what all warps of a CTA have to wait for costs
 // four times as much.  So the line of steps (as in paged_rows.cu, but of UNIT tokens each) is cut into a share for every warp,
@@ -30,7 +30,7 @@
 // were a quarter of a step's instructions (74 -> 70 us below).
 //
 // Measured on one B200 (6540 GB/s copied; bf16, 32 heads of 128 on 8, groups of 64): 64 histories of up to 8192 tokens 68 - 71 us, 4.6
-// TB/s (floor 49); 4 of up to 131072, 4 key heads, groups of 128 43 us, 3.9 TB/s; 200 of up to 2048, 16 heads of 64, f16, groups of 32
+// TB/s (floor 49); 4 of up to 131072, 4 key heads, groups of 128 44 us, 3.9 TB/s; 200 of up to 2048, 16 heads of 64, f16, groups of 32
 // 86 us, 3.2 TB/s; one of 2000 10.4 us, the reads one after another of two launches.  Bound by what a step of 64 tokens costs beside
 // its bytes, 900 instructions on two warps per scheduler, of which the ALU's are the masks (256 of 64 tokens' codes).  Tiles of sixteen
 // rows of heads of 128 are out of registers and spill (36 to 530 bytes; f16 with groups of 32 most).
@@ -149,7 +149,8 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
   // Columns of a product are the tile's rows, or these twice: then the upper half of the columns has the upper half of the groups.
   constexpr int COPIES = TILE == 4 && GROUPS > 1 ? 2 : 1, COLUMNS = ROWS / COPIES, SETS = GROUPS / COPIES;
   constexpr bool SPLIT = std::is_same<T, __half>::value;                // weights in two bf16 parts
-  constexpr float WEIGHT = SPLIT ? 1.f : 0x1p-64f;                      // what weights, 2^64 times what they are, come with in `middle`
+  // The 2^64 of the product with codes, on the weights (f16) or on the scales (bf16, whose minima times 2^64 would leave f32's range).
+  constexpr float OF_WEIGHTS = SPLIT ? 64.f : 0.f, UNIT_OF_WEIGHTS = SPLIT ? 0x1p-64f : 1.f, OF_SCALES = SPLIT ? 1.f : 0x1p64f;
   extern __shared__ unsigned char smem_raw[];
   programmatic_begin();
   const uint32_t base = (smem_u32(smem_raw) + 127u) & ~127u;
@@ -254,8 +255,7 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
   const float centre = lane & 4 ? 7.f : 8.f;             // of the codes of this thread's tokens, which are odd or even
   const int upper = COPIES == 2 ? (lane & 3) >> 1 : 0;   // this thread's half of the groups
   // Sums of weight times the middle of the codes (f16: times the minimum, and of what stands for weight times scale in the product,
-  // times the middle code), of this thread's tokens.  For bf16 without the weights' 2^64, which large minima of many tokens would
-  // take beyond f32.
+  // times the middle code), of this thread's tokens.
   float middle[NT][2][SETS];
   float top[NT][2];
   uint64_t weight_sum[NT];               // of both rows
@@ -481,7 +481,7 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
 #pragma unroll
               for (int d = 4; d < 32; d *= 2) mean += __shfl_xor_sync(0xffffffffu, mean, d);
               mean *= 1.f / GROUP;
-              middle[nt][e][g] = fmaf(mean * 0x1p66f, 0x1p64f * WEIGHT, middle[nt][e][g]);          // (an eighth of 2^69 in each of eight lanes)
+              middle[nt][e][g] = fmaf(mean * 0x1p66f, 1.f / UNIT_OF_WEIGHTS, middle[nt][e][g]);          // (an eighth of 2^69 in each of eight lanes)
 #pragma unroll
               for (int c = 0; c < CHUNKS; ++c) {
                 if (c / OF_GROUP % SETS != g) continue;
@@ -490,12 +490,13 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
               }
             }
       }
-      // weights, 2^64 times what they are
+      // weights
       const uint64_t scales = two(scale, scale);
       uint64_t origins[NT];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
-        origins[nt] = two(64.f - (top[nt][0] == -infinity ? 0.f : top[nt][0]), 64.f - (top[nt][1] == -infinity ? 0.f : top[nt][1]));
+        origins[nt] = two(OF_WEIGHTS - (top[nt][0] == -infinity ? 0.f : top[nt][0]),
+                          OF_WEIGHTS - (top[nt][1] == -infinity ? 0.f : top[nt][1]));
       auto add_values = [&](auto whole) {
         float centres[NT][SETS][4] = {}; // minus the centre's part of what this step adds to o, in its places
 #pragma unroll
@@ -515,7 +516,7 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
 #pragma unroll
             for (int g = 0; g < SETS; ++g) {
               const float by = Elem<T>::to_float(uint16_t(w.w[g])), from = Elem<T>::to_float(uint16_t(w.w[g] >> 16));
-              const float middle_here = SPLIT ? from : fmaf(centre, by, from) * WEIGHT;
+              const float middle_here = SPLIT ? from : fmaf(centre, by, from), factor = by * OF_SCALES;
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
                 float scaled[2];
@@ -523,7 +524,7 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
                 for (int e = 0; e < 2; ++e) {
                   // (what is hidden may be anything, and 0 * NaN is NaN)
                   const bool seen = decltype(whole)::value || !(hidden[nt] >> (4 * m + 2 * h + e) & 1);
-                  scaled[e] = seen ? s[nt][m][2 * h + e] * by : 0.f;
+                  scaled[e] = seen ? s[nt][m][2 * h + e] * factor : 0.f;
                   if (seen) middle[nt][e][g] = fmaf(s[nt][m][2 * h + e], middle_here, middle[nt][e][g]);
                 }
                 const uint32_t rounded = Elem<Wide>::pack2(scaled[0], scaled[1]);
@@ -603,14 +604,14 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
           float sum_all = e ? apart(weight_sum[nt]).y : apart(weight_sum[nt]).x;
 #pragma unroll
           for (int d = 4; d < 32; d *= 2) sum_all += __shfl_xor_sync(0xffffffffu, sum_all, d);
-          sum_all *= 0x1p-64f;
+          sum_all *= UNIT_OF_WEIGHTS;
           float constant[SETS];
 #pragma unroll
           for (int g = 0; g < SETS; ++g) {
             float m = middle[nt][e][g];
 #pragma unroll
             for (int d = 4; d < 32; d *= 2) m += __shfl_xor_sync(0xffffffffu, m, d);
-            constant[g] = m * (0x1p-64f / WEIGHT);
+            constant[g] = m * UNIT_OF_WEIGHTS;
           }
           const int token = (tile_row + min(r, rows - 1)) / p.group, of_group = tile_row + min(r, rows - 1) - token * p.group;
           uint16_t* to = p.out + (int64_t(work.s.first_row + token) * p.q_heads + work.head * p.group + of_group) * D + 4 * (lane >> 2);

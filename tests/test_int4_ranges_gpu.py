@@ -52,17 +52,19 @@ def test_sums_of_queries_beside_large_minima(cuda_device, seed):
 
 
 @pytest.mark.parametrize("single", [True, False])
-@pytest.mark.parametrize("power", [60, 64, 100])
+@pytest.mark.parametrize("power", [-100, 60, 64, 100])
 @pytest.mark.parametrize("HQ,D,group", [(4, 128, 64), (16, 64, 32), (32, 128, 128)])
-def test_values_with_large_minima(cuda_device, single, power, HQ, D, group):
-    """Groups of equal numbers (their scale is 0), thousands of them as large as the type allows beside a weight."""
+def test_values_of_every_size(cuda_device, single, power, HQ, D, group):
+    """Groups of equal numbers (their scale is 0): thousands of them as large as the type allows beside a weight, or very small."""
     data = make([2500, 3], [1, 1] if single else [2, 3], HQ, 2, D, 32, group, "bf16")
     q, cache, table, offsets, n = data
-    cache[3] = cache[3].unflatten(-1, (-1, 2)).mul(torch.tensor([0.0, 2.0 ** power])).flatten(-2).bfloat16()
+    cache[3] = cache[3].unflatten(-1, (-1, 2)).mul(torch.tensor([0.0, 1.0])).flatten(-2).bfloat16()
     cache[3].masked_fill_(cache[1].isnan(), math.nan)
+    expected = reference(data, group), of_rounded(data, group)
     program = ib.programs.paged_decode_attention_int4 if single else ib.programs.paged_attention_int4
     artifact = ib.compile(program, constexprs={"GROUP_SIZE": group})
-    assert_close(run(artifact, cuda_device, data, single), reference(data, group), of_rounded(data, group))
+    out = run(artifact, cuda_device, (q, [*cache[:3], cache[3] * 2.0 ** power], table, offsets, n), single)
+    assert_close(out.double() * 2.0 ** -power, *expected)
 
 
 @pytest.mark.parametrize("HQ,D,group", [(4, 128, 64), (8, 64, 32), (16, 128, 128)])
