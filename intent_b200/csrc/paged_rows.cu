@@ -66,6 +66,60 @@ constexpr int smem_bytes() {
 static_assert(smem_bytes<128, 2>() <= 227 * 1024 && smem_bytes<128, 1>() <= 227 * 1024 && smem_bytes<64, 2>() <= 227 * 1024,
               "shared memory of a CTA");
 
+// The warps' parts of a tile, [WARPS][ROWS][D] with pieces of eight elements in the order that swaps them by row, their maxima and
+// sums: the result where the CTA has the whole tile, a part for the join where it has not.
+template <typename T, int D, int ROWS, int WARPS>
+__device__ __forceinline__ void put_together(const PagedParams& p, int share, const float* join_here, const float* max_here,
+                                             const float* sum_here, RowsJoin* entry, int tile_row, int rows, int head, int first_row,
+                                             int sequence, int item_begin, int item_end) {
+  constexpr int THREADS = 32 * WARPS;
+  const float infinity = __int_as_float(0x7f800000);
+  const int cta = blockIdx.x, tid = threadIdx.x;
+  const bool begins = item_begin >= 0, whole = begins && item_end <= share;
+  float* part = p.parts + size_t(2 * cta + begins) * (ROWS * (D + 2));
+  auto place = [&](int r) {
+    const int token = (tile_row + r) / p.group, of_group = tile_row + r - token * p.group;
+    return p.out + (int64_t(first_row + token) * p.q_heads + head * p.group + of_group) * D;
+  };
+  for (int w = tid; w < rows * (D / 8); w += THREADS) {
+    const int r = w / (D / 8), c = w - r * (D / 8);
+    float m = -infinity, l = 0.f, x[8] = {};
+#pragma unroll
+    for (int v = 0; v < WARPS; ++v) m = fmaxf(m, max_here[v * ROWS + r]);
+    const float origin = m == -infinity ? 0.f : m;
+#pragma unroll
+    for (int v = 0; v < WARPS; ++v) {
+      const float f = exp2_fast(max_here[v * ROWS + r] - origin);
+      l = fmaf(sum_here[v * ROWS + r], f, l);
+      const float* from = join_here + (v * ROWS + r) * D + 8 * (c ^ (r >> 1 & 3));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = fmaf(from[e], f, x[e]);
+    }
+    if (whole) {
+      const float inverse = l == 0.f ? of_nothing(p, sequence, first_row + (tile_row + r) / p.group) : 1.f / l;
+      *reinterpret_cast<uint4*>(place(r) + 8 * c) =
+          make_uint4(Elem<T>::pack2(x[0] * inverse, x[1] * inverse), Elem<T>::pack2(x[2] * inverse, x[3] * inverse),
+                     Elem<T>::pack2(x[4] * inverse, x[5] * inverse), Elem<T>::pack2(x[6] * inverse, x[7] * inverse));
+    } else {
+      float4* to = reinterpret_cast<float4*>(part + r * D + 8 * c);
+      to[0] = make_float4(x[0], x[1], x[2], x[3]);
+      to[1] = make_float4(x[4], x[5], x[6], x[7]);
+      if (c == 0) {
+        part[ROWS * D + r] = m;
+        part[ROWS * (D + 1) + r] = l;
+      }
+    }
+  }
+  if (tid == 0 && !whole && begins) {
+    entry->row = first_row;
+    entry->head = head;
+    entry->tile_row = tile_row;
+    entry->rows = rows;
+    entry->sequence = sequence;
+    entry->last_cta = cta + (item_end - 1) / share;
+  }
+}
+
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(32 * Ring<D>::WARPS, 1)
 paged_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedParams p) {
