@@ -16,7 +16,8 @@
 //
 // Measured on one B200: 8192 tokens, 32 + 8 + 8 heads of 128, norm, bf16, with paged_kv_read_int4 of them 55 us (floor 33), of which the
 // read is 9, queries take 20 alone, keys 12 and values 6: bound by instructions, two thirds of the issue slots.  All keys in 64
-// bits 59; keys' blocks ahead of the others 63; with four rows of keys and 102 registers 76.
+// bits 59; keys' blocks ahead of the others 63; with four rows of keys and 102 registers 76.  (With norms and several rows a group the
+// 64 registers do not hold everything: 40 to 48 bytes are spilled.)
 #include "common.cuh"
 #include "paged.cuh"
 #include "rotate.cuh"

@@ -39,9 +39,11 @@ int device_sms() {
 //    (5.8 M) 306 and 212; and if there is no long one 16 of 4 tokens 40 and 47, 64 of 2 of up to 300 26 and 31, 4 of 4 of up to
 //    65536 105 and 113.
 // A cache in 4 bits is read four times as fast, and more of the time goes to what both kernels do with its codes: the rows kernel's
-// tiles are worth it for more rows.  us for the 64 sequences of up to 4000 tokens, 1 / 4 / 8 / 16 new ones each, groups of 64:
-// rows 41 / 67 / 116 / 211, chunk 146 / 147 / 149 / 148; heads of 64 28 / 39 / 69 / 114, chunk 130 throughout; 8 of up to 16000, 4 / 8
-// / 16: rows 41 / 71 / 122, chunk 82.  The launch that may find nothing to do costs 12 us there (64 of 4 tokens: 67 and 79).
+// tiles are worth it for more rows.  us for the 64 sequences of up to 4000 tokens, 1 / 4 / 8 new ones each, bf16, groups of 64: rows
+// 40 / 85 / 133, from four on with the 12 of a launch that finds nothing to do; 16, by the chunk kernel, 155 (4 to 16 all take it 146 -
+// 155).  Heads of 64: rows 29 / 47 / 77, 16 of them 126, chunk 130; 8 of up to 16000: rows 28 / 54 / 78, chunk 89.  (f16's tiles of
+// sixteen rows are slower: 8 new ones 168, with groups of 32 271, where the chunk kernel takes about 155.  The limits are the same for both
+// types, as what a call's workspace holds is asked for without one.  MOST is that of 16-bit elements.)
 struct Choice {
   int tile_rows;           // of the rows kernel; 0: it is not needed
   int few;                 // rows up to which a sequence is its

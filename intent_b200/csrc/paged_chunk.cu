@@ -21,8 +21,9 @@
 // Of a cache in 4 bits (GROUP > 0) codes and scales come by bulk copies, a run of bytes per page, and four warps turn them into the
 // operands, numbers of the 16-bit type, in the ring's slots.  Rounding them is what reading the cache back would do.  A pair of codes
 // costs four instructions for keys, three for values, whose columns then lie in another order (column_of).  4096 tokens behind 12288
-// take 1014 us with groups of 32, the same call on 16-bit elements 920.  (With three for keys, too, which would need the queries in
-// that order, it is the same time.)
+// take 1010 - 1018 us with groups of 32, the same call on 16-bit elements 920.  (With three for keys, too, which would need the
+// queries in that order, it is the same time.)  The rows' threads have 208 registers here in place of 224, and 38 to 46 bytes of
+// them are spilled.
 //
 // Measured on one B200: 4096 tokens behind 12288, 32 heads of 128 on 8 key heads, bf16: 0.92 ms, 1.05 PFLOP/s of what the queries
 // see, at the power cap (1.6 GHz, 1000 W).  A step takes 3500 cycles there: the tensor core is busy for 58 % of them (a half's two

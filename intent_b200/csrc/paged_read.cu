@@ -3,7 +3,7 @@
 // A slot outside the cache (-1) gives a row of zeros.
 //
 // Bound by HBM, and by what it writes: 2 D bytes a row for D / 2 + 4 D / GROUP read.  A thread turns eight codes of keys and eight of
-// values of two rows into 16 bytes each (65536 tokens, 8 heads of 128, bf16: with one row 73 us, with two 59, with four 60; 5.7 TB/s).
+// values of two rows into 16 bytes each (65536 tokens, 8 heads of 128, bf16: with one row 73 us, with two 59 - 61, with four 60; 5.6 TB/s).
 #include "common.cuh"
 #include "paged.cuh"
 
