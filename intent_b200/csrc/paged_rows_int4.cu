@@ -16,9 +16,9 @@
 // the rounding left over, too.
 //
 // A product cuts, instead of rounding, what it adds to, and a sum of codes only grows: after 131072 tokens of a row in one warp it
-// was too small by a fifth of the result.  So the middle is taken off in every step, and in every LEVEL-th (or where a maximum is
-// raised) what the sums of a row's group have in common goes to the middle's sum.  What is cut is a part of what is left then
-// (131072 tokens, f16: results off by 2.5 10^-4, of which 2.1 are their own rounding; skewed values 3.1).
+// was too small by a fifth of the result.  So the middle is taken off in every step, and in every LEVEL-th what the sums of a row's
+// group have in common goes to the middle's sum.  What is cut is a part of what is left then (131072 tokens, f16: results off by
+// 2.5 10^-4, of which 2.1 are their own rounding; skewed values 3.1).
 //
 // With a quarter of the bytes of 16-bit elements there is a quarter of the time, and what all warps of a CTA have to wait for costs
 // four times as much.  So the line of steps (as in paged_rows.cu, but of UNIT tokens each) is cut into a share for every warp,
@@ -33,7 +33,7 @@
 // TB/s (floor 49); 4 of up to 131072, 4 key heads, groups of 128 44 us, 3.9 TB/s; 200 of up to 2048, 16 heads of 64, f16, groups of 32
 // 86 us, 3.2 TB/s; one of 2000 10.4 us, the reads one after another of two launches.  Bound by what a step of 64 tokens costs beside
 // its bytes, 900 instructions on two warps per scheduler, of which the ALU's are the masks (256 of 64 tokens' codes).  Tiles of sixteen
-// rows of heads of 128 are out of registers and spill (36 to 530 bytes; f16 with groups of 32 most).
+// rows of heads of 128 are out of registers and spill (28 to 136 bytes; f16 88 to 116, with groups of 32 532).
 // Tried and not kept: twelve warps with keys and values in slots of their own (more instructions issued, and more of them: 72 us where
 // eight warps took 70), steps of 32 or 48 tokens for sixteen or twelve (80, 76), of 32 for tiles of
 // sixteen rows (64 sequences of 16 heads of 64 on one: 151 us, 122 with 64), codes asked for in the second-level cache a step
@@ -442,7 +442,8 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
           for (int m = 1; m < PARTS; ++m) here[nt][e] = fmaxf(here[nt][e], fmaxf(s[nt][m][e], s[nt][m][e + 2]));
           raise |= here[nt][e] * scale > top[nt][e] + SLACK;           // (from -inf: any)
         }
-      if (__any_sync(0xffffffffu, raise || work.step % LEVEL == LEVEL - 1)) {
+      const bool level = work.step % LEVEL == LEVEL - 1;
+      if (__any_sync(0xffffffffu, raise || level)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float factor[2];
@@ -464,31 +465,36 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
 #pragma unroll
               for (int t = 0; t < 2; ++t) o[nt][c][t][e] *= factor[e & 1];
         }
-        // What the elements of a row's group have in common goes to its middle.
+        // What the elements of a row's group have in common goes to its middle.  (In this branch, which is rarely taken: behind the
+        // product with values it cost 3 to 9 %.  Where registers are spilled, whenever it is taken: 8 new tokens for each of 64 sequences,
+        // groups of 32, 177 us, 202 with a branch of its own; other tiles are 1 to 2 % faster with that.)
+        if (level || SETS * NT > 4) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int g = 0; g < SETS; ++g)
+            for (int g = 0; g < SETS; ++g)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float mean = 0.f;          // of this thread's four elements of a chunk, as codes in the lowest four bits
+              for (int e = 0; e < 2; ++e) {
+                float mean = 0.f;          // of this thread's four elements of a chunk, as codes in the lowest four bits
 #pragma unroll
-              for (int c = 0; c < CHUNKS; ++c) {
-                if (c / OF_GROUP % SETS != g || (COPIES == 2 && c / OF_GROUP / SETS != upper)) continue;
+                for (int c = 0; c < CHUNKS; ++c) {
+                  if (c / OF_GROUP % SETS != g || (COPIES == 2 && c / OF_GROUP / SETS != upper)) continue;
 #pragma unroll
-                for (int t = 0; t < 2; ++t) mean += fmaf(o[nt][c][t][e + 2], 0x1p-4f, o[nt][c][t][e]);
+                  for (int t = 0; t < 2; ++t) mean += fmaf(o[nt][c][t][e + 2], 0x1p-4f, o[nt][c][t][e]);
+                }
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2) mean += __shfl_xor_sync(0xffffffffu, mean, d);
+                mean *= 1.f / GROUP;
+                // (an eighth of 2^69 in each of eight lanes)
+                middle[nt][e][g] = fmaf(mean * 0x1p66f, 1.f / UNIT_OF_WEIGHTS, middle[nt][e][g]);
+#pragma unroll
+                for (int c = 0; c < CHUNKS; ++c) {
+                  if (c / OF_GROUP % SETS != g) continue;
+#pragma unroll
+                  for (int t = 0; t < 2; ++t) o[nt][c][t][e] -= mean, o[nt][c][t][e + 2] = fmaf(mean, -16.f, o[nt][c][t][e + 2]);
+                }
               }
-#pragma unroll
-              for (int d = 4; d < 32; d *= 2) mean += __shfl_xor_sync(0xffffffffu, mean, d);
-              mean *= 1.f / GROUP;
-              middle[nt][e][g] = fmaf(mean * 0x1p66f, 1.f / UNIT_OF_WEIGHTS, middle[nt][e][g]);          // (an eighth of 2^69 in each of eight lanes)
-#pragma unroll
-              for (int c = 0; c < CHUNKS; ++c) {
-                if (c / OF_GROUP % SETS != g) continue;
-#pragma unroll
-                for (int t = 0; t < 2; ++t) o[nt][c][t][e] -= mean, o[nt][c][t][e + 2] = fmaf(mean, -16.f, o[nt][c][t][e + 2]);
-              }
-            }
+        }
       }
       // weights
       const uint64_t scales = two(scale, scale);
