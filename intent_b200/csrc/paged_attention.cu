@@ -40,10 +40,10 @@ int device_sms() {
 //    65536 105 and 113.
 // A cache in 4 bits is read four times as fast, and more of the time goes to what both kernels do with its codes: the rows kernel's
 // tiles are worth it for more rows.  us for the 64 sequences of up to 4000 tokens, 1 / 4 / 8 new ones each, bf16, groups of 64: rows
-// 40 / 84 / 130, from four on with the 12 of a launch that finds nothing to do; 16, by the chunk kernel, 155 (4 to 16 all take it 146 -
-// 155).  Heads of 64: rows 29 / 47 / 77, 16 of them 126, chunk 130; 8 of up to 16000: rows 28 / 54 / 78, chunk 89.  (f16's tiles of
-// sixteen rows are slower: 8 new ones 167, with groups of 32 270, where the chunk kernel takes about 155.  The limits are the same for both
-// types, as what a call's workspace holds is asked for without one.  MOST is that of 16-bit elements.)
+// 40 / 83 / 130, from four on with the 12 of a launch that finds nothing to do; 16, by the chunk kernel, 155 (4 to 16 all take it 146 -
+// 155).  Heads of 64: rows 29 / 47 / 77, 16 of them 126, chunk 130; 8 of up to 16000: rows 28 / 54 / 78, chunk 89.  (8 new ones
+// in f16 151; groups of 32 179, f16 210, where the chunk kernel would be faster: the limits are the same for all groups and types, as
+// what a call's workspace holds is asked for without them.  MOST is that of 16-bit elements.)
 struct Choice {
   int tile_rows;           // of the rows kernel; 0: it is not needed
   int few;                 // rows up to which a sequence is its

@@ -13,12 +13,12 @@
 // All statistics and sums are in f32, or in three bf16 parts that have its bits.  A weight times its scale is rounded to bf16 for the
 // product with the codes.  The same rounded numbers times the middle of the codes (8 and 7 in turn) are taken off, and the middle's
 // share is added up apart: the rounding is worth what it is for a product with v_j.  For f16 results the product is made with what
-// the rounding left over, too.
+// the rounding left over, too, and nothing is taken off.
 //
 // A product cuts, instead of rounding, what it adds to, and a sum of codes only grows: after 131072 tokens of a row in one warp it
-// was too small by a fifth of the result.  So the middle is taken off in every step, and in every LEVEL-th what the sums of a row's
-// group have in common goes to the middle's sum.  What is cut is a part of what is left then (131072 tokens, f16: results off by
-// 2.5 10^-4, of which 2.1 are their own rounding; skewed values 3.1).
+// was too small by a fifth of the result.  So the middle is taken off in every step (bf16), and in every LEVEL-th what the sums of a
+// row's group have in common goes to the sum of minima or middles.  What is cut is a part of what is left then (131072 tokens: f16
+// results are off by 2.9 10^-4, of which 2.1 are their own rounding, bf16 by 2.4 10^-3 and 1.7; skewed values 2.3 10^-4 and 2.9 10^-3).
 //
 // With a quarter of the bytes of 16-bit elements there is a quarter of the time, and what all warps of a CTA have to wait for costs
 // four times as much.  So the line of steps (as in paged_rows.cu, but of UNIT tokens each) is cut into a share for every warp,
@@ -31,9 +31,9 @@
 //
 // Measured on one B200 (6540 GB/s copied; bf16, 32 heads of 128 on 8, groups of 64): 64 histories of up to 8192 tokens 68 - 71 us, 4.6
 // TB/s (floor 49); 4 of up to 131072, 4 key heads, groups of 128 44 us, 3.9 TB/s; 200 of up to 2048, 16 heads of 64, f16, groups of 32
-// 86 us, 3.2 TB/s; one of 2000 10.4 us, the reads one after another of two launches.  Bound by what a step of 64 tokens costs beside
+// 81 us, 3.4 TB/s; one of 2000 10.5 us, the reads one after another of two launches.  Bound by what a step of 64 tokens costs beside
 // its bytes, 900 instructions on two warps per scheduler, of which the ALU's are the masks (256 of 64 tokens' codes).  Tiles of sixteen
-// rows of heads of 128 are out of registers and spill (28 to 136 bytes; f16 88 to 116, with groups of 32 532).
+// rows of heads of 128 are out of registers and spill (28 to 136 bytes).
 // Tried and not kept: twelve warps with keys and values in slots of their own (more instructions issued, and more of them: 72 us where
 // eight warps took 70), steps of 32 or 48 tokens for sixteen or twelve (80, 76), of 32 for tiles of
 // sixteen rows (64 sequences of 16 heads of 64 on one: 151 us, 122 with 64), codes asked for in the second-level cache a step
@@ -117,7 +117,6 @@ using Wide = __nv_bfloat16;              // the type of the weights' product wit
 constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u;
 // The middle of the codes of an even token and of the odd one behind it, 8 and 7, negative, in the same places
 constexpr uint32_t LOW_CENTRE = 0x80078008u, HIGH_CENTRE = 0x80708080u;
-constexpr int LEVEL = 16;                // steps after which sums of codes are brought back to nothing on average
 
 // What the scores of keys' codes are multiplied with
 template <typename T>
@@ -149,6 +148,11 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
   // Columns of a product are the tile's rows, or these twice: then the upper half of the columns has the upper half of the groups.
   constexpr int COPIES = TILE == 4 && GROUPS > 1 ? 2 : 1, COLUMNS = ROWS / COPIES, SETS = GROUPS / COPIES;
   constexpr bool SPLIT = std::is_same<T, __half>::value;                // weights in two bf16 parts
+  // Steps after which sums of codes are brought back to nothing on average.  (f16, for whose two products the middle is not taken off
+  // before, us of 200 histories of up to 2048, 16 heads of 64 / what results over 131072 tokens in one warp are off by, in 10^-4: 2
+  // steps 82.7 / 2.6, 4 81.1 / 2.9, 8 80.3 / 3.8; taken off in every step and 16 of these 85.4 / 2.5, and tiles of sixteen rows 10 - 30 %
+  // slower.)
+  constexpr int LEVEL = SPLIT ? 4 : 16;
   // The 2^64 of the product with codes, on the weights (f16) or on the scales (bf16, whose minima times 2^64 would leave f32's range).
   constexpr float OF_WEIGHTS = SPLIT ? 64.f : 0.f, UNIT_OF_WEIGHTS = SPLIT ? 0x1p-64f : 1.f, OF_SCALES = SPLIT ? 1.f : 0x1p64f;
   extern __shared__ unsigned char smem_raw[];
@@ -252,10 +256,9 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
   float q_sum[NT][2][GROUPS];
   uint32_t q_parts[NT][2];
   float o[NT][CHUNKS][2][4];             // sums of codes: elements 32 c + 4 (lane / 4) + 2 t (+ 1, times 16) of rows 2 (lane % 4) (+ 1)
-  const float centre = lane & 4 ? 7.f : 8.f;             // of the codes of this thread's tokens, which are odd or even
+  const float centre = lane & 4 ? 7.f : 8.f;             // of the codes of this thread's tokens, which are odd or even (bf16)
   const int upper = COPIES == 2 ? (lane & 3) >> 1 : 0;   // this thread's half of the groups
-  // Sums of weight times the middle of the codes (f16: times the minimum, and of what stands for weight times scale in the product,
-  // times the middle code), of this thread's tokens.
+  // Sums of weight times the middle of the codes (f16: times the minimum) of this thread's tokens
   float middle[NT][2][SETS];
   float top[NT][2];
   uint64_t weight_sum[NT];               // of both rows
@@ -465,7 +468,7 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
 #pragma unroll
               for (int t = 0; t < 2; ++t) o[nt][c][t][e] *= factor[e & 1];
         }
-        // What the elements of a row's group have in common goes to its middle.  (In this branch, which is rarely taken: behind the
+        // What the elements of a row's group have in common goes to `middle`.  (In this branch, which is rarely taken: behind the
         // product with values it cost 3 to 9 %.  Where registers are spilled, whenever it is taken: 8 new tokens for each of 64 sequences,
         // groups of 32, 177 us, 202 with a branch of its own; other tiles are 1 to 2 % faster with that.)
         if (level || SETS * NT > 4) {
@@ -504,7 +507,7 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
         origins[nt] = two(OF_WEIGHTS - (top[nt][0] == -infinity ? 0.f : top[nt][0]),
                           OF_WEIGHTS - (top[nt][1] == -infinity ? 0.f : top[nt][1]));
       auto add_values = [&](auto whole) {
-        float centres[NT][SETS][4] = {}; // minus the centre's part of what this step adds to o, in its places
+        float centres[NT][SETS][4] = {}; // (bf16) minus the centre's part of what this step adds to o, in its places
 #pragma unroll
         for (int m = 0; m < PARTS; ++m) {
           uint32_t pf[NT][SETS][2], rest[NT][SETS][2];                 // (weights times scales)^T as B fragments
@@ -538,19 +541,19 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
                 if (SPLIT) {
                   const float a = Elem<Wide>::to_float(uint16_t(rounded)), b = Elem<Wide>::to_float(uint16_t(rounded >> 16));
                   rest[nt][g][h] = movmatrix(Elem<Wide>::pack2(scaled[0] - a, scaled[1] - b));
-                  middle[nt][0][g] = fmaf(a, centre, middle[nt][0][g]);
-                  middle[nt][1][g] = fmaf(b, centre, middle[nt][1][g]);
                 }
               }
             }
           }
+          if (!SPLIT) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int g = 0; g < SETS; ++g) {
-              const uint32_t(&f)[2] = pf[nt][g];
-              Elem<Wide>::mma16816(centres[nt][g], LOW_CENTRE, HIGH_CENTRE, LOW_CENTRE, HIGH_CENTRE, f[0], f[1]);
-            }
+              for (int g = 0; g < SETS; ++g) {
+                const uint32_t(&f)[2] = pf[nt][g];
+                Elem<Wide>::mma16816(centres[nt][g], LOW_CENTRE, HIGH_CENTRE, LOW_CENTRE, HIGH_CENTRE, f[0], f[1]);
+              }
+          }
 #pragma unroll
           for (int pair = 0; pair < CHUNKS / 2; ++pair) {
             // codes of tokens 16 m + 2 (lane % 4) (+ 1; + 8): elements 32 c + 4 (lane / 4) .. of chunks 2 pair and 2 pair + 1
@@ -575,14 +578,16 @@ paged_rows_int4_kernel(const Int4Cache cache, const PagedParams p) {
               }
           }
         }
+        if (!SPLIT) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int c = 0; c < CHUNKS; ++c)
+            for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+              for (int t = 0; t < 2; ++t)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o[nt][c][t][e] += centres[nt][c / OF_GROUP % SETS][e];
+                for (int e = 0; e < 4; ++e) o[nt][c][t][e] += centres[nt][c / OF_GROUP % SETS][e];
+        }
       };
       if (all) add_values(Bool<true>{});
       else add_values(Bool<false>{});
