@@ -88,8 +88,8 @@ def test_sums_over_long_histories(cuda_device, dtype, skew, HQ, D, group):
     """So many sequences that one warp has a whole one of 65536 tokens, of which its sums must not lose what is below their last bits.
     For a step of 64 tokens four products (f16: eight) are added to a sum of codes, and as many to what is taken off it for the
     middle of the codes.  An addition may cut the sum, by 2^-23 of it, which is at most what sixteen steps leave between them (7.5
-    scales a weight) and one puts on top (15).  Whatever else is rounded goes either way: the mean of the results is four of its
-    deviations from that at most."""
+    scales a weight) and one puts on top (15); f16's sum is of four steps (15 each) and has less.  Whatever else is rounded goes
+    either way: the mean of the results is four of its deviations from that at most."""
     L, B = 65536, 2400
     q, cache, table, _, n = make([L], [1], HQ, 1, D, 64, group, dtype)
     g = torch.Generator().manual_seed(1)
